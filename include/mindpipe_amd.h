@@ -419,6 +419,69 @@ int mp_smooth_scales(const float *act_max, const float *w_colmax, int64_t k, dou
  * (smooth_ln_fcs_llama_like, smooth.py:91-101). */
 int mp_scale_columns(void *w, int dtype, int64_t rows, int64_t k, const void *scales, int divide, mp_stream_t stream);
 
+/* ---------------------------------------------------------------- serving over a paged key-value cache
+ *
+ * No counterpart in the reference (its runtimes bring their own attention and sampling): what a server of the W4A16 /
+ * W8A8 stacks runs between their linears.  fp16 or bf16 (`dtype`).  Strides are in elements, multiples of 8; base
+ * pointers are 16-byte aligned; the values of a position or head are contiguous. */
+
+/* One layer's cache.  k and v: pools of `pages` pages of `page_size` positions (a power of two from 8 to 32768) of every
+ * key-value head.  table int32 [batch, width], dense: the pages of each sequence in order (width * page_size up to
+ * 2^30).  A page number outside [0, pages) is an empty page: nothing is written there, its positions are not attended. */
+typedef struct mp_pages {
+  void *k, *v;
+  int64_t k_page, k_head, k_row, v_page, v_head, v_row; /* strides of a page, a head, a position */
+  int64_t pages;
+  int page_size;
+  const int32_t *table;
+  int64_t width;
+} mp_pages;
+
+/* Packed rows of new tokens, qkv [rows, nh + 2 kvh, head_dim] (row stride qkv_row): rotates queries and keys, writes keys
+ * and values into the cache and the queries to q_out [rows, nh, head_dim], dense.  Rows starts[b] .. starts[b + 1] - 1
+ * (starts int32 [batch + 1], ascending) are the last positions of sequence b, which has lens[b] positions once they are
+ * in; without starts row b is the last position of sequence b.  The first `rotary` values of a head (a multiple of
+ * 16) are rotated in fp32 by cos_t / sin_t [angles, rotary / 2] (fp32, 16-byte aligned) of the position and rounded
+ * once; pairs: values (2 i, 2 i + 1), else (i, i + rotary / 2).  head_dim a multiple of 16.  A row of no sequence, or
+ * whose position has no angle, gives a zero query and is not written to the cache; nor is one past the table's width.
+ * Where the table gives two positions of a call the same place, either's values may be left there. */
+int mp_paged_rope_append(const void *qkv, int64_t qkv_row, int64_t rows, int nh, int kvh, int head_dim, const float *cos_t,
+                         const float *sin_t, int rotary, int64_t angles, int pairs, void *q_out, const mp_pages *cache,
+                         const int32_t *lens, const int32_t *starts, int64_t batch, int dtype, mp_stream_t stream);
+
+/* out [batch, nh, head_dim], dense = softmax(scale q k^T) v of one query per sequence over its first lens[b] positions
+ * (held to what the table has room for), head_dim 64, 128 or 256, nh a multiple of kvh; nothing to attend gives zeros.
+ * Weights and sums in fp32, the weights rounded to the dtype for the product with v.  Long caches are split over
+ * workgroups and joined, always in the same order.  workspace: mp_paged_decode_workspace_bytes of the current device,
+ * 16-byte aligned, not shared by calls that may run at once. */
+size_t mp_paged_decode_workspace_bytes(int64_t batch, int nh, int kvh, int head_dim);
+int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q_head, int64_t batch, int nh, int kvh, int head_dim,
+                              const mp_pages *cache, const int32_t *lens, float scale, void *out, int dtype,
+                              void *workspace, size_t workspace_bytes, mp_stream_t stream);
+
+/* Causal attention of packed sequences: rows starts[b] .. starts[b + 1] - 1 of q [rows, nh, head_dim], k and v [rows, kvh,
+ * head_dim] are sequence b.  out [rows, nh, head_dim], dense; rows of no sequence are zeros.  head_dim 64, 128, 256. */
+int mp_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const void *k, int64_t k_row, int64_t k_head,
+                        const void *v, int64_t v_row, int64_t v_head, int64_t rows, int nh, int kvh, int head_dim,
+                        const int32_t *starts, int64_t batch, float scale, void *out, int dtype, mp_stream_t stream);
+
+/* The same with keys and values in the cache: the packed rows of sequence b are its last positions of lens[b] (as
+ * mp_paged_rope_append puts them there), and each sees the positions up to its own. */
+int mp_paged_prompt_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh, int head_dim,
+                              const mp_pages *cache, const int32_t *lens, const int32_t *starts, int64_t batch,
+                              float scale, void *out, int dtype, mp_stream_t stream);
+
+/* A token for each row of logits [rows, vocab] (row stride `stride`; fp16, bf16 or fp32; vocab up to 2^19) at the random
+ * number u in [0, 1): weights exp((x - max) / temperature) of the top_k largest values (equal ones: the lowest indexes;
+ * <= 0: all), of those the shortest run from the largest down that has top_p of their weight (>= 1: all; at least
+ * one), of those the ones of at least min_p times the largest weight; the first index at which their running sum
+ * in index order exceeds u times their sum.  temperature, top_k, top_p, min_p: one per row, NULL for 1, all, 1, 0.
+ * temperature <= 0: the largest value's first index.  Weights are summed in units of 2^-44 of the largest: what weighs
+ * less than half of that is never taken, nor are NaN and -inf; a row of nothing else gives -1 and -inf.  logprobs: the logarithm of the kept tokens' probability of the one taken (0 with temperature <= 0). */
+int mp_sample_tokens(const void *logits, int64_t stride, int64_t rows, int64_t vocab, int dtype, const float *u,
+                     const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                     int64_t *tokens, float *logprobs, mp_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,14 @@ ABI_VERSION = 2
 
 _vp, _i64, _i32, _sz = C.c_void_p, C.c_int64, C.c_int, C.c_size_t
 
+
+
+class Pages(C.Structure):
+    """``mp_pages``: the pools, strides and table of a paged key-value cache."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_page", _i64), ("k_head", _i64), ("k_row", _i64), ("v_page", _i64),
+                ("v_head", _i64), ("v_row", _i64), ("pages", _i64), ("page_size", _i32), ("table", _vp), ("width", _i64)]
+
+
 # name -> (restype, argtypes); mirrors include/mindpipe_amd.h one to one.
 SIGNATURES = {
     "mp_strerror": (C.c_char_p, [_i32]),
@@ -73,6 +81,16 @@ SIGNATURES = {
                                    _vp, C.c_size_t, _vp]),
     "mp_dq_linear": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp]),
     "mp_fake_quant_rows": (_i32, [_vp, _i32, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "mp_paged_rope_append": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _i64,
+                                    _i32, _vp]),
+    "mp_paged_decode_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "mp_paged_decode_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, C.c_float, _vp, _i32, _vp, _sz,
+                                         _vp]),
+    "mp_prompt_attention": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _i64,
+                                   C.c_float, _vp, _i32, _vp]),
+    "mp_paged_prompt_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, C.c_float, _vp, _i32,
+                                         _vp]),
+    "mp_sample_tokens": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mp_moe_unpermute_combine": (_i32, [_vp, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _i32, _vp]),
 }
 

@@ -115,13 +115,13 @@ class _Op(torch.library.CustomOpDef):
         return super().__call__(*args, **kwargs)
 
 
-def _op(name, ns="mindpipe_amd"):
+def _op(name, ns="mindpipe_amd", mutates=()):
     def register(fn):
-        op = torch.library.custom_op(f"{ns}::{name}", mutates_args=())(fn)
+        op = torch.library.custom_op(f"{ns}::{name}", mutates_args=mutates)(fn)
         op.__class__ = _Op  # torch.library.custom_op is the only way to make a CustomOpDef
         op.cuda_impl = f"{ns}/{name}/CUDA"
         op.light_name, op.__name__, op.__doc__ = name, fn.__name__, fn.__doc__
-        _LIGHT.define(name + torch.library.infer_schema(fn, mutates_args=()))
+        _LIGHT.define(name + torch.library.infer_schema(fn, mutates_args=mutates))
         _LIGHT.impl(name, fn, "CompositeExplicitAutograd")
         op.light = getattr(torch.ops.mindpipe_amd_light, name).default
         return op
@@ -1078,6 +1078,270 @@ def silu_mul(gate_up: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch
         _lib.check(_lib.load().mp_silu_mul(gate_up.data_ptr(), rows, two_i // 2, out.data_ptr(), _DT[gate_up.dtype],
                                            _stream()), "mp_silu_mul")
     return out
+
+
+# ---------------------------------------------------------------- serving over a paged key-value cache
+_HALF = (torch.float16, torch.bfloat16)
+
+
+def _need_strided(t: torch.Tensor, name: str, dtype, ndim: int) -> None:
+    """A GPU tensor whose last dimension is contiguous; the other strides are free, in steps of 16 bytes (the kernels
+    load rows in 16-byte pieces)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be on the GPU (mindpipe_amd has no CPU path)")
+    if t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+        raise RuntimeError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if t.dim() != ndim:
+        raise RuntimeError(f"{name} must be {ndim}-D, got shape {tuple(t.shape)}")
+    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or
+                      any(t.stride(i) % 8 for i in range(ndim - 1) if t.shape[i] > 1)):
+        raise RuntimeError(f"{name} must have contiguous values and rows in steps of 16 bytes, got strides {t.stride()}")
+
+
+def _same_device(t: torch.Tensor, **others: Optional[torch.Tensor]) -> None:
+    for name, o in others.items():
+        if o is not None and o.device != t.device:
+            raise RuntimeError(f"{name} is on {o.device}, expected {t.device}")
+
+
+def _step(t: torch.Tensor, dim: int) -> int:
+    """The stride of a dimension (0 of one that holds a single entry, whatever it says)."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, dtype):
+    """Checks the cache's tensors against each other; its description for the C entry points."""
+    _need_strided(k_pages, "k_pages", dtype, 4)
+    _need_strided(v_pages, "v_pages", dtype, 4)
+    _need(table, "table", torch.int32, 2)
+    _need(lens, "lens", torch.int32, 1)
+    _same_device(k_pages, v_pages=v_pages, table=table, lens=lens)
+    if v_pages.shape != k_pages.shape:
+        raise RuntimeError(f"v_pages {tuple(v_pages.shape)} must have the shape of k_pages {tuple(k_pages.shape)}")
+    pages, kvh, size, _ = k_pages.shape
+    if size < 8 or size > 32768 or size & (size - 1):
+        raise RuntimeError(f"a page holds a power of two of positions from 8 to 32768, got {size}")
+    if not pages or not kvh or not table.shape[1]:
+        raise RuntimeError("k_pages, v_pages and table must hold at least one page and one head")
+    if table.shape[0] != lens.shape[0]:
+        raise RuntimeError(f"table {tuple(table.shape)} and lens {tuple(lens.shape)} must have one row per sequence")
+    if table.shape[1] * size > 1 << 30:
+        raise RuntimeError(f"a sequence has at most 2^30 positions, the table has room for {table.shape[1] * size}")
+    return _lib.C.byref(_lib.Pages(
+        k_pages.data_ptr(), v_pages.data_ptr(), _step(k_pages, 0), _step(k_pages, 1), _step(k_pages, 2), _step(v_pages, 0),
+        _step(v_pages, 1), _step(v_pages, 2), pages, size, table.data_ptr(), table.shape[1]))
+
+
+def _attention_heads(q: torch.Tensor, kvh: int, dim: int) -> None:
+    if q.shape[2] != dim or dim not in (64, 128, 256):
+        raise RuntimeError(f"heads of 64, 128 or 256 values are taken, the same in q and the keys: got {q.shape[2]} and {dim}")
+    if not kvh or q.shape[1] % kvh or not q.shape[1]:
+        raise RuntimeError(f"{q.shape[1]} query heads cannot share {kvh} key-value heads")
+
+
+def _need_starts(starts: torch.Tensor, batch: Optional[int]) -> int:
+    _need(starts, "starts", torch.int32, 1)
+    if starts.shape[0] < 1 or (batch is not None and starts.shape[0] != batch + 1):
+        raise RuntimeError(f"starts must be [sequences + 1], got {tuple(starts.shape)}")
+    return starts.shape[0] - 1
+
+
+@_op("paged_rope_append", mutates=("k_pages", "v_pages"))
+def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                      table: torch.Tensor, lens: torch.Tensor, starts: Optional[torch.Tensor] = None,
+                      pairs: bool = True) -> torch.Tensor:
+    """Rotates the queries and keys of packed new tokens, writes keys and values into a paged cache and returns the
+    rotated queries ``[rows, nh, dim]``.
+
+    ``qkv [rows, (nh + 2 kvh) * dim]`` fp16 or bf16 (rows may be strided) holds the query, key and value heads of each
+    token.  ``k_pages`` / ``v_pages [pages, kvh, page, dim]`` are the pools (any strides over 16-byte rows), ``table``
+    int32 ``[sequences, width]`` lists each sequence's pages in order, and ``lens`` int32 counts each sequence's
+    positions with the new tokens.  Rows ``starts[b] .. starts[b + 1] - 1`` (``starts`` int32 ``[sequences + 1]``,
+    ascending) are the last positions of sequence b; without ``starts`` each sequence has one row.  The first ``2 *
+    cos.shape[1]`` values of a head turn by ``cos`` / ``sin`` fp32 ``[positions, rotary / 2]`` of the token's position, in
+    fp32 with one rounding: values ``(2 i, 2 i + 1)`` as ``decode_rope_append`` pairs them, or with ``pairs=False``
+    ``(i, i + rotary / 2)``.
+
+    Rows behind the last sequence, and positions without an angle, give zero queries and leave the cache as it is, and so
+    do the keys and values of a position past the table's width or in a page whose number is not the pool's.
+    Where the table gives two positions of one call the same place, either's values may be left there."""
+    _need_strided(qkv, "qkv", _HALF, 2)
+    cache = _paged_cache(k_pages, v_pages, table, lens, qkv.dtype)
+    _need(cos, "cos", torch.float32, 2)
+    _need(sin, "sin", torch.float32, 2)
+    _same_device(qkv, cos=cos, sin=sin, k_pages=k_pages, starts=starts)
+    _, kvh, _, dim = k_pages.shape
+    rows, batch = qkv.shape[0], lens.shape[0]
+    if dim % 16 or dim > 1024:
+        raise RuntimeError(f"heads of a multiple of 16 values up to 1024 are taken, got {dim}")
+    if qkv.shape[1] % dim or qkv.shape[1] // dim <= 2 * kvh:
+        raise RuntimeError(f"qkv {tuple(qkv.shape)} does not hold query heads and 2 x {kvh} heads of {dim}")
+    nh = qkv.shape[1] // dim - 2 * kvh
+    if sin.shape != cos.shape or not cos.shape[0] or not cos.shape[1] or cos.shape[1] % 8 or 2 * cos.shape[1] > dim:
+        raise RuntimeError(f"cos and sin must be [positions, rotary / 2] with rotary a multiple of 16 up to {dim}, got "
+                           f"{tuple(cos.shape)} and {tuple(sin.shape)}")
+    if cos.data_ptr() % 16 or sin.data_ptr() % 16:
+        raise RuntimeError("cos and sin must be 16-byte aligned")
+    if starts is not None:
+        _need_starts(starts, batch)
+    elif rows != batch:
+        raise RuntimeError(f"without starts each of the {batch} sequences has one row, got {rows}")
+    if not batch:
+        return torch.zeros((rows, nh, dim), dtype=qkv.dtype, device=qkv.device)
+    q = torch.empty((rows, nh, dim), dtype=qkv.dtype, device=qkv.device)
+    if rows:
+        with _dev(qkv):
+            _lib.check(_lib.load().mp_paged_rope_append(
+                qkv.data_ptr(), qkv.stride(0) if rows > 1 else qkv.shape[1], rows, nh, kvh, dim, cos.data_ptr(),
+                sin.data_ptr(), 2 * cos.shape[1], cos.shape[0], int(pairs), q.data_ptr(), cache, lens.data_ptr(),
+                _ptr(starts), batch, _DT[qkv.dtype], _stream()), "mp_paged_rope_append")
+    return q
+
+
+@paged_rope_append.register_fake
+def _(qkv, cos, sin, k_pages, v_pages, table, lens, starts=None, pairs=True):
+    dim = k_pages.shape[3]
+    return qkv.new_empty((qkv.shape[0], qkv.shape[1] // dim - 2 * k_pages.shape[1], dim))
+
+
+@_op("paged_decode_attention")
+def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                           lens: torch.Tensor, scale: float) -> torch.Tensor:
+    """Attention of one query per sequence, ``q [sequences, nh, dim]`` (fp16 or bf16, ``dim`` 64, 128 or 256), over the
+    first ``lens[b]`` positions of its pages (``paged_rope_append`` describes the cache); ``nh / kvh`` consecutive query
+    heads share a key-value head.  Returns ``[sequences, nh, dim]``; a sequence with nothing to attend gives zeros.
+    Long caches are split over workgroups and joined in a fixed order."""
+    _need_strided(q, "q", _HALF, 3)
+    cache = _paged_cache(k_pages, v_pages, table, lens, q.dtype)
+    _same_device(q, k_pages=k_pages)
+    b, nh, dim = q.shape
+    kvh = k_pages.shape[1]
+    _attention_heads(q, kvh, k_pages.shape[3])
+    if lens.shape[0] != b:
+        raise RuntimeError(f"q {tuple(q.shape)} and lens {tuple(lens.shape)} must have one row per sequence")
+    out = torch.empty((b, nh, dim), dtype=q.dtype, device=q.device)
+    if not b:
+        return out
+    lib = _lib.load()
+    with _dev(q):
+        wsb = lib.mp_paged_decode_workspace_bytes(b, nh, kvh, dim)
+        ws = torch.empty((wsb,), dtype=torch.uint8, device=q.device)
+        _lib.check(lib.mp_paged_decode_attention(
+            q.data_ptr(), _step(q, 0), _step(q, 1), b, nh, kvh, dim, cache, lens.data_ptr(), scale, out.data_ptr(),
+            _DT[q.dtype], ws.data_ptr(), wsb, _stream()), "mp_paged_decode_attention")
+    return out
+
+
+@paged_decode_attention.register_fake
+def _(q, k_pages, v_pages, table, lens, scale):
+    return q.new_empty(q.shape)
+
+
+@_op("prompt_attention")
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, scale: float) -> torch.Tensor:
+    """Causal attention of packed prompts: rows ``starts[b] .. starts[b + 1] - 1`` (int32 ``[sequences + 1]``, ascending) of
+    ``q [rows, nh, dim]`` and ``k``, ``v [rows, kvh, dim]`` are sequence b (fp16 or bf16, ``dim`` 64, 128 or 256; views of a
+    fused projection's rows are taken as they are).  Returns ``[rows, nh, dim]``; rows behind the last sequence are zeros."""
+    _need_strided(q, "q", _HALF, 3)
+    _need_strided(k, "k", q.dtype, 3)
+    _need_strided(v, "v", q.dtype, 3)
+    batch = _need_starts(starts, None)
+    _same_device(q, k=k, v=v, starts=starts)
+    rows, nh, dim = q.shape
+    if v.shape != k.shape or k.shape[0] != rows:
+        raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be alike, with a row for each of q {tuple(q.shape)}")
+    _attention_heads(q, k.shape[1], k.shape[2])
+    if not batch or not rows:
+        return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
+    out = torch.empty((rows, nh, dim), dtype=q.dtype, device=q.device)
+    with _dev(q):
+        _lib.check(_lib.load().mp_prompt_attention(
+            q.data_ptr(), _step(q, 0), _step(q, 1), k.data_ptr(), _step(k, 0), _step(k, 1), v.data_ptr(), _step(v, 0),
+            _step(v, 1), rows, nh, k.shape[1], dim, starts.data_ptr(), batch, scale, out.data_ptr(), _DT[q.dtype],
+            _stream()), "mp_prompt_attention")
+    return out
+
+
+@prompt_attention.register_fake
+def _(q, k, v, starts, scale):
+    return q.new_empty(q.shape)
+
+
+@_op("paged_prompt_attention")
+def paged_prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                           lens: torch.Tensor, starts: torch.Tensor, scale: float) -> torch.Tensor:
+    """Causal attention of packed new tokens over a paged cache that holds them (``paged_rope_append``): the rows of
+    sequence b in ``q [rows, nh, dim]`` are its last positions of ``lens[b]``, and each sees the positions up to its own:
+    whole prompts, chunks of one, or prompts behind a shared prefix.  Returns ``[rows, nh, dim]``; rows that see nothing,
+    those behind the last sequence among them, are zeros."""
+    _need_strided(q, "q", _HALF, 3)
+    cache = _paged_cache(k_pages, v_pages, table, lens, q.dtype)
+    batch = _need_starts(starts, lens.shape[0])
+    _same_device(q, k_pages=k_pages, starts=starts)
+    rows, nh, dim = q.shape
+    _attention_heads(q, k_pages.shape[1], k_pages.shape[3])
+    if not batch or not rows:
+        return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
+    out = torch.empty((rows, nh, dim), dtype=q.dtype, device=q.device)
+    with _dev(q):
+        _lib.check(_lib.load().mp_paged_prompt_attention(
+            q.data_ptr(), _step(q, 0), _step(q, 1), rows, nh, k_pages.shape[1], dim, cache, lens.data_ptr(),
+            starts.data_ptr(), batch, scale, out.data_ptr(), _DT[q.dtype], _stream()), "mp_paged_prompt_attention")
+    return out
+
+
+@paged_prompt_attention.register_fake
+def _(q, k_pages, v_pages, table, lens, starts, scale):
+    return q.new_empty(q.shape)
+
+
+@_op("sample_tokens")
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+                  top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                  min_p: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A token for each row of ``logits [rows, vocab]`` (fp16, bf16 or fp32; rows may be strided) at the random numbers ``u``
+    fp32 ``[rows]`` in ``[0, 1)``: ``(tokens int64, logprobs fp32)``.
+
+    One value per row, ``None`` where none is wanted: ``temperature`` fp32 (``<= 0``: the largest logit), ``top_k`` int32 (the
+    k largest, of equal ones those of the lowest index; ``<= 0``: all), ``top_p`` fp32 (of those the shortest run from the
+    largest down that has this share of their weight, one at least; ``>= 1``: all), ``min_p`` fp32 (of those the ones of
+    at least this share of the largest one's weight).  The token is the first, in index order, at which the running sum of
+    what is kept exceeds ``u`` times the whole, and its logprob the logarithm of its share (0 with ``temperature <= 0``).
+    Weights are summed in units of 2^-44 of the largest: a token of less than half of that is never taken, nor are NaN and
+    ``-inf``; a row of nothing else gives -1 and ``-inf``.  The same inputs give the same tokens."""
+    if not isinstance(logits, torch.Tensor):
+        raise TypeError("logits must be a tensor")
+    if not logits.is_cuda:
+        raise RuntimeError("logits must be on the GPU (mindpipe_amd has no CPU path)")
+    if logits.dtype not in _DT or logits.dim() != 2:
+        raise RuntimeError(f"logits must be fp16, bf16 or fp32 [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    stride = logits.stride(0) if rows > 1 else vocab
+    if vocab < 1 or vocab > 1 << 19 or (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
+        raise RuntimeError(f"logits must be rows of 1 to 2^19 contiguous values, got {tuple(logits.shape)} with strides "
+                           f"{logits.stride()}")
+    for name, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                        ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if t is not None or name == "u":
+            _need(t, name, dt, 1)
+            if t.shape[0] != rows:
+                raise RuntimeError(f"{name} must have one value for each of the {rows} rows, got {tuple(t.shape)}")
+    _same_device(logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    if rows:
+        with _dev(logits):
+            _lib.check(_lib.load().mp_sample_tokens(
+                logits.data_ptr(), stride, rows, vocab, _DT[logits.dtype], u.data_ptr(), _ptr(temperature), _ptr(top_k),
+                _ptr(top_p), _ptr(min_p), tokens.data_ptr(), logprobs.data_ptr(), _stream()), "mp_sample_tokens")
+    return tokens, logprobs
+
+
+@sample_tokens.register_fake
+def _(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    return (logits.new_empty(logits.shape[0], dtype=torch.int64), logits.new_empty(logits.shape[0], dtype=torch.float32))
 
 
 # ------------------------------------------------------------------ SmoothQuant smoothing
