@@ -17,6 +17,7 @@ namespace {
 
 typedef __bf16 abf8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 abf2_t __attribute__((ext_vector_type(2)));
+typedef short as2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 ah2_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -42,6 +43,16 @@ __device__ __forceinline__ uint32_t attn_pack2(float a, float b) {
     const abf2_t v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
     return __builtin_bit_cast(uint32_t, v);
   }
+}
+
+// sum + the two packed values: weights are summed as they are rounded for the second product, so that the rounding of a weight
+// that dominates cancels in the quotient.
+template <int DT>
+__device__ __forceinline__ float attn_add2(uint32_t w, float sum) {
+  if constexpr (DT == MP_F16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(ah2_t, w), ah2_t{1, 1}, sum, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(as2_t, w), as2_t{0x3F80, 0x3F80}, sum, false);
 }
 
 // The lowest fp16 magnitudes lose bits; weights are raised by 2^7 there, so that with the lag they end below 2^15 and keep

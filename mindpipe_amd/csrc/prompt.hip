@@ -1,14 +1,64 @@
 // Causal attention of packed new tokens: whole prompts (keys and values packed alike) or chunks of new tokens behind what
 // a paged cache holds of their sequences.
 //
-// The queries of the heads that share a key-value head are rows of one problem: row = token * group + head.  A workgroup
-// takes kRows consecutive rows of a sequence and a key-value head; row r sees the positions up to its token's.  The tiles of
-// the last rows, which see most, are started first.
+// The queries of the heads that share a key-value head are rows of one problem: row = token * group + head, and a row sees
+// the positions up to its token's.  A workgroup takes kRows consecutive rows of a sequence and a key-value head, 32 to
+// each wave, and walks over the positions in tiles:
+//
+//   S = K . Q^T,  P = exp2(scale S - m),  O^T += V^T . P^T   (MFMA 32x32x16)
+//
+// Both products have the query row as their column, so a row's maximum m, sum l, weights and outputs stay in its two lanes
+// (l & 31) and the weights go from the first product's accumulators to the second's operand without crossing lanes.
+// K and V tiles come by direct-to-LDS loads, a tile ahead; V is read transposed (ds_read_b64_tr_b16).  Rows of LDS are
+// swizzled in 16-byte chunks so that neither reads a bank twice at a time.
+#include <cfloat>
+#include <cmath>
+#include <type_traits>
+
 #include "attn_common.h"
 
 namespace {
 
-constexpr int kRows = 64;  // 16 for each of four waves
+constexpr int kWaves = 4, kRows = 32 * kWaves;
+
+typedef short as4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) as4_t *lds_as4;
+
+// Through buffer descriptors and integers, in non-template functions: the compiler makes LDS reads wait for the LDS loads that it
+// recognises as such.  Offsets are below 2^31 (the launch sees to it) and rows inside the tensors.
+__device__ __forceinline__ void prompt_lds_load16(const uint16_t *base, uint32_t offset, int8_t *lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      mp_rsrc(base, 0x80000000u), reinterpret_cast<__attribute__((address_space(3))) void *>(reinterpret_cast<uintptr_t>(lds)),
+      16, offset, 0, 0, 0);
+}
+// Four rows' values of one column: lane i of 16 gives 8 bytes of row i / 4 and gets column i of the four rows.
+__device__ __forceinline__ as4_t prompt_read_tr(const __restrict__ lds_as4 p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
+__device__ __forceinline__ uint2 prompt_read_tr(const int8_t *lds) {
+  return __builtin_bit_cast(uint2, prompt_read_tr((lds_as4) reinterpret_cast<uintptr_t>(lds)));
+}
+
+template <int DT>
+__device__ __forceinline__ f16_t prompt_mfma(uint4 a, uint4 b, f16_t c) {
+  if constexpr (DT == MP_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(abf8_t, a), __builtin_bit_cast(abf8_t, b), c, 0, 0,
+                                                   0);
+}
+
+template <int D>
+struct PromptTile {
+  static constexpr int kTile = D == 256 ? 32 : 64;  // positions
+  static constexpr int kChunks = D / 8;             // of 16 bytes in a row
+  static constexpr int kBytes = kTile * D * 2;      // of K or of V
+  static constexpr int kLoads = kBytes / 1024 / kWaves;
+  // LDS chunk of a row's chunk c (and back).  K is read by 16 rows at a time in one column of chunks, V by four rows at a time
+  // in four columns; 256 bytes are all banks.
+  static __device__ __forceinline__ int k_chunk(int row, int c) { return c ^ (D == 64 ? (row >> 1) & 7 : row & 15); }
+  static __device__ __forceinline__ int v_chunk(int row, int c) {
+    return c ^ (D == 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3));
+  }
+};
 
 struct PackedPlan {
   const int32_t *starts;
@@ -21,59 +71,215 @@ struct PackedPlan {
   }
 };
 
-template <int D, int DT, bool PAGED>
-__global__ __launch_bounds__(256) void prompt_attention_kernel(
-    const uint16_t *__restrict__ q, int64_t q_row, int64_t q_head, const uint16_t *__restrict__ k, int64_t kpage,
-    int64_t khead, int64_t krow, const uint16_t *__restrict__ v, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
-    int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
-    const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, int tiles, float scale2,
-    uint16_t *__restrict__ out) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, j = lane >> 4;
-  const int kh = blockIdx.x % kvh;
-  const PackedPlan plan{starts, batch, rows, grp};
-  int b, part, parts;
-  if (!attn_find_part(plan, batch + 1, kRows, tiles - 1 - static_cast<int>(blockIdx.x / kvh), b, part, parts)) return;
-  const int first = plan.first(b), n = plan.end(b) - first;
-  int len = 0;  // positions of the sequence, the new tokens' included
-  if (b < batch) len = PAGED ? min(max(lens[b], 0), width << shift) : n;
-  const int at = part * kRows + wave * 16 + i16;  // row of this lane
-  const bool row = at < n * grp;
-  const int token = row ? at / grp : 0, head = kh * grp + (row ? at - token * grp : 0);
-  // behind the last sequence (b == batch) nothing is seen, and zeros are written
-  const int sees = row && b < batch ? max(len - n + token + 1, 0) : 0;
-  int full = row ? sees : len, end = sees;
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    full = min(full, __shfl_xor(full, o, 64));
-    end = max(end, __shfl_xor(end, o, 64));
-  }
-  full = __builtin_amdgcn_readfirstlane(full);
-  end = __builtin_amdgcn_readfirstlane(end);
-
+// Rows r0 .. r0 + 15 by the wave alone, K and V straight from memory.
+template <int D, int DT, bool PAGED, class Seen>
+__device__ __forceinline__ void prompt_rows16(const KvSource<PAGED> &src, const uint16_t *q, int64_t q_row, int64_t q_head,
+                                              int r0, int all, int grp, Seen seen, float scale2, uint16_t *out, int64_t out_row) {
+  const int lane = threadIdx.x & 63, i16 = lane & 15, j = lane >> 4, at = min(r0 + i16, all - 1);
+  const int token = at / grp, head = at - token * grp;
+  const int full = __builtin_amdgcn_readfirstlane(seen(r0)), end = __builtin_amdgcn_readfirstlane(seen(r0 + 15));
   uint4 qf[D / 32];
-  const uint16_t *qp = q + (first + token) * q_row + head * q_head + 8 * j;
+  const uint16_t *qp = q + token * q_row + head * q_head + 8 * j;
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) qf[c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
-  KvSource<PAGED> src;
-  if constexpr (PAGED)
-    src = {k + kh * khead, v + kh * vhead, kpage, krow, vpage, vrow, table + static_cast<int64_t>(min(b, batch - 1)) * width,
-           shift, (1 << shift) - 1, pages, len > 0 ? (len - 1) >> shift : 0};
-  else
-    src = {k + first * krow + kh * khead, v + first * vrow + kh * vhead, krow, vrow, n - 1};
   AttnRows<D> a;
   attn_clear(a);
-  attn_walk<D, DT>(a, src, qf, 0, end, 32, sees, end, full, scale2, lane);
+  attn_walk<D, DT>(a, src, qf, 0, end, 32, seen(at), end, full, scale2, lane);
   const float l = attn_row_sum(a.l);
-  if (!row) return;
-  uint16_t *y = out + (static_cast<int64_t>(first + token) * kvh * grp + head) * D + (D / 16) * 4 * j;
+  if (r0 + i16 >= all) return;
+  uint16_t *y = out + token * out_row + head * D + (D / 16) * 4 * j;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
+  for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int c = 0; c < D / 16; c += 2) {
       const float lo = l == 0.f ? 0.f : a.o[c][r] / l, hi = l == 0.f ? 0.f : a.o[c + 1][r] / l;
       *reinterpret_cast<uint32_t *>(y + (D / 16) * r + c) = attn_pack2<DT>(lo, hi);
     }
+}
+
+template <int D, int DT, bool PAGED>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attention_kernel(
+    const uint16_t *__restrict__ q, int64_t q_row, int64_t q_head, const uint16_t *__restrict__ k, int64_t kpage,
+    int64_t khead, int64_t krow, const uint16_t *__restrict__ v, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
+    int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
+    const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, int tiles, float scale2,
+    uint32_t flip, uint16_t *__restrict__ out) {
+  using T = PromptTile<D>;
+  constexpr int kTile = T::kTile, kStage = 2 * T::kBytes, kS = kTile / 32;
+  extern __shared__ __attribute__((aligned(1024))) int8_t prompt_smem[];  // two stages of K and V
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i32 = lane & 31, h = lane >> 5;
+  const int kh = blockIdx.x % kvh;
+  const PackedPlan plan{starts, batch, rows, grp};
+  int b, part, parts;
+  if (!attn_find_part(plan, batch + 1, kRows, tiles - 1 - static_cast<int>(blockIdx.x / kvh), b, part, parts)) return;
+  const int first = plan.first(b), n = plan.end(b) - first, all = n * grp;
+  int len = 0;  // positions of the sequence, the new tokens' included; none behind the last sequence
+  if (b < batch) len = PAGED ? min(max(lens[b], 0), width << shift) : n;
+  // positions seen by row r of the sequence, and by none of a wave's or workgroup's rows past their last
+  const int before = len - n + 1;
+  const auto seen = [&](int r) { return b < batch ? max(before + min(r, all - 1) / grp, 0) : 0; };
+  const int r0 = part * kRows + wave * 32, at = r0 + i32;
+  const bool row = at < all;
+  const int token = row ? at / grp : 0, head = kh * grp + (row ? at - token * grp : 0);
+  const int sees = row ? seen(at) : 0;
+  const int full = r0 < all ? __builtin_amdgcn_readfirstlane(seen(r0)) : 0;
+  const int wend = r0 < all ? __builtin_amdgcn_readfirstlane(seen(r0 + 31)) : 0;
+  const int end = __builtin_amdgcn_readfirstlane(seen(part * kRows + kRows - 1));
+
+  uint4 qf[D / 16];
+  const uint16_t *qp = q + (first + token) * q_row + head * q_head + 8 * h;
+#pragma unroll
+  for (int c = 0; c < D / 16; ++c) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(qp + 16 * c);
+    qf[c] = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
   }
+
+  const uint16_t *kb = k + kh * khead + (PAGED ? 0 : first * krow), *vb = v + kh * vhead + (PAGED ? 0 : first * vrow);
+  const int32_t *pg = PAGED ? table + static_cast<int64_t>(min(b, batch - 1)) * width : nullptr;
+  // page of the tile's position `lane` (positions past the end: the last one's)
+  const auto entry = [&](int tile) { return PAGED ? pg[min(tile + lane, end - 1) >> shift] : 0; };
+  const auto load = [&](int tile, int id, int8_t *stage) {
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) {
+      const int slot = (wave * T::kLoads + i) * 64, r = slot / T::kChunks + lane / T::kChunks, c = lane % T::kChunks;
+      const int p = min(tile + r, end - 1);
+      // the rows of one load lie in one page
+      const int64_t pid = PAGED ? __builtin_amdgcn_readlane(id, slot / T::kChunks) : 0;
+      const uint32_t off = PAGED ? p & ((1 << shift) - 1) : p - tile;
+      prompt_lds_load16(kb + (PAGED ? pid * kpage : tile * krow), 2 * (off * static_cast<uint32_t>(krow) + 8 * T::k_chunk(r, c)),
+                        stage + slot * 16);
+      prompt_lds_load16(vb + (PAGED ? pid * vpage : tile * vrow), 2 * (off * static_cast<uint32_t>(vrow) + 8 * T::v_chunk(r, c)),
+                        stage + T::kBytes + slot * 16);
+    }
+  };
+
+  f16_t o[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  const auto fix = [&](int id, uint64_t &there) {  // page numbers outside the pool: page 0, unseen
+    if constexpr (!PAGED) return 0;
+    const bool ok = id >= 0 && id < pages;
+    there = __ballot(ok || lane >= kTile);
+    return ok ? id : 0;
+  };
+  uint64_t there = ~uint64_t(0), next_there = there;
+  int ahead = 0;
+  if (end > 0) {
+    load(0, fix(entry(0), there), prompt_smem);
+    ahead = entry(kTile);
+  }
+  int stage = 0;
+  uint32_t odd = 0;  // an infinity or NaN in V where only some of the wave's rows see it
+  for (int tile = 0; tile < end; tile += kTile) {
+    // this tile's loads have landed, every wave's, and the other stage has been read
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (tile + kTile < end) {
+      load(tile + kTile, fix(ahead, next_there), prompt_smem + (stage ^ 1) * kStage);
+      ahead = entry(tile + 2 * kTile);
+    }
+    const int8_t *ks = prompt_smem + stage * kStage, *vs = ks + T::kBytes;
+    stage ^= 1;
+    const uint64_t ok = there;
+    there = next_there;
+    if (tile >= wend) continue;  // rows that see nothing more load for the others
+    f16_t s[kS];
+#pragma unroll
+    for (int t = 0; t < kS; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+      const int r = 32 * t + i32;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        const i4_t kf = *reinterpret_cast<const i4_t *>(ks + r * (D * 2) + 16 * T::k_chunk(r, 2 * c + h));
+        s[t] = prompt_mfma<DT>(__builtin_bit_cast(uint4, kf), qf[c], s[t]);
+      }
+    }
+    // s[t][r]: position 32 t + 8 (r >> 2) + 4 h + (r & 3) of the tile
+    if (tile + kTile > full || ok != ~uint64_t(0)) {
+      const uint64_t vis = ok >> (4 * h);
+#pragma unroll
+      for (int t = 0; t < kS; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int p = 32 * t + 8 * (r >> 2) + (r & 3);
+          s[t][r] = tile + p + 4 * h < sees && ((vis >> p) & 1) ? s[t][r] : -INFINITY;
+        }
+      for (int e = lane; e < T::kBytes / 16; e += 64) {
+        const i4_t x = *reinterpret_cast<const i4_t *>(vs + 16 * e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd |= attn_odd16<DT>(x[i]) || attn_odd16<DT>(static_cast<uint32_t>(x[i]) >> 16);
+      }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < kS; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+    top *= scale2;
+    if (__any(top > m + kMaxLag)) {
+      const float new_m = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+      const float f = m == new_m ? 1.0f : __builtin_amdgcn_exp2f(m - new_m);
+      l *= f;
+      m = new_m;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= f;
+    }
+    const float base = m == -INFINITY ? 0.f : m - kRaise<DT>;
+    uint32_t w[kS][8];
+#pragma unroll
+    for (int t = 0; t < kS; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        w[t][r / 2] = attn_pack2<DT>(__builtin_amdgcn_exp2f(fmaf(s[t][r], scale2, -base)),
+                                     __builtin_amdgcn_exp2f(fmaf(s[t][r + 1], scale2, -base)));
+        l = attn_add2<DT>(w[t][r / 2], l);
+      }
+    // O^T: step c of 16 positions, whose weights are w[c / 2][4 (c & 1) ..]: positions 16 c + 4 h + {0..3, 8..11}
+    const int trow = 4 * h + ((lane & 15) >> 2), tcol = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+#pragma unroll
+    for (int c = 0; c < kTile / 16; ++c) {
+      const uint4 wf = make_uint4(w[c / 2][4 * (c & 1)], w[c / 2][4 * (c & 1) + 1], w[c / 2][4 * (c & 1) + 2],
+                                  w[c / 2][4 * (c & 1) + 3]);
+      const int ra = 16 * c + trow, rb = ra + 8;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) {
+        const uint2 lo = prompt_read_tr(vs + ra * (D * 2) + 16 * T::v_chunk(ra, 4 * d + tcol) + 8 * (lane & 1));
+        const uint2 hi = prompt_read_tr(vs + rb * (D * 2) + 16 * T::v_chunk(rb, 4 * d + tcol) + 8 * (lane & 1));
+        o[d] = prompt_mfma<DT>(make_uint4(lo.x, lo.y, hi.x, hi.y), wf, o[d]);
+      }
+    }
+  }
+  if (__any(odd)) {
+    // 0 times an infinity is no zero: these rows once more, with what they do not see left out one position at a time
+    KvSource<PAGED> src;
+    if constexpr (PAGED) src = {kb, vb, kpage, krow, vpage, vrow, pg, shift, (1 << shift) - 1, pages, (len - 1) >> shift};
+    else src = {kb, vb, krow, vrow, n - 1};
+    const int64_t out_row = static_cast<int64_t>(kvh) * grp * D;
+    for (int half = 0; half < 2; ++half)
+      if (r0 + 16 * half < all)
+        prompt_rows16<D, DT, PAGED>(src, q + first * q_row + kh * grp * q_head, q_row, q_head, r0 + 16 * half, all, grp, seen,
+                                    flip ? -scale2 : scale2, out + first * out_row + kh * grp * D, out_row);
+    return;
+  }
+  if (!row) return;
+  l += __shfl_xor(l, 32, 64);
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  uint16_t *y = out + (static_cast<int64_t>(first + token) * kvh * grp + head) * D + 4 * h;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = l == 0.f ? 0.f : o[d][r + i] * inv;
+      *reinterpret_cast<uint2 *>(y + 32 * d + 2 * r) = make_uint2(attn_pack2<DT>(x[0], x[1]), attn_pack2<DT>(x[2], x[3]));
+    }
 }
 
 struct PromptCall {
@@ -94,6 +300,7 @@ struct PromptCall {
 template <bool PAGED>
 int prompt_launch(const PromptCall &c) {
   if (c.dtype != MP_F16 && c.dtype != MP_BF16) return MP_ERR_DTYPE;
+  if (!std::isfinite(c.scale)) return MP_ERR_ARG;
   if (c.rows < 0 || c.rows > INT32_MAX || c.batch < 1 || c.batch > INT32_MAX - 64) return MP_ERR_SHAPE;
   if (c.nh < 1 || c.kvh < 1 || c.nh > 65536 || c.nh % c.kvh) return MP_ERR_SHAPE;
   if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return MP_ERR_SHAPE;
@@ -101,25 +308,44 @@ int prompt_launch(const PromptCall &c) {
     if (s < 0 || s % 8) return MP_ERR_SHAPE;
   for (const void *p : {c.q, c.k, c.v, static_cast<const void *>(c.out)})
     if (!mp_aligned(p, 16)) return MP_ERR_ALIGN;
+  // byte offsets inside a page, or a tile, are 32 bits
+  const int64_t span = PAGED ? int64_t(1) << c.shift : 64, reach = (int64_t(1) << 30) - 256;
+  if (c.krow > reach / span || c.vrow > reach / span) return MP_ERR_SHAPE;
   if (c.rows == 0) return MP_OK;
   const int64_t grp = c.nh / c.kvh;
   // a part of a tile for each sequence, and for the rows behind the last one
   const int64_t tiles = c.rows * grp / kRows + c.batch + 1, blocks = tiles * c.kvh;
   if (c.rows * grp > INT32_MAX - kRows || blocks > INT32_MAX) return MP_ERR_SHAPE;
+  // the sign of the scale goes to the queries, so that the largest product gives the largest score; a scale of 0 becomes the
+  // smallest normal number, which leaves every finite score 0 and a masked one -inf
+  const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
+  const float scale2 = fmaxf(fabsf(c.scale) * kLog2e, FLT_MIN);
 #define MP_PROMPT(D, DT)                                                                                                  \
-  hipLaunchKernelGGL((prompt_attention_kernel<D, DT, PAGED>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, c.stream, \
+  if (hipFuncSetAttribute(reinterpret_cast<const void *>(prompt_attention_kernel<D, DT, PAGED>),                          \
+                          hipFuncAttributeMaxDynamicSharedMemorySize, 4 * PromptTile<D>::kBytes) != hipSuccess)           \
+    return MP_ERR_HIP;                                                                                                    \
+  hipLaunchKernelGGL((prompt_attention_kernel<D, DT, PAGED>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),     \
+                     4 * PromptTile<D>::kBytes, c.stream,                                                                 \
                      static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(c.k), c.kpage,  \
                      c.khead, c.krow, static_cast<const uint16_t *>(c.v), c.vpage, c.vhead, c.vrow, c.pages, c.shift,     \
                      c.table, c.width, c.lens, c.starts, static_cast<int>(c.batch), static_cast<int>(c.rows), c.kvh,      \
-                     static_cast<int>(grp), static_cast<int>(tiles), c.scale * kLog2e, static_cast<uint16_t *>(c.out))
+                     static_cast<int>(grp), static_cast<int>(tiles), scale2, flip, static_cast<uint16_t *>(c.out))
   if (c.dtype == MP_F16) {
-    if (c.head_dim == 64) MP_PROMPT(64, MP_F16);
-    else if (c.head_dim == 128) MP_PROMPT(128, MP_F16);
-    else MP_PROMPT(256, MP_F16);
+    if (c.head_dim == 64) {
+      MP_PROMPT(64, MP_F16);
+    } else if (c.head_dim == 128) {
+      MP_PROMPT(128, MP_F16);
+    } else {
+      MP_PROMPT(256, MP_F16);
+    }
   } else {
-    if (c.head_dim == 64) MP_PROMPT(64, MP_BF16);
-    else if (c.head_dim == 128) MP_PROMPT(128, MP_BF16);
-    else MP_PROMPT(256, MP_BF16);
+    if (c.head_dim == 64) {
+      MP_PROMPT(64, MP_BF16);
+    } else if (c.head_dim == 128) {
+      MP_PROMPT(128, MP_BF16);
+    } else {
+      MP_PROMPT(256, MP_BF16);
+    }
   }
 #undef MP_PROMPT
   MP_CHECK_LAUNCH();
