@@ -7,74 +7,264 @@
 //
 // A token is decided by which side of a border a sum over the vocabulary falls on, so weights are computed in 64 bits
 // and summed as whole numbers of 2^-44: sums of up to 2^19 of them fit 63 bits, and no order of additions changes them.
+//
+// Nothing is sorted.  A workgroup takes a row.  It counts the values into 2048 bins of equal width below the maximum (counts for
+// top-k, weights for top-p) and so finds the bin that the border of the kept is in.  The values down to that bin, few as a
+// rule, are copied to LDS in index order, and the rest is done on them (on the whole row, where they are more than
+// kListed): the bin's values are counted into bins of neighbouring values down to single ones, which gives the border, a
+// value and how many of its ties; then weights are summed by spans of indexes and the token looked up.
 #include "mp_common.h"
 
 namespace {
 
-constexpr int kThreads = 1024, kWavesPerRow = kThreads / 64;
+constexpr int kMaxWaves = 16;
 constexpr int kMaxVocab = 1 << 19;
-constexpr int kSpan = 512;                     // indexes of one wave step: eight per lane
-constexpr int kMaxSpans = kMaxVocab / kSpan;
+constexpr int kSpan = 512;                     // indexes of one step of a wave: eight neighbours per lane
+constexpr int kMaxSpans = kMaxVocab / kSpan + kMaxWaves;  // the waves' counts are rounded up
 constexpr int kBins = 2048;
+constexpr int kTable = 1024;                   // 2^(j / 1024)
 constexpr double kOne = 17592186044416.0;      // 2^44
 constexpr float kReach = 32.0f;                // e^-32 < 2^-46: past it a weight is no part of 2^-44
 
-__device__ __forceinline__ float sample_value(const void *x, int64_t i, int dt) {
-  const float v = mp_load_as_f32(x, i, dt);
-  return v != v ? -INFINITY : v + 0.0f;  // NaN is never taken; -0 is 0
-}
+constexpr int kListed = kSpan;                 // values of a wave that LDS has room for
 
-// Eight values from index i on, past the end -inf.
+struct SampleShared {
+  double table[kTable];
+  uint64_t mass[kBins];
+  uint64_t span_mass[kMaxSpans];
+  uint64_t wave_mass[kMaxWaves];
+  uint64_t before_mass;
+  uint32_t count[kBins];
+  uint32_t span_ties[kMaxSpans];
+  uint32_t wave_count[kMaxWaves];
+  float top[kMaxWaves];
+  int at[kMaxWaves];
+  int found;
+  uint32_t before_count;
+  float value[kMaxWaves][kListed];
+  int index[kMaxWaves][kListed];
+  int listed[kMaxWaves];
+};
+
+// Eight neighbouring values from index i on, past the end -inf.
 template <int DT>
-__device__ __forceinline__ void sample_load8(const uint8_t *row, int i, int vocab, bool vec, float (&v)[8]) {
-  if (vec && i + 8 <= vocab) {
-    constexpr int N = MpChunk16<DT>::N;
-    const uint4 *p = reinterpret_cast<const uint4 *>(row + static_cast<int64_t>(i) * (16 / N));
+struct Eight {
+  static constexpr int kWords = DT == MP_F32 ? 8 : 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const uint8_t *row, int i, int vocab, bool vec) {
+    if (vec && i + 8 <= vocab) {
+      const uint4 *p = reinterpret_cast<const uint4 *>(row + static_cast<int64_t>(i) * (kWords / 2));
 #pragma unroll
-    for (int c = 0; c < 8 / N; ++c) {
-      float f[N];
-      mp_chunk_to_f32<DT>(p[c], f);
-#pragma unroll
-      for (int e = 0; e < N; ++e) v[c * N + e] = f[e] != f[e] ? -INFINITY : f[e] + 0.0f;
+      for (int c = 0; c < kWords / 4; ++c) {
+        const uint4 x = p[c];
+        w[4 * c] = x.x;
+        w[4 * c + 1] = x.y;
+        w[4 * c + 2] = x.z;
+        w[4 * c + 3] = x.w;
+      }
+      return;
     }
-    return;
-  }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = i + e < vocab ? sample_value(row, i + e, DT) : -INFINITY;
-}
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (DT == MP_F32) {
+        w[e] = i + e < vocab ? reinterpret_cast<const uint32_t *>(row)[i + e] : 0xFF800000u;
+      } else {
+        const uint32_t h = i + e < vocab ? reinterpret_cast<const uint16_t *>(row)[i + e] : (DT == MP_F16 ? 0xFC00u : 0xFF80u);
+        w[e / 2] = e & 1 ? w[e / 2] | h << 16 : h;
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (DT == MP_F32) v[e] = __uint_as_float(w[e]);
+      else if constexpr (DT == MP_BF16) v[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
+      else v[e] = mp_h2f(static_cast<uint16_t>(e & 1 ? w[e / 2] >> 16 : w[e / 2]));
+    }
+  }
+};
+
+__device__ __forceinline__ void sample_renew(uint32_t &w) { asm volatile("" : "+v"(w)); }
+
+// The row: in registers where it has up to CH chunks, or else (CH = 0) in memory, read anew in every pass (from the L2,
+// past the first).
+template <int DT, int CH>
+struct SampleRow {
+  const uint8_t *row;
+  int vocab, chunks;  // a wave's steps of kSpan values: wave w has the spans w * chunks ..
+  bool vec;
+  bool infinite = false;  // the maximum is +inf: such values are 0, all others -inf
+  Eight<DT> held[CH > 0 ? CH : 1];
+
+  __device__ __forceinline__ int first(int c) const { return ((threadIdx.x >> 6) * chunks + c) * kSpan + 8 * (threadIdx.x & 63); }
+  __device__ __forceinline__ void load() {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (c < chunks) held[c].load(row, first(c), vocab, vec);
+  }
+  template <bool RAW>
+  __device__ __forceinline__ void values(const Eight<DT> &x, float (&v)[8]) const {
+    x.get(v);
+    if (!RAW) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fmaxf(v[e], -INFINITY);  // NaN
+    }
+    if (infinite) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = v[e] == INFINITY ? 0.f : -INFINITY;
+    }
+  }
+  // f(chunk, its eight values); RAW: NaN as it is, for what compares with it or takes it for the last bin
+  template <bool RAW = false, class F>
+  __device__ __forceinline__ void each(F f) {
+    if constexpr (CH > 0) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (c < chunks) {
+          // the words are new to the compiler in every pass: it would keep what it unpacked in the last one, and spill it
+#pragma unroll
+          for (int i = 0; i < Eight<DT>::kWords; ++i) sample_renew(held[c].w[i]);
+          float v[8];
+          values<RAW>(held[c], v);
+          f(c, v);
+        }
+      return;
+    }
+    constexpr int kAhead = DT == MP_F32 ? 2 : 4;  // steps that are asked for before they are looked at
+    Eight<DT> x[kAhead];
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c)
+      if (c < chunks) x[c].load(row, first(c), vocab, vec);
+    for (int c0 = 0; c0 < chunks; c0 += kAhead) {
+#pragma unroll
+      for (int c = 0; c < kAhead; ++c) {
+        if (c0 + c >= chunks) break;
+        const Eight<DT> now = x[c];
+        if (c0 + c + kAhead < chunks) x[c].load(row, first(c0 + c + kAhead), vocab, vec);
+        float v[8];
+        values<RAW>(now, v);
+        f(c0 + c, v);
+      }
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void one(int c, F f) const {
+    Eight<DT> x;
+    x.load(row, first(c), vocab, vec);
+    float v[8];
+    values<false>(x, v);
+    f(c, v);
+  }
+  __device__ __forceinline__ int index(int c, int e) const { return first(c) + e; }
+  __device__ __forceinline__ int span(int c) const { return (threadIdx.x >> 6) * chunks + c; }
+};
+
+// What of it is in LDS, in the same order: one chunk, `per` neighbours to a thread.
+template <int W>
+struct SampleList {
+  const SampleShared *s;
+  static constexpr int chunks = 1;
+  int per, all;
+  float v[8];
+  // wave and place of the list's entry i
+  __device__ __forceinline__ void find(int i, int &wave, int &at) const {
+    wave = 0;
+    at = i;
+#pragma unroll
+    for (int w = 0; w < W - 1; ++w) {
+      const bool on = wave == w && at >= s->listed[w];
+      at -= on ? s->listed[w] : 0;
+      wave += on ? 1 : 0;
+    }
+  }
+  __device__ __forceinline__ void load() {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = -INFINITY;
+      if (e < per && per * static_cast<int>(threadIdx.x) + e < all) {
+        int wave, at;
+        find(per * threadIdx.x + e, wave, at);
+        v[e] = s->value[wave][at];
+      }
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void each(F f) { f(0, v); }
+  template <class F>
+  __device__ __forceinline__ void one(int, F f) const { f(0, v); }
+  __device__ __forceinline__ int index(int, int e) const {
+    int wave, at;
+    find(per * threadIdx.x + e, wave, at);
+    return s->index[wave][at];
+  }
+  __device__ __forceinline__ int span(int) const { return threadIdx.x >> 6; }
+};
 
 // Order of the values as unsigned numbers, without the trailing bits that are alike in all values of the type.
 template <int DT>
+constexpr int kDrop = DT == MP_F32 ? 0 : DT == MP_F16 ? 13 : 16;
+template <int DT>
 __device__ __forceinline__ uint32_t sample_key(float v) {
-  constexpr int kDrop = DT == MP_F32 ? 0 : DT == MP_F16 ? 13 : 16;
-  const uint32_t b = __float_as_uint(v);
-  return (b & 0x80000000u ? ~b : b | 0x80000000u) >> kDrop;
+  const uint32_t b = __float_as_uint(v + 0.0f);  // -0 is 0
+  return (b & 0x80000000u ? ~b : b | 0x80000000u) >> kDrop<DT>;
+}
+template <int DT>
+__device__ __forceinline__ float sample_value(uint32_t key) {
+  const uint32_t k = key << kDrop<DT>, low = (1u << kDrop<DT>) - 1;
+  return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~(k | low));
 }
 
-__device__ __forceinline__ uint64_t sample_weight(float v, float top, double inv_t) {
-  if (v == top) return static_cast<uint64_t>(kOne);
-  const double d = (static_cast<double>(v) - static_cast<double>(top)) * inv_t;
-  return d > -kReach ? static_cast<uint64_t>(exp(d) * kOne + 0.5) : 0;  // also -inf
-}
-
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-__device__ __forceinline__ uint64_t wave_scan64(uint64_t v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t u = __shfl_up(v, o, 64);
-    v += lane >= o ? u : 0;
+struct Weight {
+  const double *table;  // LDS
+  double top, rate;     // the largest value, log2 e / T
+  // exp((v - top) / T) in units of 2^-44: 2^(k / 1024) from the table, and the rest of the exponent, below 2^-11, by a cubic
+  // (off by less than 2^-50)
+  __device__ __forceinline__ uint64_t operator()(float v) const {
+    const double y = (static_cast<double>(v) - top) * rate;
+    const double magic = 1.5 * 0x1p42;  // a sum with it ends in 2^-10
+    const double t = y + magic;
+    const double r = y - (t - magic);
+    const int k = __double2loint(t);
+    const double q = r * fma(r, fma(r, 0.05550410866482158, 0.24022650695910072), 0.6931471805599453);
+    const double b = table[k & (kTable - 1)];
+    const double w = ldexp(fma(b, q, b), (k >> 10) + 44) + 0x1p52;  // below 2^45: the sum's last bits are the number
+    const uint64_t n = static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
+    return y > -46.0 ? n : 0;  // also -inf
   }
+};
+
+// One step of a scan over the wave: lanes whose row or bank is masked, or whose source is none, add 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_from(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_from(uint64_t v) {
+  const uint32_t lo = dpp_from<CTRL, ROWS>(static_cast<uint32_t>(v)), hi = dpp_from<CTRL, ROWS>(static_cast<uint32_t>(v >> 32));
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+// Sums up to and with each lane: within rows of 16 (row_shr 1, 2, 4, 8), then row 0 into 1 and 2 into 3, then 1 into 2 and 3.
+template <class U>
+__device__ __forceinline__ U wave_scan(U v) {
+  v += dpp_from<0x111, 0xF>(v);
+  v += dpp_from<0x112, 0xF>(v);
+  v += dpp_from<0x114, 0xF>(v);
+  v += dpp_from<0x118, 0xF>(v);
+  v += dpp_from<0x142, 0xA>(v);  // row_bcast 15
+  v += dpp_from<0x143, 0xC>(v);  // row_bcast 31
   return v;
 }
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) { return __builtin_amdgcn_readlane(v, 63); }
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
+  return static_cast<uint64_t>(last_lane(static_cast<uint32_t>(v >> 32))) << 32 | last_lane(static_cast<uint32_t>(v));
+}
+template <class U>
+__device__ __forceinline__ U wave_sum(U v) {
+  return last_lane(wave_scan(v));
+}
 
-struct Border {       // the kept: keys above `key`, and the first `ties` indexes at it
-  uint32_t key;
-  uint32_t ties;
-  uint64_t mass;      // weight of the kept
+struct Border {  // the kept: keys above `key`, and the first `ties` indexes at it
+  uint32_t key, ties;
 };
 
 // What a border is looked for by: so many values, or so much weight.
@@ -84,365 +274,467 @@ struct Target {
   double mass;
 };
 
-struct SampleShared {
-  uint64_t mass[kBins];
-  uint32_t count[kBins];
-  uint64_t span_mass[kMaxSpans];
-  uint32_t span_ties[kMaxSpans];
-  float top[kWavesPerRow];
-  int at[kWavesPerRow];
-  uint64_t wave_mass[kWavesPerRow];
-  uint32_t wave_count[kWavesPerRow];
-  int found;
-  uint64_t before_mass;
-  uint32_t before_count;
-};
-
-// The first bin, from bin 0 up, at which the running count or mass reaches the target, with what lies before it.  The last
-// bin where none does.  All threads; kThreads = kBins / 2.
-__device__ __forceinline__ int find_bin(SampleShared &s, const Target &t, uint32_t &count, uint64_t &mass) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
-  const uint64_t m0 = s.mass[2 * tid], m1 = s.mass[2 * tid + 1];
-  uint64_t upto = wave_scan64(m0 + m1, lane);
-  uint32_t cupto = static_cast<uint32_t>(wave_scan64(c0 + c1, lane));
-  if (lane == 63) {
-    s.wave_mass[wave] = upto;
-    s.wave_count[wave] = cupto;
-  }
-  if (tid == 0) s.found = kBins - 1;
+template <int W>
+__device__ __forceinline__ void clear_bins(SampleShared &s) {
   __syncthreads();
-  for (int w = 0; w < wave; ++w) {
-    upto += s.wave_mass[w];
-    cupto += s.wave_count[w];
-  }
-  const auto there = [&](uint32_t c, uint64_t m) {
-    return t.by_mass ? static_cast<double>(m) >= t.mass : c >= t.count;
-  };
-  if (there(cupto - c1, upto - m1)) atomicMin(&s.found, 2 * tid);
-  else if (there(cupto, upto)) atomicMin(&s.found, 2 * tid + 1);
-  __syncthreads();
-  const int bin = s.found;
-  if (bin >> 1 == tid) {
-    const bool odd = bin & 1;
-    s.before_count = cupto - c1 - (odd ? 0 : c0);
-    s.before_mass = upto - m1 - (odd ? 0 : m0);
+#pragma unroll
+  for (int b = 0; b < kBins; b += 64 * W) {
+    s.mass[b + threadIdx.x] = 0;
+    s.count[b + threadIdx.x] = 0;
   }
   __syncthreads();
-  count = s.before_count;
-  mass = s.before_mass;
-  return bin;
 }
 
-// The border inside the values of [low, high] (keys; those above `high` are `count` with weight `mass`): bins of keys,
-// refined until a bin is one key.
-template <int DT>
-__device__ __forceinline__ Border find_border(SampleShared &s, const uint8_t *row, int vocab, bool vec, float top, double inv_t,
-                                              uint32_t low, uint32_t high, Target t, uint32_t count, uint64_t mass) {
+// Sum of the waves' `v` before this wave; `all`: of all of them.  One barrier.
+template <int W, class U>
+__device__ __forceinline__ U waves_before(U *of_wave, U v, U &all) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (lane == 0) of_wave[wave] = v;
+  __syncthreads();
+  const U upto = wave_scan(lane < W ? of_wave[lane] : U(0));
+  all = last_lane(upto);
+  return __shfl(upto, wave, 64) - v;
+}
+
+// The first bin, from bin 0 up, at which the running count or mass reaches the target, with what lies before it; the last
+// bin where none does.  The thread whose bins the target is reached in says so.
+template <int W>
+__device__ __forceinline__ int find_bin(SampleShared &s, const Target &t, uint32_t &count, uint64_t &mass) {
+  constexpr int kOwn = kBins / 64 / W;  // a thread's bins
   const int tid = threadIdx.x;
+  if (t.by_mass) {
+    uint64_t own[kOwn], sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) sum += own[i] = s.mass[kOwn * tid + i];
+    const uint64_t scan = wave_scan(sum);
+    uint64_t at = scan - sum + waves_before<W>(s.wave_mass, last_lane(scan), all);
+    bool open = tid == 0 || static_cast<double>(at) < t.mass;
+    if (open && (static_cast<double>(at + sum) >= t.mass || tid == 64 * W - 1)) {
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        if (open && (static_cast<double>(at + own[i]) >= t.mass || i == kOwn - 1)) {
+          s.found = kOwn * tid + i;
+          s.before_mass = at;
+          open = false;
+        }
+        at += own[i];
+      }
+    }
+  } else {
+    uint32_t own[kOwn], sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) sum += own[i] = s.count[kOwn * tid + i];
+    const uint32_t scan = wave_scan(sum);
+    uint32_t at = scan - sum + waves_before<W>(s.wave_count, last_lane(scan), all);
+    bool open = tid == 0 || at < t.count;
+    if (open && (at + sum >= t.count || tid == 64 * W - 1)) {
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        if (open && (at + own[i] >= t.count || i == kOwn - 1)) {
+          s.found = kOwn * tid + i;
+          s.before_count = at;
+          open = false;
+        }
+        at += own[i];
+      }
+    }
+  }
+  __syncthreads();
+  if (t.by_mass) mass = s.before_mass;
+  else count = s.before_count;
+  return s.found;
+}
+
+struct RowCall {
+  float t, top, per;
+  int k;                   // 0: all
+  bool by_p;
+  float p, floor_p, u;
+  int64_t *token;
+  float *logprob;
+};
+
+__device__ __forceinline__ int bin_of(float v, float top, float per) {
+  return static_cast<int>(fminf((top - v) * per, static_cast<float>(kBins - 1)));  // also of -inf
+}
+
+// The border inside a bin: `count` and `mass` lie before the bin, of it the values above from.key, and from.ties at it.
+template <int DT, int W, class X>
+__device__ __forceinline__ Border find_border(SampleShared &s, X &x, const RowCall &c, const Weight &weight, int bin,
+                                              const Target &goal, uint32_t count, uint64_t mass, Border from) {
+  const int tid = threadIdx.x;
+  // keys that may fall into the bin: its edges, with a margin for the roundings of bin_of
+  const float near = bin / c.per, far = (bin + 1) / c.per;
+  const float hi_v = c.top - near * (1.f - 0x1p-20f) + 0x1p-21f * (fabsf(c.top) + near);
+  const float lo_v = c.top - far * (1.f + 0x1p-20f) - 0x1p-21f * (fabsf(c.top) + far);
+  const uint32_t top_key = sample_key<DT>(c.top);
+  uint32_t high = bin > 0 && hi_v < c.top ? min(top_key, sample_key<DT>(hi_v) + 1) : top_key;
+  uint32_t low = lo_v == lo_v ? max(from.key, sample_key<DT>(lo_v)) : from.key;
+  low = min(low, high);
   for (;;) {
     const int shift = max(0, 21 - __clz((high - low) | 1));  // 11 bits of the range
-    __syncthreads();
-    for (int b = tid; b < kBins; b += kThreads) {
-      s.mass[b] = 0;
-      s.count[b] = 0;
-    }
-    __syncthreads();
-    for (int i = tid * 8; i < vocab; i += kThreads * 8) {
-      float v[8];
-      sample_load8<DT>(row, i, vocab, vec, v);
+    clear_bins<W>(s);
+    x.each([&](int, const float (&v)[8]) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t key = sample_key<DT>(v[e]);
-        if (key >= low && key <= high && i + e < vocab) {
-          const uint32_t bin = (high - key) >> shift;
-          atomicAdd(&s.count[bin], 1u);
-          atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[bin]),
-                    static_cast<unsigned long long>(sample_weight(v[e], top, inv_t)));
-        }
+        if (key < low || key > high || key <= from.key || bin_of(v[e], c.top, c.per) != bin) continue;
+        atomicAdd(&s.count[(high - key) >> shift], 1u);
+        if (goal.by_mass && shift > 0)
+          atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[(high - key) >> shift]),
+                    static_cast<unsigned long long>(weight(v[e])));
       }
-    }
+    });
     __syncthreads();
-    Target rest = t;
-    rest.count = t.count - count;
-    rest.mass = t.mass - static_cast<double>(mass);
-    uint32_t c;
-    uint64_t m;
-    const uint32_t bin = find_bin(s, rest, c, m);
-    const uint32_t n = s.count[bin];
-    const uint64_t in = s.mass[bin];
-    count += c;
-    mass += m;
-    if (shift == 0) {
-      // one key: all of its values weigh the same
-      const uint32_t key = high - bin;
-      uint32_t ties = t.count - count;
-      if (t.by_mass) {
-        const uint64_t w = n ? in / n : 0;
-        const double need = t.mass - static_cast<double>(mass);
-        ties = w ? static_cast<uint32_t>(fmin(ceil(need / static_cast<double>(w)), static_cast<double>(n))) : n;
+    if (from.ties && from.key >= low && from.key <= high) {
+      const float v = sample_value<DT>(from.key);
+      if (tid == 0 && bin_of(v, c.top, c.per) == bin) {
+        s.count[(high - from.key) >> shift] += from.ties;
+        s.mass[(high - from.key) >> shift] += from.ties * weight(v);
       }
-      ties = min(max(ties, 1u), n);
-      return {key, ties, mass + (n ? in / n * ties : 0)};
+      __syncthreads();
     }
-    const uint32_t up = high - (bin << shift);
-    const uint32_t down = up - low > (1u << shift) - 1 ? up - ((1u << shift) - 1) : low;
+    if (goal.by_mass && shift == 0) {  // one key a bin: its values weigh the same
+#pragma unroll
+      for (int b = tid; b < kBins; b += 64 * W)
+        if (s.count[b]) s.mass[b] = s.count[b] * weight(sample_value<DT>(high - b));
+      __syncthreads();
+    }
+    Target rest = goal;
+    rest.count = goal.count - count;
+    rest.mass = goal.mass - static_cast<double>(mass);
+    uint32_t c2 = 0;
+    uint64_t m2 = 0;
+    const uint32_t bin2 = find_bin<W>(s, rest, c2, m2);
+    const uint32_t n = s.count[bin2];
+    const uint64_t in = s.mass[bin2];
+    count += c2;
+    mass += m2;
+    if (shift == 0) {
+      uint32_t ties = goal.count - count;
+      if (goal.by_mass) {
+        const double need = goal.mass - static_cast<double>(mass), w = n ? static_cast<double>(in / n) : 0.0;
+        ties = w > 0.0 ? static_cast<uint32_t>(fmin(ceil(need / w), static_cast<double>(n))) : n;
+      }
+      ties = ties > n ? n : ties;
+      return Border{high - bin2, ties < 1 ? 1 : ties};
+    }
+    const uint32_t up = high - (bin2 << shift), room = (1u << shift) - 1;
+    low = up - low > room ? up - room : low;
     high = up;
-    low = down;
   }
 }
 
-// One workgroup per row.
-template <int DT>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const uint8_t *__restrict__ logits, int64_t stride, int vocab,
-                                                          const float *__restrict__ u, const float *__restrict__ temperature,
-                                                          const int32_t *__restrict__ top_k, const float *__restrict__ top_p,
-                                                          const float *__restrict__ min_p, int64_t *__restrict__ tokens,
-                                                          float *__restrict__ logprobs) {
-  extern __shared__ uint8_t sample_smem[];
-  SampleShared &s = *reinterpret_cast<SampleShared *>(sample_smem);
-  constexpr int kSize = DT == MP_F32 ? 4 : 2;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r = blockIdx.x;
-  const uint8_t *row = logits + r * stride * kSize;
-  const bool vec = reinterpret_cast<uintptr_t>(row) % 16 == 0;
-
-  // the maximum and its first index
-  float top = -INFINITY;
-  int at = INT32_MAX;
-  for (int i = tid * 8; i < vocab; i += kThreads * 8) {
-    float v[8];
-    sample_load8<DT>(row, i, vocab, vec, v);
+// Weights by bins, of the values above from.key and from.ties at it; returns their sum.
+template <int DT, int W, bool RAW, class X>
+__device__ __forceinline__ uint64_t bin_weights(SampleShared &s, X &x, const RowCall &c, const Weight &weight, Border from) {
+  const int tid = threadIdx.x;
+  clear_bins<W>(s);
+  const auto add = [&](int, const float (&v)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (v[e] > top) {
-        top = v[e];
-        at = i + e;
-      }
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float v = __shfl_xor(top, o, 64);
-    const int a = __shfl_xor(at, o, 64);
-    if (v > top || (v == top && a < at)) {
-      top = v;
-      at = a;
+    for (int e = 0; e < 8; ++e) {
+      const int bin = bin_of(v[e], c.top, c.per);
+      if (bin < kBins - 1 && (from.key == 0 || sample_key<DT>(v[e]) > from.key))
+        atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[bin]), static_cast<unsigned long long>(weight(v[e])));
     }
-  }
-  if (lane == 0) {
-    s.top[wave] = top;
-    s.at[wave] = at;
-  }
+  };
+  if constexpr (RAW) x.template each<true>(add);
+  else x.each(add);
   __syncthreads();
-  for (int w = 0; w < kWavesPerRow; ++w)
-    if (s.top[w] > top || (s.top[w] == top && s.at[w] < at)) {
-      top = s.top[w];
-      at = s.at[w];
-    }
-  const float t = temperature ? temperature[r] : 1.0f;
-  if (top == -INFINITY || !(t > 0.f)) {  // nothing may be taken, or the largest is
-    if (tid == 0) {
-      tokens[r] = top == -INFINITY ? -1 : at;
-      logprobs[r] = top == -INFINITY ? -INFINITY : 0.f;
-    }
-    return;
-  }
-  const double inv_t = 1.0 / static_cast<double>(t);
-  const int k = top_k ? top_k[r] : 0;
-  const float p = top_p ? top_p[r] : 1.0f;
-  const bool by_k = k > 0 && k < vocab, by_p = p < 1.0f;
-
-  Border border{0, 0xFFFFFFFFu, 0};
-  if (by_k || by_p) {
-    // bins of equal width below the maximum, down to where weights end
-    const float per = static_cast<float>((kBins - 1) / (kReach * static_cast<double>(t)));
-    const auto bin_of = [&](float v) {
-      const float d = (top - v) * per;  // NaN for two infinities
-      return v == top ? 0 : static_cast<int>(fminf(d, static_cast<float>(kBins - 1)));
-    };
-    for (int b = tid; b < kBins; b += kThreads) {
-      s.mass[b] = 0;
-      s.count[b] = 0;
-    }
+  if (from.ties) {
+    const float v = sample_value<DT>(from.key);
+    if (tid == 0) s.mass[bin_of(v, c.top, c.per)] += from.ties * weight(v);
     __syncthreads();
-    uint32_t rest = 0;
-    for (int i = tid * 8; i < vocab; i += kThreads * 8) {
-      float v[8];
-      sample_load8<DT>(row, i, vocab, vec, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (i + e >= vocab) continue;
-        const int bin = bin_of(v[e]);
-        if (bin == kBins - 1) {
-          ++rest;
-        } else {
-          atomicAdd(&s.count[bin], 1u);
-          atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[bin]),
-                    static_cast<unsigned long long>(sample_weight(v[e], top, inv_t)));
-        }
-      }
-    }
-    // the last bin's weights are below 2^-45 each
-    rest = static_cast<uint32_t>(wave_sum64(rest));
-    if (lane == 0 && rest) atomicAdd(&s.count[kBins - 1], rest);
-    __syncthreads();
-    uint64_t total = 0;
-    // keys of a bin: the values of the row that fall into it, found by its edges with a step of slack
-    const auto border_of = [&](const Target &target) {
-      uint32_t count;
-      uint64_t mass;
-      const int bin = find_bin(s, target, count, mass);
-      if (bin == kBins - 1) return Border{0, 0xFFFFFFFFu, mass};  // what weighs nothing is never taken
-      // smallest and largest key of the bin
-      if (tid == 0) {
-        s.count[0] = 0xFFFFFFFFu;
-        s.count[1] = 0;
-      }
-      __syncthreads();
-      uint32_t low = 0xFFFFFFFFu, high = 0;
-      for (int i = tid * 8; i < vocab; i += kThreads * 8) {
-        float v[8];
-        sample_load8<DT>(row, i, vocab, vec, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (i + e < vocab && bin_of(v[e]) == bin) {
-            low = min(low, sample_key<DT>(v[e]));
-            high = max(high, sample_key<DT>(v[e]));
-          }
-      }
-      atomicMin(&s.count[0], low);
-      atomicMax(&s.count[1], high);
-      __syncthreads();
-      low = s.count[0];
-      high = s.count[1];
-      return find_border<DT>(s, row, vocab, vec, top, inv_t, low, high, target, count, mass);
-    };
-    if (by_p && !by_k) {
-      uint64_t mine = s.mass[2 * tid] + s.mass[2 * tid + 1];
-      mine = wave_sum64(mine);
-      if (lane == 0) s.wave_mass[wave] = mine;
-      __syncthreads();
-      for (int w = 0; w < kWavesPerRow; ++w) total += s.wave_mass[w];
-      __syncthreads();
-      border = border_of({true, 0, static_cast<double>(p) * static_cast<double>(total)});
-    } else {
-      border = border_of({false, static_cast<uint32_t>(k), 0.0});
-      if (by_p) {
-        // the same search over the kept alone
-        const uint32_t key = border.key, ties = border.ties;
-        const double need = static_cast<double>(p) * static_cast<double>(border.mass);
-        const Border q = find_border<DT>(s, row, vocab, vec, top, inv_t, key, sample_key<DT>(top), {true, 0, need}, 0, 0);
-        border = q.key > key ? q : Border{key, min(q.ties, ties), 0};
-      }
-    }
   }
-
-  // kept weight of each span of the row, with the ties at the border counted apart
-  const uint64_t floor_w = min_p && min_p[r] > 0.f
-                               ? static_cast<uint64_t>(fmin(static_cast<double>(min_p[r]), 1.0) * kOne + 0.5)
-                               : 0;
-  const int spans = (vocab + kSpan - 1) / kSpan;
-  __shared__ uint64_t tie_w;
-  if (tid == 0) tie_w = 0;
+  uint64_t own = 0, total;
+#pragma unroll
+  for (int b = tid; b < kBins; b += 64 * W) own += s.mass[b];
+  waves_before<W>(s.wave_mass, wave_sum(own), total);
   __syncthreads();
-  for (int sp = wave; sp < spans; sp += kWavesPerRow) {
-    const int i = sp * kSpan + lane * 8;
-    float v[8];
-    sample_load8<DT>(row, i, vocab, vec, v);
-    uint64_t mass = 0;
+  return total;
+}
+
+// The bin that the k-th largest value is in, and how many values are in those before it.
+template <int DT, int W, class X>
+__device__ __forceinline__ int find_bin_of_count(SampleShared &s, X &x, const RowCall &c, const Target &goal, uint32_t &count) {
+  clear_bins<W>(s);
+  x.each([&](int, const float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int bin = bin_of(v[e], c.top, c.per);
+      if (bin < kBins - 1) atomicAdd(&s.count[bin], 1u);
+    }
+  });
+  __syncthreads();
+  uint64_t mass;
+  return find_bin<W>(s, goal, count, mass);
+}
+
+// From the values of a row, or those of them that may be kept, to the token.  `bin`, with `count` or `mass` before it: where
+// the border of `goal` is, if there is one.
+template <int DT, int W, class X>
+__device__ __forceinline__ void draw_token(SampleShared &s, X &x, const RowCall &c, const Weight &weight, bool filtered,
+                                           const Target &goal, int bin, uint32_t count, uint64_t mass) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Border border{0, 0};
+  if (filtered) {
+    border = find_border<DT, W>(s, x, c, weight, bin, goal, count, mass, border);
+    if (!goal.by_mass && c.by_p) {  // of the k largest, those down to p of their weight
+      const uint64_t total = bin_weights<DT, W, false>(s, x, c, weight, border);
+      const Target part{true, 0, static_cast<double>(c.p) * static_cast<double>(total)};
+      const int at = find_bin<W>(s, part, count, mass);
+      border = find_border<DT, W>(s, x, c, weight, at, part, 0, mass, border);
+    }
+  }
+
+  // kept weight of each span, the ties at the border counted apart
+  const uint64_t floor_w =
+      c.floor_p > 0.f ? static_cast<uint64_t>(fmin(static_cast<double>(c.floor_p), 1.0) * kOne + 0.5) : 0;
+  uint64_t tie_w = border.ties ? weight(sample_value<DT>(border.key)) : 0;
+  if (tie_w < floor_w) tie_w = 0;
+  x.each([&](int ch, const float (&v)[8]) {
+    uint64_t m = 0;
     uint32_t ties = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t key = sample_key<DT>(v[e]);
-      if (key < border.key || i + e >= vocab) continue;
-      const uint64_t w = sample_weight(v[e], top, inv_t);
-      if (w < floor_w) continue;
+      ties += key == border.key ? 1 : 0;
       if (key > border.key) {
-        mass += w;
-      } else {
-        ++ties;
-        tie_w = w;  // the same for all
+        const uint64_t w = weight(v[e]);
+        m += w >= floor_w ? w : 0;
       }
     }
-    mass = wave_sum64(mass);
-    ties = static_cast<uint32_t>(wave_sum64(ties));
-    if (lane == 0) {
-      s.span_mass[sp] = mass;
-      s.span_ties[sp] = ties;
+    if (__any(ties || m)) {
+      m = wave_sum(m);
+      ties = wave_sum(ties);
     }
-  }
+    if (lane == 0) {
+      s.span_mass[x.span(ch)] = m;
+      s.span_ties[x.span(ch)] = ties;
+    }
+  });
   __syncthreads();
-  if (wave != 0) return;
 
-  // one wave: ties to weights, the sum, the span that the token is in, the token
+  // every wave: ties to weights, the sum, the span that the token is in; its wave finds the token
+  const int spans = x.chunks * W;
   uint64_t total = 0;
   uint32_t taken = 0;
   for (int b = 0; b < spans; b += 64) {
     const bool in = b + lane < spans;
-    const uint32_t ties = in ? s.span_ties[b + lane] : 0;
-    const uint32_t upto = static_cast<uint32_t>(wave_scan64(ties, lane));
-    const uint32_t before = taken + upto - ties;
-    const uint32_t room = border.ties > before ? border.ties - before : 0;
-    const uint32_t mine = min(ties, room);
-    uint64_t m = in ? s.span_mass[b + lane] + tie_w * mine : 0;
-    if (in) {
-      s.span_mass[b + lane] = m;
-      s.span_ties[b + lane] = before;  // ties before the span
-    }
-    taken += __builtin_amdgcn_readlane(upto, 63);
-    total += wave_sum64(m);
+    const uint32_t ties = in ? s.span_ties[b + lane] : 0, upto = wave_scan(ties), before = taken + upto - ties;
+    total += in ? s.span_mass[b + lane] + tie_w * min(ties, border.ties > before ? border.ties - before : 0) : 0;
+    taken += last_lane(upto);
   }
-  // u below 1 leaves the target below the sum; rounding and other u are held there
-  const double target = fmin(fmax(static_cast<double>(u[r]), 0.0) * static_cast<double>(total),
+  total = wave_sum(total);
+  // u below 1 leaves the target below the sum; other u, and NaN, are held there
+  const double target = fmin(fmax(static_cast<double>(c.u), 0.0) * static_cast<double>(total),
                              static_cast<double>(total) * (1.0 - 0x1p-52) - 1.0);
   uint64_t run = 0;
+  uint32_t ties_before = 0;
   int span = spans - 1;
+  taken = 0;
   for (int b = 0; b < spans; b += 64) {
-    const uint64_t m = b + lane < spans ? s.span_mass[b + lane] : 0;
-    const uint64_t upto = run + wave_scan64(m, lane);
-    const uint64_t past = __ballot(b + lane < spans && static_cast<double>(upto) > target);
+    const bool in = b + lane < spans;
+    const uint32_t ties = in ? s.span_ties[b + lane] : 0, tupto = wave_scan(ties), before = taken + tupto - ties;
+    const uint64_t m = in ? s.span_mass[b + lane] + tie_w * min(ties, border.ties > before ? border.ties - before : 0) : 0;
+    const uint64_t upto = run + wave_scan(m);
+    const uint64_t past = __ballot(in && static_cast<double>(upto) > target);
     if (past) {
       const int l = __builtin_ctzll(past);
       span = b + l;
       run = __shfl(upto - m, l, 64);
+      ties_before = __builtin_amdgcn_readlane(before, l);
       break;
     }
-    run = __shfl(upto, 63, 64);
+    run = last_lane(upto);
+    taken += last_lane(tupto);
   }
-  const int i = span * kSpan + lane * 8;
-  float v[8];
-  sample_load8<DT>(row, i, vocab, vec, v);
-  uint64_t w[8], mass = 0;
-  uint32_t ties = 0;
+  if (span / x.chunks != wave) return;
+  x.one(span % x.chunks, [&](int ch, const float (&v)[8]) {
+    uint64_t w[8], m = 0;
+    uint32_t ties = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t key = sample_key<DT>(v[e]);
-    w[e] = key >= border.key && i + e < vocab ? sample_weight(v[e], top, inv_t) : 0;
-    if (w[e] < floor_w) w[e] = 0;
-    ties += key == border.key && w[e] ? 1 : 0;
-  }
-  uint32_t before = s.span_ties[span] + static_cast<uint32_t>(wave_scan64(ties, lane)) - ties;
+    for (int e = 0; e < 8; ++e) ties += sample_key<DT>(v[e]) == border.key ? 1 : 0;
+    uint32_t before = ties_before + wave_scan(ties) - ties;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if (sample_key<DT>(v[e]) == border.key && w[e]) w[e] = before++ < border.ties ? w[e] : 0;
-    mass += w[e];
-  }
-  uint64_t upto = run + wave_scan64(mass, lane) - mass;
-  int found = INT32_MAX;
-  uint64_t weight = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    upto += w[e];
-    if (w[e] && static_cast<double>(upto) > target && found == INT32_MAX) {
-      found = i + e;
-      weight = w[e];
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t key = sample_key<DT>(v[e]);
+      w[e] = key > border.key ? weight(v[e]) : 0;
+      if (w[e] < floor_w) w[e] = 0;
+      if (key == border.key) w[e] = before++ < border.ties ? tie_w : 0;
+      m += w[e];
     }
+    uint64_t upto = run + wave_scan(m) - m, own = 0;
+    int found = INT32_MAX;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      upto += w[e];
+      if (w[e] && static_cast<double>(upto) > target && found == INT32_MAX) {
+        found = e;
+        own = w[e];
+      }
+    }
+    const uint64_t who = __ballot(found != INT32_MAX);
+    if (who && lane == __builtin_ctzll(who)) {
+      *c.token = x.index(ch, found);
+      *c.logprob = static_cast<float>(log(static_cast<double>(own) / static_cast<double>(total)));
+    }
+  });
+}
+
+template <int DT, int W, int CH>
+__global__ __launch_bounds__(64 * W) void sample_kernel(const uint8_t *__restrict__ logits, int64_t stride, int vocab,
+                                                          const float *__restrict__ u, const float *__restrict__ temperature,
+                                                          const int32_t *__restrict__ top_k, const float *__restrict__ top_p,
+                                                          const float *__restrict__ min_p, int64_t *__restrict__ tokens,
+                                                          float *__restrict__ logprobs) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t sample_smem[];
+  SampleShared &s = *reinterpret_cast<SampleShared *>(sample_smem);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t r = blockIdx.x;
+  SampleRow<DT, CH> x;
+  x.row = logits + r * stride * (DT == MP_F32 ? 4 : 2);
+  x.vocab = vocab;
+  x.chunks = (vocab + W * kSpan - 1) / (W * kSpan);
+  x.vec = reinterpret_cast<uintptr_t>(x.row) % 16 == 0;
+  x.load();
+  RowCall c;
+  c.t = temperature ? temperature[r] : 1.0f;
+  c.k = top_k ? top_k[r] : 0;
+  c.k = c.k > 0 && c.k < vocab ? c.k : 0;
+  c.p = top_p ? top_p[r] : 1.0f;
+  c.by_p = c.p < 1.0f;
+  c.floor_p = min_p ? min_p[r] : 0.f;
+  c.u = u[r];
+  c.token = tokens + r;
+  c.logprob = logprobs + r;
+
+  float top = -INFINITY;
+  x.template each<true>([&](int, const float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, v[e]);
+  });
+  const float mine = top;  // this thread's
+  top = mp_wave_max(top);
+  if (lane == 0) s.top[wave] = top;
+  for (int i = tid; i < kTable; i += 64 * W) s.table[i] = exp2(static_cast<double>(i) / kTable);  // for the weights
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) top = fmaxf(top, s.top[w]);
+  if (top == -INFINITY) {  // nothing may be taken
+    if (tid == 0) {
+      *c.token = -1;
+      *c.logprob = -INFINITY;
+    }
+    return;
   }
-  const uint64_t who = __ballot(found != INT32_MAX);
-  if (who && lane == __builtin_ctzll(who)) {
-    tokens[r] = found;
-    logprobs[r] = static_cast<float>(log(static_cast<double>(weight) / static_cast<double>(total)));
+  if (!(c.t > 0.f)) {  // the largest is: its first index
+    int at = INT32_MAX;
+    x.each([&](int ch, const float (&v)[8]) {
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (v[e] == top) at = min(at, x.index(ch, e));
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
+    if (lane == 0) s.at[wave] = at;
+    __syncthreads();
+    for (int w = 0; w < W; ++w) at = min(at, s.at[w]);
+    if (tid == 0) {
+      *c.token = at;
+      *c.logprob = 0.f;
+    }
+    return;
   }
+  x.infinite = top == INFINITY;
+  c.top = top = x.infinite ? 0.f : top;
+  c.per = static_cast<float>((kBins - 1) / (kReach * static_cast<double>(c.t)));
+  const double rate = 1.4426950408889634 / static_cast<double>(c.t);
+  const Weight weight{s.table, static_cast<double>(top), rate};
+
+  // the bin that the border is in
+  Target goal{!c.k, static_cast<uint32_t>(c.k), 0.0};
+  int bin = kBins - 1;
+  uint32_t count = 0;
+  uint64_t mass = 0;
+  // at least k values are in this bin or above: of the threads' maxima are
+  bool bounded = c.k > 0 && c.k <= 64 * W && !x.infinite;
+  if (bounded) {
+    clear_bins<W>(s);
+    const int b = bin_of(mine, top, c.per);
+    if (b < kBins - 1) atomicAdd(&s.count[b], 1u);
+    __syncthreads();
+    bin = find_bin<W>(s, goal, count, mass);
+    bounded = bin < kBins - 1;
+  }
+  if (c.k && !bounded) {
+    bin = find_bin_of_count<DT, W>(s, x, c, goal, count);
+    if (bin == kBins - 1) goal.by_mass = true;  // all that weighs anything is among the k largest
+  }
+  if (bin == kBins - 1 && c.by_p) {
+    goal.mass = static_cast<double>(c.p) * static_cast<double>(bin_weights<DT, W, true>(s, x, c, weight, Border{0, 0}));
+    bin = find_bin<W>(s, goal, count, mass);
+  }
+  const bool filtered = bin < kBins - 1;
+
+  // to be listed: the values of that bin and above, or else those not below min-p's floor; a few more do no harm, which
+  // leaves a margin for the roundings.  (Where top-p sums weights up, min-p has to wait for it.)
+  const float reach = filtered ? (bin + 1) / c.per : c.t * -logf(fminf(c.floor_p, 1.0f));
+  const float least = top - reach * (1.f + 0x1p-10f) - 0x1p-10f * (c.t + 0x1p-10f * fabsf(top));
+  bool list = (filtered || c.floor_p > 0.f) && least == least;
+  if (list) {  // each wave its own, in index order
+    uint32_t n = 0;
+    x.template each<true>([&](int ch, const float (&v)[8]) {
+      float most = v[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) most = fmaxf(most, v[e]);
+      if (!__any(most >= least) || n > kListed) return;
+      uint32_t own = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) own += v[e] >= least ? 1 : 0;
+      const uint32_t upto = wave_scan(own);
+      uint32_t at = n + upto - own;
+      n += last_lane(upto);
+      if (n > kListed) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v[e] >= least) {
+          s.value[wave][at] = v[e];
+          s.index[wave][at++] = x.index(ch, e);
+        }
+    });
+    if (lane == 0) s.listed[wave] = n;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) list = list && s.listed[w] <= kListed;
+  }
+  if (list) {
+    SampleList<W> l;
+    l.s = &s;
+    l.all = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) l.all += s.listed[w];
+    l.per = (l.all + 64 * W - 1) / (64 * W);
+    l.load();
+    if (bounded) bin = find_bin_of_count<DT, W>(s, l, c, goal, count);
+    draw_token<DT, W>(s, l, c, weight, filtered, goal, bin, count, mass);
+  } else {
+    if (bounded) bin = find_bin_of_count<DT, W>(s, x, c, goal, count);
+    draw_token<DT, W>(s, x, c, weight, filtered, goal, bin, count, mass);
+  }
+}
+
+template <int DT, int W, int CH>
+int sample_launch(const void *logits, int64_t stride, int64_t rows, int vocab, const float *u, const float *temperature,
+                  const int32_t *top_k, const float *top_p, const float *min_p, int64_t *tokens, float *logprobs,
+                  hipStream_t s) {
+  if (hipFuncSetAttribute(reinterpret_cast<const void *>(sample_kernel<DT, W, CH>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                          sizeof(SampleShared)) != hipSuccess)
+    return MP_ERR_HIP;
+  hipLaunchKernelGGL((sample_kernel<DT, W, CH>), dim3(static_cast<unsigned>(rows)), dim3(64 * W), sizeof(SampleShared), s,
+                     static_cast<const uint8_t *>(logits), stride, vocab, u, temperature, top_k, top_p, min_p, tokens, logprobs);
+  MP_CHECK_LAUNCH();
+  return MP_OK;
 }
 
 }  // namespace
@@ -455,17 +747,14 @@ extern "C" int mp_sample_tokens(const void *logits, int64_t stride, int64_t rows
   if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > kMaxVocab || stride < vocab) return MP_ERR_SHAPE;
   if (!mp_aligned(logits, dtype == MP_F32 ? 4 : 2)) return MP_ERR_ALIGN;
   if (rows == 0) return MP_OK;
-  const dim3 grid(static_cast<unsigned>(rows));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const auto *x = static_cast<const uint8_t *>(logits);
   const int n = static_cast<int>(vocab);
-#define MP_SAMPLE(DT)                                                                                                       \
-  hipLaunchKernelGGL(sample_kernel<DT>, grid, dim3(kThreads), sizeof(SampleShared), s, x, stride, n, u, temperature, top_k, \
-                     top_p, min_p, tokens, logprobs)
-  if (dtype == MP_F16) MP_SAMPLE(MP_F16);
-  else if (dtype == MP_BF16) MP_SAMPLE(MP_BF16);
-  else MP_SAMPLE(MP_F32);
+#define MP_SAMPLE(DT) \
+  (n <= 8 * 8 * kSpan \
+       ? sample_launch<DT, 8, 8>(logits, stride, rows, n, u, temperature, top_k, top_p, min_p, tokens, logprobs, s) \
+       : sample_launch<DT, 16, 0>(logits, stride, rows, n, u, temperature, top_k, top_p, min_p, tokens, logprobs, s))
+  if (dtype == MP_F16) return MP_SAMPLE(MP_F16);
+  if (dtype == MP_BF16) return MP_SAMPLE(MP_BF16);
+  return MP_SAMPLE(MP_F32);
 #undef MP_SAMPLE
-  MP_CHECK_LAUNCH();
-  return MP_OK;
 }
