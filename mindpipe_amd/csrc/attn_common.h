@@ -11,7 +11,7 @@
 //     them in registers: operand c holds value D/16 i + c of the eight rows.
 // K and V go from memory to registers and no LDS is used.
 #pragma once
-#include "mp_common.h"
+#include "wave_scan.h"
 
 namespace {
 
@@ -179,8 +179,8 @@ __device__ __forceinline__ void attn_clear(AttnRows<D> &a) {
 // One tile into the rows' state.  `sees`: positions below it are visible to this lane's row; `end`: to any row of the wave;
 // `full`: to all.  Rows that see nothing of the tile are left as they are, whatever its masked places hold: masked scores
 // become -inf, V rows that no row sees are cleared, and a tile whose V has an infinity or NaN where only some rows see it
-// is added position by position, to those rows alone (0 times an infinity is no zero).
-template <int D, int DT>
+// is added position by position, to those rows alone (0 times an infinity is no zero).  CAUSAL: rows see different positions.
+template <int D, int DT, bool CAUSAL>
 __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const uint4 (&q)[D / 32], int tile, int sees,
                                           int end, int full, float scale2, int lane) {
   const int j = lane >> 4, p0 = tile + 8 * j;
@@ -204,10 +204,10 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         t.v[i][c] = p0 + i < any ? t.v[i][c] : 0u;
-        odd |= attn_odd16<DT>(t.v[i][c]) || attn_odd16<DT>(t.v[i][c] >> 16);
+        if (CAUSAL) odd |= attn_odd16<DT>(t.v[i][c]) || attn_odd16<DT>(t.v[i][c] >> 16);
       }
     }
-    apart = tile + 32 > full && __any(odd);
+    if (CAUSAL) apart = tile + 32 > full && __any(odd);
   }
   float top = x[0];
 #pragma unroll
@@ -224,15 +224,13 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
   const float base = a.m == -INFINITY ? 0.f : a.m - kRaise<DT>;
   float p[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    p[i] = __builtin_amdgcn_exp2f(x[i] - base);
-    a.l += p[i];
-  }
+  for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(x[i] - base);
   // the weights in the values' type, for the matrix cores: half a step of 2^-11 (fp16) or 2^-8 (bf16) each, which averages out
-  // over the positions; the sum keeps the unrounded ones
+  // over the positions
   uint4 w = make_uint4(attn_pack2<DT>(p[0], p[1]), attn_pack2<DT>(p[2], p[3]), attn_pack2<DT>(p[4], p[5]),
                        attn_pack2<DT>(p[6], p[7]));
-  if (!apart) {
+  a.l = attn_add2<DT>(w.w, attn_add2<DT>(w.z, attn_add2<DT>(w.y, attn_add2<DT>(w.x, a.l))));
+  if (!CAUSAL || !apart) {
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
       const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;
@@ -272,7 +270,7 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
 
 // Tiles first, first + step, ... below `to` into the rows' state.  The next tile's rows and the table entries of the one
 // after it are asked for before a tile is computed.
-template <int D, int DT, bool PAGED>
+template <int D, int DT, bool CAUSAL, bool PAGED>
 __device__ __forceinline__ void attn_walk(AttnRows<D> &a, const KvSource<PAGED> &src, const uint4 (&q)[D / 32], int first,
                                           int to, int step, int sees, int end, int full, float scale2, int lane) {
   if (first >= to) return;
@@ -287,7 +285,7 @@ __device__ __forceinline__ void attn_walk(AttnRows<D> &a, const KvSource<PAGED> 
       attn_load_tile<D>(src, next, tile + step, lane, ahead);
       next = after;
     }
-    attn_tile<D, DT>(a, cur, q, tile, sees, end, full, scale2, lane);
+    attn_tile<D, DT, CAUSAL>(a, cur, q, tile, sees, end, full, scale2, lane);
     cur = ahead;
   }
 }
@@ -307,12 +305,7 @@ __device__ __forceinline__ bool attn_find_part(N n, int batch, int per, int at, 
   for (int b0 = 0; b0 < batch; b0 += 64) {
     const int b = b0 + lane;
     const int parts = b < batch ? n(b, per) : 0;
-    int upto = parts;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(upto, o, 64);
-      upto += lane >= o ? v : 0;
-    }
+    const int upto = static_cast<int>(wave_scan(static_cast<uint32_t>(parts)));
     const uint64_t past = __ballot(upto > at);
     if (past) {
       const int l = __builtin_ctzll(past);

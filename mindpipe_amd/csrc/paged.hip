@@ -96,147 +96,170 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(
 }
 
 // ---------------------------------------------------------------- one new token per sequence
-// Positions are split into chunks of one size for all sequences, the smallest multiple of kChunk that leaves about `goal`
-// workgroups in all: a sequence has ceil(length / chunk) of them (an empty one has one, which writes its zeros).
+// The sequences' positions, in blocks of kBlock (an empty sequence has one, which writes its zeros), follow each other in one
+// row of blocks for every key-value head, and the workgroups of a head (`share`, or one per block) take equal runs of it: run w
+// is blocks w T / share .. (w + 1) T / share of T.  However ragged the lengths are, all have the same to read.  A sequence that lies
+// in several runs is joined from its parts: a workgroup leaves at most two, that of the sequence its run begins inside of
+// (slot 2 w) and that of the sequence its run ends inside of (slot 2 w + 1).
 constexpr int kWaves = 4;
-constexpr int kChunk = 32 * kWaves;
+constexpr int kBlock = 32 * kWaves;
 
 struct DecodePlan {
   const int32_t *lens;
-  int capacity;  // positions that the table has room for
+  int batch, capacity;  // capacity: positions that the table has room for
   __device__ __forceinline__ int len(int b) const { return min(max(lens[b], 0), capacity); }
-  __device__ __forceinline__ int operator()(int b, int chunk) const {
-    const int n = len(b);
-    return n > 0 ? (n - 1) / chunk + 1 : 1;
+  __device__ __forceinline__ int operator()(int b, int) const { return max((len(b) + kBlock - 1) / kBlock, 1); }
+  __device__ __forceinline__ uint32_t blocks() const {
+    uint32_t n = 0;
+    for (int b = threadIdx.x & 63; b < batch; b += 64) n += (*this)(b, 0);
+    return wave_sum(n);
   }
 };
 
-__device__ __forceinline__ int decode_chunk(const DecodePlan &plan, int batch, int heads, int goal) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  for (int b = lane; b < batch; b += 64) total += plan.len(b);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-  // a sequence is shorter than 2^30: a longer chunk says no more
-  const int64_t chunk = min((total * heads / goal + kChunk) / kChunk * kChunk, static_cast<int64_t>(1) << 30);
-  return __builtin_amdgcn_readfirstlane(static_cast<int>(chunk));
+// Workgroups of a head: as many as fit the card at once (kRound of D per CU), and not more.
+constexpr int decode_round(int dim) { return dim == 64 ? 4 : dim == 128 ? 2 : 1; }
+inline int decode_share(int64_t heads, int dim) {
+  const int64_t n = static_cast<int64_t>(decode_round(dim)) * mp_cu_count() / heads;
+  return static_cast<int>(n > 1 ? n : 1);
 }
 
-// Workgroups that a plan may need: the goal's and one more per sequence, of each head.
-inline int64_t decode_parts(int64_t batch, int64_t heads, int64_t goal) { return goal / heads + 1 + batch; }
-
 template <int D, int DT>
-__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(
+__global__ __launch_bounds__(64 * kWaves, decode_round(D)) void paged_decode_kernel(
     const uint16_t *__restrict__ q, int64_t q_row, int64_t q_head, const uint16_t *__restrict__ k_pages, int64_t kpage,
     int64_t khead, int64_t krow, const uint16_t *__restrict__ v_pages, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
     int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens, int batch, int kvh, int grp,
-    int tiles, int goal, float scale2, float *__restrict__ part_o, float *__restrict__ part_ml, uint16_t *__restrict__ out) {
+    int tiles, int share, float scale2, float *__restrict__ part_o, float *__restrict__ part_ml, int4 *__restrict__ joins,
+    uint16_t *__restrict__ out) {
   extern __shared__ float sm[];  // [kWaves][rows][D] outputs, then [kWaves][rows][2] maxima and sums
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, j = lane >> 4;
-  const int heads = kvh * tiles, h = blockIdx.x % heads, kh = h / tiles;
-  const DecodePlan plan{lens, width << shift};
-  const int chunk = decode_chunk(plan, batch, heads, goal);
-  int b, part, parts;
-  if (!attn_find_part(plan, batch, chunk, blockIdx.x / heads, b, part, parts)) return;  // uniform over the workgroup
-  const int len = plan.len(b), t0 = part * chunk, t1 = min(t0 + chunk, len);
+  const int heads = kvh * tiles, h = blockIdx.x % heads, kh = h / tiles, run = blockIdx.x / heads;
+  const DecodePlan plan{lens, batch, width << shift};
+  const uint64_t all = plan.blocks();
+  share = static_cast<int>(min(static_cast<uint64_t>(share), all));  // no run is empty
+  const int from = static_cast<int>(run * all / share), to = static_cast<int>((run + 1) * all / share);
+  int b, at, blocks;  // the sequence, and the block of it, that the run begins with
+  if (run >= share || !attn_find_part(plan, batch, 0, from, b, at, blocks)) return;  // uniform over the workgroup
   const int g0 = h % tiles * 16, rows = min(16, grp - g0);  // query heads of this workgroup
   const int nh = kvh * grp;
-
-  uint4 qf[D / 32];
-  const uint16_t *qp = q + b * q_row + static_cast<int64_t>(kh * grp + g0 + min(i16, rows - 1)) * q_head + 8 * j;
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) qf[c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
-
-  KvSource<true> src{k_pages + kh * khead, v_pages + kh * vhead, kpage, krow, vpage, vrow,
-                     table + static_cast<int64_t>(b) * width, shift, (1 << shift) - 1, pages,
-                     len > 0 ? (len - 1) >> shift : 0};
-  AttnRows<D> a;
-  attn_clear(a);
-  attn_walk<D, DT>(a, src, qf, t0 + 32 * wave, t1, kChunk, t1, t1, t1, scale2, lane);
-  a.l = attn_row_sum(a.l);
-
-  // the four waves' states meet
   float *ml = sm + kWaves * rows * D;
-  if (i16 < rows) {
-    float *o = sm + (wave * rows + i16) * D + (D / 16) * 4 * j;
+  KvSource<true> src{k_pages + kh * khead, v_pages + kh * vhead, kpage, krow, vpage, vrow, nullptr, shift, (1 << shift) - 1, pages, 0};
+
+  for (int left = to - from; left > 0; ++b, at = 0) {
+    const int len = plan.len(b);
+    blocks = plan(b, 0);
+    const int end = min(at + left, blocks), t1 = min(end * kBlock, len);
+    const bool whole = at == 0 && end == blocks;
+    uint4 qf[D / 32];
+    const uint16_t *qp = q + b * q_row + static_cast<int64_t>(kh * grp + g0 + min(i16, rows - 1)) * q_head + 8 * j;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int c = 0; c < D / 32; ++c) qf[c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
+    src.table = table + static_cast<int64_t>(b) * width;
+    src.last = len > 0 ? (len - 1) >> shift : 0;
+    AttnRows<D> a;
+    attn_clear(a);
+    attn_walk<D, DT, false>(a, src, qf, at * kBlock + 32 * wave, t1, kBlock, t1, t1, t1, scale2, lane);
+    a.l = attn_row_sum(a.l);
+
+    // the four waves' states meet
+    if (i16 < rows) {
+      float *o = sm + (wave * rows + i16) * D + (D / 16) * 4 * j;
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) o[(D / 16) * r + c] = a.o[c][r];
-    if (j == 0) {
-      ml[(wave * rows + i16) * 2] = a.m;
-      ml[(wave * rows + i16) * 2 + 1] = a.l;
-    }
-  }
-  __syncthreads();
-  const int64_t slot = static_cast<int64_t>(blockIdx.x) * min(grp, 16);
-  for (int e = threadIdx.x; e < rows * D; e += 64 * kWaves) {
-    const int row = e / D, d = e % D;
-    float m = -INFINITY;
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[(w * rows + row) * 2]);
-    float o = 0.f, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float mw = ml[(w * rows + row) * 2];
-      const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-      o += f * sm[(w * rows + row) * D + d];
-      l += f * ml[(w * rows + row) * 2 + 1];
-    }
-    if (parts == 1) {
-      const float v = l == 0.f ? 0.f : o / l;
-      out[(static_cast<int64_t>(b) * nh + kh * grp + g0 + row) * D + d] = DT == MP_F16 ? mp_f2h(v) : mp_f2bf(v);
-    } else {
-      part_o[(slot + row) * D + d] = o;
-      if (d == 0) {
-        part_ml[(slot + row) * 2] = m;
-        part_ml[(slot + row) * 2 + 1] = l;
+        for (int c = 0; c < D / 16; ++c) o[(D / 16) * r + c] = a.o[c][r];
+      if (j == 0) {
+        ml[(wave * rows + i16) * 2] = a.m;
+        ml[(wave * rows + i16) * 2 + 1] = a.l;
       }
     }
+    __syncthreads();
+    const int64_t slot = (static_cast<int64_t>(2 * run + (left < to - from ? 1 : 0)) * heads + h) * min(grp, 16);
+    if (at == 0 && threadIdx.x == 0) {
+      const int last = static_cast<int>(((to - left + blocks) * static_cast<uint64_t>(share) - 1) / all);  // run of its last block
+      joins[b * heads + h] = make_int4(run, last - run + 1, left < to - from ? 1 : 0, 0);
+    }
+    for (int e = threadIdx.x; e < rows * D; e += 64 * kWaves) {
+      const int row = e / D, d = e % D;
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[(w * rows + row) * 2]);
+      float o = 0.f, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float mw = ml[(w * rows + row) * 2];
+        const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+        o += f * sm[(w * rows + row) * D + d];
+        l += f * ml[(w * rows + row) * 2 + 1];
+      }
+      if (whole) {
+        const float v = l == 0.f ? 0.f : o / l;
+        out[(static_cast<int64_t>(b) * nh + kh * grp + g0 + row) * D + d] = DT == MP_F16 ? mp_f2h(v) : mp_f2bf(v);
+      } else {
+        part_o[(slot + row) * D + d] = o;
+        if (d == 0) {
+          part_ml[(slot + row) * 2] = m;
+          part_ml[(slot + row) * 2 + 1] = l;
+        }
+      }
+    }
+    left -= end - at;
+    if (left > 0) __syncthreads();  // the next sequence's states go to the same place
   }
 }
 
-// The chunks of a sequence's query head meet: one wave each.
+// The parts of a sequence's query head meet, in one workgroup: D / 4 threads take a part's output, 1024 / D parts at a time.
+// joins, of (sequence, head tile): the first run, how many runs, and whether the first run begins before the sequence.
 template <int D, int DT>
-__global__ __launch_bounds__(256) void paged_decode_join_kernel(const int32_t *__restrict__ lens, int capacity, int batch, int kvh,
-                                                                int grp, int tiles, int goal, const float *__restrict__ part_o,
+__global__ __launch_bounds__(256) void paged_decode_join_kernel(int heads, int kvh, int grp, const float *__restrict__ part_o,
                                                                 const float *__restrict__ part_ml,
-                                                                uint16_t *__restrict__ out) {
-  const int nh = kvh * grp, heads = kvh * tiles;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (unit >= static_cast<int64_t>(batch) * nh) return;  // uniform over the wave
-  const int b = __builtin_amdgcn_readfirstlane(static_cast<int>(unit / nh)), qh = static_cast<int>(unit % nh);
-  const DecodePlan plan{lens, capacity};
-  const int chunk = decode_chunk(plan, batch, heads, goal);
-  const int parts = plan(b, chunk);
-  if (parts == 1) return;
-  int before = 0;
-  for (int s = lane; s < b; s += 64) before += plan(s, chunk);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
-  const int kh = qh / grp, g = qh % grp, per = min(grp, 16);
-  const auto slot = [&](int p) {
-    return (static_cast<int64_t>(before + p) * heads + kh * tiles + g / 16) * per + g % 16;
+                                                                const int4 *__restrict__ joins, uint16_t *__restrict__ out) {
+  constexpr int kCols = D / 4, kAt = 256 / kCols;
+  __shared__ float4 acc[kAt][kCols];
+  __shared__ float sums[kAt], tops[4];
+  const int nh = kvh * grp, b = blockIdx.x / nh, qh = blockIdx.x % nh, per = min(grp, 16);
+  const int kh = qh / grp, g = qh % grp, h = kh * (heads / kvh) + g / 16;
+  const int4 of = joins[b * heads + h];
+  if (of.y == 1) return;  // written already
+  const auto at_part = [&](int p) {
+    return (static_cast<int64_t>(2 * (of.x + p) + (p == 0 ? of.z : 0)) * heads + h) * per + g % 16;
   };
   float m = -INFINITY;
-  for (int p = lane; p < parts; p += 64) m = fmaxf(m, part_ml[slot(p) * 2]);
+  for (int p = threadIdx.x; p < of.y; p += 256) m = fmaxf(m, part_ml[at_part(p) * 2]);
   m = mp_wave_max(m);
-  float o[D / 64], l = 0.f;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
-  for (int p = 0; p < parts; ++p) {
-    const float mp = part_ml[slot(p) * 2];
-    const float f = mp == m ? 1.0f : __builtin_amdgcn_exp2f(mp - m);
-    l += f * part_ml[slot(p) * 2 + 1];
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] += f * part_o[slot(p) * D + 64 * i + lane];
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const int col = threadIdx.x % kCols, at = threadIdx.x / kCols;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int p = at; p < of.y; p += kAt) {
+    const float2 ml = reinterpret_cast<const float2 *>(part_ml)[at_part(p)];
+    const float4 x = reinterpret_cast<const float4 *>(part_o)[at_part(p) * kCols + col];
+    const float f = ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m);
+    l += f * ml.y;
+    o.x += f * x.x;
+    o.y += f * x.y;
+    o.z += f * x.z;
+    o.w += f * x.w;
   }
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const float v = l == 0.f ? 0.f : o[i] / l;
-    out[(static_cast<int64_t>(b) * nh + qh) * D + 64 * i + lane] = DT == MP_F16 ? mp_f2h(v) : mp_f2bf(v);
+  acc[at][col] = o;
+  if (col == 0) sums[at] = l;
+  __syncthreads();
+  if (at != 0) return;
+  for (int i = 1; i < kAt; ++i) {
+    const float4 x = acc[i][col];
+    l += sums[i];
+    o.x += x.x;
+    o.y += x.y;
+    o.z += x.z;
+    o.w += x.w;
   }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const bool none = l == 0.f;
+  reinterpret_cast<uint2 *>(out)[static_cast<int64_t>(blockIdx.x) * kCols + col] =
+      make_uint2(attn_pack2<DT>(none ? 0.f : o.x * inv, none ? 0.f : o.y * inv),
+                 attn_pack2<DT>(none ? 0.f : o.z * inv, none ? 0.f : o.w * inv));
 }
 
 inline bool strides8(int64_t a, int64_t b, int64_t c) { return a % 8 == 0 && b % 8 == 0 && c % 8 == 0 && a >= 0 && b >= 0 && c >= 0; }
@@ -247,9 +270,6 @@ inline int page_shift(int page) {
     if (page == 1 << s) return s;
   return -1;
 }
-
-// Workgroups wanted for the decode attention: two of four waves on each CU.
-inline int decode_goal() { return 2 * mp_cu_count(); }
 
 }  // namespace
 
@@ -298,7 +318,8 @@ extern "C" size_t mp_paged_decode_workspace_bytes(int64_t batch, int nh, int kvh
   const int cus = mp_cu_count();
   if (batch <= 0 || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || cus <= 0) return 0;
   const int64_t grp = nh / kvh, heads = kvh * mp_cdiv(grp, 16), per = grp < 16 ? grp : 16;
-  return static_cast<size_t>(decode_parts(batch, heads, decode_goal()) * heads * per) * (head_dim + 2) * sizeof(float);
+  return static_cast<size_t>(2 * decode_share(heads, head_dim) * heads * per) * (head_dim + 2) * sizeof(float) +
+         static_cast<size_t>(batch * heads) * sizeof(int4);
 }
 
 extern "C" int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q_head, int64_t batch, int nh, int kvh,
@@ -319,11 +340,12 @@ extern "C" int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q
   if (batch == 0) return MP_OK;
   if (mp_cu_count() <= 0) return MP_ERR_HIP;
   if (workspace_bytes < mp_paged_decode_workspace_bytes(batch, nh, kvh, head_dim)) return MP_ERR_WORKSPACE;
-  const int grp = nh / kvh, tiles = static_cast<int>(mp_cdiv(grp, 16)), per = grp < 16 ? grp : 16, goal = decode_goal();
-  const int64_t heads = static_cast<int64_t>(kvh) * tiles, parts = decode_parts(batch, heads, goal), blocks = parts * heads;
-  if (blocks > INT32_MAX || batch * nh > INT32_MAX) return MP_ERR_SHAPE;
-  float *part_o = static_cast<float *>(workspace), *part_ml = part_o + blocks * per * head_dim;
-  const int capacity = static_cast<int>(cache->width << shift);
+  const int grp = nh / kvh, tiles = static_cast<int>(mp_cdiv(grp, 16)), per = grp < 16 ? grp : 16;
+  const int64_t heads = static_cast<int64_t>(kvh) * tiles, share = decode_share(heads, head_dim), blocks = share * heads;
+  float *part_o = static_cast<float *>(workspace), *part_ml = part_o + 2 * blocks * per * head_dim;
+  int4 *joins = reinterpret_cast<int4 *>(part_ml + 2 * blocks * per * 2);
+  const int64_t capacity = cache->width << shift;
+  if (blocks > INT32_MAX || batch * nh > INT32_MAX || batch * mp_cdiv(capacity, kBlock) > INT32_MAX) return MP_ERR_SHAPE;
   const float scale2 = scale * kLog2e;
   const int lds = kWaves * per * (head_dim + 2) * static_cast<int>(sizeof(float));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -337,13 +359,12 @@ extern "C" int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q
                        static_cast<const uint16_t *>(cache->k), cache->k_page, cache->k_head, cache->k_row,               \
                        static_cast<const uint16_t *>(cache->v), cache->v_page, cache->v_head, cache->v_row,               \
                        static_cast<int>(cache->pages), shift, cache->table, static_cast<int>(cache->width), lens,         \
-                       static_cast<int>(batch), kvh, grp, tiles, goal, scale2, part_o, part_ml,                           \
+                       static_cast<int>(batch), kvh, grp, tiles, static_cast<int>(share), scale2, part_o, part_ml, joins,                    \
                        static_cast<uint16_t *>(out));                                                                     \
     MP_CHECK_LAUNCH();                                                                                                    \
-    if (capacity > kChunk) { /* else every sequence is one chunk */                                                       \
-      hipLaunchKernelGGL((paged_decode_join_kernel<D, DT>), dim3(static_cast<unsigned>(mp_cdiv(batch * nh, 4))),          \
-                         dim3(256), 0, s, lens, capacity, static_cast<int>(batch), kvh, grp, tiles, goal, part_o,         \
-                         part_ml, static_cast<uint16_t *>(out));                                                          \
+    if (capacity > kBlock) { /* else every sequence is one block */                                                       \
+      hipLaunchKernelGGL((paged_decode_join_kernel<D, DT>), dim3(static_cast<unsigned>(batch * nh)), dim3(256), 0, s,     \
+                         static_cast<int>(heads), kvh, grp, part_o, part_ml, joins, static_cast<uint16_t *>(out));        \
       MP_CHECK_LAUNCH();                                                                                                  \
     }                                                                                                                     \
   } while (0)

@@ -84,7 +84,7 @@ __device__ __forceinline__ void prompt_rows16(const KvSource<PAGED> &src, const 
   for (int c = 0; c < D / 32; ++c) qf[c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
   AttnRows<D> a;
   attn_clear(a);
-  attn_walk<D, DT>(a, src, qf, 0, end, 32, seen(at), end, full, scale2, lane);
+  attn_walk<D, DT, true>(a, src, qf, 0, end, 32, seen(at), end, full, scale2, lane);
   const float l = attn_row_sum(a.l);
   if (r0 + i16 >= all) return;
   uint16_t *y = out + token * out_row + head * D + (D / 16) * 4 * j;
@@ -321,9 +321,6 @@ int prompt_launch(const PromptCall &c) {
   const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
   const float scale2 = fmaxf(fabsf(c.scale) * kLog2e, FLT_MIN);
 #define MP_PROMPT(D, DT)                                                                                                  \
-  if (hipFuncSetAttribute(reinterpret_cast<const void *>(prompt_attention_kernel<D, DT, PAGED>),                          \
-                          hipFuncAttributeMaxDynamicSharedMemorySize, 4 * PromptTile<D>::kBytes) != hipSuccess)           \
-    return MP_ERR_HIP;                                                                                                    \
   hipLaunchKernelGGL((prompt_attention_kernel<D, DT, PAGED>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),     \
                      4 * PromptTile<D>::kBytes, c.stream,                                                                 \
                      static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(c.k), c.kpage,  \

@@ -1091,61 +1091,69 @@ def _need_strided(t: torch.Tensor, name: str, dtype, ndim: int) -> None:
         raise TypeError(f"{name} must be a tensor")
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be on the GPU (mindpipe_amd has no CPU path)")
-    if t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+    if t.dtype is not dtype and t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
         raise RuntimeError(f"{name} has dtype {t.dtype}, expected {dtype}")
-    if t.dim() != ndim:
-        raise RuntimeError(f"{name} must be {ndim}-D, got shape {tuple(t.shape)}")
-    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or
-                      any(t.stride(i) % 8 for i in range(ndim - 1) if t.shape[i] > 1)):
-        raise RuntimeError(f"{name} must have contiguous values and rows in steps of 16 bytes, got strides {t.stride()}")
+    shape = t.shape
+    if len(shape) != ndim:
+        raise RuntimeError(f"{name} must be {ndim}-D, got shape {tuple(shape)}")
+    if t.data_ptr() % 16 or not (shape[-1] % 8 == 0 and t.is_contiguous()):
+        stride = t.stride()
+        if t.numel() and (stride[-1] != 1 or t.data_ptr() % 16 or
+                          any(stride[i] % 8 for i in range(ndim - 1) if shape[i] > 1)):
+            raise RuntimeError(f"{name} must have contiguous values and rows in steps of 16 bytes, got strides {stride}")
 
 
 def _same_device(t: torch.Tensor, **others: Optional[torch.Tensor]) -> None:
+    device = t.device
     for name, o in others.items():
-        if o is not None and o.device != t.device:
-            raise RuntimeError(f"{name} is on {o.device}, expected {t.device}")
+        if o is not None and o.device != device:
+            raise RuntimeError(f"{name} is on {o.device}, expected {device}")
 
 
-def _step(t: torch.Tensor, dim: int) -> int:
-    """The stride of a dimension (0 of one that holds a single entry, whatever it says)."""
-    return t.stride(dim) if t.shape[dim] > 1 else 0
+def _steps(t: torch.Tensor):
+    """The strides, 0 of a dimension that holds a single entry, whatever it says."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
 
 
 def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, dtype):
-    """Checks the cache's tensors against each other; its description for the C entry points."""
+    """Checks the cache's tensors against each other; its description for the C entry points (``mp_pages``)."""
     _need_strided(k_pages, "k_pages", dtype, 4)
     _need_strided(v_pages, "v_pages", dtype, 4)
     _need(table, "table", torch.int32, 2)
     _need(lens, "lens", torch.int32, 1)
     _same_device(k_pages, v_pages=v_pages, table=table, lens=lens)
-    if v_pages.shape != k_pages.shape:
-        raise RuntimeError(f"v_pages {tuple(v_pages.shape)} must have the shape of k_pages {tuple(k_pages.shape)}")
-    pages, kvh, size, _ = k_pages.shape
+    shape = k_pages.shape
+    if v_pages.shape != shape:
+        raise RuntimeError(f"v_pages {tuple(v_pages.shape)} must have the shape of k_pages {tuple(shape)}")
+    pages, kvh, size, _ = shape
+    batch, width = table.shape
     if size < 8 or size > 32768 or size & (size - 1):
         raise RuntimeError(f"a page holds a power of two of positions from 8 to 32768, got {size}")
-    if not pages or not kvh or not table.shape[1]:
+    if not pages or not kvh or not width:
         raise RuntimeError("k_pages, v_pages and table must hold at least one page and one head")
-    if table.shape[0] != lens.shape[0]:
+    if batch != lens.shape[0]:
         raise RuntimeError(f"table {tuple(table.shape)} and lens {tuple(lens.shape)} must have one row per sequence")
-    if table.shape[1] * size > 1 << 30:
-        raise RuntimeError(f"a sequence has at most 2^30 positions, the table has room for {table.shape[1] * size}")
-    return _lib.C.byref(_lib.Pages(
-        k_pages.data_ptr(), v_pages.data_ptr(), _step(k_pages, 0), _step(k_pages, 1), _step(k_pages, 2), _step(v_pages, 0),
-        _step(v_pages, 1), _step(v_pages, 2), pages, size, table.data_ptr(), table.shape[1]))
+    if width * size > 1 << 30:
+        raise RuntimeError(f"a sequence has at most 2^30 positions, the table has room for {width * size}")
+    ks, vs = _steps(k_pages), _steps(v_pages)
+    return _lib.PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages, size,
+                           table.data_ptr(), width)
 
 
 def _attention_heads(q: torch.Tensor, kvh: int, dim: int) -> None:
-    if q.shape[2] != dim or dim not in (64, 128, 256):
-        raise RuntimeError(f"heads of 64, 128 or 256 values are taken, the same in q and the keys: got {q.shape[2]} and {dim}")
-    if not kvh or q.shape[1] % kvh or not q.shape[1]:
-        raise RuntimeError(f"{q.shape[1]} query heads cannot share {kvh} key-value heads")
+    _, nh, qdim = q.shape
+    if qdim != dim or dim not in (64, 128, 256):
+        raise RuntimeError(f"heads of 64, 128 or 256 values are taken, the same in q and the keys: got {qdim} and {dim}")
+    if not kvh or nh % kvh or not nh:
+        raise RuntimeError(f"{nh} query heads cannot share {kvh} key-value heads")
 
 
 def _need_starts(starts: torch.Tensor, batch: Optional[int]) -> int:
     _need(starts, "starts", torch.int32, 1)
-    if starts.shape[0] < 1 or (batch is not None and starts.shape[0] != batch + 1):
+    n = starts.shape[0]
+    if n < 1 or (batch is not None and n != batch + 1):
         raise RuntimeError(f"starts must be [sequences + 1], got {tuple(starts.shape)}")
-    return starts.shape[0] - 1
+    return n - 1
 
 
 @_op("paged_rope_append", mutates=("k_pages", "v_pages"))
@@ -1173,13 +1181,13 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
     _need(sin, "sin", torch.float32, 2)
     _same_device(qkv, cos=cos, sin=sin, k_pages=k_pages, starts=starts)
     _, kvh, _, dim = k_pages.shape
-    rows, batch = qkv.shape[0], lens.shape[0]
+    (rows, values), batch, (angles, half) = qkv.shape, lens.shape[0], cos.shape
     if dim % 16 or dim > 1024:
         raise RuntimeError(f"heads of a multiple of 16 values up to 1024 are taken, got {dim}")
-    if qkv.shape[1] % dim or qkv.shape[1] // dim <= 2 * kvh:
+    if values % dim or values // dim <= 2 * kvh:
         raise RuntimeError(f"qkv {tuple(qkv.shape)} does not hold query heads and 2 x {kvh} heads of {dim}")
-    nh = qkv.shape[1] // dim - 2 * kvh
-    if sin.shape != cos.shape or not cos.shape[0] or not cos.shape[1] or cos.shape[1] % 8 or 2 * cos.shape[1] > dim:
+    nh = values // dim - 2 * kvh
+    if sin.shape != cos.shape or not angles or not half or half % 8 or 2 * half > dim:
         raise RuntimeError(f"cos and sin must be [positions, rotary / 2] with rotary a multiple of 16 up to {dim}, got "
                            f"{tuple(cos.shape)} and {tuple(sin.shape)}")
     if cos.data_ptr() % 16 or sin.data_ptr() % 16:
@@ -1194,8 +1202,8 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
     if rows:
         with _dev(qkv):
             _lib.check(_lib.load().mp_paged_rope_append(
-                qkv.data_ptr(), qkv.stride(0) if rows > 1 else qkv.shape[1], rows, nh, kvh, dim, cos.data_ptr(),
-                sin.data_ptr(), 2 * cos.shape[1], cos.shape[0], int(pairs), q.data_ptr(), cache, lens.data_ptr(),
+                qkv.data_ptr(), qkv.stride(0) if rows > 1 else values, rows, nh, kvh, dim, cos.data_ptr(),
+                sin.data_ptr(), 2 * half, angles, int(pairs), q.data_ptr(), cache, lens.data_ptr(),
                 _ptr(starts), batch, _DT[qkv.dtype], _stream()), "mp_paged_rope_append")
     return q
 
@@ -1224,12 +1232,12 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     out = torch.empty((b, nh, dim), dtype=q.dtype, device=q.device)
     if not b:
         return out
-    lib = _lib.load()
+    lib, qs = _lib.load(), _steps(q)
     with _dev(q):
         wsb = lib.mp_paged_decode_workspace_bytes(b, nh, kvh, dim)
         ws = torch.empty((wsb,), dtype=torch.uint8, device=q.device)
         _lib.check(lib.mp_paged_decode_attention(
-            q.data_ptr(), _step(q, 0), _step(q, 1), b, nh, kvh, dim, cache, lens.data_ptr(), scale, out.data_ptr(),
+            q.data_ptr(), qs[0], qs[1], b, nh, kvh, dim, cache, lens.data_ptr(), scale, out.data_ptr(),
             _DT[q.dtype], ws.data_ptr(), wsb, _stream()), "mp_paged_decode_attention")
     return out
 
@@ -1255,11 +1263,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     _attention_heads(q, k.shape[1], k.shape[2])
     if not batch or not rows:
         return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
-    out = torch.empty((rows, nh, dim), dtype=q.dtype, device=q.device)
+    out, qs, ks, vs = torch.empty((rows, nh, dim), dtype=q.dtype, device=q.device), _steps(q), _steps(k), _steps(v)
     with _dev(q):
         _lib.check(_lib.load().mp_prompt_attention(
-            q.data_ptr(), _step(q, 0), _step(q, 1), k.data_ptr(), _step(k, 0), _step(k, 1), v.data_ptr(), _step(v, 0),
-            _step(v, 1), rows, nh, k.shape[1], dim, starts.data_ptr(), batch, scale, out.data_ptr(), _DT[q.dtype],
+            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], rows, nh, k.shape[1], dim, starts.data_ptr(), batch, scale, out.data_ptr(), _DT[q.dtype],
             _stream()), "mp_prompt_attention")
     return out
 
@@ -1284,10 +1291,10 @@ def paged_prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     _attention_heads(q, k_pages.shape[1], k_pages.shape[3])
     if not batch or not rows:
         return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
-    out = torch.empty((rows, nh, dim), dtype=q.dtype, device=q.device)
+    out, qs = torch.empty((rows, nh, dim), dtype=q.dtype, device=q.device), _steps(q)
     with _dev(q):
         _lib.check(_lib.load().mp_paged_prompt_attention(
-            q.data_ptr(), _step(q, 0), _step(q, 1), rows, nh, k_pages.shape[1], dim, cache, lens.data_ptr(),
+            q.data_ptr(), qs[0], qs[1], rows, nh, k_pages.shape[1], dim, cache, lens.data_ptr(),
             starts.data_ptr(), batch, scale, out.data_ptr(), _DT[q.dtype], _stream()), "mp_paged_prompt_attention")
     return out
 

@@ -105,7 +105,7 @@ def test_c_entry_points_refuse():
     def cache(**over):
         f = dict(k=p, v=p, k_page=2048, k_head=1024, k_row=64, v_page=2048, v_head=1024, v_row=64, pages=6, page_size=16, table=p,
                  width=4)
-        return ctypes.byref(_lib.Pages(**{**f, **over}))
+        return _lib.PAGES.pack(*(v or 0 for v in {**f, **over}.values()))
 
     def decode(c, q=p, b=3, nh=4, kvh=2, d=64, dt=0, ws=p, wsb=1 << 40):
         return lib.mp_paged_decode_attention(q, 256, 64, b, nh, kvh, d, c, p, 0.1, p, dt, ws, wsb, None)
