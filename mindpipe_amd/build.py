@@ -34,10 +34,12 @@ FLAGS = [
 ]
 
 
-# Per-source extra flags.  w4a16.hip: MFMA results in ordinary VGPRs (its
-# kernels scale every MFMA result in VALU code; results in accumulation registers
+# Per-source extra flags.  w4a16.hip, paged.hip, prompt.hip: MFMA results in ordinary VGPRs
+# (their kernels scale MFMA results in VALU code; results in accumulation registers
 # would each need a copy first).
 FILE_FLAGS = {
+    "paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "w4a16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

@@ -31,6 +31,11 @@ __device__ __forceinline__ void prompt_lds_load16(const uint16_t *base, uint32_t
       mp_rsrc(base, 0x80000000u), reinterpret_cast<__attribute__((address_space(3))) void *>(reinterpret_cast<uintptr_t>(lds)),
       16, offset, 0, 0, 0);
 }
+// At most N of the wave's loads still on their way, every wave so far.
+template <int N>
+__device__ __forceinline__ void prompt_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 // Four rows' values of one column: lane i of 16 gives 8 bytes of row i / 4 and gets column i of the four rows.
 __device__ __forceinline__ as4_t prompt_read_tr(const __restrict__ lds_as4 p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
 __device__ __forceinline__ uint2 prompt_read_tr(const int8_t *lds) {
@@ -52,6 +57,8 @@ struct PromptTile {
   static constexpr int kChunks = D / 8;             // of 16 bytes in a row
   static constexpr int kBytes = kTile * D * 2;      // of K or of V
   static constexpr int kLoads = kBytes / 1024 / kWaves;
+  // Stages of K and V.  One workgroup a CU (D = 256) has nothing else to do while a tile is on its way: three tiles are.
+  static constexpr int kStages = D == 256 ? 4 : 2;
   // LDS chunk of a row's chunk c (and back).  K is read by 16 rows at a time in one column of chunks, V by four rows at a time
   // in four columns; 256 bytes are all banks.
   static __device__ __forceinline__ int k_chunk(int row, int c) { return c ^ (D == 64 ? (row >> 1) & 7 : row & 15); }
@@ -71,23 +78,33 @@ struct PackedPlan {
   }
 };
 
-// Rows r0 .. r0 + 15 by the wave alone, K and V straight from memory.
-template <int D, int DT, bool PAGED, class Seen>
-__device__ __forceinline__ void prompt_rows16(const KvSource<PAGED> &src, const uint16_t *q, int64_t q_row, int64_t q_head,
-                                              int r0, int all, int grp, Seen seen, float scale2, uint16_t *out, int64_t out_row) {
-  const int lane = threadIdx.x & 63, i16 = lane & 15, j = lane >> 4, at = min(r0 + i16, all - 1);
-  const int token = at / grp, head = at - token * grp;
+// Rows r0 .. r0 + 15 of a sequence and key-value head by the wave alone, K and V straight from memory.  A function of its own:
+// inlined, its registers would be the kernel's.
+template <bool PAGED>
+struct PromptRows {
+  KvSource<PAGED> src;
+  const uint16_t *q;
+  uint16_t *out;
+  int64_t q_row, q_head, out_row;
+  int all, grp, before;  // rows, heads of a token, positions that row 0 sees
+  float scale2;
+};
+template <int D, int DT, bool PAGED>
+__device__ __attribute__((noinline)) void prompt_rows16(const PromptRows<PAGED> &p, int r0) {
+  const int lane = threadIdx.x & 63, i16 = lane & 15, j = lane >> 4, at = min(r0 + i16, p.all - 1);
+  const int token = at / p.grp, head = at - token * p.grp;
+  const auto seen = [&](int r) { return max(p.before + min(r, p.all - 1) / p.grp, 0); };
   const int full = __builtin_amdgcn_readfirstlane(seen(r0)), end = __builtin_amdgcn_readfirstlane(seen(r0 + 15));
   uint4 qf[D / 32];
-  const uint16_t *qp = q + token * q_row + head * q_head + 8 * j;
+  const uint16_t *qp = p.q + token * p.q_row + head * p.q_head + 8 * j;
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) qf[c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
   AttnRows<D> a;
   attn_clear(a);
-  attn_walk<D, DT, true>(a, src, qf, 0, end, 32, seen(at), end, full, scale2, lane);
+  attn_walk<D, DT, true>(a, p.src, qf, 0, end, 32, seen(at), end, full, p.scale2, lane);
   const float l = attn_row_sum(a.l);
-  if (r0 + i16 >= all) return;
-  uint16_t *y = out + token * out_row + head * D + (D / 16) * 4 * j;
+  if (r0 + i16 >= p.all) return;
+  uint16_t *y = p.out + token * p.out_row + head * D + (D / 16) * 4 * j;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -106,7 +123,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
     uint32_t flip, uint16_t *__restrict__ out) {
   using T = PromptTile<D>;
   constexpr int kTile = T::kTile, kStage = 2 * T::kBytes, kS = kTile / 32;
-  extern __shared__ __attribute__((aligned(1024))) int8_t prompt_smem[];  // two stages of K and V
+  extern __shared__ __attribute__((aligned(1024))) int8_t prompt_smem[];  // kStages of K and V
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i32 = lane & 31, h = lane >> 5;
   const int kh = blockIdx.x % kvh;
   const PackedPlan plan{starts, batch, rows, grp};
@@ -139,6 +156,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
   // page of the tile's position `lane` (positions past the end: the last one's)
   const auto entry = [&](int tile) { return PAGED ? pg[min(tile + lane, end - 1) >> shift] : 0; };
   const auto load = [&](int tile, int id, int8_t *stage) {
+    tile = min(tile, end - 1);  // past the last tile: rows that nothing reads
 #pragma unroll
     for (int i = 0; i < T::kLoads; ++i) {
       const int slot = (wave * T::kLoads + i) * 64, r = slot / T::kChunks + lane / T::kChunks, c = lane % T::kChunks;
@@ -161,30 +179,36 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
   float m = -INFINITY, l = 0.f;
 
   const auto fix = [&](int id, uint64_t &there) {  // page numbers outside the pool: page 0, unseen
+    there = ~uint64_t(0);
     if constexpr (!PAGED) return 0;
     const bool ok = id >= 0 && id < pages;
     there = __ballot(ok || lane >= kTile);
     return ok ? id : 0;
   };
-  uint64_t there = ~uint64_t(0), next_there = there;
-  int ahead = 0;
+  // there[i]: which positions of the i-th tile from here exist
+  constexpr int kAhead = T::kStages - 1, kOneTile = 2 * T::kLoads + (PAGED ? 1 : 0);
+  uint64_t there[kAhead + 1];
+  int next_entry = 0, fill = 0, stage = 0;
   if (end > 0) {
-    load(0, fix(entry(0), there), prompt_smem);
-    ahead = entry(kTile);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      load(i * kTile, fix(entry(i * kTile), there[i]), prompt_smem + i * kStage);
+      fill = i + 1;
+    }
+    next_entry = entry(kAhead * kTile);
   }
-  int stage = 0;
   uint32_t odd = 0;  // an infinity or NaN in V where only some of the wave's rows see it
   for (int tile = 0; tile < end; tile += kTile) {
-    // this tile's loads have landed, every wave's, and the other stage has been read
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    if (tile + kTile < end) {
-      load(tile + kTile, fix(ahead, next_there), prompt_smem + (stage ^ 1) * kStage);
-      ahead = entry(tile + 2 * kTile);
-    }
+    // this tile's loads have landed, every wave's, and the stage of the last tile has been read
+    prompt_wait<(kAhead - 1) * kOneTile>();
+    load(tile + kAhead * kTile, fix(next_entry, there[kAhead]), prompt_smem + fill * kStage);
+    next_entry = entry(tile + (kAhead + 1) * kTile);
     const int8_t *ks = prompt_smem + stage * kStage, *vs = ks + T::kBytes;
-    stage ^= 1;
-    const uint64_t ok = there;
-    there = next_there;
+    stage = stage + 1 == T::kStages ? 0 : stage + 1;
+    fill = fill + 1 == T::kStages ? 0 : fill + 1;
+    const uint64_t ok = there[0];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) there[i] = there[i + 1];
     if (tile >= wend) continue;  // rows that see nothing more load for the others
     f16_t s[kS];
 #pragma unroll
@@ -255,16 +279,23 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
       }
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing on its way to LDS when the workgroup ends
   if (__any(odd)) {
     // 0 times an infinity is no zero: these rows once more, with what they do not see left out one position at a time
-    KvSource<PAGED> src;
-    if constexpr (PAGED) src = {kb, vb, kpage, krow, vpage, vrow, pg, shift, (1 << shift) - 1, pages, (len - 1) >> shift};
-    else src = {kb, vb, krow, vrow, n - 1};
-    const int64_t out_row = static_cast<int64_t>(kvh) * grp * D;
+    PromptRows<PAGED> p;
+    if constexpr (PAGED) p.src = {kb, vb, kpage, krow, vpage, vrow, pg, shift, (1 << shift) - 1, pages, (len - 1) >> shift};
+    else p.src = {kb, vb, krow, vrow, n - 1};
+    p.q = q + first * q_row + kh * grp * q_head;
+    p.q_row = q_row;
+    p.q_head = q_head;
+    p.out_row = static_cast<int64_t>(kvh) * grp * D;
+    p.out = out + first * p.out_row + kh * grp * D;
+    p.all = all;
+    p.grp = grp;
+    p.before = before;
+    p.scale2 = flip ? -scale2 : scale2;
     for (int half = 0; half < 2; ++half)
-      if (r0 + 16 * half < all)
-        prompt_rows16<D, DT, PAGED>(src, q + first * q_row + kh * grp * q_head, q_row, q_head, r0 + 16 * half, all, grp, seen,
-                                    flip ? -scale2 : scale2, out + first * out_row + kh * grp * D, out_row);
+      if (r0 + 16 * half < all) prompt_rows16<D, DT, PAGED>(p, r0 + 16 * half);
     return;
   }
   if (!row) return;
@@ -321,8 +352,13 @@ int prompt_launch(const PromptCall &c) {
   const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
   const float scale2 = fmaxf(fabsf(c.scale) * kLog2e, FLT_MIN);
 #define MP_PROMPT(D, DT)                                                                                                  \
+  if (2 * PromptTile<D>::kStages * PromptTile<D>::kBytes > 64 * 1024 &&                                                   \
+      hipFuncSetAttribute(reinterpret_cast<const void *>(prompt_attention_kernel<D, DT, PAGED>),                          \
+                          hipFuncAttributeMaxDynamicSharedMemorySize,                                                     \
+                          2 * PromptTile<D>::kStages * PromptTile<D>::kBytes) != hipSuccess)                              \
+    return MP_ERR_HIP;                                                                                                    \
   hipLaunchKernelGGL((prompt_attention_kernel<D, DT, PAGED>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),     \
-                     4 * PromptTile<D>::kBytes, c.stream,                                                                 \
+                     2 * PromptTile<D>::kStages * PromptTile<D>::kBytes, c.stream,                                                                 \
                      static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(c.k), c.kpage,  \
                      c.khead, c.krow, static_cast<const uint16_t *>(c.v), c.vpage, c.vhead, c.vrow, c.pages, c.shift,     \
                      c.table, c.width, c.lens, c.starts, static_cast<int>(c.batch), static_cast<int>(c.rows), c.kvh,      \
