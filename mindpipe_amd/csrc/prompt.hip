@@ -212,14 +212,27 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
     if (tile >= wend) continue;  // rows that see nothing more load for the others
     f16_t s[kS];
 #pragma unroll
-    for (int t = 0; t < kS; ++t) {
+    for (int t = 0; t < kS; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
-      const int r = 32 * t + i32;
+    {
+      constexpr int kC = D / 16, kAheadK = 2;  // pairs of operands that are read before they are used
+      i4_t kf[kAheadK + 1][kS];
+      const auto keys = [&](int c) {
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        const i4_t kf = *reinterpret_cast<const i4_t *>(ks + r * (D * 2) + 16 * T::k_chunk(r, 2 * c + h));
-        s[t] = prompt_mfma<DT>(__builtin_bit_cast(uint4, kf), qf[c], s[t]);
+        for (int t = 0; t < kS; ++t) {
+          const int r = 32 * t + i32;
+          kf[c % (kAheadK + 1)][t] = *reinterpret_cast<const i4_t *>(ks + r * (D * 2) + 16 * T::k_chunk(r, 2 * c + h));
+        }
+      };
+#pragma unroll
+      for (int c = 0; c < kAheadK; ++c) keys(c);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        if (c + kAheadK < kC) keys(c + kAheadK);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < kS; ++t) s[t] = prompt_mfma<DT>(__builtin_bit_cast(uint4, kf[c % (kAheadK + 1)][t]), qf[c], s[t]);
       }
     }
     // s[t][r]: position 32 t + 8 (r >> 2) + 4 h + (r & 3) of the tile
@@ -255,29 +268,43 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
         for (int r = 0; r < 16; ++r) o[d][r] *= f;
     }
     const float base = m == -INFINITY ? 0.f : m - kRaise<DT>;
-    uint32_t w[kS][8];
-#pragma unroll
-    for (int t = 0; t < kS; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        w[t][r / 2] = attn_pack2<DT>(__builtin_amdgcn_exp2f(fmaf(s[t][r], scale2, -base)),
-                                     __builtin_amdgcn_exp2f(fmaf(s[t][r + 1], scale2, -base)));
-        l = attn_add2<DT>(w[t][r / 2], l);
-      }
-    // O^T: step c of 16 positions, whose weights are w[c / 2][4 (c & 1) ..]: positions 16 c + 4 h + {0..3, 8..11}
+    // O^T: step c of 16 positions, whose weights are those of positions 16 c + 4 h + {0..3, 8..11}: s[c / 2][8 (c & 1) ..].  The
+    // next step's weights are made, and its V read, between the matrix instructions of this one.
+    constexpr int kSteps = kTile / 16, kD = D / 32;
     const int trow = 4 * h + ((lane & 15) >> 2), tcol = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-#pragma unroll
-    for (int c = 0; c < kTile / 16; ++c) {
-      const uint4 wf = make_uint4(w[c / 2][4 * (c & 1)], w[c / 2][4 * (c & 1) + 1], w[c / 2][4 * (c & 1) + 2],
-                                  w[c / 2][4 * (c & 1) + 3]);
+    uint32_t w[2][4];
+    uint4 vf[2][kD];
+    const auto weight = [&](int c, int i) {
+      const int r = 8 * (c & 1) + 2 * i;
+      w[c & 1][i] = attn_pack2<DT>(__builtin_amdgcn_exp2f(fmaf(s[c / 2][r], scale2, -base)),
+                                   __builtin_amdgcn_exp2f(fmaf(s[c / 2][r + 1], scale2, -base)));
+      l = attn_add2<DT>(w[c & 1][i], l);
+    };
+    const auto values = [&](int c, int d) {
       const int ra = 16 * c + trow, rb = ra + 8;
+      const uint2 lo = prompt_read_tr(vs + ra * (D * 2) + 16 * T::v_chunk(ra, 4 * d + tcol) + 8 * (lane & 1));
+      const uint2 hi = prompt_read_tr(vs + rb * (D * 2) + 16 * T::v_chunk(rb, 4 * d + tcol) + 8 * (lane & 1));
+      vf[c & 1][d] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    };
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) {
-        const uint2 lo = prompt_read_tr(vs + ra * (D * 2) + 16 * T::v_chunk(ra, 4 * d + tcol) + 8 * (lane & 1));
-        const uint2 hi = prompt_read_tr(vs + rb * (D * 2) + 16 * T::v_chunk(rb, 4 * d + tcol) + 8 * (lane & 1));
-        o[d] = prompt_mfma<DT>(make_uint4(lo.x, lo.y, hi.x, hi.y), wf, o[d]);
+    for (int d = 0; d < kD; ++d) values(0, d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) weight(0, i);
+#pragma unroll
+    for (int c = 0; c < kSteps; ++c) {
+      const uint4 wf = make_uint4(w[c & 1][0], w[c & 1][1], w[c & 1][2], w[c & 1][3]);
+#pragma unroll
+      for (int d = 0; d < kD; ++d) {
+        __builtin_amdgcn_sched_barrier(0);
+        o[d] = prompt_mfma<DT>(vf[c & 1][d], wf, o[d]);
+        if (c + 1 < kSteps) {
+          values(c + 1, d);
+#pragma unroll
+          for (int i = 4 * d / kD; i < 4 * (d + 1) / kD; ++i) weight(c + 1, i);
+        }
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing on its way to LDS when the workgroup ends
   if (__any(odd)) {
