@@ -17,11 +17,17 @@ the current position from device memory, so a step is shape-static and can be
 captured into a HIP graph.  ``decode_step_torch`` is the same step in PyTorch ops
 (masked attention over the whole cache), kept as the numerical reference.  Prefill
 uses PyTorch attention (SDPA) around the same W4A16 linears and fused norm / SiLU-mul kernels.
+
+``PagedKVCache`` holds sequences of different lengths in pages instead.  ``forward_paged`` runs packed
+new tokens of any of them (whole prompts, chunks of prompts, one token each) on the paged operators:
+append with rotation, decode or prompt attention.  ``generate_paged`` serves prompts with it, the
+tokens drawn by ``ops.sample_tokens``.
 """
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import List, Optional, Sequence
 
 import torch
 
@@ -96,6 +102,72 @@ class _W4:
 def _rms(x, w, eps):
     xf = x.float()
     return (xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)).half() * w
+
+
+class PagedKVCache:
+    """Keys and values of up to ``sequences`` sequences in pages of ``page`` positions, ``positions`` in all.
+
+    ``k`` / ``v [layers, pages, kv_heads, page, head_dim]`` are the pools; ``table`` (int32, a row of pages for each
+    sequence) and ``lens`` (int32) are what the paged operators read, in device memory and updated in place, so a
+    captured step goes on working while the sequences grow.  Which pages are free is kept on the host."""
+
+    def __init__(self, cfg: DecoderConfig, sequences: int, positions: int, page: int = 64, max_len: Optional[int] = None,
+                 device="cuda", dtype=torch.float16):
+        if sequences < 1 or positions < 1 or page < 8 or page & (page - 1):
+            raise ValueError("sequences and positions must be positive, page a power of two from 8")
+        pages = -(-positions // page)
+        self.page, self.max_len = page, max_len if max_len is not None else pages * page
+        shape = (cfg.layers, pages, cfg.kv_heads, page, cfg.head_dim)
+        self.k = torch.zeros(shape, device=device, dtype=dtype)
+        self.v = torch.zeros(shape, device=device, dtype=dtype)
+        self.table = torch.zeros(sequences, -(-self.max_len // page), device=device, dtype=torch.int32)
+        self.lens = torch.zeros(sequences, device=device, dtype=torch.int32)
+        self.length = [0] * sequences                      # of lens, on the host
+        self._held: List[List[int]] = [[] for _ in range(sequences)]
+        self._free = list(range(pages - 1, -1, -1))
+
+    def free_positions(self) -> int:
+        return len(self._free) * self.page
+
+    @torch.no_grad()
+    def extend(self, news: Sequence[int]) -> Optional[torch.Tensor]:
+        """Makes room for ``news[b]`` more positions of each sequence b, whose keys and values the next ``forward_paged``
+        writes: takes pages, updates ``table`` and ``lens``.  Returns the offsets of the sequences' tokens in their packed
+        order (``starts``), or ``None`` where every sequence has one.  Raises, and changes nothing, if a sequence gets too
+        long or the pages do not suffice."""
+        if len(news) != len(self.length) or any(n < 0 for n in news):
+            raise ValueError(f"one count for each of the {len(self.length)} sequences, got {list(news)}")
+        want = [-(-(l + n) // self.page) - len(h) for l, n, h in zip(self.length, news, self._held)]
+        if any(l + n > self.max_len for l, n in zip(self.length, news)):
+            raise RuntimeError(f"a sequence would pass {self.max_len} positions")
+        if sum(want) > len(self._free):
+            raise RuntimeError(f"{sum(want)} pages are wanted and {len(self._free)} are free")
+        device = self.table.device
+        rows, cols, pages = [], [], []
+        for b, n in enumerate(want):
+            for _ in range(n):
+                rows.append(b)
+                cols.append(len(self._held[b]))
+                pages.append(self._free.pop())
+                self._held[b].append(pages[-1])
+        if pages:
+            self.table[torch.tensor(rows, device=device), torch.tensor(cols, device=device)] = \
+                torch.tensor(pages, device=device, dtype=torch.int32)
+        self.length = [l + n for l, n in zip(self.length, news)]
+        self.lens.copy_(torch.tensor(self.length, dtype=torch.int32))
+        if all(n == 1 for n in news):
+            return None
+        starts = torch.zeros(len(news) + 1, dtype=torch.int32)
+        starts[1:] = torch.tensor(news, dtype=torch.int32).cumsum(0)
+        return starts.to(device)
+
+    @torch.no_grad()
+    def release(self, sequence: int) -> None:
+        """Ends a sequence: its pages are free again."""
+        self._free += reversed(self._held[sequence])
+        self._held[sequence] = []
+        self.length[sequence] = 0
+        self.lens[sequence] = 0
 
 
 class W4Decoder:
@@ -294,3 +366,73 @@ class W4Decoder:
             x = x + l["down"].reference(act.contiguous())
         logits = self.lm_head.reference(_rms(x, self.norm, cfg.eps).contiguous())
         return logits if return_logits else logits.argmax(-1)
+
+    def paged_cache(self, sequences: int, positions: int, page: int = 64) -> PagedKVCache:
+        """A paged cache for this model: up to ``positions`` in all, ``max_len`` of one sequence."""
+        return PagedKVCache(self.cfg, sequences, positions, page, self.max_len, self.embed.device)
+
+    def _angles(self):
+        """cos / sin of every position in fp32, from angles in 64 bits (far positions lose theirs in 32)."""
+        if getattr(self, "_cos_sin", None) is None:
+            hd, device = self.cfg.head_dim, self.embed.device
+            inv = self.cfg.rope_theta ** (-torch.arange(0, hd, 2, device=device, dtype=torch.float64) / hd)
+            angle = torch.outer(torch.arange(self.max_len, device=device, dtype=torch.float64), inv)
+            self._cos_sin = angle.cos().float(), angle.sin().float()
+        return self._cos_sin
+
+    @torch.no_grad()
+    def forward_paged(self, tokens, cache: PagedKVCache, starts: Optional[torch.Tensor] = None):
+        """Logits ``[sequences, vocab]`` after the last of each sequence's new tokens.  ``tokens`` (int64) are the packed new
+        tokens and ``starts`` their offsets, both for the positions that ``cache.extend`` has just made room for; without
+        ``starts`` each sequence has one.  A sequence without new tokens gets the logits of some other row.  Reads lengths
+        and pages from device memory: a step without ``starts`` can be captured and replayed after each ``extend``."""
+        cfg = self.cfg
+        hd, nh, kvh = cfg.head_dim, cfg.heads, cfg.kv_heads
+        scale, (cos, sin) = 1.0 / math.sqrt(hd), self._angles()
+        x, delta = self.embed[tokens], None
+        for li, l in enumerate(self.layers):
+            if delta is None:
+                hn = ops.add_rms_norm_quant(x, None, l["ln1"], cfg.eps, quant=False)[0]
+            else:
+                hn, _, _, x = ops.add_rms_norm_quant(delta, x, l["ln1"], cfg.eps, quant=False)
+            k, v = cache.k[li], cache.v[li]
+            q = ops.paged_rope_append(l["qkv"](hn), cos, sin, k, v, cache.table, cache.lens, starts)
+            if starts is None:
+                att = ops.paged_decode_attention(q, k, v, cache.table, cache.lens, scale)
+            else:
+                att = ops.paged_prompt_attention(q, k, v, cache.table, cache.lens, starts, scale)
+            hn, _, _, x = ops.add_rms_norm_quant(l["o"](att.view(-1, nh * hd)), x, l["ln2"], cfg.eps, quant=False)
+            delta = l["down"](l["gate_up"].swiglu(hn))
+        if starts is not None:  # the last row of each sequence
+            last = (starts[1:].long() - 1).clamp(min=0)
+            delta, x = delta[last], x[last]
+        return self.lm_head(ops.add_rms_norm_quant(delta, x, self.norm, cfg.eps, quant=False)[0])
+
+    @torch.no_grad()
+    def generate_paged(self, prompts: Sequence[torch.Tensor], new_tokens: int, cache: Optional[PagedKVCache] = None,
+                       temperature=None, top_k=None, top_p=None, min_p=None, generator: Optional[torch.Generator] = None):
+        """``new_tokens`` tokens after each of ``prompts`` (int64 tensors of different lengths): the prompts in one packed
+        pass, then a token of every sequence per step.  ``temperature``, ``top_k``, ``top_p``, ``min_p``: one value per prompt
+        or ``None`` (``ops.sample_tokens``); ``temperature`` ``None`` takes the largest logit.  Returns ``[prompts,
+        new_tokens]``."""
+        device = self.embed.device
+        lengths = [int(p.numel()) for p in prompts]
+        if not lengths or min(lengths) < 1 or new_tokens < 1:
+            raise ValueError("prompts must hold a token at least, and new_tokens must be positive")
+        if cache is None:
+            page = 64
+            cache = self.paged_cache(len(prompts), sum(-(-(n + new_tokens) // page) * page for n in lengths), page)
+        if temperature is None:
+            temperature = torch.zeros(len(prompts), device=device)
+
+        def sample(logits):
+            u = torch.rand(len(prompts), device=device, generator=generator)
+            return ops.sample_tokens(logits, u, temperature, top_k, top_p, min_p)[0]
+
+        starts = cache.extend(lengths)
+        tokens = sample(self.forward_paged(torch.cat([p.reshape(-1) for p in prompts]).to(device), cache, starts))
+        out = [tokens]
+        for _ in range(new_tokens - 1):
+            cache.extend([1] * len(prompts))
+            out.append(sample(self.forward_paged(out[-1], cache)))
+        return torch.stack(out, 1)
