@@ -460,16 +460,22 @@ int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q_head, int6
                               void *workspace, size_t workspace_bytes, mp_stream_t stream);
 
 /* Causal attention of packed sequences: rows starts[b] .. starts[b + 1] - 1 of q [rows, nh, head_dim], k and v [rows, kvh,
- * head_dim] are sequence b.  out [rows, nh, head_dim], dense; rows of no sequence are zeros.  head_dim 64, 128, 256. */
+ * head_dim] are sequence b.  out [rows, nh, head_dim], dense; rows of no sequence are zeros.  head_dim 64, 128, 256.
+ * Few rows have their positions split over workgroups, which needs the workspace that mp_prompt_workspace_bytes says for
+ * the current device (reach: the most positions a sequence can have, rows here and width * page_size of a cache; 0: none
+ * is needed), 16-byte aligned, not shared by calls that may run at once. */
+size_t mp_prompt_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch, int64_t reach);
 int mp_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const void *k, int64_t k_row, int64_t k_head,
                         const void *v, int64_t v_row, int64_t v_head, int64_t rows, int nh, int kvh, int head_dim,
-                        const int32_t *starts, int64_t batch, float scale, void *out, int dtype, mp_stream_t stream);
+                        const int32_t *starts, int64_t batch, float scale, void *out, int dtype, void *workspace,
+                        size_t workspace_bytes, mp_stream_t stream);
 
 /* The same with keys and values in the cache: the packed rows of sequence b are its last positions of lens[b] (as
  * mp_paged_rope_append puts them there), and each sees the positions up to its own. */
 int mp_paged_prompt_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh, int head_dim,
                               const mp_pages *cache, const int32_t *lens, const int32_t *starts, int64_t batch,
-                              float scale, void *out, int dtype, mp_stream_t stream);
+                              float scale, void *out, int dtype, void *workspace, size_t workspace_bytes,
+                              mp_stream_t stream);
 
 /* A token for each row of logits [rows, vocab] (row stride `stride`; fp16, bf16 or fp32; vocab up to 2^19) at the random
  * number u in [0, 1): weights exp((x - max) / temperature) of the top_k largest values (equal ones: the lowest indexes;

@@ -87,9 +87,10 @@ SIGNATURES = {
     "mp_paged_decode_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, C.c_float, _vp, _i32, _vp, _sz,
                                          _vp]),
     "mp_prompt_attention": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _i64,
-                                   C.c_float, _vp, _i32, _vp]),
+                                   C.c_float, _vp, _i32, _vp, _sz, _vp]),
+    "mp_prompt_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64, _i64]),
     "mp_paged_prompt_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, C.c_float, _vp, _i32,
-                                         _vp]),
+                                         _vp, _sz, _vp]),
     "mp_sample_tokens": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mp_moe_unpermute_combine": (_i32, [_vp, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _i32, _vp]),
 }

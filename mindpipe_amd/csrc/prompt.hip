@@ -11,6 +11,9 @@
 // (l & 31) and the weights go from the first product's accumulators to the second's operand without crossing lanes.
 // K and V tiles come by direct-to-LDS loads, a tile ahead; V is read transposed (ds_read_b64_tr_b16).  Rows of LDS are
 // swizzled in 16-byte chunks so that neither reads a bank twice at a time.
+//
+// Few rows leave most CUs without a workgroup: then the positions are split over `splits` workgroups, which leave their sums,
+// maxima and outputs, unnormalised, in the workspace, and a second launch joins them.
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -87,7 +90,10 @@ struct PromptRows {
   uint16_t *out;
   int64_t q_row, q_head, out_row;
   int all, grp, before;  // rows, heads of a token, positions that row 0 sees
+  int from, to;          // positions that are looked at
   float scale2;
+  float *part;           // [tokens, heads][dim + 2], row stride part_row; null: outputs are final
+  int64_t part_row;
 };
 template <int D, int DT, bool PAGED>
 __device__ __attribute__((noinline)) void prompt_rows16(const PromptRows<PAGED> &p, int r0) {
@@ -101,9 +107,21 @@ __device__ __attribute__((noinline)) void prompt_rows16(const PromptRows<PAGED> 
   for (int c = 0; c < D / 32; ++c) qf[c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
   AttnRows<D> a;
   attn_clear(a);
-  attn_walk<D, DT, true>(a, p.src, qf, 0, end, 32, seen(at), end, full, p.scale2, lane);
+  attn_walk<D, DT, true>(a, p.src, qf, p.from, min(end, p.to), 32, seen(at), end, full, p.scale2, lane);
   const float l = attn_row_sum(a.l);
   if (r0 + i16 >= p.all) return;
+  if (p.part) {
+    float *z = p.part + token * p.part_row + head * (D + 2);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) z[(D / 16) * (4 * j + r) + c] = a.o[c][r];
+    if (j == 0) {
+      z[D] = a.m;
+      z[D + 1] = l;
+    }
+    return;
+  }
   uint16_t *y = p.out + token * p.out_row + head * D + (D / 16) * 4 * j;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -120,15 +138,15 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
     int64_t khead, int64_t krow, const uint16_t *__restrict__ v, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
     int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
     const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, int tiles, float scale2,
-    uint32_t flip, uint16_t *__restrict__ out) {
+    uint32_t flip, int splits, float *__restrict__ parts, uint16_t *__restrict__ out) {
   using T = PromptTile<D>;
   constexpr int kTile = T::kTile, kStage = 2 * T::kBytes, kS = kTile / 32;
   extern __shared__ __attribute__((aligned(1024))) int8_t prompt_smem[];  // kStages of K and V
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i32 = lane & 31, h = lane >> 5;
-  const int kh = blockIdx.x % kvh;
+  const int kh = blockIdx.x % kvh, unit = blockIdx.x / kvh, sp = unit % splits;
   const PackedPlan plan{starts, batch, rows, grp};
-  int b, part, parts;
-  if (!attn_find_part(plan, batch + 1, kRows, tiles - 1 - static_cast<int>(blockIdx.x / kvh), b, part, parts)) return;
+  int b, part, count;
+  if (!attn_find_part(plan, batch + 1, kRows, tiles - 1 - unit / splits, b, part, count)) return;
   const int first = plan.first(b), n = plan.end(b) - first, all = n * grp;
   int len = 0;  // positions of the sequence, the new tokens' included; none behind the last sequence
   if (b < batch) len = PAGED ? min(max(lens[b], 0), width << shift) : n;
@@ -139,9 +157,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
   const bool row = at < all;
   const int token = row ? at / grp : 0, head = kh * grp + (row ? at - token * grp : 0);
   const int sees = row ? seen(at) : 0;
+  // this workgroup's positions: `from` up to `end`, of them this wave's up to `wend`
+  const int reach = seen(part * kRows + kRows - 1), share = (reach + kTile * splits - 1) / (kTile * splits) * kTile;
+  const int from = __builtin_amdgcn_readfirstlane(min(sp * share, reach)), end = __builtin_amdgcn_readfirstlane(min(from + share, reach));
   const int full = r0 < all ? __builtin_amdgcn_readfirstlane(seen(r0)) : 0;
-  const int wend = r0 < all ? __builtin_amdgcn_readfirstlane(seen(r0 + 31)) : 0;
-  const int end = __builtin_amdgcn_readfirstlane(seen(part * kRows + kRows - 1));
+  const int wend = r0 < all ? min(__builtin_amdgcn_readfirstlane(seen(r0 + 31)), end) : 0;
 
   uint4 qf[D / 16];
   const uint16_t *qp = q + (first + token) * q_row + head * q_head + 8 * h;
@@ -189,16 +209,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
   constexpr int kAhead = T::kStages - 1, kOneTile = 2 * T::kLoads + (PAGED ? 1 : 0);
   uint64_t there[kAhead + 1];
   int next_entry = 0, fill = 0, stage = 0;
-  if (end > 0) {
+  if (end > from) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      load(i * kTile, fix(entry(i * kTile), there[i]), prompt_smem + i * kStage);
+      load(from + i * kTile, fix(entry(from + i * kTile), there[i]), prompt_smem + i * kStage);
       fill = i + 1;
     }
-    next_entry = entry(kAhead * kTile);
+    next_entry = entry(from + kAhead * kTile);
   }
   uint32_t odd = 0;  // an infinity or NaN in V where only some of the wave's rows see it
-  for (int tile = 0; tile < end; tile += kTile) {
+  for (int tile = from; tile < end; tile += kTile) {
     // this tile's loads have landed, every wave's, and the stage of the last tile has been read
     prompt_wait<(kAhead - 1) * kOneTile>();
     load(tile + kAhead * kTile, fix(next_entry, there[kAhead]), prompt_smem + fill * kStage);
@@ -320,13 +340,26 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
     p.all = all;
     p.grp = grp;
     p.before = before;
+    p.from = from;
+    p.to = end;
     p.scale2 = flip ? -scale2 : scale2;
+    p.part_row = static_cast<int64_t>(kvh) * grp * (D + 2);
+    p.part = splits > 1 ? parts + sp * rows * p.part_row + first * p.part_row + kh * grp * (D + 2) : nullptr;
     for (int half = 0; half < 2; ++half)
       if (r0 + 16 * half < all) prompt_rows16<D, DT, PAGED>(p, r0 + 16 * half);
     return;
   }
   if (!row) return;
   l += __shfl_xor(l, 32, 64);
+  if (splits > 1) {
+    float *z = parts + ((static_cast<int64_t>(sp) * rows + first + token) * kvh * grp + head) * (D + 2);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) *reinterpret_cast<float2 *>(z + 32 * d + 8 * (r >> 2) + 4 * h + (r & 3)) = make_float2(o[d][r], o[d][r + 1]);
+    if (h == 0) *reinterpret_cast<float2 *>(z + D) = make_float2(m, l);
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   uint16_t *y = out + (static_cast<int64_t>(first + token) * kvh * grp + head) * D + 4 * h;
 #pragma unroll
@@ -338,6 +371,48 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
       for (int i = 0; i < 4; ++i) x[i] = l == 0.f ? 0.f : o[d][r + i] * inv;
       *reinterpret_cast<uint2 *>(y + 32 * d + 2 * r) = make_uint2(attn_pack2<DT>(x[0], x[1]), attn_pack2<DT>(x[2], x[3]));
     }
+}
+
+// The splits of a row meet, one wave each.
+template <int D, int DT>
+__global__ __launch_bounds__(256) void prompt_join_kernel(const float *__restrict__ parts, int splits, int64_t rows,
+                                                          uint16_t *__restrict__ out) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 63;
+  const float *z = parts + row * (D + 2);
+  const int64_t step = rows * (D + 2);
+  float m = -INFINITY;
+  for (int s = lane; s < splits; s += 64) m = fmaxf(m, z[s * step + D]);
+  m = mp_wave_max(m);
+  float o[D / 64], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float ms = z[s * step + D], f = ms == m ? 1.0f : __builtin_amdgcn_exp2f(ms - m);
+    l += f * z[s * step + D + 1];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) o[i] += f * z[s * step + 64 * i + lane];
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    const float v = l == 0.f ? 0.f : o[i] * inv;
+    out[row * D + 64 * i + lane] = DT == MP_F16 ? mp_f2h(v) : mp_f2bf(v);
+  }
+}
+
+// Row tiles of all sequences, at most: a part of one for each, and for the rows behind the last.
+inline int64_t prompt_tiles(int64_t rows, int64_t grp, int64_t batch) { return rows * grp / kRows + batch + 1; }
+
+// Splits of the positions (at most `reach`): as many as there are CUs (two workgroups each; one of heads of 256) for every
+// row tile, where that leaves each four tiles of positions at least.  With half as many workgroups as that there is none:
+// what the join reads and writes would cost more than the idle CUs.
+inline int prompt_splits(int64_t rows, int64_t nh, int64_t kvh, int64_t dim, int64_t batch, int64_t reach) {
+  const int64_t slots = (dim == 256 ? 1 : 2) * mp_cu_count(), blocks = prompt_tiles(rows, nh / kvh, batch) * kvh;
+  const int64_t s = slots / blocks, most = reach / 256;
+  return static_cast<int>(s < 2 || most < 2 ? 1 : s < most ? s : most);
 }
 
 struct PromptCall {
@@ -352,6 +427,8 @@ struct PromptCall {
   float scale;
   void *out;
   int dtype;
+  void *workspace;
+  size_t workspace_bytes;
   hipStream_t stream;
 };
 
@@ -371,9 +448,17 @@ int prompt_launch(const PromptCall &c) {
   if (c.krow > reach / span || c.vrow > reach / span) return MP_ERR_SHAPE;
   if (c.rows == 0) return MP_OK;
   const int64_t grp = c.nh / c.kvh;
-  // a part of a tile for each sequence, and for the rows behind the last one
-  const int64_t tiles = c.rows * grp / kRows + c.batch + 1, blocks = tiles * c.kvh;
-  if (c.rows * grp > INT32_MAX - kRows || blocks > INT32_MAX) return MP_ERR_SHAPE;
+  const int64_t tiles = prompt_tiles(c.rows, grp, c.batch);
+  if (c.rows * c.nh > INT32_MAX - kRows || tiles * c.kvh > INT32_MAX) return MP_ERR_SHAPE;
+  if (mp_cu_count() <= 0) return MP_ERR_HIP;
+  const int splits = prompt_splits(c.rows, c.nh, c.kvh, c.head_dim, c.batch, PAGED ? static_cast<int64_t>(c.width) << c.shift : c.rows);
+  const int64_t blocks = tiles * c.kvh * splits;
+  if (splits > 1) {
+    if (!c.workspace) return MP_ERR_ARG;
+    if (!mp_aligned(c.workspace, 16)) return MP_ERR_ALIGN;
+    if (c.workspace_bytes < splits * c.rows * c.nh * (c.head_dim + 2) * sizeof(float)) return MP_ERR_WORKSPACE;
+  }
+  float *parts = static_cast<float *>(c.workspace);
   // the sign of the scale goes to the queries, so that the largest product gives the largest score; a scale of 0 becomes the
   // smallest normal number, which leaves every finite score 0 and a masked one -inf
   const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
@@ -389,22 +474,28 @@ int prompt_launch(const PromptCall &c) {
                      static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(c.k), c.kpage,  \
                      c.khead, c.krow, static_cast<const uint16_t *>(c.v), c.vpage, c.vhead, c.vrow, c.pages, c.shift,     \
                      c.table, c.width, c.lens, c.starts, static_cast<int>(c.batch), static_cast<int>(c.rows), c.kvh,      \
-                     static_cast<int>(grp), static_cast<int>(tiles), scale2, flip, static_cast<uint16_t *>(c.out))
+                     static_cast<int>(grp), static_cast<int>(tiles), scale2, flip, splits, parts,                         \
+                     static_cast<uint16_t *>(c.out));                                                                    \
+  if (splits > 1) {                                                                                                       \
+    MP_CHECK_LAUNCH();                                                                                                    \
+    hipLaunchKernelGGL((prompt_join_kernel<D, DT>), dim3(static_cast<unsigned>(mp_cdiv(c.rows * c.nh, 4))), dim3(256), 0, \
+                       c.stream, parts, splits, c.rows * c.nh, static_cast<uint16_t *>(c.out));                          \
+  }
   if (c.dtype == MP_F16) {
     if (c.head_dim == 64) {
-      MP_PROMPT(64, MP_F16);
+      MP_PROMPT(64, MP_F16)
     } else if (c.head_dim == 128) {
-      MP_PROMPT(128, MP_F16);
+      MP_PROMPT(128, MP_F16)
     } else {
-      MP_PROMPT(256, MP_F16);
+      MP_PROMPT(256, MP_F16)
     }
   } else {
     if (c.head_dim == 64) {
-      MP_PROMPT(64, MP_BF16);
+      MP_PROMPT(64, MP_BF16)
     } else if (c.head_dim == 128) {
-      MP_PROMPT(128, MP_BF16);
+      MP_PROMPT(128, MP_BF16)
     } else {
-      MP_PROMPT(256, MP_BF16);
+      MP_PROMPT(256, MP_BF16)
     }
   }
 #undef MP_PROMPT
@@ -414,18 +505,26 @@ int prompt_launch(const PromptCall &c) {
 
 }  // namespace
 
+extern "C" size_t mp_prompt_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch, int64_t reach) {
+  if (rows <= 0 || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || batch <= 0 || reach <= 0 || mp_cu_count() <= 0) return 0;
+  const int splits = prompt_splits(rows, nh, kvh, head_dim, batch, reach);
+  return splits > 1 ? static_cast<size_t>(splits) * rows * nh * (head_dim + 2) * sizeof(float) : 0;
+}
+
 extern "C" int mp_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const void *k, int64_t k_row, int64_t k_head,
                                    const void *v, int64_t v_row, int64_t v_head, int64_t rows, int nh, int kvh, int head_dim,
-                                   const int32_t *starts, int64_t batch, float scale, void *out, int dtype,
-                                   mp_stream_t stream) {
+                                   const int32_t *starts, int64_t batch, float scale, void *out, int dtype, void *workspace,
+                                   size_t workspace_bytes, mp_stream_t stream) {
   if (!q || !k || !v || !starts || !out) return MP_ERR_ARG;
   return prompt_launch<false>({q, q_row, q_head, k, v, 0, k_head, k_row, 0, v_head, v_row, 0, 0, 0, nullptr, nullptr, starts,
-                               batch, rows, nh, kvh, head_dim, scale, out, dtype, reinterpret_cast<hipStream_t>(stream)});
+                               batch, rows, nh, kvh, head_dim, scale, out, dtype, workspace, workspace_bytes,
+                               reinterpret_cast<hipStream_t>(stream)});
 }
 
 extern "C" int mp_paged_prompt_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh,
                                          int head_dim, const mp_pages *cache, const int32_t *lens, const int32_t *starts,
-                                         int64_t batch, float scale, void *out, int dtype, mp_stream_t stream) {
+                                         int64_t batch, float scale, void *out, int dtype, void *workspace,
+                                         size_t workspace_bytes, mp_stream_t stream) {
   if (!q || !cache || !cache->k || !cache->v || !cache->table || !lens || !starts || !out) return MP_ERR_ARG;
   int shift = -1;
   for (int s = 3; s < 16; ++s)
@@ -435,5 +534,5 @@ extern "C" int mp_paged_prompt_attention(const void *q, int64_t q_row, int64_t q
   return prompt_launch<true>({q, q_row, q_head, cache->k, cache->v, cache->k_page, cache->k_head, cache->k_row, cache->v_page,
                               cache->v_head, cache->v_row, static_cast<int>(cache->pages), shift,
                               static_cast<int>(cache->width), cache->table, lens, starts, batch, rows, nh, kvh, head_dim,
-                              scale, out, dtype, reinterpret_cast<hipStream_t>(stream)});
+                              scale, out, dtype, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream)});
 }

@@ -1264,10 +1264,13 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     if not batch or not rows:
         return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
     out, qs, ks, vs = torch.empty((rows, nh, dim), dtype=q.dtype, device=q.device), _steps(q), _steps(k), _steps(v)
+    lib, kvh = _lib.load(), k.shape[1]
     with _dev(q):
-        _lib.check(_lib.load().mp_prompt_attention(
-            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], rows, nh, k.shape[1], dim, starts.data_ptr(), batch, scale, out.data_ptr(), _DT[q.dtype],
-            _stream()), "mp_prompt_attention")
+        wsb = lib.mp_prompt_workspace_bytes(rows, nh, kvh, dim, batch, rows)
+        ws = torch.empty((wsb,), dtype=torch.uint8, device=q.device) if wsb else None
+        _lib.check(lib.mp_prompt_attention(
+            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], rows, nh, kvh, dim, starts.data_ptr(), batch, scale, out.data_ptr(), _DT[q.dtype],
+            _ptr(ws), wsb, _stream()), "mp_prompt_attention")
     return out
 
 
@@ -1292,10 +1295,13 @@ def paged_prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if not batch or not rows:
         return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
     out, qs = torch.empty((rows, nh, dim), dtype=q.dtype, device=q.device), _steps(q)
+    lib, (_, kvh, size, _) = _lib.load(), k_pages.shape
     with _dev(q):
-        _lib.check(_lib.load().mp_paged_prompt_attention(
-            q.data_ptr(), qs[0], qs[1], rows, nh, k_pages.shape[1], dim, cache, lens.data_ptr(),
-            starts.data_ptr(), batch, scale, out.data_ptr(), _DT[q.dtype], _stream()), "mp_paged_prompt_attention")
+        wsb = lib.mp_prompt_workspace_bytes(rows, nh, kvh, dim, batch, table.shape[1] * size)
+        ws = torch.empty((wsb,), dtype=torch.uint8, device=q.device) if wsb else None
+        _lib.check(lib.mp_paged_prompt_attention(
+            q.data_ptr(), qs[0], qs[1], rows, nh, kvh, dim, cache, lens.data_ptr(), starts.data_ptr(), batch, scale,
+            out.data_ptr(), _DT[q.dtype], _ptr(ws), wsb, _stream()), "mp_paged_prompt_attention")
     return out
 
 

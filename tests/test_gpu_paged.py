@@ -189,6 +189,28 @@ def test_later_tokens_do_not_reach_back(dtype, dim):
                 assert torch.isnan(got[at:70]).all()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_few_rows_over_long_contexts(dtype, dim):
+    """Positions split over workgroups and joined: rows that see all of a split, a part of it, or nothing, missing pages, and a
+    NaN that only the last rows see."""
+    lens, news = [2500, 700, 30, 0], [20, 1, 30, 0]
+    k, v, table, ln = _cache(lens, 2, dim, 32, dtype, 41)
+    table[0, 3], table[1, 2] = -1, 1 << 20
+    starts = torch.tensor([0, 20, 21, 51, 51], dtype=torch.int32)
+    q = (1.5 * torch.randn(54, 6, dim, generator=torch.Generator().manual_seed(42))).to(dtype).to(DEV)
+    args = (q, k, v, table, ln, starts.to(DEV), dim ** -0.5)
+    got = _ops().paged_prompt_attention(*args)
+    ref.check(got, *ref.paged_attention(q, k, v, table, ln, starts, dim ** -0.5))
+    assert torch.equal(got, _ops().paged_prompt_attention(*args))
+    page, row = int(table[0, 2490 // 32]), 2490 % 32
+    v[page, 1, row] = float("nan")
+    k[page, 0, row] = float("nan")
+    got = _ops().paged_prompt_attention(*args)
+    ref.check(got, *ref.paged_attention(q, k, v, table, ln, starts, dim ** -0.5))
+    assert torch.isfinite(got[:10]).all() and torch.isnan(got[10:20]).all()
+
+
 def test_paged_prompt_bad_pages_and_short_lengths():
     """Missing pages, lengths smaller than the number of new tokens, and lengths past the table's room."""
     k, v, table, ln = _cache([90, 40, 64], 2, 128, 16, F16, 11)

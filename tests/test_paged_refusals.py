@@ -119,7 +119,7 @@ def test_c_entry_points_refuse():
     for bad in (dict(page_size=24), dict(page_size=4), dict(pages=0), dict(width=0), dict(width=1 << 27), dict(k_row=60),
                 dict(v_head=-64)):
         assert decode(cache(**bad)) == SHAPE
-        assert lib.mp_paged_prompt_attention(p, 256, 64, 9, 4, 2, 64, cache(**bad), p, p, 3, 0.1, p, 0, None) == SHAPE
+        assert lib.mp_paged_prompt_attention(p, 256, 64, 9, 4, 2, 64, cache(**bad), p, p, 3, 0.1, p, 0, p, 1 << 40, None) == SHAPE
         assert lib.mp_paged_rope_append(p, 512, 3, 4, 2, 64, p, p, 64, 20, 1, p, cache(**bad), p, None, 3, 0, None) == SHAPE
     for bad in ((p, 500, 3, 4, 2, 64, p, p, 64), (p, 512, 3, 4, 2, 60, p, p, 48), (p, 512, 3, 4, 2, 64, p, p, 80),
                 (p, 512, 3, 4, 2, 64, p, p, 8), (p, 512, 4, 4, 2, 64, p, p, 64)):
@@ -127,7 +127,7 @@ def test_c_entry_points_refuse():
     assert lib.mp_paged_rope_append(p, 512, 3, 4, 2, 64, p, p, 64, 0, 1, p, cache(), p, None, 3, 0, None) == SHAPE
     assert lib.mp_paged_rope_append(p, 512, 3, 4, 2, 64, p, p, 64, 20, 1, None, cache(), p, None, 3, 0, None) == ARG
     prompt = lambda *a, nh=4, kvh=2, d=64, rows=9, b=3, row=256, dt=0: lib.mp_prompt_attention(  # noqa: E731
-        p, row, 64, p, 128, 64, p, 128, 64, rows, nh, kvh, d, *(a or (p,)), b, 0.1, p, dt, None)
+        p, row, 64, p, 128, 64, p, 128, 64, rows, nh, kvh, d, *(a or (p,)), b, 0.1, p, dt, p, 1 << 40, None)
     assert prompt(None) == ARG and prompt(nh=3) == SHAPE and prompt(d=80) == SHAPE and prompt(b=0) == SHAPE
     assert prompt(row=-8) == SHAPE and prompt(row=252) == SHAPE and prompt(dt=2) == DTYPE and prompt(rows=1 << 40) == SHAPE
     sample = lambda x=p, stride=50, rows=3, vocab=50, dt=0, u=p: lib.mp_sample_tokens(  # noqa: E731
