@@ -406,12 +406,14 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const float *__restric
 // Row tiles of all sequences, at most: a part of one for each, and for the rows behind the last.
 inline int64_t prompt_tiles(int64_t rows, int64_t grp, int64_t batch) { return rows * grp / kRows + batch + 1; }
 
-// Splits of the positions (at most `reach`): as many as there are CUs (two workgroups each; one of heads of 256) for every
-// row tile, where that leaves each four tiles of positions at least.  With half as many workgroups as that there is none:
-// what the join reads and writes would cost more than the idle CUs.
+// Splits of the positions (at most `reach`): so many that the workgroups come nearest to what the CUs hold at once (two each;
+// one of heads of 256), with four tiles of positions each at least.  16 rows behind 32768 positions (32 / 8 heads of 128):
+// 666 us whole, 341 / 176 / 95 us in 2 / 4 / 8 splits, 40 us in the 32 that this gives; 1068 rows of 16 / 4 heads of 256
+// (144 workgroups): 143 us whole, 108 in 2, 113 in 3; 1737 rows of 32 heads of 128 (480 workgroups): 180 whole, 197 in 2, the
+// join reads and writes more than idle CUs cost.
 inline int prompt_splits(int64_t rows, int64_t nh, int64_t kvh, int64_t dim, int64_t batch, int64_t reach) {
   const int64_t slots = (dim == 256 ? 1 : 2) * mp_cu_count(), blocks = prompt_tiles(rows, nh / kvh, batch) * kvh;
-  const int64_t s = slots / blocks, most = reach / 256;
+  const int64_t s = (slots + blocks / 2) / blocks, most = reach / 256;
   return static_cast<int>(s < 2 || most < 2 ? 1 : s < most ? s : most);
 }
 
