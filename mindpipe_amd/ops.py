@@ -1110,22 +1110,33 @@ def _same_device(t: torch.Tensor, **others: Optional[torch.Tensor]) -> None:
             raise RuntimeError(f"{name} is on {o.device}, expected {device}")
 
 
+def _fits(t, device, dtype, ndim: int) -> bool:
+    """What ``_need`` and ``_same_device`` ask for, in one look (a call's checks take as long as its launch)."""
+    return (type(t) in _PLAIN and t.dtype is dtype and t.dim() == ndim and t.device == device and t.is_contiguous())
+
+
+def _need_plain(t: torch.Tensor, name: str, like: torch.Tensor, dtype, ndim: int) -> None:
+    if not _fits(t, like.device, dtype, ndim):
+        _need(t, name, dtype, ndim)
+        _same_device(like, **{name: t})
+
+
 def _steps(t: torch.Tensor):
     """The strides, 0 of a dimension that holds a single entry, whatever it says."""
     return [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
 
 
-def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, dtype):
-    """Checks the cache's tensors against each other; its description for the C entry points (``mp_pages``)."""
-    _need_strided(k_pages, "k_pages", dtype, 4)
-    _need_strided(v_pages, "v_pages", dtype, 4)
-    _need(table, "table", torch.int32, 2)
-    _need(lens, "lens", torch.int32, 1)
-    _same_device(k_pages, v_pages=v_pages, table=table, lens=lens)
-    shape = k_pages.shape
-    if v_pages.shape != shape:
-        raise RuntimeError(f"v_pages {tuple(v_pages.shape)} must have the shape of k_pages {tuple(shape)}")
-    pages, kvh, size, _ = shape
+def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, like: torch.Tensor):
+    """Checks the cache's tensors against each other and ``like``; its description for the C entry points (``mp_pages``)."""
+    _need_strided(k_pages, "k_pages", like.dtype, 4)
+    _need_strided(v_pages, "v_pages", like.dtype, 4)
+    _need_plain(table, "table", like, torch.int32, 2)
+    _need_plain(lens, "lens", like, torch.int32, 1)
+    if k_pages.device != like.device or v_pages.device != like.device:
+        _same_device(like, k_pages=k_pages, v_pages=v_pages)
+    shape = pages, kvh, size, dim = k_pages.shape
+    if v_pages.shape != k_pages.shape:
+        raise RuntimeError(f"v_pages {tuple(v_pages.shape)} must have the shape of k_pages {shape}")
     batch, width = table.shape
     if size < 8 or size > 32768 or size & (size - 1):
         raise RuntimeError(f"a page holds a power of two of positions from 8 to 32768, got {size}")
@@ -1135,7 +1146,10 @@ def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
         raise RuntimeError(f"table {tuple(table.shape)} and lens {tuple(lens.shape)} must have one row per sequence")
     if width * size > 1 << 30:
         raise RuntimeError(f"a sequence has at most 2^30 positions, the table has room for {width * size}")
-    ks, vs = _steps(k_pages), _steps(v_pages)
+    if k_pages.is_contiguous() and v_pages.is_contiguous():
+        ks = vs = kvh * size * dim, size * dim, dim
+    else:
+        ks, vs = _steps(k_pages), _steps(v_pages)
     return _lib.PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages, size,
                            table.data_ptr(), width)
 
@@ -1148,8 +1162,8 @@ def _attention_heads(q: torch.Tensor, kvh: int, dim: int) -> None:
         raise RuntimeError(f"{nh} query heads cannot share {kvh} key-value heads")
 
 
-def _need_starts(starts: torch.Tensor, batch: Optional[int]) -> int:
-    _need(starts, "starts", torch.int32, 1)
+def _need_starts(starts: torch.Tensor, like: torch.Tensor, batch: Optional[int]) -> int:
+    _need_plain(starts, "starts", like, torch.int32, 1)
     n = starts.shape[0]
     if n < 1 or (batch is not None and n != batch + 1):
         raise RuntimeError(f"starts must be [sequences + 1], got {tuple(starts.shape)}")
@@ -1176,10 +1190,9 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
     do the keys and values of a position past the table's width or in a page whose number is not the pool's.
     Where the table gives two positions of one call the same place, either's values may be left there."""
     _need_strided(qkv, "qkv", _HALF, 2)
-    cache = _paged_cache(k_pages, v_pages, table, lens, qkv.dtype)
-    _need(cos, "cos", torch.float32, 2)
-    _need(sin, "sin", torch.float32, 2)
-    _same_device(qkv, cos=cos, sin=sin, k_pages=k_pages, starts=starts)
+    cache = _paged_cache(k_pages, v_pages, table, lens, qkv)
+    _need_plain(cos, "cos", qkv, torch.float32, 2)
+    _need_plain(sin, "sin", qkv, torch.float32, 2)
     _, kvh, _, dim = k_pages.shape
     (rows, values), batch, (angles, half) = qkv.shape, lens.shape[0], cos.shape
     if dim % 16 or dim > 1024:
@@ -1193,12 +1206,12 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
     if cos.data_ptr() % 16 or sin.data_ptr() % 16:
         raise RuntimeError("cos and sin must be 16-byte aligned")
     if starts is not None:
-        _need_starts(starts, batch)
+        _need_starts(starts, qkv, batch)
     elif rows != batch:
         raise RuntimeError(f"without starts each of the {batch} sequences has one row, got {rows}")
     if not batch:
         return torch.zeros((rows, nh, dim), dtype=qkv.dtype, device=qkv.device)
-    q = torch.empty((rows, nh, dim), dtype=qkv.dtype, device=qkv.device)
+    q = qkv.new_empty((rows, nh, dim))
     if rows:
         with _dev(qkv):
             _lib.check(_lib.load().mp_paged_rope_append(
@@ -1222,14 +1235,13 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     heads share a key-value head.  Returns ``[sequences, nh, dim]``; a sequence with nothing to attend gives zeros.
     Long caches are split over workgroups and joined in a fixed order."""
     _need_strided(q, "q", _HALF, 3)
-    cache = _paged_cache(k_pages, v_pages, table, lens, q.dtype)
-    _same_device(q, k_pages=k_pages)
+    cache = _paged_cache(k_pages, v_pages, table, lens, q)
     b, nh, dim = q.shape
     kvh = k_pages.shape[1]
     _attention_heads(q, kvh, k_pages.shape[3])
     if lens.shape[0] != b:
         raise RuntimeError(f"q {tuple(q.shape)} and lens {tuple(lens.shape)} must have one row per sequence")
-    out = torch.empty((b, nh, dim), dtype=q.dtype, device=q.device)
+    out = q.new_empty((b, nh, dim))
     if not b:
         return out
     lib, qs = _lib.load(), _steps(q)
@@ -1255,15 +1267,16 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     _need_strided(q, "q", _HALF, 3)
     _need_strided(k, "k", q.dtype, 3)
     _need_strided(v, "v", q.dtype, 3)
-    batch = _need_starts(starts, None)
-    _same_device(q, k=k, v=v, starts=starts)
+    batch = _need_starts(starts, q, None)
+    if k.device != q.device or v.device != q.device:
+        _same_device(q, k=k, v=v)
     rows, nh, dim = q.shape
     if v.shape != k.shape or k.shape[0] != rows:
         raise RuntimeError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be alike, with a row for each of q {tuple(q.shape)}")
     _attention_heads(q, k.shape[1], k.shape[2])
     if not batch or not rows:
         return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
-    out, qs, ks, vs = torch.empty((rows, nh, dim), dtype=q.dtype, device=q.device), _steps(q), _steps(k), _steps(v)
+    out, qs, ks, vs = q.new_empty((rows, nh, dim)), _steps(q), _steps(k), _steps(v)
     lib, kvh = _lib.load(), k.shape[1]
     with _dev(q):
         wsb = lib.mp_prompt_workspace_bytes(rows, nh, kvh, dim, batch, rows)
@@ -1287,14 +1300,13 @@ def paged_prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     whole prompts, chunks of one, or prompts behind a shared prefix.  Returns ``[rows, nh, dim]``; rows that see nothing,
     those behind the last sequence among them, are zeros."""
     _need_strided(q, "q", _HALF, 3)
-    cache = _paged_cache(k_pages, v_pages, table, lens, q.dtype)
-    batch = _need_starts(starts, lens.shape[0])
-    _same_device(q, k_pages=k_pages, starts=starts)
+    cache = _paged_cache(k_pages, v_pages, table, lens, q)
+    batch = _need_starts(starts, q, lens.shape[0])
     rows, nh, dim = q.shape
     _attention_heads(q, k_pages.shape[1], k_pages.shape[3])
     if not batch or not rows:
         return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
-    out, qs = torch.empty((rows, nh, dim), dtype=q.dtype, device=q.device), _steps(q)
+    out, qs = q.new_empty((rows, nh, dim)), _steps(q)
     lib, (_, kvh, size, _) = _lib.load(), k_pages.shape
     with _dev(q):
         wsb = lib.mp_prompt_workspace_bytes(rows, nh, kvh, dim, batch, table.shape[1] * size)
@@ -1338,10 +1350,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[t
     for name, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
                         ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
         if t is not None or name == "u":
-            _need(t, name, dt, 1)
+            _need_plain(t, name, logits, dt, 1)
             if t.shape[0] != rows:
                 raise RuntimeError(f"{name} must have one value for each of the {rows} rows, got {tuple(t.shape)}")
-    _same_device(logits, u=u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
     logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
     if rows:
