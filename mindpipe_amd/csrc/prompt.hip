@@ -175,19 +175,41 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
   const int32_t *pg = PAGED ? table + static_cast<int64_t>(min(b, batch - 1)) * width : nullptr;
   // page of the tile's position `lane` (positions past the end: the last one's)
   const auto entry = [&](int tile) { return PAGED ? pg[min(tile + lane, end - 1) >> shift] : 0; };
+  // Over pages, byte offsets of this lane's pieces in a whole tile are kept, from its first row or that of its page: they are
+  // the same for all tiles, which start at multiples of kTile.  (1737 rows of 32 heads behind contexts 160 -> 151 us.  Packed
+  // rows, whose offsets take less to work out, lose by the registers, 466 -> 472 us at 64 / 8 heads, and so do heads of 256,
+  // 99 -> 120 us.)
+  constexpr bool kKept = PAGED && D < 256;
+  const int mask = PAGED ? (1 << shift) - 1 : 0;
+  uint32_t koff[kKept ? T::kLoads : 1], voff[kKept ? T::kLoads : 1];
+  if constexpr (kKept) {
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) {
+      const int r = (wave * T::kLoads + i) * 64 / T::kChunks + lane / T::kChunks, c = lane % T::kChunks;
+      koff[i] = 2 * ((r & mask) * static_cast<uint32_t>(krow) + 8 * T::k_chunk(r, c));
+      voff[i] = 2 * ((r & mask) * static_cast<uint32_t>(vrow) + 8 * T::v_chunk(r, c));
+    }
+  }
   const auto load = [&](int tile, int id, int8_t *stage) {
+    const bool whole = kKept && tile + kTile <= end;
     tile = min(tile, end - 1);  // past the last tile: rows that nothing reads
 #pragma unroll
     for (int i = 0; i < T::kLoads; ++i) {
-      const int slot = (wave * T::kLoads + i) * 64, r = slot / T::kChunks + lane / T::kChunks, c = lane % T::kChunks;
-      const int p = min(tile + r, end - 1);
+      const int slot = (wave * T::kLoads + i) * 64;
       // the rows of one load lie in one page
       const int64_t pid = PAGED ? __builtin_amdgcn_readlane(id, slot / T::kChunks) : 0;
-      const uint32_t off = PAGED ? p & ((1 << shift) - 1) : p - tile;
-      prompt_lds_load16(kb + (PAGED ? pid * kpage : tile * krow), 2 * (off * static_cast<uint32_t>(krow) + 8 * T::k_chunk(r, c)),
-                        stage + slot * 16);
-      prompt_lds_load16(vb + (PAGED ? pid * vpage : tile * vrow), 2 * (off * static_cast<uint32_t>(vrow) + 8 * T::v_chunk(r, c)),
-                        stage + T::kBytes + slot * 16);
+      if (whole) {
+        const int64_t at = tile & mask;
+        prompt_lds_load16(kb + pid * kpage + at * krow, koff[kKept ? i : 0], stage + slot * 16);
+        prompt_lds_load16(vb + pid * vpage + at * vrow, voff[kKept ? i : 0], stage + T::kBytes + slot * 16);
+      } else {
+        const int r = slot / T::kChunks + lane / T::kChunks, c = lane % T::kChunks, p = min(tile + r, end - 1);
+        const uint32_t off = PAGED ? p & mask : p - tile;
+        prompt_lds_load16(kb + (PAGED ? pid * kpage : tile * krow), 2 * (off * static_cast<uint32_t>(krow) + 8 * T::k_chunk(r, c)),
+                          stage + slot * 16);
+        prompt_lds_load16(vb + (PAGED ? pid * vpage : tile * vrow), 2 * (off * static_cast<uint32_t>(vrow) + 8 * T::v_chunk(r, c)),
+                          stage + T::kBytes + slot * 16);
+      }
     }
   };
 
