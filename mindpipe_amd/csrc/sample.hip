@@ -316,7 +316,7 @@ __device__ __forceinline__ int find_bin(SampleShared &s, const Target &t, uint32
 }
 
 struct RowCall {
-  float t, top, per;
+  float t, top, half, per;  // half of the maximum, bins per unit of half the distance to it (distances may pass fp32's range)
   int k;                   // 0: all
   bool by_p;
   float p, floor_p, u;
@@ -324,8 +324,8 @@ struct RowCall {
   float *logprob;
 };
 
-__device__ __forceinline__ int bin_of(float v, float top, float per) {
-  return static_cast<int>(fminf((top - v) * per, static_cast<float>(kBins - 1)));  // also of -inf
+__device__ __forceinline__ int bin_of(float v, const RowCall &c) {
+  return static_cast<int>(fminf(fmaf(-0.5f, v, c.half) * c.per, static_cast<float>(kBins - 1)));  // also of -inf
 }
 
 // The border inside a bin: `count` and `mass` lie before the bin, of it the values above from.key, and from.ties at it.
@@ -334,9 +334,9 @@ __device__ __forceinline__ Border find_border(SampleShared &s, X &x, const RowCa
                                               const Target &goal, uint32_t count, uint64_t mass, Border from) {
   const int tid = threadIdx.x;
   // keys that may fall into the bin: its edges, with a margin for the roundings of bin_of
-  const float near = bin / c.per, far = (bin + 1) / c.per;
-  const float hi_v = c.top - near * (1.f - 0x1p-20f) + 0x1p-21f * (fabsf(c.top) + near);
-  const float lo_v = c.top - far * (1.f + 0x1p-20f) - 0x1p-21f * (fabsf(c.top) + far);
+  const float near = bin / c.per, far = (bin + 1) / c.per, margin = 0x1p-21f * fabsf(c.half);
+  const float hi_v = 2.f * (c.half - near * (1.f - 0x1p-20f) + (margin + 0x1p-21f * near));
+  const float lo_v = 2.f * (c.half - far * (1.f + 0x1p-20f) - (margin + 0x1p-21f * far));
   const uint32_t top_key = sample_key<DT>(c.top);
   uint32_t high = bin > 0 && hi_v < c.top ? min(top_key, sample_key<DT>(hi_v) + 1) : top_key;
   uint32_t low = lo_v == lo_v ? max(from.key, sample_key<DT>(lo_v)) : from.key;
@@ -348,7 +348,7 @@ __device__ __forceinline__ Border find_border(SampleShared &s, X &x, const RowCa
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t key = sample_key<DT>(v[e]);
-        if (key < low || key > high || key <= from.key || bin_of(v[e], c.top, c.per) != bin) continue;
+        if (key < low || key > high || key <= from.key || bin_of(v[e], c) != bin) continue;
         atomicAdd(&s.count[(high - key) >> shift], 1u);
         if (goal.by_mass && shift > 0)
           atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[(high - key) >> shift]),
@@ -358,7 +358,7 @@ __device__ __forceinline__ Border find_border(SampleShared &s, X &x, const RowCa
     __syncthreads();
     if (from.ties && from.key >= low && from.key <= high) {
       const float v = sample_value<DT>(from.key);
-      if (tid == 0 && bin_of(v, c.top, c.per) == bin) {
+      if (tid == 0 && bin_of(v, c) == bin) {
         s.count[(high - from.key) >> shift] += from.ties;
         s.mass[(high - from.key) >> shift] += from.ties * weight(v);
       }
@@ -403,7 +403,7 @@ __device__ __forceinline__ uint64_t bin_weights(SampleShared &s, X &x, const Row
   const auto add = [&](int, const float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int bin = bin_of(v[e], c.top, c.per);
+      const int bin = bin_of(v[e], c);
       if (bin < kBins - 1 && (from.key == 0 || sample_key<DT>(v[e]) > from.key))
         atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[bin]), static_cast<unsigned long long>(weight(v[e])));
     }
@@ -413,7 +413,7 @@ __device__ __forceinline__ uint64_t bin_weights(SampleShared &s, X &x, const Row
   __syncthreads();
   if (from.ties) {
     const float v = sample_value<DT>(from.key);
-    if (tid == 0) s.mass[bin_of(v, c.top, c.per)] += from.ties * weight(v);
+    if (tid == 0) s.mass[bin_of(v, c)] += from.ties * weight(v);
     __syncthreads();
   }
   uint64_t own = 0, total;
@@ -431,7 +431,7 @@ __device__ __forceinline__ int find_bin_of_count(SampleShared &s, X &x, const Ro
   x.each([&](int, const float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int bin = bin_of(v[e], c.top, c.per);
+      const int bin = bin_of(v[e], c);
       if (bin < kBins - 1) atomicAdd(&s.count[bin], 1u);
     }
   });
@@ -618,7 +618,8 @@ __global__ __launch_bounds__(64 * W) void sample_kernel(const uint8_t *__restric
   }
   x.infinite = top == INFINITY;
   c.top = top = x.infinite ? 0.f : top;
-  c.per = static_cast<float>((kBins - 1) / (kReach * static_cast<double>(c.t)));
+  c.half = 0.5f * top;
+  c.per = static_cast<float>(fmin(2 * (kBins - 1) / (kReach * static_cast<double>(c.t)), 0x1p127));
   const double rate = 1.4426950408889634 / static_cast<double>(c.t);
   const Weight weight{s.table, static_cast<double>(top), rate};
 
@@ -631,7 +632,7 @@ __global__ __launch_bounds__(64 * W) void sample_kernel(const uint8_t *__restric
   bool bounded = c.k > 0 && c.k <= 64 * W && !x.infinite;
   if (bounded) {
     clear_bins<W>(s);
-    const int b = bin_of(mine, top, c.per);
+    const int b = bin_of(mine, c);
     if (b < kBins - 1) atomicAdd(&s.count[b], 1u);
     __syncthreads();
     bin = find_bin<W>(s, goal, count, mass);
@@ -649,7 +650,7 @@ __global__ __launch_bounds__(64 * W) void sample_kernel(const uint8_t *__restric
 
   // to be listed: the values of that bin and above, or else those not below min-p's floor; a few more do no harm, which
   // leaves a margin for the roundings.  (Where top-p sums weights up, min-p has to wait for it.)
-  const float reach = filtered ? (bin + 1) / c.per : c.t * -logf(fminf(c.floor_p, 1.0f));
+  const float reach = filtered ? 2.f * ((bin + 1) / c.per) : c.t * -logf(fminf(c.floor_p, 1.0f));
   const float least = top - reach * (1.f + 0x1p-10f) - 0x1p-10f * (c.t + 0x1p-10f * fabsf(top));
   bool list = (filtered || c.floor_p > 0.f) && least == least;
   if (list) {  // each wave its own, in index order

@@ -446,3 +446,19 @@ def test_gradients_are_refused():
     out = ops.prompt_attention(q, q[:, :1].detach(), q[:, 1:].detach(), _ints([0, 4]), 0.1)
     with pytest.raises((RuntimeError, NotImplementedError)):
         out.sum().backward()
+
+
+# ---------------------------------------------------------------- calls at the edges
+def test_sample_temperatures_of_every_size():
+    """Temperatures and logits whose quotients, or differences, pass the range of fp32."""
+    g = torch.Generator().manual_seed(51)
+    vocab = 2000
+    ties, small = torch.zeros(vocab), torch.randn(vocab, generator=g)
+    big = (torch.rand(vocab, generator=g) * 2 - 1) * 3e38
+    two = torch.where(torch.rand(vocab, generator=g) < 0.5, 3e38, -3e38)
+    x = torch.stack([ties, small, big, two]).to(DEV)
+    for t in (1e-44, 1e-38, 1e-30, 1e30, 5e37, 2e38, math.inf):
+        for k, p in ((0, 1.0), (1, 1.0), (7, 1.0), (1500, 1.0), (0, 0.6), (1500, 0.99)):
+            f = [torch.full((4,), a, device=DEV, dtype=torch.int32 if i == 1 else torch.float32) for i, a in enumerate((t, k, p))]
+            _say("temperature", t, k, p)
+            _check_sample(x, torch.tensor([0.99, 0.7, 0.6, 0.8], device=DEV), *f)
