@@ -73,9 +73,9 @@ struct PromptTile {
 struct PackedPlan {
   const int32_t *starts;
   int batch, rows, grp;
-  // offsets of a sequence; sequence `batch` is what lies behind the last one
-  __device__ __forceinline__ int first(int b) const { return min(max(starts[b], 0), rows); }
-  __device__ __forceinline__ int end(int b) const { return b < batch ? max(first(b), first(b + 1)) : rows; }
+  // offsets of a sequence; sequence `batch` is what lies behind the last one, and batch + 1 what lies before the first
+  __device__ __forceinline__ int first(int b) const { return b > batch ? 0 : min(max(starts[b], 0), rows); }
+  __device__ __forceinline__ int end(int b) const { return b < batch ? max(first(b), first(b + 1)) : b == batch ? rows : first(0); }
   __device__ __forceinline__ int operator()(int b, int per) const {
     return static_cast<int>((static_cast<int64_t>(end(b) - first(b)) * grp + per - 1) / per);
   }
@@ -146,9 +146,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
   const int kh = blockIdx.x % kvh, unit = blockIdx.x / kvh, sp = unit % splits;
   const PackedPlan plan{starts, batch, rows, grp};
   int b, part, count;
-  if (!attn_find_part(plan, batch + 1, kRows, tiles - 1 - unit / splits, b, part, count)) return;
+  if (!attn_find_part(plan, batch + 2, kRows, tiles - 1 - unit / splits, b, part, count)) return;
   const int first = plan.first(b), n = plan.end(b) - first, all = n * grp;
-  int len = 0;  // positions of the sequence, the new tokens' included; none behind the last sequence
+  int len = 0;  // positions of the sequence, the new tokens' included; none outside of the sequences
   if (b < batch) len = PAGED ? min(max(lens[b], 0), width << shift) : n;
   // positions seen by row r of the sequence, and by none of a wave's or workgroup's rows past their last
   const int before = len - n + 1;
@@ -425,8 +425,8 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const float *__restric
   }
 }
 
-// Row tiles of all sequences, at most: a part of one for each, and for the rows behind the last.
-inline int64_t prompt_tiles(int64_t rows, int64_t grp, int64_t batch) { return rows * grp / kRows + batch + 1; }
+// Row tiles of all sequences, at most: a part of one for each, and for the rows before the first and behind the last.
+inline int64_t prompt_tiles(int64_t rows, int64_t grp, int64_t batch) { return rows * grp / kRows + batch + 2; }
 
 // Splits of the positions (at most `reach`): so many that the workgroups come nearest to what the CUs hold at once (two each;
 // one of heads of 256), with four tiles of positions each at least.  16 rows behind 32768 positions (32 / 8 heads of 128):

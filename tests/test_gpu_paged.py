@@ -449,6 +449,26 @@ def test_gradients_are_refused():
 
 
 # ---------------------------------------------------------------- calls at the edges
+@pytest.mark.parametrize("paged", [False, True])
+def test_rows_before_the_first_sequence(paged):
+    """Rows before the first sequence are no sequence's, as those behind the last: zeros, over memory that held other values."""
+    rows, nh, kvh, dim = 300, 4, 2, 64
+    starts = torch.tensor([140, 150, 260], dtype=torch.int32)
+    q = torch.randn(rows, nh, dim, device=DEV, dtype=F16)
+    for _ in range(2):
+        torch.full((rows, nh, dim), math.nan, device=DEV, dtype=F16)  # what the allocator hands out next
+        if paged:
+            k, v, table, ln = _cache([30, 200], kvh, dim, 16, F16, 41)
+            got = _ops().paged_prompt_attention(q, k, v, table, ln, starts.to(DEV), 0.1)
+            want, tol = ref.paged_attention(q[140:260], k, v, table, ln, starts - 140, 0.1)
+        else:
+            k, v = torch.randn(2, rows, kvh, dim, device=DEV, dtype=F16).unbind()
+            got = _ops().prompt_attention(q, k, v, starts.to(DEV), 0.1)
+            want, tol = ref.prompt_attention(q[140:260], k[140:260], v[140:260], starts - 140, 0.1)
+        ref.check(got[140:260], want, tol)
+        assert not got[:140].any() and not got[260:].any()
+
+
 def test_sample_temperatures_of_every_size():
     """Temperatures and logits whose quotients, or differences, pass the range of fp32."""
     g = torch.Generator().manual_seed(51)
