@@ -450,7 +450,8 @@ int mp_paged_rope_append(const void *qkv, int64_t qkv_row, int64_t rows, int nh,
                          const int32_t *lens, const int32_t *starts, int64_t batch, int dtype, mp_stream_t stream);
 
 /* out [batch, nh, head_dim], dense = softmax(scale q k^T) v of one query per sequence over its first lens[b] positions
- * (held to what the table has room for), head_dim 64, 128 or 256, nh a multiple of kvh; nothing to attend gives zeros.
+ * (held to what the table has room for), head_dim 64, 128 or 256, nh a multiple of kvh, scale finite (with log2 e in it);
+ * nothing to attend gives zeros.
  * Weights and sums in fp32, the weights rounded to the dtype for the product with v.  Long caches are split over
  * workgroups and joined, always in the same order.  workspace: mp_paged_decode_workspace_bytes of the current device,
  * 16-byte aligned, not shared by calls that may run at once. */

@@ -6,6 +6,7 @@
 // sequences grow and can be captured into a graph.  A page number outside the pool is an empty page: nothing is
 // written to it, and its positions are not attended.
 #include <climits>
+#include <cmath>
 
 #include "attn_common.h"
 
@@ -316,7 +317,7 @@ extern "C" int mp_paged_rope_append(const void *qkv, int64_t qkv_row, int64_t ro
 
 extern "C" size_t mp_paged_decode_workspace_bytes(int64_t batch, int nh, int kvh, int head_dim) {
   const int cus = mp_cu_count();
-  if (batch <= 0 || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || cus <= 0) return 0;
+  if (batch <= 0 || batch > INT32_MAX || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || cus <= 0) return 0;
   const int64_t grp = nh / kvh, heads = kvh * mp_cdiv(grp, 16), per = grp < 16 ? grp : 16;
   return static_cast<size_t>(2 * decode_share(heads, head_dim) * heads * per) * (head_dim + 2) * sizeof(float) +
          static_cast<size_t>(batch * heads) * sizeof(int4);
@@ -327,6 +328,7 @@ extern "C" int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q
                                          int dtype, void *workspace, size_t workspace_bytes, mp_stream_t stream) {
   if (!q || !cache || !cache->k || !cache->v || !cache->table || !lens || !out || !workspace) return MP_ERR_ARG;
   if (dtype != MP_F16 && dtype != MP_BF16) return MP_ERR_DTYPE;
+  if (!std::isfinite(scale * kLog2e)) return MP_ERR_ARG;
   const int shift = page_shift(cache->page_size);
   if (batch < 0 || batch > INT32_MAX - 64 || nh < 1 || kvh < 1 || nh > 65536 || nh % kvh) return MP_ERR_SHAPE;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return MP_ERR_SHAPE;

@@ -459,7 +459,7 @@ struct PromptCall {
 template <bool PAGED>
 int prompt_launch(const PromptCall &c) {
   if (c.dtype != MP_F16 && c.dtype != MP_BF16) return MP_ERR_DTYPE;
-  if (!std::isfinite(c.scale)) return MP_ERR_ARG;
+  if (!std::isfinite(c.scale * kLog2e)) return MP_ERR_ARG;
   if (c.rows < 0 || c.rows > INT32_MAX || c.batch < 1 || c.batch > INT32_MAX - 64) return MP_ERR_SHAPE;
   if (c.nh < 1 || c.kvh < 1 || c.nh > 65536 || c.nh % c.kvh) return MP_ERR_SHAPE;
   if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return MP_ERR_SHAPE;
@@ -530,7 +530,9 @@ int prompt_launch(const PromptCall &c) {
 }  // namespace
 
 extern "C" size_t mp_prompt_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch, int64_t reach) {
-  if (rows <= 0 || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || batch <= 0 || reach <= 0 || mp_cu_count() <= 0) return 0;
+  if (rows <= 0 || rows > INT32_MAX || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || batch <= 0 || batch > INT32_MAX ||
+      reach <= 0 || mp_cu_count() <= 0)
+    return 0;
   const int splits = prompt_splits(rows, nh, kvh, head_dim, batch, reach);
   return splits > 1 ? static_cast<size_t>(splits) * rows * nh * (head_dim + 2) * sizeof(float) : 0;
 }

@@ -482,3 +482,58 @@ def test_sample_temperatures_of_every_size():
             f = [torch.full((4,), a, device=DEV, dtype=torch.int32 if i == 1 else torch.float32) for i, a in enumerate((t, k, p))]
             _say("temperature", t, k, p)
             _check_sample(x, torch.tensor([0.99, 0.7, 0.6, 0.8], device=DEV), *f)
+
+
+def test_workspaces_that_are_too_small_are_refused():
+    import ctypes
+    from mindpipe_amd import _lib
+    lib = _lib.load()
+    k, v, table, ln = _cache([400, 30], 2, 64, 16, F16, 61)
+    q = torch.randn(2, 4, 64, device=DEV, dtype=F16)
+    out, ws = torch.empty_like(q), torch.empty(1 << 24, device=DEV, dtype=torch.uint8)
+    cache = _lib.PAGES.pack(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], k.shape[0], 16, table.data_ptr(),
+                            table.shape[1])
+    starts, at = _ints([0, 1, 2]), torch.cuda.current_stream().cuda_stream
+    need = lib.mp_paged_decode_workspace_bytes(2, 4, 2, 64)
+    also = lib.mp_prompt_workspace_bytes(2, 4, 2, 64, 2, table.shape[1] * 16 * 40)
+    assert need > 0 and also > 0
+    decode = lambda scale, n: lib.mp_paged_decode_attention(  # noqa: E731
+        q.data_ptr(), 256, 64, 2, 4, 2, 64, cache, ln.data_ptr(), scale, out.data_ptr(), 0, ws.data_ptr(), n, at)
+    assert decode(0.1, need - 1) == 6 and decode(0.1, need) == 0
+    want, tol = ref.paged_attention(q, k, v, table, ln, None, 0.1)
+    torch.cuda.synchronize()
+    ref.check(out, want, tol)
+    for scale in (math.nan, math.inf, 3e38):
+        assert decode(scale, need) == 5
+    wide = table.repeat(1, 40)
+    cache = _lib.PAGES.pack(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], k.shape[0], 16, wide.data_ptr(),
+                            wide.shape[1])
+    prompt = lambda scale, n: lib.mp_paged_prompt_attention(  # noqa: E731
+        q.data_ptr(), 256, 64, 2, 4, 2, 64, cache, ln.data_ptr(), starts.data_ptr(), 2, scale, out.data_ptr(), 0, ws.data_ptr(),
+        n, at)
+    assert prompt(0.1, also - 1) == 6 and prompt(0.1, also) == 0 and prompt(3e38, also) == 5
+    torch.cuda.synchronize()
+    ref.check(out, want, tol)
+
+
+def test_calls_on_two_streams_at_once():
+    """Two streams with their own calls under way together: each gets what it gets alone."""
+    ops = _ops()
+    calls = []
+    for seed, lens in ((71, [3000, 10, 900]), (72, [50, 4000, 1])):
+        k, v, table, ln = _cache(lens, 2, 128, 16, BF16, seed)
+        q = torch.randn(3, 8, 128, device=DEV).to(BF16)
+        calls.append((q, k, v, table, ln))
+    starts = _ints([0, 1, 2, 3])
+    run = lambda c: (ops.paged_decode_attention(*c, 0.1), ops.paged_prompt_attention(*c, starts, 0.1))  # noqa: E731
+    alone = [run(c) for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(calls[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for g in got[i] for a, b in zip(g, alone[i]))
