@@ -369,12 +369,15 @@ class W4Decoder:
 
     def paged_cache(self, sequences: int, positions: int, page: int = 64) -> PagedKVCache:
         """A paged cache for this model: up to ``positions`` in all, ``max_len`` of one sequence."""
+        self._angles()  # before a step may be captured
         return PagedKVCache(self.cfg, sequences, positions, page, self.max_len, self.embed.device)
 
     def _angles(self):
         """cos / sin of every position in fp32, from angles in 64 bits (far positions lose theirs in 32)."""
         if getattr(self, "_cos_sin", None) is None:
             hd, device = self.cfg.head_dim, self.embed.device
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a step has to run, or paged_cache be called, before one is captured")
             inv = self.cfg.rope_theta ** (-torch.arange(0, hd, 2, device=device, dtype=torch.float64) / hd)
             angle = torch.outer(torch.arange(self.max_len, device=device, dtype=torch.float64), inv)
             self._cos_sin = angle.cos().float(), angle.sin().float()
@@ -387,6 +390,10 @@ class W4Decoder:
         ``starts`` each sequence has one.  A sequence without new tokens gets the logits of some other row.  Reads lengths
         and pages from device memory: a step without ``starts`` can be captured and replayed after each ``extend``."""
         cfg = self.cfg
+        if tokens.dim() != 1 or not tokens.numel():
+            raise ValueError(f"tokens must be packed in one dimension and hold one at least, got {tuple(tokens.shape)}")
+        if max(cache.length) > self.max_len:
+            raise RuntimeError(f"a sequence of {max(cache.length)} positions, the model has {self.max_len}")
         hd, nh, kvh = cfg.head_dim, cfg.heads, cfg.kv_heads
         scale, (cos, sin) = 1.0 / math.sqrt(hd), self._angles()
         x, delta = self.embed[tokens], None
@@ -404,7 +411,7 @@ class W4Decoder:
             hn, _, _, x = ops.add_rms_norm_quant(l["o"](att.view(-1, nh * hd)), x, l["ln2"], cfg.eps, quant=False)
             delta = l["down"](l["gate_up"].swiglu(hn))
         if starts is not None:  # the last row of each sequence
-            last = (starts[1:].long() - 1).clamp(min=0)
+            last = (starts[1:].long() - 1).clamp(0, len(tokens) - 1)
             delta, x = delta[last], x[last]
         return self.lm_head(ops.add_rms_norm_quant(delta, x, self.norm, cfg.eps, quant=False)[0])
 

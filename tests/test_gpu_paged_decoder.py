@@ -131,3 +131,31 @@ def test_cache_keeps_its_pages():
     starts = cache.extend([1, 1, 1])
     assert starts is None and cache.lens.tolist() == [1, 9, 2]
     assert cache.extend([0, 2, 0]).tolist() == [0, 0, 2, 2]
+
+
+def test_calls_that_are_refused():
+    from mindpipe_amd.decoder import PagedKVCache
+    model = _model(2, 2, max_len=20)
+    cache = PagedKVCache(model.cfg, 2, 100, 8)
+    graph, tokens = torch.cuda.CUDAGraph(), torch.zeros(2, device=DEV, dtype=torch.int64)
+    cache.extend([1, 1])
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            model.forward_paged(tokens, cache)
+    for bad in (tokens[:0], tokens.view(1, 2)):
+        with pytest.raises(ValueError, match="tokens"):
+            model.forward_paged(bad, cache)
+    with pytest.raises(RuntimeError):
+        model.forward_paged(tokens[:1], cache)
+    starts = cache.extend([20, 0])
+    with pytest.raises(RuntimeError, match="positions"):
+        model.forward_paged(torch.zeros(20, device=DEV, dtype=torch.int64), cache, starts)
+
+
+def test_fewer_tokens_than_the_offsets_say():
+    """What such a call returns is open; it reads no token that is not there."""
+    model = _model(2, 2)
+    cache = model.paged_cache(2, 100, 8)
+    starts = cache.extend([30, 5])
+    assert model.forward_paged(_tokens(10)[0], cache, starts).shape == (2, 512)
+    torch.cuda.synchronize()
