@@ -13,6 +13,11 @@
 // rule, are copied to LDS in index order, and the rest is done on them (on the whole row, where they are more than
 // kListed): the bin's values are counted into bins of neighbouring values down to single ones, which gives the border, a
 // value and how many of its ties; then weights are summed by spans of indexes and the token looked up.
+//
+// A row's bytes are read once where registers hold it (256 rows of 128256 bf16 are 66 MB, 10 us at the rate of a read), and the
+// weights bound it: some 30 instructions each, twice over the row with top-p (once for the sum that p is a share of, once for
+// the spans).  Those rows, by filter: none 57 us, top-k 33, min-p 30, top-k and top-p 38, top-p alone 105 (128256 values of
+// which more than the list holds are kept).
 #include "wave_scan.h"
 
 namespace {
@@ -22,7 +27,7 @@ constexpr int kMaxVocab = 1 << 19;
 constexpr int kSpan = 512;                     // indexes of one step of a wave: eight neighbours per lane
 constexpr int kMaxSpans = kMaxVocab / kSpan + kMaxWaves;  // the waves' counts are rounded up
 constexpr int kBins = 2048;
-constexpr int kTable = 1024;                   // 2^(j / 1024)
+constexpr int kTable = 1024;                   // 2^(44 + j / 1024)
 constexpr double kOne = 17592186044416.0;      // 2^44
 constexpr float kReach = 32.0f;                // e^-32 < 2^-46: past it a weight is no part of 2^-44
 
@@ -188,7 +193,7 @@ struct SampleList {
       }
     }
   }
-  template <class F>
+  template <bool RAW = false, class F>
   __device__ __forceinline__ void each(F f) { f(0, v); }
   template <class F>
   __device__ __forceinline__ void one(int, F f) const { f(0, v); }
@@ -215,27 +220,28 @@ __device__ __forceinline__ float sample_value(uint32_t key) {
 }
 
 struct Weight {
-  const double *table;  // LDS
-  double top, rate;     // the largest value, log2 e / T
-  // exp((v - top) / T) in units of 2^-44: 2^(k / 1024) from the table, and the rest of the exponent, below 2^-11, by a cubic
-  // (off by less than 2^-50)
+  const double *table;  // LDS: 2^(44 + j / 1024)
+  double top, rate;     // the largest value, 1024 log2 e / T
+  // exp((v - top) / T) in units of 2^-44: 2^(k / 1024) from the table, its whole powers added to the exponent, and the rest of
+  // the exponent, up to 2^-11, by a cubic (off by less than 2^-50).  -inf and NaN weigh 0, as what is below 2^-45 does.
   __device__ __forceinline__ uint64_t operator()(float v) const {
-    const double y = (static_cast<double>(v) - top) * rate;
-    const double magic = 1.5 * 0x1p42;  // a sum with it ends in 2^-10
-    const double t = y + magic;
-    const double r = y - (t - magic);
+    const double magic = 1.5 * 0x1p52;  // a sum with it is whole
+    const double y = fmax((static_cast<double>(v) - top) * rate, -64.0 * kTable);
+    const double t = y + magic, r = y - (t - magic);
     const int k = __double2loint(t);
-    const double q = r * fma(r, fma(r, 0.05550410866482158, 0.24022650695910072), 0.6931471805599453);
-    const double b = table[k & (kTable - 1)];
-    const double w = ldexp(fma(b, q, b), (k >> 10) + 44) + 0x1p52;  // below 2^45: the sum's last bits are the number
-    const uint64_t n = static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
-    return y > -46.0 ? n : 0;  // also -inf
+    const double q = r * fma(r, fma(r, 5.169222938345892e-11, 2.290978498068816e-07), 0.0006769015435155716);
+    const double e = table[k & (kTable - 1)];
+    const double b = __hiloint2double(__double2hiint(e) + ((k & ~(kTable - 1)) << 10), __double2loint(e));
+    const double w = fma(b, q, b) + 0x1p52;  // below 2^45: the sum's last bits are the number
+    return static_cast<uint64_t>(__double_as_longlong(w)) & 0xFFFFFFFFFFFFFull;
   }
 };
 
 struct Border {  // the kept: keys above `key`, and the first `ties` indexes at it
   uint32_t key, ties;
 };
+template <int DT>
+__device__ __forceinline__ float border_value(const Border &b) { return b.key ? sample_value<DT>(b.key) : -INFINITY; }
 
 // What a border is looked for by: so many values, or so much weight.
 struct Target {
@@ -344,9 +350,11 @@ __device__ __forceinline__ Border find_border(SampleShared &s, X &x, const RowCa
   for (;;) {
     const int shift = max(0, 21 - __clz((high - low) | 1));  // 11 bits of the range
     clear_bins<W>(s);
-    x.each([&](int, const float (&v)[8]) {
+    const float from_v = low ? sample_value<DT>(low) : -INFINITY, to_v = sample_value<DT>(high);
+    x.template each<true>([&](int, const float (&v)[8]) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
+        if (!(v[e] >= from_v && v[e] <= to_v)) continue;
         const uint32_t key = sample_key<DT>(v[e]);
         if (key < low || key > high || key <= from.key || bin_of(v[e], c) != bin) continue;
         atomicAdd(&s.count[(high - key) >> shift], 1u);
@@ -396,20 +404,20 @@ __device__ __forceinline__ Border find_border(SampleShared &s, X &x, const RowCa
 }
 
 // Weights by bins, of the values above from.key and from.ties at it; returns their sum.
-template <int DT, int W, bool RAW, class X>
+template <int DT, int W, class X>
 __device__ __forceinline__ uint64_t bin_weights(SampleShared &s, X &x, const RowCall &c, const Weight &weight, Border from) {
   const int tid = threadIdx.x;
   clear_bins<W>(s);
+  const float above = border_value<DT>(from);
   const auto add = [&](int, const float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int bin = bin_of(v[e], c);
-      if (bin < kBins - 1 && (from.key == 0 || sample_key<DT>(v[e]) > from.key))
+      if (bin < kBins - 1 && v[e] > above)
         atomicAdd(reinterpret_cast<unsigned long long *>(&s.mass[bin]), static_cast<unsigned long long>(weight(v[e])));
     }
   };
-  if constexpr (RAW) x.template each<true>(add);
-  else x.each(add);
+  x.template each<true>(add);
   __syncthreads();
   if (from.ties) {
     const float v = sample_value<DT>(from.key);
@@ -450,7 +458,7 @@ __device__ __forceinline__ void draw_token(SampleShared &s, X &x, const RowCall 
   if (filtered) {
     border = find_border<DT, W>(s, x, c, weight, bin, goal, count, mass, border);
     if (!goal.by_mass && c.by_p) {  // of the k largest, those down to p of their weight
-      const uint64_t total = bin_weights<DT, W, false>(s, x, c, weight, border);
+      const uint64_t total = bin_weights<DT, W>(s, x, c, weight, border);
       const Target part{true, 0, static_cast<double>(c.p) * static_cast<double>(total)};
       const int at = find_bin<W>(s, part, count, mass);
       border = find_border<DT, W>(s, x, c, weight, at, part, 0, mass, border);
@@ -460,19 +468,17 @@ __device__ __forceinline__ void draw_token(SampleShared &s, X &x, const RowCall 
   // kept weight of each span, the ties at the border counted apart
   const uint64_t floor_w =
       c.floor_p > 0.f ? static_cast<uint64_t>(fmin(static_cast<double>(c.floor_p), 1.0) * kOne + 0.5) : 0;
+  const float above = border_value<DT>(border);
   uint64_t tie_w = border.ties ? weight(sample_value<DT>(border.key)) : 0;
   if (tie_w < floor_w) tie_w = 0;
-  x.each([&](int ch, const float (&v)[8]) {
+  x.template each<true>([&](int ch, const float (&v)[8]) {
     uint64_t m = 0;
     uint32_t ties = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint32_t key = sample_key<DT>(v[e]);
-      ties += key == border.key ? 1 : 0;
-      if (key > border.key) {
-        const uint64_t w = weight(v[e]);
-        m += w >= floor_w ? w : 0;
-      }
+      const uint64_t w = weight(v[e]);
+      m += v[e] > above && w >= floor_w ? w : 0;
+      ties += v[e] == above ? 1 : 0;
     }
     if (__any(ties || m)) {
       m = wave_sum(m);
@@ -524,14 +530,13 @@ __device__ __forceinline__ void draw_token(SampleShared &s, X &x, const RowCall 
     uint64_t w[8], m = 0;
     uint32_t ties = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ties += sample_key<DT>(v[e]) == border.key ? 1 : 0;
+    for (int e = 0; e < 8; ++e) ties += v[e] == above ? 1 : 0;
     uint32_t before = ties_before + wave_scan(ties) - ties;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint32_t key = sample_key<DT>(v[e]);
-      w[e] = key > border.key ? weight(v[e]) : 0;
+      w[e] = v[e] > above ? weight(v[e]) : 0;
       if (w[e] < floor_w) w[e] = 0;
-      if (key == border.key) w[e] = before++ < border.ties ? tie_w : 0;
+      if (v[e] == above) w[e] = before++ < border.ties ? tie_w : 0;
       m += w[e];
     }
     uint64_t upto = run + wave_scan(m) - m, own = 0;
@@ -587,7 +592,7 @@ __global__ __launch_bounds__(64 * W) void sample_kernel(const uint8_t *__restric
   const float mine = top;  // this thread's
   top = mp_wave_max(top);
   if (lane == 0) s.top[wave] = top;
-  for (int i = tid; i < kTable; i += 64 * W) s.table[i] = exp2(static_cast<double>(i) / kTable);  // for the weights
+  for (int i = tid; i < kTable; i += 64 * W) s.table[i] = kOne * exp2(static_cast<double>(i) / kTable);  // for the weights
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < W; ++w) top = fmaxf(top, s.top[w]);
@@ -620,7 +625,7 @@ __global__ __launch_bounds__(64 * W) void sample_kernel(const uint8_t *__restric
   c.top = top = x.infinite ? 0.f : top;
   c.half = 0.5f * top;
   c.per = static_cast<float>(fmin(2 * (kBins - 1) / (kReach * static_cast<double>(c.t)), 0x1p127));
-  const double rate = 1.4426950408889634 / static_cast<double>(c.t);
+  const double rate = kTable * 1.4426950408889634 / static_cast<double>(c.t);
   const Weight weight{s.table, static_cast<double>(top), rate};
 
   // the bin that the border is in
@@ -643,7 +648,7 @@ __global__ __launch_bounds__(64 * W) void sample_kernel(const uint8_t *__restric
     if (bin == kBins - 1) goal.by_mass = true;  // all that weighs anything is among the k largest
   }
   if (bin == kBins - 1 && c.by_p) {
-    goal.mass = static_cast<double>(c.p) * static_cast<double>(bin_weights<DT, W, true>(s, x, c, weight, Border{0, 0}));
+    goal.mass = static_cast<double>(c.p) * static_cast<double>(bin_weights<DT, W>(s, x, c, weight, Border{0, 0}));
     bin = find_bin<W>(s, goal, count, mass);
   }
   const bool filtered = bin < kBins - 1;
@@ -720,12 +725,18 @@ extern "C" int mp_sample_tokens(const void *logits, int64_t stride, int64_t rows
   if (rows == 0) return MP_OK;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int n = static_cast<int>(vocab);
-#define MP_SAMPLE(DT) \
-  (n <= 8 * 8 * kSpan \
-       ? sample_launch<DT, 8, 8>(logits, stride, rows, n, u, temperature, top_k, top_p, min_p, tokens, logprobs, s) \
-       : sample_launch<DT, 16, 0>(logits, stride, rows, n, u, temperature, top_k, top_p, min_p, tokens, logprobs, s))
-  if (dtype == MP_F16) return MP_SAMPLE(MP_F16);
-  if (dtype == MP_BF16) return MP_SAMPLE(MP_BF16);
-  return MP_SAMPLE(MP_F32);
+  // Waves of a row, and whether their registers hold it.  Eight hold up to 32768 values; sixteen 131072 of 16 bits, and past that
+  // the row is read again in every pass.  256 rows of 128256 bf16, read again or held: no filter 57.9 / 56.1 us, top-k 36.6 /
+  // 32.6, top-p 114.7 / 104.6.  Rows of 32000 in sixteen waves or eight: one row, top-k 17.0 / 14.9 us (the eight have fewer
+  // counts to join); 256 rows 19.7 / 18.4, top-p 39.4 / 41.1.
+#define MP_SAMPLE(DT, CH)                                                                                                     \
+  (n <= 8 * 8 * kSpan                                                                                                         \
+       ? sample_launch<DT, 8, 8>(logits, stride, rows, n, u, temperature, top_k, top_p, min_p, tokens, logprobs, s)           \
+       : n <= 16 * CH * kSpan                                                                                                 \
+             ? sample_launch<DT, 16, CH>(logits, stride, rows, n, u, temperature, top_k, top_p, min_p, tokens, logprobs, s)   \
+             : sample_launch<DT, 16, 0>(logits, stride, rows, n, u, temperature, top_k, top_p, min_p, tokens, logprobs, s))
+  if (dtype == MP_F16) return MP_SAMPLE(MP_F16, 16);
+  if (dtype == MP_BF16) return MP_SAMPLE(MP_BF16, 16);
+  return MP_SAMPLE(MP_F32, 0);
 #undef MP_SAMPLE
 }
