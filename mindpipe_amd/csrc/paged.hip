@@ -34,7 +34,8 @@ __device__ __forceinline__ float at16(uint32_t w, int half) {
 
 // One workgroup per packed row and 256 of its 16-value pieces (a piece: eight pairs of a rotated head, or 16 values that
 // are copied).  Pairs are (2 i, 2 i + 1), or (i, i + rotary / 2).  Rotated in fp32 and rounded once.
-// Bound by its bytes: a row is read once and written once, the tables' rows come from the caches.
+// Bound by its bytes: a row is read once and written once, the tables' rows come from the caches.  9219 rows of 64 / 8 heads of
+// 128 in bf16, 382 MB: 70 us, 5.4 TB/s, what a large copy reaches.  A row per workgroup keeps the look for its sequence uniform.
 template <int DT, bool PAIRS>
 __global__ __launch_bounds__(256) void paged_rope_append_kernel(
     const uint16_t *__restrict__ qkv, int64_t qkv_row, int nh, int kvh, int dim, const float *__restrict__ cos_t,
@@ -102,6 +103,13 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(
 // is blocks w T / share .. (w + 1) T / share of T.  However ragged the lengths are, all have the same to read.  A sequence that lies
 // in several runs is joined from its parts: a workgroup leaves at most two, that of the sequence its run begins inside of
 // (slot 2 w) and that of the sequence its run ends inside of (slot 2 w + 1).
+//
+// The heads that share a key-value head are the columns of one matrix product, up to 16 in a wave, so K and V are read once for
+// all of them:  S = K . Q^T,  P = exp2(scale S - m),  O^T += V^T . P^T  (MFMA 16x16x32; attn_tile).  The four waves take the 32
+// positions of a block each, straight from memory to registers: nothing is read twice, so LDS would only delay it.  Bound by
+// those reads: 64 sequences of up to 8192 positions, 64 / 8 heads of 128 in bf16 (945 MB), 170 us, 5.5 TB/s, and two of 131071
+// (1.07 GB) 184 us, 5.8 TB/s, of the 6.4 TB/s that reads reach here; 200 short ones of 14 / 2 heads of 64 (75 MB), 20 us,
+// where a workgroup's first loads wait for its look at the lengths, the table and a page in turn.
 constexpr int kWaves = 4;
 constexpr int kBlock = 32 * kWaves;
 
@@ -117,7 +125,8 @@ struct DecodePlan {
   }
 };
 
-// Workgroups of a head: as many as fit the card at once (kRound of D per CU), and not more.
+// Workgroups of a head: as many as fit the card at once (decode_round of D per CU: their registers hold two tiles each), and not
+// more.  64 sequences as above: each sequence cut into parts of its own 188 us, equal runs 176, joins included.
 constexpr int decode_round(int dim) { return dim == 64 ? 4 : dim == 128 ? 2 : 1; }
 inline int decode_share(int64_t heads, int dim) {
   const int64_t n = static_cast<int64_t>(decode_round(dim)) * mp_cu_count() / heads;
@@ -209,7 +218,8 @@ __global__ __launch_bounds__(64 * kWaves, decode_round(D)) void paged_decode_ker
 }
 
 // The parts of a sequence's query head meet, in one workgroup: D / 4 threads take a part's output, 1024 / D parts at a time.
-// joins, of (sequence, head tile): the first run, how many runs, and whether the first run begins before the sequence.
+// joins, of (sequence, head tile): the first run, how many runs, and whether the first run begins before the sequence.  A launch
+// of its own, 3 to 7 us: joined by the last of its workgroups, a sequence would need fences and counters over the XCDs' L2s.
 template <int D, int DT>
 __global__ __launch_bounds__(256) void paged_decode_join_kernel(int heads, int kvh, int grp, const float *__restrict__ part_o,
                                                                 const float *__restrict__ part_ml,
