@@ -1170,7 +1170,7 @@ def _need_starts(starts: torch.Tensor, like: torch.Tensor, batch: Optional[int])
     return n - 1
 
 
-@_op("paged_rope_append", mutates=("k_pages", "v_pages"))
+@_op("paged_rope_append", "mindpipe_amd_serve", mutates=("k_pages", "v_pages"))
 def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                       table: torch.Tensor, lens: torch.Tensor, starts: Optional[torch.Tensor] = None,
                       pairs: bool = True) -> torch.Tensor:
@@ -1218,6 +1218,9 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
                 qkv.data_ptr(), qkv.stride(0) if rows > 1 else values, rows, nh, kvh, dim, cos.data_ptr(),
                 sin.data_ptr(), 2 * half, angles, int(pairs), q.data_ptr(), cache, lens.data_ptr(),
                 _ptr(starts), batch, _DT[qkv.dtype], _stream()), "mp_paged_rope_append")
+        for t in (k_pages, v_pages):
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)  # a backward that saved the pool notices
     return q
 
 
@@ -1227,7 +1230,7 @@ def _(qkv, cos, sin, k_pages, v_pages, table, lens, starts=None, pairs=True):
     return qkv.new_empty((qkv.shape[0], qkv.shape[1] // dim - 2 * k_pages.shape[1], dim))
 
 
-@_op("paged_decode_attention")
+@_op("paged_decode_attention", "mindpipe_amd_serve")
 def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
                            lens: torch.Tensor, scale: float) -> torch.Tensor:
     """Attention of one query per sequence, ``q [sequences, nh, dim]`` (fp16 or bf16, ``dim`` 64, 128 or 256), over the
@@ -1259,7 +1262,7 @@ def _(q, k_pages, v_pages, table, lens, scale):
     return q.new_empty(q.shape)
 
 
-@_op("prompt_attention")
+@_op("prompt_attention", "mindpipe_amd_serve")
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, scale: float) -> torch.Tensor:
     """Causal attention of packed prompts: rows ``starts[b] .. starts[b + 1] - 1`` (int32 ``[sequences + 1]``, ascending) of
     ``q [rows, nh, dim]`` and ``k``, ``v [rows, kvh, dim]`` are sequence b (fp16 or bf16, ``dim`` 64, 128 or 256; views of a
@@ -1292,7 +1295,7 @@ def _(q, k, v, starts, scale):
     return q.new_empty(q.shape)
 
 
-@_op("paged_prompt_attention")
+@_op("paged_prompt_attention", "mindpipe_amd_serve")
 def paged_prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
                            lens: torch.Tensor, starts: torch.Tensor, scale: float) -> torch.Tensor:
     """Causal attention of packed new tokens over a paged cache that holds them (``paged_rope_append``): the rows of
@@ -1322,7 +1325,7 @@ def _(q, k_pages, v_pages, table, lens, starts, scale):
     return q.new_empty(q.shape)
 
 
-@_op("sample_tokens")
+@_op("sample_tokens", "mindpipe_amd_serve")
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
                   top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
                   min_p: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -422,13 +422,13 @@ def test_registered_operators():
     cos, sin = torch.rand(30, 32, device=DEV), torch.rand(30, 32, device=DEV)
     qkv, q = torch.randn(2, 4 * 64, device=DEV, dtype=F16), torch.randn(2, 2, 64, device=DEV, dtype=F16)
     tests = ("test_schema", "test_faketensor", "test_autograd_registration")
-    torch.library.opcheck(torch.ops.mindpipe_amd.paged_rope_append.default, (qkv, cos, sin, k, v, table, ln), test_utils=tests)
-    torch.library.opcheck(torch.ops.mindpipe_amd.paged_decode_attention.default, (q, k, v, table, ln, 0.1), test_utils=tests)
-    torch.library.opcheck(torch.ops.mindpipe_amd.paged_prompt_attention.default,
+    torch.library.opcheck(torch.ops.mindpipe_amd_serve.paged_rope_append.default, (qkv, cos, sin, k, v, table, ln), test_utils=tests)
+    torch.library.opcheck(torch.ops.mindpipe_amd_serve.paged_decode_attention.default, (q, k, v, table, ln, 0.1), test_utils=tests)
+    torch.library.opcheck(torch.ops.mindpipe_amd_serve.paged_prompt_attention.default,
                           (q, k, v, table, ln, _ints([0, 1, 2]), 0.1), test_utils=tests)
-    torch.library.opcheck(torch.ops.mindpipe_amd.prompt_attention.default, (q, q[:, :1], q[:, 1:], _ints([0, 2]), 0.1),
+    torch.library.opcheck(torch.ops.mindpipe_amd_serve.prompt_attention.default, (q, q[:, :1], q[:, 1:], _ints([0, 2]), 0.1),
                           test_utils=tests)
-    torch.library.opcheck(torch.ops.mindpipe_amd.sample_tokens.default, (qkv, torch.rand(2, device=DEV)), test_utils=tests)
+    torch.library.opcheck(torch.ops.mindpipe_amd_serve.sample_tokens.default, (qkv, torch.rand(2, device=DEV)), test_utils=tests)
 
     def f(qkv, k, v):
         q = ops.paged_rope_append(qkv, cos, sin, k, v, table, ln)
@@ -537,3 +537,21 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(a, b) for g in got[i] for a, b in zip(g, alone[i]))
+
+
+def test_append_tells_autograd_of_the_pools():
+    """A backward that saved a pool before an append notices; tensors of inference mode, which keep no count, are taken."""
+    ops = _ops()
+    k, v, table, ln = _cache([20, 5], 1, 64, 8, F16, 81)
+    cos, sin = torch.rand(30, 32, device=DEV), torch.rand(30, 32, device=DEV)
+    qkv = torch.randn(2, 4 * 64, device=DEV, dtype=F16)
+    w = torch.ones_like(k, requires_grad=True)
+    y = (w * k).sum()
+    ops.paged_rope_append(qkv, cos, sin, k, v, table, ln)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    want = k.clone()
+    with torch.inference_mode():
+        k2, v2 = k.clone(), v.clone()
+        q = ops.paged_rope_append(qkv, cos, sin, k2, v2, table, ln)
+        assert torch.equal(k2, want) and q.shape == (2, 2, 64)
