@@ -555,3 +555,36 @@ def test_append_tells_autograd_of_the_pools():
         k2, v2 = k.clone(), v.clone()
         q = ops.paged_rope_append(qkv, cos, sin, k2, v2, table, ln)
         assert torch.equal(k2, want) and q.shape == (2, 2, 64)
+
+
+def test_sequences_that_share_pages():
+    """Two sequences and one of them twice over the same first pages, as behind a common prefix; decode and chunks."""
+    k, v, table, ln = _cache([200, 70, 40], 2, 128, 16, F16, 91)
+    table[1, :4] = table[0, :4]
+    table[2] = table[0]
+    starts = _ints([0, 20, 21, 45])
+    q = torch.randn(45, 6, 128, device=DEV, dtype=F16)
+    got = _ops().paged_prompt_attention(q, k, v, table, ln, starts, 0.09)
+    ref.check(got, *ref.paged_attention(q, k, v, table, ln, starts, 0.09))
+    got = _ops().paged_decode_attention(q[:3], k, v, table, ln, 0.09)
+    ref.check(got, *ref.paged_attention(q[:3], k, v, table, ln, None, 0.09))
+
+
+def test_chunks_over_far_pages_and_repeated_keys():
+    """Chunks over pools whose offsets pass 32 bits; prompts whose keys and values are one row, or one head, repeated."""
+    pages = (1 << 31) // (8 * 128 * 128) + 40
+    k = torch.empty(pages, 8, 128, 128, device=DEV, dtype=BF16)
+    v = torch.empty_like(k)
+    table = _ints([[pages - 1, 3, pages - 20, pages // 2 + 7]])
+    few = table[0].long()
+    k[few], v[few] = (torch.randn(4, 8, 128, 128, device=DEV).to(BF16) for _ in range(2))
+    q = torch.randn(30, 16, 128, device=DEV).to(BF16)
+    got = _ops().paged_prompt_attention(q, k, v, table, _ints([450]), _ints([0, 30]), 0.09)
+    ref.check(got, *ref.paged_attention(q, k[few], v[few], _ints([[0, 1, 2, 3]]), _ints([450]), _ints([0, 30]), 0.09))
+    del k, v
+    starts = torch.tensor([0, 70, 100], dtype=torch.int32)
+    q, one, head = torch.randn(100, 4, 64, device=DEV, dtype=F16), torch.randn(1, 2, 64, device=DEV, dtype=F16), \
+        torch.randn(100, 1, 64, device=DEV, dtype=F16)
+    for kv in (one.expand(100, 2, 64), head.expand(100, 2, 64)):
+        got = _ops().prompt_attention(q, kv, kv, starts.to(DEV), 0.1)
+        ref.check(got, *ref.prompt_attention(q, kv, kv, starts, 0.1))
