@@ -13,10 +13,10 @@
 // swizzled in 16-byte chunks so that neither reads a bank twice at a time.
 //
 // Bound by the matrix cores and the vector units in turn: three sequences of 1933 to 4096 tokens, 64 / 8 heads of 128 in bf16
-// (420 GFLOP that are seen), 463 us, 0.91 PFLOP/s, where a large matrix product reaches 1.37.  Matrix instructions are 45% of
+// (420 GFLOP that are seen), 448 us, 0.94 PFLOP/s, where a large matrix product reaches 1.37.  Matrix instructions are 47% of
 // the time, the softmax's another 55%; the two waves of a SIMD cover part of it.  32 rows a wave, so that an operand from LDS
 // serves 32 x 32 x 16 products (with 16, straight from memory, 2374 us).  Eight waves in two groups that take turns: 716 us; the
-// next tile's scores ahead of a tile's weights in one wave, or wave priorities: 463 to 516 us.
+// next tile's scores ahead of a tile's weights in one wave, or wave priorities: no faster.
 //
 // Few rows leave most CUs without a workgroup: then the positions are split over `splits` workgroups, which leave their sums,
 // maxima and outputs, unnormalised, in the workspace, and a second launch joins them.
@@ -29,6 +29,7 @@
 namespace {
 
 constexpr int kWaves = 4, kRows = 32 * kWaves;
+constexpr int kTile = 64;  // positions
 
 typedef short as4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) as4_t *lds_as4;
@@ -40,11 +41,8 @@ __device__ __forceinline__ void prompt_lds_load16(const uint16_t *base, uint32_t
       mp_rsrc(base, 0x80000000u), reinterpret_cast<__attribute__((address_space(3))) void *>(reinterpret_cast<uintptr_t>(lds)),
       16, offset, 0, 0, 0);
 }
-// At most N of the wave's loads still on their way, every wave so far.
-template <int N>
-__device__ __forceinline__ void prompt_wait() {
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
-}
+// The wave's loads have landed, and every wave is so far.
+__device__ __forceinline__ void prompt_wait() { asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory"); }
 // Four rows' values of one column: lane i of 16 gives 8 bytes of row i / 4 and gets column i of the four rows.
 __device__ __forceinline__ as4_t prompt_read_tr(const __restrict__ lds_as4 p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
 __device__ __forceinline__ uint2 prompt_read_tr(const int8_t *lds) {
@@ -62,12 +60,10 @@ __device__ __forceinline__ f16_t prompt_mfma(uint4 a, uint4 b, f16_t c) {
 
 template <int D>
 struct PromptTile {
-  static constexpr int kTile = D == 256 ? 32 : 64;  // positions
-  static constexpr int kChunks = D / 8;             // of 16 bytes in a row
-  static constexpr int kBytes = kTile * D * 2;      // of K or of V
+  static constexpr int kChunks = D / 8;         // of 16 bytes in a row
+  static constexpr int kBytes = kTile * D * 2;  // of K or of V
+  static constexpr int kStage = 2 * kBytes;     // of both; two stages, 32 / 64 / 128 KB
   static constexpr int kLoads = kBytes / 1024 / kWaves;
-  // Stages of K and V.  One workgroup a CU (D = 256) has nothing else to do while a tile is on its way: three tiles are.
-  static constexpr int kStages = D == 256 ? 4 : 2;
   // LDS chunk of a row's chunk c (and back).  K is read by 16 rows at a time in one column of chunks, V by four rows at a time
   // in four columns; 256 bytes are all banks.
   static __device__ __forceinline__ int k_chunk(int row, int c) { return c ^ (D == 64 ? (row >> 1) & 7 : row & 15); }
@@ -146,8 +142,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
     const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, int tiles, float scale2,
     uint32_t flip, int splits, float *__restrict__ parts, uint16_t *__restrict__ out) {
   using T = PromptTile<D>;
-  constexpr int kTile = T::kTile, kStage = 2 * T::kBytes, kS = kTile / 32;
-  extern __shared__ __attribute__((aligned(1024))) int8_t prompt_smem[];  // kStages of K and V
+  constexpr int kStage = T::kStage, kS = kTile / 32;
+  extern __shared__ __attribute__((aligned(1024))) int8_t prompt_smem[];  // two stages of K and V
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i32 = lane & 31, h = lane >> 5;
   const int kh = blockIdx.x % kvh, unit = blockIdx.x / kvh, sp = unit % splits;
   const PackedPlan plan{starts, batch, rows, grp};
@@ -184,7 +180,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
   // Over pages, byte offsets of this lane's pieces in a whole tile are kept, from its first row or that of its page: they are
   // the same for all tiles, which start at multiples of kTile.  (1737 rows of 32 heads behind contexts 160 -> 151 us.  Packed
   // rows, whose offsets take less to work out, lose by the registers, 466 -> 472 us at 64 / 8 heads, and so do heads of 256,
-  // 99 -> 120 us.)
+  // 92 -> 102 us.)
   constexpr bool kKept = PAGED && D < 256;
   const int mask = PAGED ? (1 << shift) - 1 : 0;
   uint32_t koff[kKept ? T::kLoads : 1], voff[kKept ? T::kLoads : 1];
@@ -230,33 +226,24 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
     there = ~uint64_t(0);
     if constexpr (!PAGED) return 0;
     const bool ok = id >= 0 && id < pages;
-    there = __ballot(ok || lane >= kTile);
+    there = __ballot(ok);
     return ok ? id : 0;
   };
-  // there[i]: which positions of the i-th tile from here exist
-  constexpr int kAhead = T::kStages - 1, kOneTile = 2 * T::kLoads + (PAGED ? 1 : 0);
-  uint64_t there[kAhead + 1];
-  int next_entry = 0, fill = 0, stage = 0;
+  uint64_t there = 0;  // which positions of the tile that is on its way exist
+  int next_entry = 0, stage = 0;
   if (end > from) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      load(from + i * kTile, fix(entry(from + i * kTile), there[i]), prompt_smem + i * kStage);
-      fill = i + 1;
-    }
-    next_entry = entry(from + kAhead * kTile);
+    load(from, fix(entry(from), there), prompt_smem);
+    next_entry = entry(from + kTile);
   }
   uint32_t odd = 0;  // an infinity or NaN in V where only some of the wave's rows see it
   for (int tile = from; tile < end; tile += kTile) {
     // this tile's loads have landed, every wave's, and the stage of the last tile has been read
-    prompt_wait<(kAhead - 1) * kOneTile>();
-    load(tile + kAhead * kTile, fix(next_entry, there[kAhead]), prompt_smem + fill * kStage);
-    next_entry = entry(tile + (kAhead + 1) * kTile);
-    const int8_t *ks = prompt_smem + stage * kStage, *vs = ks + T::kBytes;
-    stage = stage + 1 == T::kStages ? 0 : stage + 1;
-    fill = fill + 1 == T::kStages ? 0 : fill + 1;
-    const uint64_t ok = there[0];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) there[i] = there[i + 1];
+    prompt_wait();
+    const uint64_t ok = there;
+    load(tile + kTile, fix(next_entry, there), prompt_smem + (kStage - stage));
+    next_entry = entry(tile + 2 * kTile);
+    const int8_t *ks = prompt_smem + stage, *vs = ks + T::kBytes;
+    stage = kStage - stage;
     if (tile >= wend) continue;  // rows that see nothing more load for the others
     f16_t s[kS];
 #pragma unroll
@@ -264,7 +251,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
     {
-      constexpr int kC = D / 16, kAheadK = 2;  // pairs of operands that are read before they are used
+      constexpr int kC = D / 16, kAheadK = 1;  // pairs of operands that are read before they are used
       i4_t kf[kAheadK + 1][kS];
       const auto keys = [&](int c) {
 #pragma unroll
@@ -317,25 +304,27 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
     }
     const float base = m == -INFINITY ? 0.f : m - kRaise<DT>;
     // O^T: step c of 16 positions, whose weights are those of positions 16 c + 4 h + {0..3, 8..11}: s[c / 2][8 (c & 1) ..].  The
-    // next step's weights are made, and its V read, between the matrix instructions of this one.
+    // next step's weights are made between the matrix instructions of this one.
     constexpr int kSteps = kTile / 16, kD = D / 32;
     const int trow = 4 * h + ((lane & 15) >> 2), tcol = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
     uint32_t w[2][4];
-    uint4 vf[2][kD];
+    constexpr int kAheadV = 2;  // operands of V that are read before they are used (1: 461 -> 470 us, 4: 463, heads of 256 92 -> 101 and 94)
+    uint4 vf[kAheadV + 1];
     const auto weight = [&](int c, int i) {
       const int r = 8 * (c & 1) + 2 * i;
       w[c & 1][i] = attn_pack2<DT>(__builtin_amdgcn_exp2f(fmaf(s[c / 2][r], scale2, -base)),
                                    __builtin_amdgcn_exp2f(fmaf(s[c / 2][r + 1], scale2, -base)));
       l = attn_add2<DT>(w[c & 1][i], l);
     };
-    const auto values = [&](int c, int d) {
+    const auto values = [&](int j) {
+      const int c = j / kD, d = j % kD;
       const int ra = 16 * c + trow, rb = ra + 8;
       const uint2 lo = prompt_read_tr(vs + ra * (D * 2) + 16 * T::v_chunk(ra, 4 * d + tcol) + 8 * (lane & 1));
       const uint2 hi = prompt_read_tr(vs + rb * (D * 2) + 16 * T::v_chunk(rb, 4 * d + tcol) + 8 * (lane & 1));
-      vf[c & 1][d] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      vf[j % (kAheadV + 1)] = make_uint4(lo.x, lo.y, hi.x, hi.y);
     };
 #pragma unroll
-    for (int d = 0; d < kD; ++d) values(0, d);
+    for (int j = 0; j < kAheadV; ++j) values(j);
 #pragma unroll
     for (int i = 0; i < 4; ++i) weight(0, i);
 #pragma unroll
@@ -344,9 +333,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
 #pragma unroll
       for (int d = 0; d < kD; ++d) {
         __builtin_amdgcn_sched_barrier(0);
-        o[d] = prompt_mfma<DT>(vf[c & 1][d], wf, o[d]);
+        const int j = c * kD + d;
+        o[d] = prompt_mfma<DT>(vf[j % (kAheadV + 1)], wf, o[d]);
+        if (j + kAheadV < kSteps * kD) values(j + kAheadV);
         if (c + 1 < kSteps) {
-          values(c + 1, d);
 #pragma unroll
           for (int i = 4 * d / kD; i < 4 * (d + 1) / kD; ++i) weight(c + 1, i);
         }
@@ -437,7 +427,7 @@ inline int64_t prompt_tiles(int64_t rows, int64_t grp, int64_t batch) { return r
 // Splits of the positions (at most `reach`): so many that the workgroups come nearest to what the CUs hold at once (two each;
 // one of heads of 256), with four tiles of positions each at least.  16 rows behind 32768 positions (32 / 8 heads of 128):
 // 666 us whole, 341 / 176 / 95 us in 2 / 4 / 8 splits, 40 us in the 32 that this gives; 1068 rows of 16 / 4 heads of 256
-// (144 workgroups): 143 us whole, 108 in 2, 113 in 3; 1737 rows of 32 heads of 128 (480 workgroups): 180 whole, 197 in 2, the
+// (144 workgroups): 117 us whole, 91 in 2, 93 in 3; 1737 rows of 32 heads of 128 (480 workgroups): 149 whole, 168 in 2, the
 // join reads and writes more than idle CUs cost.
 inline int prompt_splits(int64_t rows, int64_t nh, int64_t kvh, int64_t dim, int64_t batch, int64_t reach) {
   const int64_t slots = (dim == 256 ? 1 : 2) * mp_cu_count(), blocks = prompt_tiles(rows, nh / kvh, batch) * kvh;
@@ -494,13 +484,13 @@ int prompt_launch(const PromptCall &c) {
   const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
   const float scale2 = fmaxf(fabsf(c.scale) * kLog2e, FLT_MIN);
 #define MP_PROMPT(D, DT)                                                                                                  \
-  if (2 * PromptTile<D>::kStages * PromptTile<D>::kBytes > 64 * 1024 &&                                                   \
+  if (2 * PromptTile<D>::kStage > 64 * 1024 &&                                                                            \
       hipFuncSetAttribute(reinterpret_cast<const void *>(prompt_attention_kernel<D, DT, PAGED>),                          \
                           hipFuncAttributeMaxDynamicSharedMemorySize,                                                     \
-                          2 * PromptTile<D>::kStages * PromptTile<D>::kBytes) != hipSuccess)                              \
+                          2 * PromptTile<D>::kStage) != hipSuccess)                                                       \
     return MP_ERR_HIP;                                                                                                    \
   hipLaunchKernelGGL((prompt_attention_kernel<D, DT, PAGED>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),     \
-                     2 * PromptTile<D>::kStages * PromptTile<D>::kBytes, c.stream,                                                                 \
+                     2 * PromptTile<D>::kStage, c.stream,                                                                 \
                      static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(c.k), c.kpage,  \
                      c.khead, c.krow, static_cast<const uint16_t *>(c.v), c.vpage, c.vhead, c.vrow, c.pages, c.shift,     \
                      c.table, c.width, c.lens, c.starts, static_cast<int>(c.batch), static_cast<int>(c.rows), c.kvh,      \
