@@ -472,7 +472,7 @@ int mp_prompt_attention(const void *q, int64_t q_row, int64_t q_head, const void
                         size_t workspace_bytes, mp_stream_t stream);
 
 /* The same with keys and values in the cache: the packed rows of sequence b are its last positions of lens[b] (as
- * mp_paged_rope_append puts them there), and each sees the positions up to its own. */
+ * mp_paged_rope_append puts them there), and each sees the positions up to its own that the table has room for. */
 int mp_paged_prompt_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh, int head_dim,
                               const mp_pages *cache, const int32_t *lens, const int32_t *starts, int64_t batch,
                               float scale, void *out, int dtype, void *workspace, size_t workspace_bytes,

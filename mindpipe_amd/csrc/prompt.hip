@@ -91,8 +91,8 @@ struct PromptRows {
   const uint16_t *q;
   uint16_t *out;
   int64_t q_row, q_head, out_row;
-  int all, grp, before;  // rows, heads of a token, positions that row 0 sees
-  int from, to;          // positions that are looked at
+  int all, grp, before, room;  // rows, heads of a token, positions up to row 0's own, positions there are
+  int from, to;                // positions that are looked at
   float scale2;
   float *part;           // [tokens, heads][dim + 2], row stride part_row; null: outputs are final
   int64_t part_row;
@@ -101,7 +101,7 @@ template <int D, int DT, bool PAGED>
 __device__ __attribute__((noinline)) void prompt_rows16(const PromptRows<PAGED> &p, int r0) {
   const int lane = threadIdx.x & 63, i16 = lane & 15, j = lane >> 4, at = min(r0 + i16, p.all - 1);
   const int token = at / p.grp, head = at - token * p.grp;
-  const auto seen = [&](int r) { return max(p.before + min(r, p.all - 1) / p.grp, 0); };
+  const auto seen = [&](int r) { return max(min(p.before + min(r, p.all - 1) / p.grp, p.room), 0); };
   const int full = __builtin_amdgcn_readfirstlane(seen(r0)), end = __builtin_amdgcn_readfirstlane(seen(r0 + 15));
   uint4 qf[D / 32];
   const uint16_t *qp = p.q + token * p.q_row + head * p.q_head + 8 * j;
@@ -150,11 +150,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
   int b, part, count;
   if (!attn_find_part(plan, batch + 2, kRows, tiles - 1 - unit / splits, b, part, count)) return;
   const int first = plan.first(b), n = plan.end(b) - first, all = n * grp;
-  int len = 0;  // positions of the sequence, the new tokens' included; none outside of the sequences
-  if (b < batch) len = PAGED ? min(max(lens[b], 0), width << shift) : n;
+  // positions of the sequence, the new tokens' included, and those that there is room for; none outside of the sequences.  A
+  // row's own position goes by the length, as the append's does: a sequence longer than its table keeps the places of its rows.
+  int len = 0, room = 0;
+  if (b < batch) {
+    len = PAGED ? max(lens[b], 0) : n;
+    room = PAGED ? width << shift : n;
+  }
   // positions seen by row r of the sequence, and by none of a wave's or workgroup's rows past their last
   const int before = len - n + 1;
-  const auto seen = [&](int r) { return b < batch ? max(before + min(r, all - 1) / grp, 0) : 0; };
+  const auto seen = [&](int r) { return max(min(before + min(r, all - 1) / grp, room), 0); };
   const int r0 = part * kRows + wave * 32, at = r0 + i32;
   const bool row = at < all;
   const int token = row ? at / grp : 0, head = kh * grp + (row ? at - token * grp : 0);
@@ -348,7 +353,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
   if (__any(odd)) {
     // 0 times an infinity is no zero: these rows once more, with what they do not see left out one position at a time
     PromptRows<PAGED> p;
-    if constexpr (PAGED) p.src = {kb, vb, kpage, krow, vpage, vrow, pg, shift, (1 << shift) - 1, pages, (len - 1) >> shift};
+    if constexpr (PAGED) p.src = {kb, vb, kpage, krow, vpage, vrow, pg, shift, (1 << shift) - 1, pages, (end - 1) >> shift};
     else p.src = {kb, vb, krow, vrow, n - 1};
     p.q = q + first * q_row + kh * grp * q_head;
     p.q_row = q_row;
@@ -358,6 +363,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
     p.all = all;
     p.grp = grp;
     p.before = before;
+    p.room = room;
     p.from = from;
     p.to = end;
     p.scale2 = flip ? -scale2 : scale2;

@@ -1299,9 +1299,9 @@ def _(q, k, v, starts, scale):
 def paged_prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
                            lens: torch.Tensor, starts: torch.Tensor, scale: float) -> torch.Tensor:
     """Causal attention of packed new tokens over a paged cache that holds them (``paged_rope_append``): the rows of
-    sequence b in ``q [rows, nh, dim]`` are its last positions of ``lens[b]``, and each sees the positions up to its own:
-    whole prompts, chunks of one, or prompts behind a shared prefix.  Returns ``[rows, nh, dim]``; rows that see nothing,
-    those behind the last sequence among them, are zeros."""
+    sequence b in ``q [rows, nh, dim]`` are its last positions of ``lens[b]``, and each sees the positions up to its own that
+    the table has room for: whole prompts, chunks of one, or prompts behind a shared prefix.  Returns ``[rows, nh, dim]``;
+    rows that see nothing, those behind the last sequence among them, are zeros."""
     _need_strided(q, "q", _HALF, 3)
     cache = _paged_cache(k_pages, v_pages, table, lens, q)
     batch = _need_starts(starts, q, lens.shape[0])

@@ -62,7 +62,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts, scale):
             k, there = gather(k_pages, table[b], length, h)
             v, _ = gather(v_pages, table[b], length, h)
             for j in range(n):
-                see = max(0, length - n + j + 1)
+                see = max(0, min(room, int(lens[b]) - n + j + 1))
                 of = there[:see]
                 for g in range(h * nh // kvh, (h + 1) * nh // kvh):
                     row, bound = attention_row(q[at[b] + j, g].double(), k[:see][of], v[:see][of], scale)
