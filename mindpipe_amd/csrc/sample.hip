@@ -6,7 +6,8 @@
 //   token: the first index, in index order, at which the kept weights' running sum exceeds u times their sum
 //
 // A token is decided by which side of a border a sum over the vocabulary falls on, so weights are computed in 64 bits
-// and summed as whole numbers of 2^-44: sums of up to 2^19 of them fit 63 bits, and no order of additions changes them.
+// and summed as whole numbers of 2^-44: sums of up to 2^19 of them, 2^63 in a row of equal values, fit unsigned 64 bits,
+// and no order of additions changes them.
 //
 // Nothing is sorted.  A workgroup takes a row.  It counts the values into 2048 bins of equal width below the maximum (counts for
 // top-k, weights for top-p) and so finds the bin that the border of the kept is in.  The values down to that bin, few as a

@@ -1,5 +1,5 @@
-"""The serving operators where several of their rules meet: chunks that pass the end of their table.  Against plain 64-bit forms
-on the CPU (``paged_reference``)."""
+"""The serving operators where several of their rules meet: chunks that pass the end of their table, packed prompts whose
+positions are split, rows of logits past what registers hold.  Against plain 64-bit forms on the CPU (``paged_reference``)."""
 import math
 import sys
 
@@ -80,3 +80,84 @@ def test_chunks_past_the_end_of_their_table(dtype, dim, grp, width, bad):
                     ref.check(got[at[b] + j, h], want, ref.allowed(bound, dtype), what=f"sequence {b} row {j} head {h}")
                 else:
                     assert not torch.isfinite(got[at[b] + j, h]).any()
+
+
+# ---------------------------------------------------------------- packed prompts whose positions are split
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,kvh,grp", [(64, 1, 2), (64, 2, 1), (128, 1, 1), (128, 2, 1), (256, 1, 2), (256, 2, 1)])
+@pytest.mark.parametrize("starts", [[0, 520], [0, 1, 300, 300, 1013], [7, 600, 640, 641]])
+def test_packed_prompts_split_over_positions(dtype, dim, kvh, grp, starts):
+    """Few heads over prompts of hundreds of tokens: workgroups take a part of the positions each and are joined.  Rows that
+    see all of a part, some of it or nothing; rows of no sequence; an infinity, and a NaN, that only later rows see."""
+    from mindpipe_amd import _lib
+    rows, nh, scale = starts[-1] + 5, kvh * grp, dim ** -0.5
+    _say("packed prompts, split", dtype, dim, kvh, grp, starts)
+    assert _lib.load().mp_prompt_workspace_bytes(rows, nh, kvh, dim, len(starts) - 1, rows) > 0
+    g = torch.Generator().manual_seed(rows + dim)
+    qkv = (1.5 * torch.randn(rows, nh + 2 * kvh, dim, generator=g)).to(dtype).to(DEV)
+    q, k, v = qkv[:, :nh], qkv[:, nh:nh + kvh], qkv[:, nh + kvh:]
+    clean, tol = ref.prompt_attention(q, k, v, torch.tensor(starts), scale)
+    got = _ops().prompt_attention(q, k, v, _ints(starts), scale)
+    ref.check(got, clean, tol)
+    assert torch.equal(got, _ops().prompt_attention(q, k, v, _ints(starts), scale))
+    # one token of the longest sequence, past its first split, inside a tile
+    first = max(range(len(starts) - 1), key=lambda b: starts[b + 1] - starts[b])
+    at, end = starts[first] + 413, starts[first + 1]
+    for value in (math.inf, math.nan):
+        v[at, 0, 3], keep = value, v[at, 0, 3].clone()
+        got = _ops().prompt_attention(q, k, v, _ints(starts), scale)
+        v[at, 0, 3] = keep
+        want = clean.clone()
+        want[at:end, :grp, 3] = math.nan
+        seen = torch.isfinite(want)
+        ref.check(torch.where(seen, got.cpu().double(), 0.0), torch.where(seen, want, 0.0), tol, what=str(value))
+        assert not torch.isfinite(got.cpu()[~seen]).any()
+
+
+# ---------------------------------------------------------------- rows of logits past what registers hold
+def _check_sample(logits, u, *filters):
+    got, logp = _ops().sample_tokens(logits, u, *filters)
+    want, wlogp = ref.sample(logits, u, *filters)
+    assert torch.equal(got.cpu(), want), [(i, int(got[i]), int(want[i])) for i in (got.cpu() != want).nonzero().flatten().tolist()]
+    fine = torch.isfinite(wlogp)
+    assert torch.equal(torch.isfinite(logp.cpu()), fine)
+    # a sum of `vocab` weights is off by half a unit of 2^-44 of the largest each, and the sum is at least that weight; a
+    # token's own weight by half a unit, of its share exp(logp) of the sum (at least one weight of 1); rounded to fp32
+    tol = 2.0 ** -23 * wlogp.abs() + 2.0 ** -44 * (logits.shape[1] + logits.shape[1] * torch.exp(-wlogp)) + 2.0 ** -48
+    assert ((logp.cpu().double() - wlogp).abs()[fine] <= tol[fine]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, torch.float32])
+@pytest.mark.parametrize("vocab", [131072, 131073, 151936, 1 << 19])
+@pytest.mark.parametrize("which", ["", "t", "tk", "tp", "tm", "tkp", "tkpm"])
+def test_sample_rows_that_are_read_again(dtype, vocab, which):
+    _say("sample", dtype, vocab, which)
+    g = torch.Generator().manual_seed(vocab)
+    rows = 4
+    x = (torch.randn(rows, vocab + 8, generator=g) * 2).to(dtype)
+    x[:2] *= 4
+    f = [torch.rand(rows, generator=g) + 0.2, torch.randint(1, 3000, (rows,), generator=g, dtype=torch.int32),
+         0.3 + 0.69 * torch.rand(rows, generator=g), torch.rand(rows, generator=g) * 0.1]
+    f = [t.to(DEV) if c in which else None for c, t in zip("tkpm", f)]
+    x = x.to(DEV)
+    u = torch.rand(rows, generator=g).to(DEV)
+    _check_sample(x[:, :vocab], u, *f)            # rows in steps of eight values
+    _check_sample(x[:, 3:3 + vocab], u, *f)       # rows that begin between them
+    _check_sample(x[:, :vocab].contiguous(), u, *f)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, torch.float32])
+@pytest.mark.parametrize("vocab", [131072, 131073, 1 << 19])
+def test_sample_flat_rows(dtype, vocab):
+    """Every weight the largest: the sum is vocab 2^44, at 2^19 values 2^63.  Ties at every border go to the lowest indexes."""
+    us = [0.0, 0.25, 0.5, 1 - 2.0 ** -23, 1 - 2.0 ** -24]
+    n = len(us)
+    x = torch.full((n, vocab), -2.5, device=DEV, dtype=dtype)
+    x[:, 0] = -math.inf
+    one = lambda a, dt=torch.float32: torch.full((n,), a, device=DEV, dtype=dt)  # noqa: E731
+    u = torch.tensor(us, device=DEV)
+    for f in ((None,) * 4, (one(0.7), one(vocab - 5, torch.int32), None, None), (None, None, one(0.5), None),
+              (one(1.5), one(70000, torch.int32), one(0.75), one(1.0)), (one(0.0), None, None, None)):
+        _check_sample(x, u, *f)
+    x[:, 0] = -2.5
+    _check_sample(x, u)
