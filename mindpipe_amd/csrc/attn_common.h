@@ -19,6 +19,7 @@ typedef __bf16 abf8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 abf2_t __attribute__((ext_vector_type(2)));
 typedef short as2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 ah2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short au2_t __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 // The maximum that scores are taken against may lag behind by this much (in powers of two): weights up to 2^8 cost no
@@ -53,6 +54,17 @@ __device__ __forceinline__ float attn_add2(uint32_t w, float sum) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(ah2_t, w), ah2_t{1, 1}, sum, false);
   else
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(as2_t, w), as2_t{0x3F80, 0x3F80}, sum, false);
+}
+
+// What the packed values w leave of a and b, packed.
+template <int DT>
+__device__ __forceinline__ uint32_t attn_rest2(uint32_t w, float a, float b) {
+  if constexpr (DT == MP_F16) {
+    const ah2_t v = __builtin_bit_cast(ah2_t, w);
+    return attn_pack2<DT>(a - static_cast<float>(v.x), b - static_cast<float>(v.y));
+  } else {
+    return attn_pack2<DT>(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xFFFF0000u));
+  }
 }
 
 // The lowest fp16 magnitudes lose bits; weights are raised by 2^7 there, so that with the lag they end below 2^15 and keep
@@ -180,6 +192,8 @@ __device__ __forceinline__ void attn_clear(AttnRows<D> &a) {
 // `full`: to all.  Rows that see nothing of the tile are left as they are, whatever its masked places hold: masked scores
 // become -inf, V rows that no row sees are cleared, and a tile whose V has an infinity or NaN where only some rows see it
 // is added position by position, to those rows alone (0 times an infinity is no zero).  CAUSAL: rows see different positions.
+// Otherwise the second product takes the weights and then what their rounding leaves, so that they count with 16 (bf16) or 22
+// bits.  That rest may be 0 or negative, which beside an infinity gives NaN: a tile whose V has one takes halves of the weights.
 template <int D, int DT, bool CAUSAL>
 __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const uint4 (&q)[D / 32], int tile, int sees,
                                           int end, int full, float scale2, int lane) {
@@ -197,17 +211,17 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
   bool apart = false;
   if (tile + 32 > full || !__all(t.ok)) {
     const int to = t.ok ? sees : 0, any = t.ok ? end : 0;
-    bool odd = false;
+    bool masked = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       x[i] = p0 + i < to ? x[i] : -INFINITY;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         t.v[i][c] = p0 + i < any ? t.v[i][c] : 0u;
-        if (CAUSAL) odd |= attn_odd16<DT>(t.v[i][c]) || attn_odd16<DT>(t.v[i][c] >> 16);
+        if (CAUSAL) masked |= attn_odd16<DT>(t.v[i][c]) || attn_odd16<DT>(t.v[i][c] >> 16);
       }
     }
-    if (CAUSAL) apart = tile + 32 > full && __any(odd);
+    if (CAUSAL) apart = tile + 32 > full && __any(masked);
   }
   float top = x[0];
 #pragma unroll
@@ -221,25 +235,46 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) a.o[c] *= f;
   }
-  const float base = a.m == -INFINITY ? 0.f : a.m - kRaise<DT>;
+  bool odd = false;  // an infinity or NaN in V
+  if constexpr (!CAUSAL) {
+    au2_t most = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(au2_t, t.v[i][c] & 0x7FFF7FFFu));
+    odd = __any(max(most.x, most.y) >= (DT == MP_F16 ? 0x7C00 : 0x7F80));
+  }
+  const float base = (a.m == -INFINITY ? 0.f : a.m - kRaise<DT>) + (odd ? 1.f : 0.f);
   float p[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(x[i] - base);
-  // the weights in the values' type, for the matrix cores: half a step of 2^-11 (fp16) or 2^-8 (bf16) each, which averages out
-  // over the positions
+  // the weights in the values' type, for the matrix cores: off by up to 2^-11 (fp16) or 2^-8 (bf16) of themselves each
   uint4 w = make_uint4(attn_pack2<DT>(p[0], p[1]), attn_pack2<DT>(p[2], p[3]), attn_pack2<DT>(p[4], p[5]),
                        attn_pack2<DT>(p[6], p[7]));
   a.l = attn_add2<DT>(w.w, attn_add2<DT>(w.z, attn_add2<DT>(w.y, attn_add2<DT>(w.x, a.l))));
-  if (!CAUSAL || !apart) {
+  const auto values = [&](int c) {
+    const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;
+    return make_uint4(__builtin_amdgcn_perm(t.v[1][c / 2], t.v[0][c / 2], sel),
+                      __builtin_amdgcn_perm(t.v[3][c / 2], t.v[2][c / 2], sel),
+                      __builtin_amdgcn_perm(t.v[5][c / 2], t.v[4][c / 2], sel),
+                      __builtin_amdgcn_perm(t.v[7][c / 2], t.v[6][c / 2], sel));
+  };
+  if constexpr (!CAUSAL) {
+    uint4 rest = make_uint4(attn_rest2<DT>(w.x, p[0], p[1]), attn_rest2<DT>(w.y, p[2], p[3]), attn_rest2<DT>(w.z, p[4], p[5]),
+                            attn_rest2<DT>(w.w, p[6], p[7]));
+    if (odd) rest = w;
+    a.l = attn_add2<DT>(rest.w, attn_add2<DT>(rest.z, attn_add2<DT>(rest.y, attn_add2<DT>(rest.x, a.l))));
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
-      const uint32_t sel = (c & 1) ? 0x07060302u : 0x05040100u;
-      const uint4 vt = make_uint4(__builtin_amdgcn_perm(t.v[1][c / 2], t.v[0][c / 2], sel),
-                                  __builtin_amdgcn_perm(t.v[3][c / 2], t.v[2][c / 2], sel),
-                                  __builtin_amdgcn_perm(t.v[5][c / 2], t.v[4][c / 2], sel),
-                                  __builtin_amdgcn_perm(t.v[7][c / 2], t.v[6][c / 2], sel));
-      a.o[c] = attn_mfma16<DT>(vt, w, a.o[c]);
+      const uint4 vt = values(c);
+      a.o[c] = attn_mfma16<DT>(vt, rest, attn_mfma16<DT>(vt, w, a.o[c]));
     }
+    return;
+  }
+  if (!apart) {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) a.o[c] = attn_mfma16<DT>(values(c), w, a.o[c]);
     return;
   }
   const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
@@ -272,7 +307,8 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
 // after it are asked for before a tile is computed.
 template <int D, int DT, bool CAUSAL, bool PAGED>
 __device__ __forceinline__ void attn_walk(AttnRows<D> &a, const KvSource<PAGED> &src, const uint4 (&q)[D / 32], int first,
-                                          int to, int step, int sees, int end, int full, float scale2, int lane) {
+                                          int to, int step, int sees, int end, int full, float scale2,
+                                          int lane) {
   if (first >= to) return;
   TilePages pg = attn_pages(src, first, lane);
   KvTile<D> cur;

@@ -1,5 +1,5 @@
-"""The serving operators where several of their rules meet: chunks that pass the end of their table, packed prompts whose
-positions are split, rows of logits past what registers hold.  Against plain 64-bit forms on the CPU (``paged_reference``)."""
+"""The serving operators where several of their rules meet: the bits of decode attention's weights, chunks that pass the end of
+their table, packed prompts whose positions are split, rows of logits past what registers hold.  Against plain 64-bit forms on the CPU (``paged_reference``)."""
 import math
 import sys
 
@@ -25,6 +25,52 @@ def _ops():
 
 def _ints(v):
     return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+# ---------------------------------------------------------------- the weights of one new token
+def _pages_of(lens, kvh, dim, page, dtype, g, signs=False):
+    width = max(-(-n // page) for n in lens)
+    shape = (len(lens) * width, kvh, page, dim)
+    k, v = torch.randn(shape, generator=g).to(dtype), torch.randn(shape, generator=g)
+    v = torch.where(v < 0, -1.0, 1.0).to(dtype) if signs else v.to(dtype)
+    return k.to(DEV), v.to(DEV), torch.randperm(shape[0], generator=g).view(len(lens), width).to(torch.int32).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,kvh,grp", [(64, 2, 7), (128, 2, 4), (256, 1, 5)])
+@pytest.mark.parametrize("lens", [[2, 3, 7, 31], [40, 129, 500, 1], [3000]])
+def test_decode_keeps_the_weights_bits(dtype, dim, kvh, grp, lens):
+    """Values of 1 and -1, whose sums cancel: a weight rounded once to the type would be off by half a step, and the output by
+    much of that.  What the rounding leaves is added, rounded itself: half a step of half a step of the sum of magnitudes."""
+    _say("decode weights", dtype, dim, kvh, grp, lens)
+    g = torch.Generator().manual_seed(dim + len(lens))
+    k, v, table = _pages_of(lens, kvh, dim, 16, dtype, g, signs=True)
+    q = torch.randn(len(lens), kvh * grp, dim, generator=g).to(dtype).to(DEV)
+    got = _ops().paged_decode_attention(q, k, v, table, _ints(lens), dim ** -0.5)
+    half = ref.HALF_STEP[dtype]
+    for b, n in enumerate(lens):
+        rows_k, rows_v = (t[table[b].long()].cpu().transpose(1, 2).reshape(-1, kvh, dim)[:n].double() for t in (k, v))
+        for h in range(kvh * grp):
+            want, (out, size, rel, low) = ref.attention_row(q[b, h].cpu().double(), rows_k[:, h // grp], rows_v[:, h // grp], dim ** -0.5)
+            tol = half * out + (half * half * (1 + half) + 1.01 * rel) * size + low + (2.0 ** -24 if dtype == F16 else 0.0)
+            ref.check(got[b, h], want, tol, what=f"sequence {b} head {h}")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,kvh,grp", [(64, 2, 7), (128, 2, 4), (256, 1, 5)])
+def test_decode_over_infinite_values(dtype, dim, kvh, grp):
+    """An infinity in a value that is attended goes to its own column, with its sign, and two of different signs give NaN; the
+    others keep their sums.  The first position of a sequence, whose weight may be a power of two, among them."""
+    lens = [1, 5, 200, 2000]
+    g = torch.Generator().manual_seed(dim)
+    k, v, table = _pages_of(lens, kvh, dim, 16, dtype, g)
+    for b, at in ((0, 0), (1, 0), (1, 4), (2, 33), (2, 199), (3, 0), (3, 1024), (3, 1999)):
+        v[int(table[b, at // 16]), :, at % 16, 2 + at % 5] = math.inf if at % 2 else -math.inf
+    for b, at in ((2, 7), (2, 150), (3, 5), (3, 1600)):
+        v[int(table[b, at // 16]), :, at % 16, 9] = math.inf if at % 2 else -math.inf
+    q = torch.randn(len(lens), kvh * grp, dim, generator=g).to(dtype).to(DEV)
+    got = _ops().paged_decode_attention(q, k, v, table, _ints(lens), dim ** -0.5)
+    ref.check(got, *ref.paged_attention(q, k, v, table, _ints(lens), None, dim ** -0.5))
 
 
 # ---------------------------------------------------------------- chunks that pass the end of their table
