@@ -421,7 +421,7 @@ class W4Decoder:
         """``new_tokens`` tokens after each of ``prompts`` (int64 tensors of different lengths): the prompts in one packed
         pass, then a token of every sequence per step.  ``temperature``, ``top_k``, ``top_p``, ``min_p``: one value per prompt
         or ``None`` (``ops.sample_tokens``); ``temperature`` ``None`` takes the largest logit.  Returns ``[prompts,
-        new_tokens]``."""
+        new_tokens]``; a sequence whose logits leave nothing to take (all NaN or -inf) has -1 from there on."""
         device = self.embed.device
         lengths = [int(p.numel()) for p in prompts]
         if not lengths or min(lengths) < 1 or new_tokens < 1:
@@ -441,5 +441,7 @@ class W4Decoder:
         out = [tokens]
         for _ in range(new_tokens - 1):
             cache.extend([1] * len(prompts))
-            out.append(sample(self.forward_paged(out[-1], cache)))
+            # a sequence that has ended goes on with the vocabulary's first token, and stays ended
+            tokens = sample(self.forward_paged(out[-1].clamp(min=0), cache))
+            out.append(torch.where(out[-1] < 0, -1, tokens))
         return torch.stack(out, 1)
