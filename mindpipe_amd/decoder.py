@@ -387,8 +387,9 @@ class W4Decoder:
     def forward_paged(self, tokens, cache: PagedKVCache, starts: Optional[torch.Tensor] = None):
         """Logits ``[sequences, vocab]`` after the last of each sequence's new tokens.  ``tokens`` (int64) are the packed new
         tokens and ``starts`` their offsets, both for the positions that ``cache.extend`` has just made room for; without
-        ``starts`` each sequence has one.  A sequence without new tokens gets the logits of some other row.  Reads lengths
-        and pages from device memory: a step without ``starts`` can be captured and replayed after each ``extend``."""
+        ``starts`` each sequence has one.  A sequence without new tokens gets -inf everywhere, from which
+        ``ops.sample_tokens`` takes no token (-1).  Reads lengths and pages from device memory: a step without ``starts`` can be
+        captured and replayed after each ``extend``."""
         cfg = self.cfg
         if tokens.dim() != 1 or not tokens.numel():
             raise ValueError(f"tokens must be packed in one dimension and hold one at least, got {tuple(tokens.shape)}")
@@ -413,7 +414,10 @@ class W4Decoder:
         if starts is not None:  # the last row of each sequence
             last = (starts[1:].long() - 1).clamp(0, len(tokens) - 1)
             delta, x = delta[last], x[last]
-        return self.lm_head(ops.add_rms_norm_quant(delta, x, self.norm, cfg.eps, quant=False)[0])
+        logits = self.lm_head(ops.add_rms_norm_quant(delta, x, self.norm, cfg.eps, quant=False)[0])
+        if starts is not None:
+            logits.masked_fill_((starts[1:] <= starts[:-1]).unsqueeze(1), -math.inf)
+        return logits
 
     @torch.no_grad()
     def generate_paged(self, prompts: Sequence[torch.Tensor], new_tokens: int, cache: Optional[PagedKVCache] = None,
