@@ -35,7 +35,7 @@ __device__ __forceinline__ float at16(uint32_t w, int half) {
 // One workgroup per packed row and 256 of its 16-value pieces (a piece: eight pairs of a rotated head, or 16 values that
 // are copied).  Pairs are (2 i, 2 i + 1), or (i, i + rotary / 2).  Rotated in fp32 and rounded once.
 // Bound by its bytes: a row is read once and written once, the tables' rows come from the caches.  9219 rows of 64 / 8 heads of
-// 128 in bf16, 382 MB: 70 us, 5.4 TB/s, what a large copy reaches.  A row per workgroup keeps the look for its sequence uniform.
+// 128 in bf16, 382 MB: 70 us, 5.4 TB/s (a copy of 2 GiB: 4.9).  A row per workgroup keeps the look for its sequence uniform.
 template <int DT, bool PAIRS>
 __global__ __launch_bounds__(256) void paged_rope_append_kernel(
     const uint16_t *__restrict__ qkv, int64_t qkv_row, int nh, int kvh, int dim, const float *__restrict__ cos_t,
@@ -107,9 +107,10 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(
 // The heads that share a key-value head are the columns of one matrix product, up to 16 in a wave, so K and V are read once for
 // all of them:  S = K . Q^T,  P = exp2(scale S - m),  O^T += V^T . P^T  (MFMA 16x16x32; attn_tile).  The four waves take the 32
 // positions of a block each, straight from memory to registers: nothing is read twice, so LDS would only delay it.  Bound by
-// those reads: 64 sequences of up to 8192 positions, 64 / 8 heads of 128 in bf16 (945 MB), 170 us, 5.5 TB/s, and two of 131071
-// (1.07 GB) 184 us, 5.8 TB/s, of the 6.4 TB/s that reads reach here; 200 short ones of 14 / 2 heads of 64 (75 MB), 20 us,
-// where a workgroup's first loads wait for its look at the lengths, the table and a page in turn.
+// those reads: 64 sequences of up to 8192 positions, 64 / 8 heads of 128 in bf16 (945 MB), 171 us, 5.5 TB/s, and two of 131071
+// (1.07 GB) 185 us, 5.8 TB/s, of the 6.4 TB/s that reads reach here; 200 short ones of 14 / 2 heads of 64 (75 MB), 21 us,
+// where a workgroup's first loads wait for its look at the lengths, the table and a page in turn.  The matrix cores are 6% busy,
+// with the weights' rest taken as well (4% without it, 1 us of 176 less).
 constexpr int kWaves = 4;
 constexpr int kBlock = 32 * kWaves;
 

@@ -13,7 +13,7 @@
 // swizzled in 16-byte chunks so that neither reads a bank twice at a time.
 //
 // Bound by the matrix cores and the vector units in turn: three sequences of 1933 to 4096 tokens, 64 / 8 heads of 128 in bf16
-// (420 GFLOP that are seen), 448 us, 0.94 PFLOP/s, where a large matrix product reaches 1.37.  Matrix instructions are 47% of
+// (420 GFLOP that are seen), 448 to 480 us by the card, 0.9 PFLOP/s, where a large matrix product reaches 1.37.  Matrix instructions are 47% of
 // the time, the softmax's another 55%; the two waves of a SIMD cover part of it.  32 rows a wave, so that an operand from LDS
 // serves 32 x 32 x 16 products (with 16, straight from memory, 2374 us).  Eight waves in two groups that take turns: 716 us; the
 // next tile's scores ahead of a tile's weights in one wave, or wave priorities: no faster.
@@ -315,6 +315,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
     uint32_t w[2][4];
     constexpr int kAheadV = 2;  // operands of V that are read before they are used (1: 461 -> 470 us, 4: 463, heads of 256 92 -> 101 and 94)
     uint4 vf[kAheadV + 1];
+    // Weights are rounded to the values' type, off by up to 2^-11 (fp16) or 2^-8 (bf16) of themselves each, and their sum takes
+    // them as rounded: errors (rms) are 1.2 (fp16) to 1.3 times (bf16; heads of 256 1.4) those of 32-bit weights, 2.1e-3 for
+    // 1.6e-3 of the packed prompts' outputs.  A second product with what the rounding leaves would take that away for 471 -> 611 us
+    // there, 153 -> 209 for chunks of 32 heads and 91 -> 107 for heads of 256.
     const auto weight = [&](int c, int i) {
       const int r = 8 * (c & 1) + 2 * i;
       w[c & 1][i] = attn_pack2<DT>(__builtin_amdgcn_exp2f(fmaf(s[c / 2][r], scale2, -base)),
@@ -431,10 +435,10 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const float *__restric
 inline int64_t prompt_tiles(int64_t rows, int64_t grp, int64_t batch) { return rows * grp / kRows + batch + 2; }
 
 // Splits of the positions (at most `reach`): so many that the workgroups come nearest to what the CUs hold at once (two each;
-// one of heads of 256), with four tiles of positions each at least.  16 rows behind 32768 positions (32 / 8 heads of 128):
+// one of heads of 256), with four tiles of positions each at least.  Workgroups are counted by the bound that the grid goes by.  16 rows behind 32768 positions (32 / 8 heads of 128):
 // 666 us whole, 341 / 176 / 95 us in 2 / 4 / 8 splits, 40 us in the 32 that this gives; 1068 rows of 16 / 4 heads of 256
-// (144 workgroups): 117 us whole, 91 in 2, 93 in 3; 1737 rows of 32 heads of 128 (480 workgroups): 149 whole, 168 in 2, the
-// join reads and writes more than idle CUs cost.
+// (148 workgroups, 136 with rows): 117 us whole, 91 in 2, 93 in 3; 1737 rows of 32 heads of 128 (640 workgroups, 480 with rows):
+// 149 whole, 168 in 2, the join reads and writes more than idle CUs cost.
 inline int prompt_splits(int64_t rows, int64_t nh, int64_t kvh, int64_t dim, int64_t batch, int64_t reach) {
   const int64_t slots = (dim == 256 ? 1 : 2) * mp_cu_count(), blocks = prompt_tiles(rows, nh / kvh, batch) * kvh;
   const int64_t s = (slots + blocks / 2) / blocks, most = reach / 256;
