@@ -452,9 +452,9 @@ int mp_paged_rope_append(const void *qkv, int64_t qkv_row, int64_t rows, int nh,
 /* out [batch, nh, head_dim], dense = softmax(scale q k^T) v of one query per sequence over its first lens[b] positions
  * (held to what the table has room for), head_dim 64, 128 or 256, nh a multiple of kvh, scale finite (with log2 e in it);
  * nothing to attend gives zeros.
- * Weights and sums in fp32; the product with v takes the first 16 (bf16) or 22 (fp16) bits of a weight.  Long caches are split over
- * workgroups and joined, always in the same order.  workspace: mp_paged_decode_workspace_bytes of the current device,
- * 16-byte aligned, not shared by calls that may run at once. */
+ * Weights and sums in fp32; the product with v takes the first 16 (bf16) or 22 (fp16) bits of a weight.  Long caches are
+ * split over workgroups and joined, always in the same order.  workspace: mp_paged_decode_workspace_bytes of the current
+ * device, 16-byte aligned, not shared by calls that may run at once. */
 size_t mp_paged_decode_workspace_bytes(int64_t batch, int nh, int kvh, int head_dim);
 int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q_head, int64_t batch, int nh, int kvh, int head_dim,
                               const mp_pages *cache, const int32_t *lens, float scale, void *out, int dtype,

@@ -307,8 +307,7 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
 // after it are asked for before a tile is computed.
 template <int D, int DT, bool CAUSAL, bool PAGED>
 __device__ __forceinline__ void attn_walk(AttnRows<D> &a, const KvSource<PAGED> &src, const uint4 (&q)[D / 32], int first,
-                                          int to, int step, int sees, int end, int full, float scale2,
-                                          int lane) {
+                                          int to, int step, int sees, int end, int full, float scale2, int lane) {
   if (first >= to) return;
   TilePages pg = attn_pages(src, first, lane);
   KvTile<D> cur;

@@ -13,10 +13,10 @@
 // swizzled in 16-byte chunks so that neither reads a bank twice at a time.
 //
 // Bound by the matrix cores and the vector units in turn: three sequences of 1933 to 4096 tokens, 64 / 8 heads of 128 in bf16
-// (420 GFLOP that are seen), 448 to 480 us by the card, 0.9 PFLOP/s, where a large matrix product reaches 1.37.  Matrix instructions are 47% of
-// the time, the softmax's another 55%; the two waves of a SIMD cover part of it.  32 rows a wave, so that an operand from LDS
-// serves 32 x 32 x 16 products (with 16, straight from memory, 2374 us).  Eight waves in two groups that take turns: 716 us; the
-// next tile's scores ahead of a tile's weights in one wave, or wave priorities: no faster.
+// (420 GFLOP that are seen), 448 to 480 us by the card, 0.9 PFLOP/s, where a large matrix product reaches 1.37.  Matrix
+// instructions are 47% of the time, the softmax's another 55%; the two waves of a SIMD cover part of it.  32 rows a wave, so
+// that an operand from LDS serves 32 x 32 x 16 products (with 16, straight from memory, 2374 us).  Eight waves in two groups
+// that take turns: 716 us; the next tile's scores ahead of a tile's weights in one wave, or wave priorities: no faster.
 //
 // Few rows leave most CUs without a workgroup: then the positions are split over `splits` workgroups, which leave their sums,
 // maxima and outputs, unnormalised, in the workspace, and a second launch joins them.
@@ -435,10 +435,10 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const float *__restric
 inline int64_t prompt_tiles(int64_t rows, int64_t grp, int64_t batch) { return rows * grp / kRows + batch + 2; }
 
 // Splits of the positions (at most `reach`): so many that the workgroups come nearest to what the CUs hold at once (two each;
-// one of heads of 256), with four tiles of positions each at least.  Workgroups are counted by the bound that the grid goes by.  16 rows behind 32768 positions (32 / 8 heads of 128):
-// 666 us whole, 341 / 176 / 95 us in 2 / 4 / 8 splits, 40 us in the 32 that this gives; 1068 rows of 16 / 4 heads of 256
-// (148 workgroups, 136 with rows): 117 us whole, 91 in 2, 93 in 3; 1737 rows of 32 heads of 128 (640 workgroups, 480 with rows):
-// 149 whole, 168 in 2, the join reads and writes more than idle CUs cost.
+// one of heads of 256), with four tiles of positions each at least.  Workgroups are counted by the bound that the grid goes by.
+// 16 rows behind 32768 positions (32 / 8 heads of 128): 666 us whole, 341 / 176 / 95 us in 2 / 4 / 8 splits, 40 us in the 32 that
+// this gives; 1068 rows of 16 / 4 heads of 256 (148 workgroups, 136 with rows): 117 us whole, 91 in 2, 93 in 3; 1737 rows of 32
+// heads of 128 (640 workgroups, 480 with rows): 149 whole, 168 in 2, the join reads and writes more than idle CUs cost.
 inline int prompt_splits(int64_t rows, int64_t nh, int64_t kvh, int64_t dim, int64_t batch, int64_t reach) {
   const int64_t slots = (dim == 256 ? 1 : 2) * mp_cu_count(), blocks = prompt_tiles(rows, nh / kvh, batch) * kvh;
   const int64_t s = (slots + blocks / 2) / blocks, most = reach / 256;
