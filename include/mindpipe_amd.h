@@ -449,6 +449,13 @@ int mp_paged_rope_append(const void *qkv, int64_t qkv_row, int64_t rows, int nh,
                          const float *sin_t, int rotary, int64_t angles, int pairs, void *q_out, const mp_pages *cache,
                          const int32_t *lens, const int32_t *starts, int64_t batch, int dtype, mp_stream_t stream);
 
+/* The same with the position that a row turns by given apart from the place it is written to: turns int32 [rows] (NULL: its place),
+ * as the nodes of a drafted tree need it, which turn by their depth.  A row whose turns[row] has no angle is not written. */
+int mp_paged_rope_append_at(const void *qkv, int64_t qkv_row, int64_t rows, int nh, int kvh, int head_dim, const float *cos_t,
+                            const float *sin_t, int rotary, int64_t angles, int pairs, void *q_out, const mp_pages *cache,
+                            const int32_t *lens, const int32_t *starts, int64_t batch, const int32_t *turns, int dtype,
+                            mp_stream_t stream);
+
 /* out [batch, nh, head_dim], dense = softmax(scale q k^T) v of one query per sequence over its first lens[b] positions
  * (held to what the table has room for), head_dim 64, 128 or 256, nh a multiple of kvh, scale finite (with log2 e in it);
  * nothing to attend gives zeros.
@@ -459,6 +466,12 @@ size_t mp_paged_decode_workspace_bytes(int64_t batch, int nh, int kvh, int head_
 int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q_head, int64_t batch, int nh, int kvh, int head_dim,
                               const mp_pages *cache, const int32_t *lens, float scale, void *out, int dtype,
                               void *workspace, size_t workspace_bytes, mp_stream_t stream);
+
+/* The same over the last `window` (1 to 2^30) of the lens[b] positions and the first `sinks` (0 to 2^30).  Pages that hold none of
+ * those are not looked at. */
+int mp_paged_decode_window_attention(const void *q, int64_t q_row, int64_t q_head, int64_t batch, int nh, int kvh, int head_dim,
+                                     const mp_pages *cache, const int32_t *lens, int64_t window, int64_t sinks, float scale,
+                                     void *out, int dtype, void *workspace, size_t workspace_bytes, mp_stream_t stream);
 
 /* Causal attention of packed sequences: rows starts[b] .. starts[b + 1] - 1 of q [rows, nh, head_dim], k and v [rows, kvh,
  * head_dim] are sequence b.  out [rows, nh, head_dim], dense; rows of no sequence are zeros.  head_dim 64, 128, 256.
@@ -477,6 +490,49 @@ int mp_paged_prompt_attention(const void *q, int64_t q_row, int64_t q_head, int6
                               const mp_pages *cache, const int32_t *lens, const int32_t *starts, int64_t batch,
                               float scale, void *out, int dtype, void *workspace, size_t workspace_bytes,
                               mp_stream_t stream);
+
+/* Attention of packed new tokens over a paged cache that holds them, where a row sees other than all positions up to its own:
+ * tree: the positions before the sequence's new tokens, and of those the ones whose bits are set: bit i of word w of masks
+ *   int64 [rows, words] (1 to 1024 words) is new token 64 w + i of the row's sequence;
+ * window: of the positions up to its own the last `window` (1 to 2^30) and the first `sinks` of the sequence (0 to 2^30).
+ * Otherwise as mp_paged_prompt_attention.  Rows that see nothing are zeros.  The tiles of all rows are split into equal runs and
+ * joined in a fixed order.  workspace: mp_masked_workspace_bytes of the current device, 16-byte aligned, not shared by calls that
+ * may run at once.  Offsets that do not ascend leave the outputs open. */
+size_t mp_masked_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch);
+int mp_paged_tree_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh, int head_dim,
+                            const mp_pages *cache, const int32_t *lens, const int32_t *starts, int64_t batch,
+                            const int64_t *masks, int64_t words, float scale, void *out, int dtype, void *workspace,
+                            size_t workspace_bytes, mp_stream_t stream);
+int mp_paged_prompt_window_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh, int head_dim,
+                                     const mp_pages *cache, const int32_t *lens, const int32_t *starts, int64_t batch,
+                                     int64_t window, int64_t sinks, float scale, void *out, int dtype, void *workspace,
+                                     size_t workspace_bytes, mp_stream_t stream);
+
+/* Pages src[i] of every layer copied to pages dst[i], i < count, the first filled[i] positions of each (filled NULL: all).  `cache`
+ * describes the first layer (its table is not used); a layer lies k_layer / v_layer elements behind the last.  Pairs with a number
+ * outside the pool are left out.  A page that is written to by two pairs, or read by one and written to by another, may hold
+ * either's values.  head_dim a multiple of 8 up to 1024, 16-bit values of any type. */
+int mp_paged_copy_pages(const mp_pages *cache, int64_t layers, int64_t k_layer, int64_t v_layer, int kvh, int head_dim,
+                        const int32_t *src, const int32_t *dst, const int32_t *filled, int64_t count, mp_stream_t stream);
+
+/* Of each sequence b the keys and values of positions first[b] + keep[j], starts[b] <= j < starts[b + 1] (starts int32 [batch + 1],
+ * ascending, up to total), of every layer are moved to positions first[b] + j - starts[b].  A sequence's entries ascend and
+ * none is below its place, so none is lost before it is moved (other entries: what was moved before may be read).  A position past
+ * the table's width or of a page outside the pool is left out.  Sequences must not share the pages that are written. */
+int mp_paged_keep_positions(const mp_pages *cache, int64_t layers, int64_t k_layer, int64_t v_layer, int kvh, int head_dim,
+                            int64_t batch, const int32_t *first, const int32_t *keep, int64_t total, const int32_t *starts,
+                            mp_stream_t stream);
+
+/* The `count` (1 to 64) best continuations of each request: of totals scores[b, k] + log softmax(logits[b beams + k])[v] over its
+ * beams (1 to 64) and the vocabulary (up to 2^19) the largest, in order, of equal ones those of the lowest beam, then token.  A
+ * beam with ended[b, k] (may be NULL) has one continuation, token `pad`, of its own score.  Totals are made in 64 bits.  NaN
+ * and -inf totals are never taken; missing ones are score -inf, beam and token -1.  With infinite logits in a row those share its
+ * weight.  logits [batch * beams, vocab] (row stride `stride`; fp16, bf16 or fp32), scores fp32 [batch, beams], outputs [batch,
+ * count].  workspace: mp_beam_select_workspace_bytes, 16-byte aligned, not shared by calls that may run at once. */
+size_t mp_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t count, int dtype);
+int mp_beam_select(const void *logits, int64_t stride, int64_t batch, int64_t beams, int64_t vocab, int dtype, const float *scores,
+                   const uint8_t *ended, int64_t pad, int64_t count, float *out_scores, int64_t *out_beams, int64_t *out_tokens,
+                   void *workspace, size_t workspace_bytes, mp_stream_t stream);
 
 /* A token for each row of logits [rows, vocab] (row stride `stride`; fp16, bf16 or fp32; vocab up to 2^19) at the random
  * number u in [0, 1): weights exp((x - max) / temperature) of the top_k largest values (equal ones: the lowest indexes;

@@ -91,6 +91,19 @@ SIGNATURES = {
     "mp_prompt_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64, _i64]),
     "mp_paged_prompt_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, C.c_float, _vp, _i32,
                                          _vp, _sz, _vp]),
+    "mp_paged_rope_append_at": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _i64,
+                                       _vp, _i32, _vp]),
+    "mp_paged_decode_window_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i64, _i64, C.c_float, _vp,
+                                                _i32, _vp, _sz, _vp]),
+    "mp_masked_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64]),
+    "mp_paged_tree_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp, _i64, C.c_float, _vp,
+                                       _i32, _vp, _sz, _vp]),
+    "mp_paged_prompt_window_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i64,
+                                                C.c_float, _vp, _i32, _vp, _sz, _vp]),
+    "mp_paged_copy_pages": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _vp]),
+    "mp_paged_keep_positions": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i64, _vp, _vp, _i64, _vp, _vp]),
+    "mp_beam_select_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32]),
+    "mp_beam_select": (_i32, [_vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "mp_sample_tokens": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mp_moe_unpermute_combine": (_i32, [_vp, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _i32, _vp]),
 }

@@ -34,10 +34,11 @@ FLAGS = [
 ]
 
 
-# Per-source extra flags.  w4a16.hip, paged.hip, prompt.hip: MFMA results in ordinary VGPRs
+# Per-source extra flags.  w4a16.hip, paged.hip, prompt.hip, masked.hip: MFMA results in ordinary VGPRs
 # (their kernels scale MFMA results in VALU code; results in accumulation registers
 # would each need a copy first).
 FILE_FLAGS = {
+    "masked.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "w4a16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],

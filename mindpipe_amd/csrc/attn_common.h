@@ -188,15 +188,26 @@ __device__ __forceinline__ void attn_clear(AttnRows<D> &a) {
   a.l = 0.f;
 }
 
-// One tile into the rows' state.  `sees`: positions below it are visible to this lane's row; `end`: to any row of the wave;
-// `full`: to all.  Rows that see nothing of the tile are left as they are, whatever its masked places hold: masked scores
+// Which positions are seen: `sees(p)` by this lane's row, `any(p)` by any row of the wave, `whole(tile)`: by all of them every
+// one of the tile.  A walk goes over virtual positions, of which `place` says the real ones (both multiples of 32), and `look`
+// comes before a tile's questions.
+struct SeenUpTo {
+  int row, wave, all;  // positions below `row` are visible to this lane's row, below `wave` to any, below `all` to all
+  __device__ __forceinline__ int place(int v) const { return v; }
+  __device__ __forceinline__ void look(int) {}
+  __device__ __forceinline__ bool sees(int p) const { return p < row; }
+  __device__ __forceinline__ bool any(int p) const { return p < wave; }
+  __device__ __forceinline__ bool whole(int tile) const { return tile + 32 <= all; }
+};
+
+// One tile into the rows' state.  Rows that see nothing of the tile are left as they are, whatever its masked places hold: masked scores
 // become -inf, V rows that no row sees are cleared, and a tile whose V has an infinity or NaN where only some rows see it
-// is added position by position, to those rows alone (0 times an infinity is no zero).  CAUSAL: rows see different positions.
+// is added position by position, to those rows alone (0 times an infinity is no zero).  APART: rows see different positions.
 // Otherwise the second product takes the weights and then what their rounding leaves, so that they count with 16 (bf16) or 22
 // bits.  That rest may be 0 or negative, which beside an infinity gives NaN: a tile whose V has one takes halves of the weights.
-template <int D, int DT, bool CAUSAL>
-__device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const uint4 (&q)[D / 32], int tile, int sees,
-                                          int end, int full, float scale2, int lane) {
+template <int D, int DT, bool APART, class Seen>
+__device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const uint4 (&q)[D / 32], int tile, const Seen &seen,
+                                          float scale2, int lane) {
   const int j = lane >> 4, p0 = tile + 8 * j;
   f4_t s[2];
 #pragma unroll
@@ -209,19 +220,19 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * scale2;
   bool apart = false;
-  if (tile + 32 > full || !__all(t.ok)) {
-    const int to = t.ok ? sees : 0, any = t.ok ? end : 0;
+  const bool whole = seen.whole(tile);
+  if (!whole || !__all(t.ok)) {
     bool masked = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      x[i] = p0 + i < to ? x[i] : -INFINITY;
+      x[i] = t.ok && seen.sees(p0 + i) ? x[i] : -INFINITY;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        t.v[i][c] = p0 + i < any ? t.v[i][c] : 0u;
-        if (CAUSAL) masked |= attn_odd16<DT>(t.v[i][c]) || attn_odd16<DT>(t.v[i][c] >> 16);
+        t.v[i][c] = t.ok && seen.any(p0 + i) ? t.v[i][c] : 0u;
+        if (APART) masked |= attn_odd16<DT>(t.v[i][c]) || attn_odd16<DT>(t.v[i][c] >> 16);
       }
     }
-    if (CAUSAL) apart = tile + 32 > full && __any(masked);
+    if (APART) apart = !whole && __any(masked);
   }
   float top = x[0];
 #pragma unroll
@@ -236,7 +247,7 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
     for (int c = 0; c < D / 16; ++c) a.o[c] *= f;
   }
   bool odd = false;  // an infinity or NaN in V
-  if constexpr (!CAUSAL) {
+  if constexpr (!APART) {
     au2_t most = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -260,7 +271,7 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
                       __builtin_amdgcn_perm(t.v[5][c / 2], t.v[4][c / 2], sel),
                       __builtin_amdgcn_perm(t.v[7][c / 2], t.v[6][c / 2], sel));
   };
-  if constexpr (!CAUSAL) {
+  if constexpr (!APART) {
     uint4 rest = make_uint4(attn_rest2<DT>(w.x, p[0], p[1]), attn_rest2<DT>(w.y, p[2], p[3]), attn_rest2<DT>(w.z, p[4], p[5]),
                             attn_rest2<DT>(w.w, p[6], p[7]));
     if (odd) rest = w;
@@ -279,7 +290,7 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
   }
   const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
   for (int pos = 0; pos < 32; ++pos) {  // one position at a time
-    const bool mine = (pos >> 3) == j, row_sees = tile + pos < sees;
+    const bool mine = (pos >> 3) == j, row_sees = seen.sees(tile + pos);
     uint4 one = make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -303,24 +314,25 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
   }
 }
 
-// Tiles first, first + step, ... below `to` into the rows' state.  The next tile's rows and the table entries of the one
-// after it are asked for before a tile is computed.
-template <int D, int DT, bool CAUSAL, bool PAGED>
+// Tiles first, first + step, ... below `to`, virtual positions, into the rows' state.  The next tile's rows and the table
+// entries of the one after it are asked for before a tile is computed.
+template <int D, int DT, bool APART, bool PAGED, class Seen>
 __device__ __forceinline__ void attn_walk(AttnRows<D> &a, const KvSource<PAGED> &src, const uint4 (&q)[D / 32], int first,
-                                          int to, int step, int sees, int end, int full, float scale2, int lane) {
+                                          int to, int step, Seen seen, float scale2, int lane) {
   if (first >= to) return;
-  TilePages pg = attn_pages(src, first, lane);
+  TilePages pg = attn_pages(src, seen.place(first), lane);
   KvTile<D> cur;
-  TilePages next = attn_pages(src, first + step, lane);
-  attn_load_tile<D>(src, pg, first, lane, cur);
+  TilePages next = attn_pages(src, seen.place(first + step), lane);
+  attn_load_tile<D>(src, pg, seen.place(first), lane, cur);
   for (int tile = first; tile < to; tile += step) {
     KvTile<D> ahead = cur;
     if (tile + step < to) {
-      const TilePages after = attn_pages(src, tile + 2 * step, lane);
-      attn_load_tile<D>(src, next, tile + step, lane, ahead);
+      const TilePages after = attn_pages(src, seen.place(tile + 2 * step), lane);
+      attn_load_tile<D>(src, next, seen.place(tile + step), lane, ahead);
       next = after;
     }
-    attn_tile<D, DT, CAUSAL>(a, cur, q, tile, sees, end, full, scale2, lane);
+    seen.look(seen.place(tile));
+    attn_tile<D, DT, APART>(a, cur, q, seen.place(tile), seen, scale2, lane);
     cur = ahead;
   }
 }

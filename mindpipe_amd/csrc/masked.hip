@@ -1,0 +1,555 @@
+// Attention of packed new tokens over a paged cache where a row sees other than all positions up to its own:
+//
+//   * trees of drafted tokens: a row sees what the cache holds before its sequence's new tokens, and of these the ones that its
+//     mask names (a node's ancestors and itself);
+//   * windows: a row sees the last `window` positions up to its own, and the first `sinks`.
+//
+// The products are those of prompt.hip (prompt_tile.h): rows are tokens times the heads that share a key-value head, 32 to a
+// wave and kRows to a workgroup, over tiles of 64 positions in LDS.  What a row sees of a tile is a word of 64 bits.
+//
+// Work is cut into equal runs.  An item is up to kRows rows of a sequence and key-value head; its tiles, those that hold
+// nothing seen left out, follow each other, and so do the items.  The workgroups of a head take equal runs of that row of tiles,
+// however ragged the sequences are.  An item that lies in several runs is joined from its parts: a workgroup leaves at most
+// two, that of the item its run begins inside of (slot 2 w) and that of the item its run ends inside of (slot 2 w + 1).
+#include <cfloat>
+#include <climits>
+#include <cmath>
+
+#include "prompt_tile.h"
+
+namespace {
+
+enum { kTree = 0, kWindow = 1 };
+
+// The lowest n bits.
+__device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1; }
+
+// What the rows see: plain arguments of a launch.
+struct MaskedRule {
+  const int64_t *masks;  // kTree: [rows, words]
+  int words;
+  int window, sinks;     // kWindow
+};
+
+// A sequence's rows and what they see, by the launch's rule.
+template <int MODE>
+struct MaskedSeq {
+  int first, n;          // its packed rows
+  int len, room;         // its positions, the new tokens' included, and those that the table has room for; none outside of the sequences
+  MaskedRule rule;
+
+  __device__ __forceinline__ int context() const { return len - n; }  // position of its first row (negative: rows without a place)
+  __device__ __forceinline__ int end() const { return min(len, room); }
+  __device__ __forceinline__ int clamped(int64_t p) const { return static_cast<int>(max(min(p, static_cast<int64_t>(end())), int64_t(0))); }
+  // Positions t .. t + 63 that token `token` of the sequence sees, as bits.  t is a multiple of 32.
+  __device__ __forceinline__ uint64_t bits(int token, int t) const {
+    if constexpr (MODE == kTree) {
+      const int d = t - context();  // node of position t
+      const int64_t *words = rule.masks + static_cast<int64_t>(first + token) * rule.words;
+      uint64_t v = bits_below(-d);
+      if (d > -64 && d < 64 * rule.words && token < n) {
+        const int w = d >> 6, s = d & 63;  // bits of nodes d .. d + 63: from word w (-1: none) and the one after it
+        if (w >= 0) v |= static_cast<uint64_t>(words[w]) >> s;
+        if (s && w + 1 < rule.words) v |= static_cast<uint64_t>(words[w + 1]) << (64 - s);
+      }
+      return v & bits_below(end() - t);
+    } else {
+      const int64_t pos = static_cast<int64_t>(context()) + token;
+      const int low = clamped(pos - rule.window + 1), upto = clamped(pos + 1);
+      return bits_below(upto - t) & (bits_below(rule.sinks - t) | ~bits_below(low - t));
+    }
+  }
+  // Rows of tokens a .. b: the tiles they look at lie below `to`, and of these none between `gap_from` and `gap_to` (multiples of
+  // 64) is seen.
+  __device__ __forceinline__ void span(int a, int b, int &to, int &gap_from, int &gap_to) const {
+    gap_from = gap_to = 0;
+    to = end();
+    if constexpr (MODE == kWindow) {
+      to = clamped(static_cast<int64_t>(context()) + b + 1);
+      gap_to = min(clamped(static_cast<int64_t>(context()) + a - rule.window + 1), to) & ~63;
+      gap_from = min((min(rule.sinks, to) + 63) & ~63, gap_to);
+    }
+  }
+  // All of tile t (64 positions) is seen by tokens a .. b.
+  __device__ __forceinline__ bool whole(int a, int b, int t) const {
+    if (t + 64 > end()) return false;
+    if constexpr (MODE == kTree) return t + 64 <= context();
+    const int64_t pos = context();
+    return t + 64 <= pos + a + 1 && (t + 64 <= rule.sinks || t >= pos + b - rule.window + 1);
+  }
+};
+
+template <int MODE>
+struct MaskedPlan {
+  PackedPlan rows;
+  const int32_t *lens;
+  int capacity;  // positions that the table has room for
+  MaskedRule rule;
+
+  __device__ __forceinline__ MaskedSeq<MODE> seq(int b) const {
+    MaskedSeq<MODE> s;
+    s.first = rows.first(b);
+    s.n = rows.end(b) - s.first;
+    s.len = b < rows.batch ? max(lens[b], 0) : 0;
+    s.room = b < rows.batch ? capacity : 0;
+    s.rule = rule;
+    return s;
+  }
+  __device__ __forceinline__ int items(const MaskedSeq<MODE> &s) const {
+    return static_cast<int>((static_cast<int64_t>(s.n) * rows.grp + kRows - 1) / kRows);
+  }
+  // Tiles of an item (one at least, which writes its zeros), with the gap among them.
+  __device__ __forceinline__ int tiles(const MaskedSeq<MODE> &s, int item, int &to, int &gap_from, int &gap_to) const {
+    const int a = item * kRows / rows.grp, b = min((item * kRows + kRows - 1) / rows.grp, s.n - 1);
+    s.span(a, b, to, gap_from, gap_to);
+    return max((to - (gap_to - gap_from) + kTile - 1) / kTile, 1);
+  }
+  __device__ __forceinline__ int tiles(const MaskedSeq<MODE> &s, int item) const {
+    int to, from, upto;
+    return tiles(s, item, to, from, upto);
+  }
+  // Tiles of a sequence.  Its items are at most (rows grp) / kRows + 1, the launch holds their tiles below 2^31.
+  __device__ __forceinline__ int operator()(int b, int) const {
+    const MaskedSeq<MODE> s = seq(b);
+    const int n = items(s);
+    if (n == 0) return 0;
+    if constexpr (MODE == kTree) return n * tiles(s, 0);
+    int sum = 0;
+    for (int i = 0; i < n; ++i) sum += tiles(s, i);
+    return sum;
+  }
+  // Tiles of all; 0 where the offsets do not ascend (then the sequences' rows add up to more than there are).
+  __device__ __forceinline__ uint32_t all() const {
+    uint32_t n = 0;
+    uint64_t held = 0;
+    for (int b = threadIdx.x & 63; b < rows.batch + 2; b += 64) {
+      n += (*this)(b, 0);
+      held += rows.end(b) - rows.first(b);
+    }
+    return wave_sum(held) == static_cast<uint64_t>(rows.rows) ? wave_sum(n) : 0;
+  }
+};
+
+// Where an item's parts and its outputs go.
+struct MaskedOut {
+  uint16_t *out;    // the item's first token and head
+  int64_t row;      // from token to token
+  float *part;      // [rows of the item][D + 2]; null: outputs are final
+};
+
+// 16 rows of an item by the wave alone, K and V straight from memory (attn_tile), for tiles whose V has an infinity or NaN that only
+// some rows see.  A function of its own: inlined, its registers would be the kernel's.
+template <int MODE>
+struct MaskedSeen {
+  MaskedSeq<MODE> s;
+  int token, gap_from, gap;  // the gap in virtual positions
+  uint32_t mine, wave;
+  bool every;
+  __device__ __forceinline__ int place(int v) const { return v < gap_from ? v : v + gap; }
+  __device__ __forceinline__ void look(int tile) {
+    mine = static_cast<uint32_t>(s.bits(token, tile));
+    every = __all(mine == ~0u);
+  }
+  __device__ __forceinline__ bool sees(int p) const { return (mine >> (p & 31)) & 1; }
+  __device__ __forceinline__ bool any(int) const { return true; }
+  __device__ __forceinline__ bool whole(int) const { return every; }
+};
+template <int MODE>
+struct MaskedRows {
+  KvSource<true> src;
+  MaskedSeen<MODE> seen;
+  const uint16_t *q;  // the item's sequence's first row, its first head
+  int64_t q_row, q_head;
+  MaskedOut to;
+  int all, grp, r0, from, end;  // rows of the sequence, heads of a token, the item's first row, virtual positions that are looked at
+  float scale2;
+};
+template <int D, int DT, int MODE>
+__device__ __attribute__((noinline)) void masked_rows16(const MaskedRows<MODE> &p, int at0) {
+  const int lane = threadIdx.x & 63, i16 = lane & 15, j = lane >> 4, at = min(p.r0 + at0 + i16, p.all - 1);
+  const int token = at / p.grp, head = at - token * p.grp;
+  uint4 qf[D / 32];
+  const uint16_t *qp = p.q + token * p.q_row + head * p.q_head + 8 * j;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) qf[c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
+  MaskedSeen<MODE> seen = p.seen;
+  seen.token = token;
+  AttnRows<D> a;
+  attn_clear(a);
+  attn_walk<D, DT, true>(a, p.src, qf, p.from, p.end, 32, seen, p.scale2, lane);
+  const float l = attn_row_sum(a.l);
+  if (p.r0 + at0 + i16 >= p.all) return;
+  if (p.to.part) {
+    float *z = p.to.part + (at0 + i16) * (D + 2);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) z[(D / 16) * (4 * j + r) + c] = a.o[c][r];
+    if (j == 0) {
+      z[D] = a.m;
+      z[D + 1] = l;
+    }
+    return;
+  }
+  uint16_t *y = p.to.out + token * p.to.row + head * D + (D / 16) * 4 * j;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < D / 16; c += 2) {
+      const float lo = l == 0.f ? 0.f : a.o[c][r] / l, hi = l == 0.f ? 0.f : a.o[c + 1][r] / l;
+      *reinterpret_cast<uint32_t *>(y + (D / 16) * r + c) = attn_pack2<DT>(lo, hi);
+    }
+}
+
+// Number of an item among all of a head, of rows that begin at packed row `first` of sequence b: no two are alike.
+__device__ __forceinline__ int64_t masked_item(int first, int grp, int b, int item) {
+  return static_cast<int64_t>(first) * grp / kRows + b + item;
+}
+// Sequences in the order of their rows: what lies before the first (batch + 1), the sequences, what lies behind the last (batch).
+__device__ __forceinline__ int masked_order(int b, int batch) { return b == batch + 1 ? 0 : b + 1; }
+
+// A run has kLeast tiles at least.
+constexpr int kLeast = 4;
+
+template <int D, int DT, int MODE>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void masked_attention_kernel(
+    const uint16_t *__restrict__ q, int64_t q_row, int64_t q_head, const uint16_t *__restrict__ k, int64_t kpage,
+    int64_t khead, int64_t krow, const uint16_t *__restrict__ v, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
+    int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
+    const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, MaskedRule rule, int share, int slot_rows,
+    float scale2, uint32_t flip, float *__restrict__ parts, int4 *__restrict__ joins, uint16_t *__restrict__ out) {
+  using T = PromptTile<D>;
+  constexpr int kStage = T::kStage, kS = kTile / 32;
+  extern __shared__ __attribute__((aligned(1024))) int8_t masked_smem[];  // two stages of K and V
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i32 = lane & 31, h = lane >> 5;
+  const int kh = blockIdx.x % kvh, run = blockIdx.x / kvh;
+  const MaskedPlan<MODE> plan{{starts, batch, rows, grp}, lens, width << shift, rule};
+  const uint64_t all = plan.all();
+  share = static_cast<int>(max(min(static_cast<uint64_t>(share), all / kLeast), uint64_t(1)));
+  if (run >= share || all == 0) return;  // uniform over the workgroup
+  const int begin = static_cast<int>(run * all / share), stop = static_cast<int>((run + 1) * all / share);
+  const int mask = (1 << shift) - 1;
+
+  for (int at = begin; at < stop;) {
+    // the item that this part of the run lies in, and which of its tiles
+    int b, part, unused;
+    if (!attn_find_part(plan, batch + 2, 0, at, b, part, unused)) return;
+    MaskedSeq<MODE> seq = plan.seq(b);
+    seq.first = __builtin_amdgcn_readfirstlane(seq.first);  // uniform: in scalar registers
+    seq.n = __builtin_amdgcn_readfirstlane(seq.n);
+    seq.len = __builtin_amdgcn_readfirstlane(seq.len);
+    int item, tile0, tiles;
+    if constexpr (MODE == kTree) {
+      tiles = plan.tiles(seq, 0);
+      item = part / tiles;
+      tile0 = part - item * tiles;
+    } else {
+      attn_find_part([&](int i, int) { return plan.tiles(seq, i); }, plan.items(seq), 0, part, item, tile0, tiles);
+    }
+    int to, gap_from, gap_to;
+    plan.tiles(seq, item, to, gap_from, gap_to);
+    const int tile1 = min(tiles, tile0 + stop - at), gap = gap_to - gap_from;
+    const bool entire = tile0 == 0 && tile1 == tiles;
+    // virtual positions of this part, and its last real one
+    const int from = tile0 * kTile, end = min(tile1 * kTile, to - gap), last = end > 0 ? (end <= gap_from ? end : end + gap) - 1 : 0;
+    const auto place = [&](int vp) { return vp < gap_from ? vp : vp + gap; };
+
+    const int n_rows = seq.n * grp, r0 = item * kRows + wave * 32, row_at = r0 + i32;
+    const bool row = row_at < n_rows;
+    const int token = row ? row_at / grp : 0, head = kh * grp + (row ? row_at - token * grp : 0);
+    const int wave_a = r0 / grp, wave_b = min((r0 + 31) / grp, seq.n - 1);
+    uint4 qf[D / 16];
+    const uint16_t *qp = q + (seq.first + token) * q_row + head * q_head + 8 * h;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const uint4 x = *reinterpret_cast<const uint4 *>(qp + 16 * c);
+      qf[c] = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+    }
+
+    const uint16_t *kb = k + kh * khead, *vb = v + kh * vhead;
+    const int32_t *pg = table + static_cast<int64_t>(min(b, batch - 1)) * width;
+    const auto entry = [&](int vp) { return pg[min(place(vp) + lane, last) >> shift]; };
+    const auto load = [&](int vp, int id, int8_t *stage) {
+      const int tile = min(place(vp), last);  // past the last tile: rows that nothing reads
+#pragma unroll
+      for (int i = 0; i < T::kLoads; ++i) {
+        const int slot = (wave * T::kLoads + i) * 64;
+        const int64_t pid = __builtin_amdgcn_readlane(id, slot / T::kChunks);  // the rows of one load lie in one page
+        const int r = slot / T::kChunks + lane / T::kChunks, c = lane % T::kChunks, p = min(tile + r, last) & mask;
+        prompt_lds_load16(kb + pid * kpage, 2 * (p * static_cast<uint32_t>(krow) + 8 * T::k_chunk(r, c)), stage + slot * 16);
+        prompt_lds_load16(vb + pid * vpage, 2 * (p * static_cast<uint32_t>(vrow) + 8 * T::v_chunk(r, c)), stage + T::kBytes + slot * 16);
+      }
+    };
+    const auto fix = [&](int id, uint64_t &there) {  // page numbers outside the pool: page 0, unseen
+      const bool ok = id >= 0 && id < pages;
+      there = __ballot(ok);
+      return ok ? id : 0;
+    };
+
+    f16_t o[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    uint64_t there = 0;  // which positions of the tile that is on its way exist
+    int next_entry = 0, stage = 0;
+    __syncthreads();  // the last item's tiles have been read
+    if (end > from) {
+      load(from, fix(entry(from), there), masked_smem);
+      next_entry = entry(from + kTile);
+    }
+    uint32_t odd = 0;  // an infinity or NaN in V where only some of the wave's rows see it
+    for (int vp = from; vp < end; vp += kTile) {
+      // this tile's loads have landed, every wave's, and the stage of the last tile has been read
+      prompt_wait();
+      const uint64_t ok = there;
+      load(vp + kTile, fix(next_entry, there), masked_smem + (kStage - stage));
+      next_entry = entry(vp + 2 * kTile);
+      const int8_t *ks = masked_smem + stage, *vs = ks + T::kBytes;
+      stage = kStage - stage;
+      if (r0 >= n_rows) continue;  // no rows: it loads for the others
+      const int tile = place(vp);
+      uint64_t vis = ~uint64_t(0);
+      const bool some = !seq.whole(wave_a, wave_b, tile) || ok != ~uint64_t(0);
+      if (some) {
+        vis = row ? seq.bits(token, tile) & ok : 0;
+        if (!__any(vis != 0)) continue;
+      }
+      f16_t s[kS];
+      prompt_scores<D, DT>(ks, qf, s, i32, h);
+      if (some) {
+        vis >>= 4 * h;
+#pragma unroll
+        for (int t = 0; t < kS; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[t][r] = (vis >> (32 * t + 8 * (r >> 2) + (r & 3))) & 1 ? s[t][r] : -INFINITY;
+        odd |= prompt_odd_values<D, DT>(vs, lane);
+      }
+      prompt_weigh<D, DT>(s, vs, o, m, l, scale2, lane);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing on its way to LDS when the item ends
+    const int64_t slot = (static_cast<int64_t>(2 * run + (at > begin ? 1 : 0)) * kvh + kh) * slot_rows;
+    MaskedOut dst{out + (static_cast<int64_t>(seq.first) * kvh * grp + kh * grp) * D, static_cast<int64_t>(kvh) * grp * D,
+                  entire ? nullptr : parts + slot * (D + 2)};
+    if (tile0 == 0 && threadIdx.x == 0) {
+      const int last_run = static_cast<int>(((at + tiles) * static_cast<uint64_t>(share) - 1) / all);  // run of its last tile
+      joins[masked_item(seq.first, grp, masked_order(b, batch), item) * kvh + kh] = make_int4(run, last_run - run + 1, at > begin ? 1 : 0, 0);
+    }
+    at += tile1 - tile0;
+    if (r0 >= n_rows) continue;
+    if (__any(odd)) {
+      // 0 times an infinity is no zero: these rows once more, with what they do not see left out one position at a time
+      MaskedRows<MODE> p;
+      p.src = {kb, vb, kpage, krow, vpage, vrow, pg, shift, mask, pages, last >> shift};
+      p.seen.s = seq;
+      p.seen.gap_from = gap_from;
+      p.seen.gap = gap;
+      p.q = q + seq.first * q_row + kh * grp * q_head;
+      p.q_row = q_row;
+      p.q_head = q_head;
+      p.to = dst;
+      p.all = n_rows;
+      p.grp = grp;
+      p.r0 = item * kRows;
+      p.from = from;
+      p.end = end;
+      p.scale2 = flip ? -scale2 : scale2;
+      for (int half = 0; half < 2; ++half)
+        if (r0 + 16 * half < n_rows) masked_rows16<D, DT, MODE>(p, 32 * wave + 16 * half);
+      continue;
+    }
+    if (!row) continue;
+    l += __shfl_xor(l, 32, 64);
+    if (!entire) {
+      float *z = dst.part + (wave * 32 + i32) * (D + 2);
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2)
+          *reinterpret_cast<float2 *>(z + 32 * d + 8 * (r >> 2) + 4 * h + (r & 3)) = make_float2(o[d][r], o[d][r + 1]);
+      if (h == 0) *reinterpret_cast<float2 *>(z + D) = make_float2(m, l);
+      continue;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint16_t *y = dst.out + token * dst.row + (head - kh * grp) * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = l == 0.f ? 0.f : o[d][r + i] * inv;
+        *reinterpret_cast<uint2 *>(y + 32 * d + 2 * r) = make_uint2(attn_pack2<DT>(x[0], x[1]), attn_pack2<DT>(x[2], x[3]));
+      }
+  }
+}
+
+// The parts of a row meet, one wave each.
+template <int D, int DT>
+__global__ __launch_bounds__(256) void masked_join_kernel(const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp,
+                                                          int slot_rows, int share, const float *__restrict__ parts,
+                                                          const int4 *__restrict__ joins, uint16_t *__restrict__ out) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int nh = kvh * grp, lane = threadIdx.x & 63;
+  if (at >= static_cast<int64_t>(rows) * nh) return;
+  const int t = static_cast<int>(at / nh), qh = static_cast<int>(at - static_cast<int64_t>(t) * nh), kh = qh / grp;
+  // the sequence of packed row t: how many of them begin at or before it
+  const PackedPlan plan{starts, batch, rows, grp};
+  int b = 0;
+  for (int b0 = 0; b0 <= batch; b0 += 64) b += __popcll(__ballot(b0 + lane <= batch && starts[min(b0 + lane, batch)] <= t));
+  b = b == 0 ? batch + 1 : b - 1;
+  const int first = plan.first(b), r = (t - first) * grp + qh - kh * grp, item = r / kRows;
+  if (t < first || t >= plan.end(b)) return;  // offsets that do not ascend: nothing was left
+  const int4 of = joins[masked_item(first, grp, masked_order(b, batch), item) * kvh + kh];
+  if (of.y == 1) return;  // written already
+  if (of.x < 0 || of.y < 1 || of.x >= share || of.y > share - of.x) return;
+  const auto at_part = [&](int p) {
+    return parts + ((static_cast<int64_t>(2 * (of.x + p) + (p == 0 ? of.z & 1 : 0)) * kvh + kh) * slot_rows + r % kRows) * (D + 2);
+  };
+  float m = -INFINITY;
+  for (int p = lane; p < of.y; p += 64) m = fmaxf(m, at_part(p)[D]);
+  m = mp_wave_max(m);
+  float o[D / 64], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
+#pragma unroll 4
+  for (int p = 0; p < of.y; ++p) {
+    const float *z = at_part(p);
+    const float f = z[D] == m ? 1.0f : __builtin_amdgcn_exp2f(z[D] - m);
+    l += f * z[D + 1];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) o[i] += f * z[64 * i + lane];
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    const float x = l == 0.f ? 0.f : o[i] * inv;
+    out[at * D + 64 * i + lane] = DT == MP_F16 ? mp_f2h(x) : mp_f2bf(x);
+  }
+}
+
+// Workgroups of a head: as many as fit the card at once (two a CU; one of heads of 256).
+inline int masked_share(int64_t kvh, int dim) {
+  const int64_t n = static_cast<int64_t>(dim == 256 ? 1 : 2) * mp_cu_count() / kvh;
+  return static_cast<int>(n > 1 ? n : 1);
+}
+inline int64_t masked_slot_rows(int64_t rows, int64_t grp) { return rows * grp < kRows ? rows * grp : kRows; }
+inline int64_t masked_items(int64_t rows, int64_t grp, int64_t batch) { return rows * grp / kRows + batch + 4; }
+
+struct MaskedCall {
+  const void *q;
+  int64_t q_row, q_head, rows;
+  int nh, kvh, head_dim;
+  const mp_pages *cache;
+  const int32_t *lens, *starts;
+  int64_t batch;
+  MaskedRule rule;
+  float scale;
+  void *out;
+  int dtype;
+  void *workspace;
+  size_t workspace_bytes;
+  hipStream_t stream;
+};
+
+size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim, int64_t batch) {
+  const int64_t grp = nh / kvh;
+  return static_cast<size_t>(masked_items(rows, grp, batch) * kvh) * sizeof(int4) +
+         static_cast<size_t>(2 * masked_share(kvh, dim) * kvh * masked_slot_rows(rows, grp)) * (dim + 2) * sizeof(float);
+}
+
+template <int D, int DT, int MODE>
+int masked_start(const MaskedCall &c, int shift) {
+  const int grp = c.nh / c.kvh, share = masked_share(c.kvh, D), slot_rows = static_cast<int>(masked_slot_rows(c.rows, grp));
+  int4 *joins = static_cast<int4 *>(c.workspace);
+  float *parts = reinterpret_cast<float *>(joins + masked_items(c.rows, grp, c.batch) * c.kvh);
+  // the sign of the scale goes to the queries, so that the largest product gives the largest score; a scale of 0 becomes the
+  // smallest normal number, which leaves every finite score 0 and a masked one -inf
+  const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
+  const float scale2 = fmaxf(fabsf(c.scale) * kLog2e, FLT_MIN);
+  constexpr int kLds = 2 * PromptTile<D>::kStage;
+  if (kLds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(masked_attention_kernel<D, DT, MODE>),
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
+    return MP_ERR_HIP;
+  const mp_pages &p = *c.cache;
+  hipLaunchKernelGGL((masked_attention_kernel<D, DT, MODE>), dim3(static_cast<unsigned>(share) * c.kvh), dim3(64 * kWaves), kLds,
+                     c.stream, static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(p.k), p.k_page,
+                     p.k_head, p.k_row, static_cast<const uint16_t *>(p.v), p.v_page, p.v_head, p.v_row, static_cast<int>(p.pages),
+                     shift, p.table, static_cast<int>(p.width), c.lens, c.starts, static_cast<int>(c.batch),
+                     static_cast<int>(c.rows), c.kvh, grp, c.rule, share, slot_rows, scale2, flip, parts, joins,
+                     static_cast<uint16_t *>(c.out));
+  MP_CHECK_LAUNCH();
+  if (share > 1) {
+    hipLaunchKernelGGL((masked_join_kernel<D, DT>), dim3(static_cast<unsigned>(mp_cdiv(c.rows * c.nh, 4))), dim3(256), 0, c.stream,
+                       c.starts, static_cast<int>(c.batch), static_cast<int>(c.rows), c.kvh, grp, slot_rows, share, parts, joins,
+                       static_cast<uint16_t *>(c.out));
+    MP_CHECK_LAUNCH();
+  }
+  return MP_OK;
+}
+
+template <int MODE>
+int masked_launch(const MaskedCall &c) {
+  if (!c.q || !c.cache || !c.cache->k || !c.cache->v || !c.cache->table || !c.lens || !c.starts || !c.out || !c.workspace)
+    return MP_ERR_ARG;
+  if (c.dtype != MP_F16 && c.dtype != MP_BF16) return MP_ERR_DTYPE;
+  if (!std::isfinite(c.scale * kLog2e)) return MP_ERR_ARG;
+  const mp_pages &p = *c.cache;
+  int shift = -1;
+  for (int s = 3; s < 16; ++s)
+    if (p.page_size == 1 << s) shift = s;
+  if (shift < 0 || p.pages < 1 || p.pages > INT32_MAX || p.width < 1 || p.width > (1 << 30) >> shift) return MP_ERR_SHAPE;
+  if (c.rows < 0 || c.rows > INT32_MAX || c.batch < 1 || c.batch > INT32_MAX - 64) return MP_ERR_SHAPE;
+  if (c.nh < 1 || c.kvh < 1 || c.nh > 65536 || c.nh % c.kvh) return MP_ERR_SHAPE;
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return MP_ERR_SHAPE;
+  for (int64_t s : {c.q_row, c.q_head, p.k_page, p.k_head, p.k_row, p.v_page, p.v_head, p.v_row})
+    if (s < 0 || s % 8) return MP_ERR_SHAPE;
+  for (const void *x : {c.q, static_cast<const void *>(p.k), static_cast<const void *>(p.v), static_cast<const void *>(c.out),
+                        static_cast<const void *>(c.workspace)})
+    if (!mp_aligned(x, 16)) return MP_ERR_ALIGN;
+  // byte offsets inside a page are 32 bits, and so are a head's tiles
+  const int64_t grp = c.nh / c.kvh, reach = (int64_t(1) << 30) - 256, span = int64_t(1) << shift;
+  if (p.k_row > reach / span || p.v_row > reach / span) return MP_ERR_SHAPE;
+  if (c.rows * c.nh > INT32_MAX - kRows) return MP_ERR_SHAPE;
+  if (masked_items(c.rows, grp, c.batch) * mp_cdiv(p.width << shift, kTile) > INT32_MAX) return MP_ERR_SHAPE;
+  if (c.rows == 0) return MP_OK;
+  if (mp_cu_count() <= 0) return MP_ERR_HIP;
+  if (c.workspace_bytes < masked_workspace(c.rows, c.nh, c.kvh, c.head_dim, c.batch)) return MP_ERR_WORKSPACE;
+#define MP_MASKED(DT)                                                        \
+  return c.head_dim == 64 ? masked_start<64, DT, MODE>(c, shift)             \
+                          : c.head_dim == 128 ? masked_start<128, DT, MODE>(c, shift) : masked_start<256, DT, MODE>(c, shift)
+  if (c.dtype == MP_F16) MP_MASKED(MP_F16);
+  MP_MASKED(MP_BF16);
+#undef MP_MASKED
+}
+
+}  // namespace
+
+extern "C" size_t mp_masked_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch) {
+  if (rows <= 0 || rows > INT32_MAX || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || batch <= 0 || batch > INT32_MAX ||
+      mp_cu_count() <= 0)
+    return 0;
+  return masked_workspace(rows, nh, kvh, head_dim, batch);
+}
+
+extern "C" int mp_paged_tree_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh, int head_dim,
+                                       const mp_pages *cache, const int32_t *lens, const int32_t *starts, int64_t batch,
+                                       const int64_t *masks, int64_t words, float scale, void *out, int dtype, void *workspace,
+                                       size_t workspace_bytes, mp_stream_t stream) {
+  if (!masks) return MP_ERR_ARG;
+  if (words < 1 || words > 1024) return MP_ERR_SHAPE;
+  return masked_launch<kTree>({q, q_row, q_head, rows, nh, kvh, head_dim, cache, lens, starts, batch,
+                               {masks, static_cast<int>(words), 0, 0}, scale, out, dtype, workspace, workspace_bytes,
+                               reinterpret_cast<hipStream_t>(stream)});
+}
+
+extern "C" int mp_paged_prompt_window_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh,
+                                                int head_dim, const mp_pages *cache, const int32_t *lens, const int32_t *starts,
+                                                int64_t batch, int64_t window, int64_t sinks, float scale, void *out, int dtype,
+                                                void *workspace, size_t workspace_bytes, mp_stream_t stream) {
+  if (window < 1 || window > 1 << 30 || sinks < 0 || sinks > 1 << 30) return MP_ERR_SHAPE;
+  return masked_launch<kWindow>({q, q_row, q_head, rows, nh, kvh, head_dim, cache, lens, starts, batch,
+                                 {nullptr, 0, static_cast<int>(window), static_cast<int>(sinks)}, scale, out, dtype, workspace,
+                                 workspace_bytes, reinterpret_cast<hipStream_t>(stream)});
+}

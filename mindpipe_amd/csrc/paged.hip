@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(
     const float *__restrict__ sin_t, int half, int64_t angles, uint16_t *__restrict__ q_out, uint16_t *__restrict__ k_pages,
     int64_t kpage, int64_t khead, int64_t krow, uint16_t *__restrict__ v_pages, int64_t vpage, int64_t vhead, int64_t vrow,
     int pages, int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
-    const int32_t *__restrict__ starts, int batch) {
+    const int32_t *__restrict__ starts, int batch, const int32_t *__restrict__ turns) {
   const int t = blockIdx.x, per = dim / 16;
   int seq = t, end = t + 1;
   if (starts) seq = seq_of_row(starts, batch, t, end);
@@ -54,11 +54,12 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(
   const bool turn = head < nh + kvh && at < 2 * half;
   const int d0 = turn && !PAIRS ? at / 2 : at, d1 = turn && !PAIRS ? half + at / 2 : at + 8;
   uint4 lo = *reinterpret_cast<const uint4 *>(x + d0), hi = *reinterpret_cast<const uint4 *>(x + d1);
-  const bool angle = pos >= 0 && pos < angles;
+  const int64_t by = turns ? turns[t] : pos;  // the position that it turns by
+  const bool angle = pos >= 0 && by >= 0 && by < angles;
   if (turn && angle) {
     float c[8], s[8];
-    const float4 *cp = reinterpret_cast<const float4 *>(cos_t + pos * half + at / 2);
-    const float4 *sp = reinterpret_cast<const float4 *>(sin_t + pos * half + at / 2);
+    const float4 *cp = reinterpret_cast<const float4 *>(cos_t + by * half + at / 2);
+    const float4 *sp = reinterpret_cast<const float4 *>(sin_t + by * half + at / 2);
     const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
     c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
     s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
@@ -114,11 +115,41 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(
 constexpr int kWaves = 4;
 constexpr int kBlock = 32 * kWaves;
 
+// With a window (WIN) a sequence sees its last `window` positions and its first `sinks`.  What lies between them is left out of its
+// blocks in steps of 32, a wave's tile: 64 sequences of up to 16384 positions with a window of 4096 read what those see and no
+// more than 62 positions each besides.
+struct DecodeSeen {  // of one sequence: SeenUpTo with a window
+  int len, sinks, low;    // seen: below len, and below sinks or from low on
+  int gap_from, gap;      // virtual positions from gap_from on lie `gap` further
+  __device__ __forceinline__ int place(int v) const { return v < gap_from ? v : v + gap; }
+  __device__ __forceinline__ void look(int) {}
+  __device__ __forceinline__ bool sees(int p) const { return p < len && (p < sinks || p >= low); }
+  __device__ __forceinline__ bool any(int p) const { return sees(p); }
+  __device__ __forceinline__ bool whole(int tile) const { return tile + 32 <= len && (tile + 32 <= sinks || tile >= low); }
+};
+template <bool WIN>
 struct DecodePlan {
   const int32_t *lens;
   int batch, capacity;  // capacity: positions that the table has room for
+  int window, sinks;
   __device__ __forceinline__ int len(int b) const { return min(max(lens[b], 0), capacity); }
-  __device__ __forceinline__ int operator()(int b, int) const { return max((len(b) + kBlock - 1) / kBlock, 1); }
+  __device__ __forceinline__ DecodeSeen seen(int b) const {
+    DecodeSeen s;
+    s.len = len(b);
+    s.sinks = sinks;
+    s.low = min(max(lens[b], 0) - min(window, max(lens[b], 0)), capacity);  // the window ends at the sequence's end, whatever the table holds
+    const int low = min(s.low, s.len) & ~31;
+    s.gap_from = min((min(sinks, s.len) + 31) & ~31, low);
+    s.gap = low - s.gap_from;
+    return s;
+  }
+  // positions to look at
+  __device__ __forceinline__ int reach(int b) const {
+    if constexpr (!WIN) return len(b);
+    const DecodeSeen s = seen(b);
+    return s.len - s.gap;
+  }
+  __device__ __forceinline__ int operator()(int b, int) const { return max((reach(b) + kBlock - 1) / kBlock, 1); }
   __device__ __forceinline__ uint32_t blocks() const {
     uint32_t n = 0;
     for (int b = threadIdx.x & 63; b < batch; b += 64) n += (*this)(b, 0);
@@ -134,17 +165,17 @@ inline int decode_share(int64_t heads, int dim) {
   return static_cast<int>(n > 1 ? n : 1);
 }
 
-template <int D, int DT>
+template <int D, int DT, bool WIN>
 __global__ __launch_bounds__(64 * kWaves, decode_round(D)) void paged_decode_kernel(
     const uint16_t *__restrict__ q, int64_t q_row, int64_t q_head, const uint16_t *__restrict__ k_pages, int64_t kpage,
     int64_t khead, int64_t krow, const uint16_t *__restrict__ v_pages, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
     int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens, int batch, int kvh, int grp,
-    int tiles, int share, float scale2, float *__restrict__ part_o, float *__restrict__ part_ml, int4 *__restrict__ joins,
+    int tiles, int share, int window, int sinks, float scale2, float *__restrict__ part_o, float *__restrict__ part_ml, int4 *__restrict__ joins,
     uint16_t *__restrict__ out) {
   extern __shared__ float sm[];  // [kWaves][rows][D] outputs, then [kWaves][rows][2] maxima and sums
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, j = lane >> 4;
   const int heads = kvh * tiles, h = blockIdx.x % heads, kh = h / tiles, run = blockIdx.x / heads;
-  const DecodePlan plan{lens, batch, width << shift};
+  const DecodePlan<WIN> plan{lens, batch, width << shift, window, sinks};
   const uint64_t all = plan.blocks();
   share = static_cast<int>(min(static_cast<uint64_t>(share), all));  // no run is empty
   const int from = static_cast<int>(run * all / share), to = static_cast<int>((run + 1) * all / share);
@@ -158,7 +189,7 @@ __global__ __launch_bounds__(64 * kWaves, decode_round(D)) void paged_decode_ker
   for (int left = to - from; left > 0; ++b, at = 0) {
     const int len = plan.len(b);
     blocks = plan(b, 0);
-    const int end = min(at + left, blocks), t1 = min(end * kBlock, len);
+    const int end = min(at + left, blocks), t1 = min(end * kBlock, plan.reach(b));
     const bool whole = at == 0 && end == blocks;
     uint4 qf[D / 32];
     const uint16_t *qp = q + b * q_row + static_cast<int64_t>(kh * grp + g0 + min(i16, rows - 1)) * q_head + 8 * j;
@@ -168,7 +199,8 @@ __global__ __launch_bounds__(64 * kWaves, decode_round(D)) void paged_decode_ker
     src.last = len > 0 ? (len - 1) >> shift : 0;
     AttnRows<D> a;
     attn_clear(a);
-    attn_walk<D, DT, false>(a, src, qf, at * kBlock + 32 * wave, t1, kBlock, t1, t1, t1, scale2, lane);
+    if constexpr (WIN) attn_walk<D, DT, false>(a, src, qf, at * kBlock + 32 * wave, t1, kBlock, plan.seen(b), scale2, lane);
+    else attn_walk<D, DT, false>(a, src, qf, at * kBlock + 32 * wave, t1, kBlock, SeenUpTo{t1, t1, t1}, scale2, lane);
     a.l = attn_row_sum(a.l);
 
     // the four waves' states meet
@@ -285,10 +317,10 @@ inline int page_shift(int page) {
 
 }  // namespace
 
-extern "C" int mp_paged_rope_append(const void *qkv, int64_t qkv_row, int64_t rows, int nh, int kvh, int head_dim,
-                                    const float *cos_t, const float *sin_t, int rotary, int64_t angles, int pairs,
-                                    void *q_out, const mp_pages *cache, const int32_t *lens, const int32_t *starts,
-                                    int64_t batch, int dtype, mp_stream_t stream) {
+extern "C" int mp_paged_rope_append_at(const void *qkv, int64_t qkv_row, int64_t rows, int nh, int kvh, int head_dim,
+                                       const float *cos_t, const float *sin_t, int rotary, int64_t angles, int pairs,
+                                       void *q_out, const mp_pages *cache, const int32_t *lens, const int32_t *starts,
+                                       int64_t batch, const int32_t *turns, int dtype, mp_stream_t stream) {
   if (!qkv || !cos_t || !sin_t || !q_out || !cache || !cache->k || !cache->v || !cache->table || !lens) return MP_ERR_ARG;
   if (dtype != MP_F16 && dtype != MP_BF16) return MP_ERR_DTYPE;
   const int shift = page_shift(cache->page_size);
@@ -313,7 +345,7 @@ extern "C" int mp_paged_rope_append(const void *qkv, int64_t qkv_row, int64_t ro
                      static_cast<uint16_t *>(cache->k), cache->k_page, cache->k_head, cache->k_row,                      \
                      static_cast<uint16_t *>(cache->v), cache->v_page, cache->v_head, cache->v_row,                      \
                      static_cast<int>(cache->pages), shift, cache->table, static_cast<int>(cache->width), lens, starts,  \
-                     static_cast<int>(batch))
+                     static_cast<int>(batch), turns)
   if (dtype == MP_F16) {
     if (pairs) MP_APPEND(MP_F16, true);
     else MP_APPEND(MP_F16, false);
@@ -326,6 +358,14 @@ extern "C" int mp_paged_rope_append(const void *qkv, int64_t qkv_row, int64_t ro
   return MP_OK;
 }
 
+extern "C" int mp_paged_rope_append(const void *qkv, int64_t qkv_row, int64_t rows, int nh, int kvh, int head_dim,
+                                    const float *cos_t, const float *sin_t, int rotary, int64_t angles, int pairs,
+                                    void *q_out, const mp_pages *cache, const int32_t *lens, const int32_t *starts,
+                                    int64_t batch, int dtype, mp_stream_t stream) {
+  return mp_paged_rope_append_at(qkv, qkv_row, rows, nh, kvh, head_dim, cos_t, sin_t, rotary, angles, pairs, q_out, cache, lens,
+                                 starts, batch, nullptr, dtype, stream);
+}
+
 extern "C" size_t mp_paged_decode_workspace_bytes(int64_t batch, int nh, int kvh, int head_dim) {
   const int cus = mp_cu_count();
   if (batch <= 0 || batch > INT32_MAX || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || cus <= 0) return 0;
@@ -334,9 +374,12 @@ extern "C" size_t mp_paged_decode_workspace_bytes(int64_t batch, int nh, int kvh
          static_cast<size_t>(batch * heads) * sizeof(int4);
 }
 
-extern "C" int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q_head, int64_t batch, int nh, int kvh,
-                                         int head_dim, const mp_pages *cache, const int32_t *lens, float scale, void *out,
-                                         int dtype, void *workspace, size_t workspace_bytes, mp_stream_t stream) {
+namespace {
+
+template <bool WIN>
+int decode_launch(const void *q, int64_t q_row, int64_t q_head, int64_t batch, int nh, int kvh, int head_dim, const mp_pages *cache,
+                  const int32_t *lens, int window, int sinks, float scale, void *out, int dtype, void *workspace,
+                  size_t workspace_bytes, mp_stream_t stream) {
   if (!q || !cache || !cache->k || !cache->v || !cache->table || !lens || !out || !workspace) return MP_ERR_ARG;
   if (dtype != MP_F16 && dtype != MP_BF16) return MP_ERR_DTYPE;
   if (!std::isfinite(scale * kLog2e)) return MP_ERR_ARG;
@@ -364,15 +407,15 @@ extern "C" int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define MP_DECODE(D, DT)                                                                                                  \
   do {                                                                                                                    \
-    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(paged_decode_kernel<D, DT>),               \
+    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(paged_decode_kernel<D, DT, WIN>),               \
                                                hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)            \
       return MP_ERR_HIP;                                                                                                  \
-    hipLaunchKernelGGL((paged_decode_kernel<D, DT>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),              \
+    hipLaunchKernelGGL((paged_decode_kernel<D, DT, WIN>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),              \
                        lds, s, static_cast<const uint16_t *>(q), q_row, q_head,        \
                        static_cast<const uint16_t *>(cache->k), cache->k_page, cache->k_head, cache->k_row,               \
                        static_cast<const uint16_t *>(cache->v), cache->v_page, cache->v_head, cache->v_row,               \
                        static_cast<int>(cache->pages), shift, cache->table, static_cast<int>(cache->width), lens,         \
-                       static_cast<int>(batch), kvh, grp, tiles, static_cast<int>(share), scale2, part_o, part_ml, joins,                    \
+                       static_cast<int>(batch), kvh, grp, tiles, static_cast<int>(share), window, sinks, scale2, part_o, part_ml, joins,                    \
                        static_cast<uint16_t *>(out));                                                                     \
     MP_CHECK_LAUNCH();                                                                                                    \
     if (capacity > kBlock) { /* else every sequence is one block */                                                       \
@@ -392,4 +435,22 @@ extern "C" int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q
   }
 #undef MP_DECODE
   return MP_OK;
+}
+
+}  // namespace
+
+extern "C" int mp_paged_decode_attention(const void *q, int64_t q_row, int64_t q_head, int64_t batch, int nh, int kvh,
+                                         int head_dim, const mp_pages *cache, const int32_t *lens, float scale, void *out,
+                                         int dtype, void *workspace, size_t workspace_bytes, mp_stream_t stream) {
+  return decode_launch<false>(q, q_row, q_head, batch, nh, kvh, head_dim, cache, lens, 0, 0, scale, out, dtype, workspace,
+                              workspace_bytes, stream);
+}
+
+extern "C" int mp_paged_decode_window_attention(const void *q, int64_t q_row, int64_t q_head, int64_t batch, int nh, int kvh,
+                                                int head_dim, const mp_pages *cache, const int32_t *lens, int64_t window,
+                                                int64_t sinks, float scale, void *out, int dtype, void *workspace,
+                                                size_t workspace_bytes, mp_stream_t stream) {
+  if (window < 1 || window > 1 << 30 || sinks < 0 || sinks > 1 << 30) return MP_ERR_SHAPE;
+  return decode_launch<true>(q, q_row, q_head, batch, nh, kvh, head_dim, cache, lens, static_cast<int>(window),
+                             static_cast<int>(sinks), scale, out, dtype, workspace, workspace_bytes, stream);
 }

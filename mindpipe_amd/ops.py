@@ -1170,10 +1170,16 @@ def _need_starts(starts: torch.Tensor, like: torch.Tensor, batch: Optional[int])
     return n - 1
 
 
+def _pools_changed(*pools: torch.Tensor) -> None:
+    for t in pools:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)  # a backward that saved the pool notices
+
+
 @_op("paged_rope_append", "mindpipe_amd_serve", mutates=("k_pages", "v_pages"))
 def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                       table: torch.Tensor, lens: torch.Tensor, starts: Optional[torch.Tensor] = None,
-                      pairs: bool = True) -> torch.Tensor:
+                      pairs: bool = True, turns: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotates the queries and keys of packed new tokens, writes keys and values into a paged cache and returns the
     rotated queries ``[rows, nh, dim]``.
 
@@ -1184,7 +1190,8 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
     ascending) are the last positions of sequence b; without ``starts`` each sequence has one row.  The first ``2 *
     cos.shape[1]`` values of a head turn by ``cos`` / ``sin`` fp32 ``[positions, rotary / 2]`` of the token's position, in
     fp32 with one rounding: values ``(2 i, 2 i + 1)`` as ``decode_rope_append`` pairs them, or with ``pairs=False``
-    ``(i, i + rotary / 2)``.
+    ``(i, i + rotary / 2)``.  With ``turns`` (int32 ``[rows]``) a row turns by the angles of that position in place of its own, as
+    the nodes of a drafted tree turn by their depth (``paged_tree_attention``).
 
     Rows behind the last sequence, and positions without an angle, give zero queries and leave the cache as it is, and so
     do the keys and values of a position past the table's width or in a page whose number is not the pool's.
@@ -1209,23 +1216,25 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
         _need_starts(starts, qkv, batch)
     elif rows != batch:
         raise RuntimeError(f"without starts each of the {batch} sequences has one row, got {rows}")
+    if turns is not None:
+        _need_plain(turns, "turns", qkv, torch.int32, 1)
+        if turns.shape[0] != rows:
+            raise RuntimeError(f"turns must have one position for each of the {rows} rows, got {tuple(turns.shape)}")
     if not batch:
         return torch.zeros((rows, nh, dim), dtype=qkv.dtype, device=qkv.device)
     q = qkv.new_empty((rows, nh, dim))
     if rows:
         with _dev(qkv):
-            _lib.check(_lib.load().mp_paged_rope_append(
+            _lib.check(_lib.load().mp_paged_rope_append_at(
                 qkv.data_ptr(), qkv.stride(0) if rows > 1 else values, rows, nh, kvh, dim, cos.data_ptr(),
                 sin.data_ptr(), 2 * half, angles, int(pairs), q.data_ptr(), cache, lens.data_ptr(),
-                _ptr(starts), batch, _DT[qkv.dtype], _stream()), "mp_paged_rope_append")
-        for t in (k_pages, v_pages):
-            if not t.is_inference():
-                torch.autograd.graph.increment_version(t)  # a backward that saved the pool notices
+                _ptr(starts), batch, _ptr(turns), _DT[qkv.dtype], _stream()), "mp_paged_rope_append_at")
+        _pools_changed(k_pages, v_pages)
     return q
 
 
 @paged_rope_append.register_fake
-def _(qkv, cos, sin, k_pages, v_pages, table, lens, starts=None, pairs=True):
+def _(qkv, cos, sin, k_pages, v_pages, table, lens, starts=None, pairs=True, turns=None):
     dim = k_pages.shape[3]
     return qkv.new_empty((qkv.shape[0], qkv.shape[1] // dim - 2 * k_pages.shape[1], dim))
 
@@ -1325,6 +1334,263 @@ def _(q, k_pages, v_pages, table, lens, starts, scale):
     return q.new_empty(q.shape)
 
 
+def _need_window(window: int, sinks: int) -> None:
+    if not 1 <= window <= 1 << 30 or not 0 <= sinks <= 1 << 30:
+        raise RuntimeError(f"a window has 1 to 2^30 positions and 0 to 2^30 sinks before it, got {window} and {sinks}")
+
+
+@_op("paged_decode_window_attention", "mindpipe_amd_serve")
+def paged_decode_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                                  lens: torch.Tensor, scale: float, window: int, sinks: int = 0) -> torch.Tensor:
+    """``paged_decode_attention`` over the last ``window`` of each sequence's ``lens[b]`` positions and its first ``sinks``.  What
+    lies between is not read, and pages that hold nothing else may be gone (any number outside the pool in the table)."""
+    _need_strided(q, "q", _HALF, 3)
+    cache = _paged_cache(k_pages, v_pages, table, lens, q)
+    b, nh, dim = q.shape
+    kvh = k_pages.shape[1]
+    _attention_heads(q, kvh, k_pages.shape[3])
+    _need_window(window, sinks)
+    if lens.shape[0] != b:
+        raise RuntimeError(f"q {tuple(q.shape)} and lens {tuple(lens.shape)} must have one row per sequence")
+    out = q.new_empty((b, nh, dim))
+    if not b:
+        return out
+    lib, qs = _lib.load(), _steps(q)
+    with _dev(q):
+        wsb = lib.mp_paged_decode_workspace_bytes(b, nh, kvh, dim)
+        ws = torch.empty((wsb,), dtype=torch.uint8, device=q.device)
+        _lib.check(lib.mp_paged_decode_window_attention(
+            q.data_ptr(), qs[0], qs[1], b, nh, kvh, dim, cache, lens.data_ptr(), window, sinks, scale, out.data_ptr(),
+            _DT[q.dtype], ws.data_ptr(), wsb, _stream()), "mp_paged_decode_window_attention")
+    return out
+
+
+@paged_decode_window_attention.register_fake
+def _(q, k_pages, v_pages, table, lens, scale, window, sinks=0):
+    return q.new_empty(q.shape)
+
+
+@_op("paged_prompt_window_attention", "mindpipe_amd_serve")
+def paged_prompt_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                                  lens: torch.Tensor, starts: torch.Tensor, scale: float, window: int,
+                                  sinks: int = 0) -> torch.Tensor:
+    """``paged_prompt_attention`` where each row sees, of the positions up to its own, the last ``window`` (its own among
+    them) and the first ``sinks`` of the sequence.  What no row sees is not read, and pages that hold nothing else may be gone."""
+    _need_strided(q, "q", _HALF, 3)
+    cache = _paged_cache(k_pages, v_pages, table, lens, q)
+    batch = _need_starts(starts, q, lens.shape[0])
+    rows, nh, dim = q.shape
+    kvh = k_pages.shape[1]
+    _attention_heads(q, kvh, k_pages.shape[3])
+    _need_window(window, sinks)
+    if not batch or not rows:
+        return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
+    out, qs, lib = q.new_empty((rows, nh, dim)), _steps(q), _lib.load()
+    with _dev(q):
+        wsb = lib.mp_masked_workspace_bytes(rows, nh, kvh, dim, batch)
+        ws = torch.empty((wsb,), dtype=torch.uint8, device=q.device)
+        _lib.check(lib.mp_paged_prompt_window_attention(
+            q.data_ptr(), qs[0], qs[1], rows, nh, kvh, dim, cache, lens.data_ptr(), starts.data_ptr(), batch, window, sinks, scale,
+            out.data_ptr(), _DT[q.dtype], ws.data_ptr(), wsb, _stream()), "mp_paged_prompt_window_attention")
+    return out
+
+
+@paged_prompt_window_attention.register_fake
+def _(q, k_pages, v_pages, table, lens, starts, scale, window, sinks=0):
+    return q.new_empty(q.shape)
+
+
+@_op("paged_tree_attention", "mindpipe_amd_serve")
+def paged_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                         starts: torch.Tensor, masks: torch.Tensor, scale: float) -> torch.Tensor:
+    """Attention of drafted tokens over a paged cache that holds them (``paged_rope_append``, with ``turns``).  The rows of
+    sequence b in ``q [rows, nh, dim]`` are its last positions of ``lens[b]``; each sees all positions before those, and of those
+    the ones whose bits are set in its row of ``masks`` (int64 ``[rows, words]``, up to 1024 words): bit ``i`` of word ``w`` is the
+    sequence's new token ``64 w + i``, for a tree the node itself and its ancestors, though any set will do.  Bits past the
+    sequence's new tokens are ignored.  Returns ``[rows, nh, dim]``; rows that see nothing, those of no sequence among them, are
+    zeros."""
+    _need_strided(q, "q", _HALF, 3)
+    cache = _paged_cache(k_pages, v_pages, table, lens, q)
+    batch = _need_starts(starts, q, lens.shape[0])
+    rows, nh, dim = q.shape
+    kvh = k_pages.shape[1]
+    _attention_heads(q, kvh, k_pages.shape[3])
+    _need_plain(masks, "masks", q, torch.int64, 2)
+    words = masks.shape[1]
+    if masks.shape[0] != rows or not 1 <= words <= 1024:
+        raise RuntimeError(f"masks must have 1 to 1024 words for each of the {rows} rows, got {tuple(masks.shape)}")
+    if not batch or not rows:
+        return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
+    out, qs, lib = q.new_empty((rows, nh, dim)), _steps(q), _lib.load()
+    with _dev(q):
+        wsb = lib.mp_masked_workspace_bytes(rows, nh, kvh, dim, batch)
+        ws = torch.empty((wsb,), dtype=torch.uint8, device=q.device)
+        _lib.check(lib.mp_paged_tree_attention(
+            q.data_ptr(), qs[0], qs[1], rows, nh, kvh, dim, cache, lens.data_ptr(), starts.data_ptr(), batch, masks.data_ptr(),
+            words, scale, out.data_ptr(), _DT[q.dtype], ws.data_ptr(), wsb, _stream()), "mp_paged_tree_attention")
+    return out
+
+
+@paged_tree_attention.register_fake
+def _(q, k_pages, v_pages, table, lens, starts, masks, scale):
+    return q.new_empty(q.shape)
+
+
+def _move_pools(k_pages: torch.Tensor, v_pages: torch.Tensor, table: Optional[torch.Tensor]):
+    """Checks the pools of one layer ``[pages, kvh, page, dim]`` or all ``[layers, pages, kvh, page, dim]``; what the C entry points
+    take: the first layer's description, layers, the strides from layer to layer, heads and their values."""
+    ndim = k_pages.dim() if isinstance(k_pages, torch.Tensor) else 0
+    if ndim != 5:
+        ndim = 4
+    _need_strided(k_pages, "k_pages", _HALF, ndim)
+    _need_strided(v_pages, "v_pages", k_pages.dtype, ndim)
+    if v_pages.shape != k_pages.shape:
+        raise RuntimeError(f"v_pages {tuple(v_pages.shape)} must have the shape of k_pages {tuple(k_pages.shape)}")
+    if v_pages.device != k_pages.device:
+        _same_device(k_pages, v_pages=v_pages)
+    pages, kvh, size, dim = k_pages.shape[-4:]
+    layers = k_pages.shape[0] if ndim == 5 else 1
+    if size < 8 or size > 32768 or size & (size - 1):
+        raise RuntimeError(f"a page holds a power of two of positions from 8 to 32768, got {size}")
+    if dim % 8 or not 8 <= dim <= 1024:
+        raise RuntimeError(f"heads of a multiple of 8 values up to 1024 are taken, got {dim}")
+    if not pages or not kvh or not layers:
+        raise RuntimeError("k_pages and v_pages must hold at least one layer, page and head")
+    ks, vs = _steps(k_pages), _steps(v_pages)
+    if any(n > 1 and not s for t, steps in ((k_pages, ks), (v_pages, vs)) for n, s in zip(t.shape, steps)):
+        raise RuntimeError("k_pages and v_pages are written to: no two of their values may lie in one place")
+    address, width = (0, 0) if table is None else (table.data_ptr(), table.shape[1])
+    cache = _lib.PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), *ks[-4:-1], *vs[-4:-1], pages, size, address, width)
+    return cache, layers, ks[0] if ndim == 5 else 0, vs[0] if ndim == 5 else 0, kvh, dim
+
+
+@_op("paged_copy_pages", "mindpipe_amd_serve", mutates=("k_pages", "v_pages"))
+def paged_copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+                     filled: Optional[torch.Tensor] = None) -> None:
+    """Copies pages ``src[i]`` of a paged cache to pages ``dst[i]`` (int32), keys and values, of one layer (``[pages, kvh, page,
+    dim]``, fp16 or bf16, strides as ``paged_rope_append`` takes them) or of all (``[layers, pages, kvh, page, dim]``); of each the
+    first ``filled[i]`` positions (int32), or all.  A sequence that is forked keeps its full pages in both tables and has the last
+    one copied.  Pairs with a number outside the pool are left out, so that a captured call may be padded with -1.  A
+    page that two pairs write, or that one reads and another writes, may hold either's values."""
+    cache, layers, k_layer, v_layer, kvh, dim = _move_pools(k_pages, v_pages, None)
+    _need_plain(src, "src", k_pages, torch.int32, 1)
+    _need_plain(dst, "dst", k_pages, torch.int32, 1)
+    if filled is not None:
+        _need_plain(filled, "filled", k_pages, torch.int32, 1)
+    n = src.shape[0]
+    if dst.shape[0] != n or (filled is not None and filled.shape[0] != n):
+        raise RuntimeError(f"src, dst and filled must have one entry for each copy, got {n}, {dst.shape[0]}"
+                           f"{'' if filled is None else f' and {filled.shape[0]}'}")
+    if n:
+        with _dev(k_pages):
+            _lib.check(_lib.load().mp_paged_copy_pages(
+                cache, layers, k_layer, v_layer, kvh, dim, src.data_ptr(), dst.data_ptr(), _ptr(filled), n, _stream()),
+                "mp_paged_copy_pages")
+        _pools_changed(k_pages, v_pages)
+
+
+@paged_copy_pages.register_fake
+def _(k_pages, v_pages, src, dst, filled=None):
+    return None
+
+
+@_op("paged_keep_positions", "mindpipe_amd_serve", mutates=("k_pages", "v_pages"))
+def paged_keep_positions(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, first: torch.Tensor, keep: torch.Tensor,
+                         starts: torch.Tensor) -> None:
+    """Moves positions of a paged cache to the front, of one layer or of all (pools as ``paged_copy_pages`` takes them): of
+    sequence b the keys and values at positions ``first[b] + keep[starts[b] + i]`` go to ``first[b] + i`` (int32; ``starts
+    [sequences + 1]`` ascends).  After a draft, ``first`` is where its nodes begin and ``keep`` names the ones that were
+    accepted, ascending; none of a sequence's entries may be below its place.  Positions past the table's width or of a page whose
+    number is not the pool's are left out.  Pages that are written must not be shared with another sequence."""
+    if not isinstance(table, torch.Tensor):
+        raise TypeError("table must be a tensor")
+    if isinstance(k_pages, torch.Tensor) and k_pages.is_cuda:
+        _need_plain(table, "table", k_pages, torch.int32, 2)
+    cache, layers, k_layer, v_layer, kvh, dim = _move_pools(k_pages, v_pages, table)
+    _need_plain(first, "first", k_pages, torch.int32, 1)
+    _need_plain(keep, "keep", k_pages, torch.int32, 1)
+    batch, width = table.shape
+    _need_starts(starts, k_pages, batch)
+    if first.shape[0] != batch:
+        raise RuntimeError(f"table {tuple(table.shape)} and first {tuple(first.shape)} must have one row per sequence")
+    if not width or width * k_pages.shape[-2] > 1 << 30:
+        raise RuntimeError(f"a sequence has 1 to 2^30 positions, the table has room for {width * k_pages.shape[-2]}")
+    total = keep.shape[0]
+    if batch and total:
+        with _dev(k_pages):
+            _lib.check(_lib.load().mp_paged_keep_positions(
+                cache, layers, k_layer, v_layer, kvh, dim, batch, first.data_ptr(), keep.data_ptr(), total, starts.data_ptr(),
+                _stream()), "mp_paged_keep_positions")
+        _pools_changed(k_pages, v_pages)
+
+
+@paged_keep_positions.register_fake
+def _(k_pages, v_pages, table, first, keep, starts):
+    return None
+
+
+def _need_logits(logits: torch.Tensor) -> int:
+    """Checks rows of logits; their stride."""
+    if not isinstance(logits, torch.Tensor):
+        raise TypeError("logits must be a tensor")
+    if not logits.is_cuda:
+        raise RuntimeError("logits must be on the GPU (mindpipe_amd has no CPU path)")
+    if logits.dtype not in _DT or logits.dim() != 2:
+        raise RuntimeError(f"logits must be fp16, bf16 or fp32 [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    stride = logits.stride(0) if rows > 1 else vocab
+    if vocab < 1 or vocab > 1 << 19 or (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
+        raise RuntimeError(f"logits must be rows of 1 to 2^19 contiguous values, got {tuple(logits.shape)} with strides "
+                           f"{logits.stride()}")
+    return stride
+
+
+@_op("beam_select", "mindpipe_amd_serve")
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int, ended: Optional[torch.Tensor] = None,
+                pad: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``count`` best continuations (1 to 64) of each request over its beams (1 to 64) and the vocabulary: ``(scores fp32,
+    beams int64, tokens int64)``, each ``[requests, count]``, from the largest total down; of equal ones those of the lowest
+    beam, then token.
+
+    ``logits [requests * beams, vocab]`` (fp16, bf16 or fp32; rows may be strided) and ``scores`` fp32 ``[requests, beams]``; a
+    total is the beam's score and the logarithm of the token's share of its row, made in 64 bits.  A beam that has ``ended``
+    (bool ``[requests, beams]``) has one continuation, the token ``pad``, of its own score; a beam of score ``-inf`` has none (the
+    beams of a request that begins: one of score 0, the others ``-inf``).  NaN and ``-inf`` are never taken; where fewer than
+    ``count`` are left, scores are ``-inf`` and beams and tokens -1.  With infinite logits in a row those share its weight."""
+    stride = _need_logits(logits)
+    _need_plain(scores, "scores", logits, torch.float32, 2)
+    (rows, vocab), (batch, beams) = logits.shape, scores.shape
+    if not 1 <= beams <= 64 or not 1 <= count <= 64:
+        raise RuntimeError(f"1 to 64 beams and continuations are taken, got {beams} and {count}")
+    if rows != batch * beams:
+        raise RuntimeError(f"logits {tuple(logits.shape)} must have a row for each of scores {tuple(scores.shape)}")
+    if not 0 <= pad < vocab:
+        raise RuntimeError(f"pad must be a token of the {vocab}, got {pad}")
+    if ended is not None:
+        _need_plain(ended, "ended", logits, torch.bool, 2)
+        if ended.shape != scores.shape:
+            raise RuntimeError(f"ended {tuple(ended.shape)} must have the shape of scores {tuple(scores.shape)}")
+    best = scores.new_empty((batch, count))
+    parents = torch.empty((batch, count), dtype=torch.int64, device=logits.device)
+    tokens = torch.empty((batch, count), dtype=torch.int64, device=logits.device)
+    if batch:
+        lib = _lib.load()
+        with _dev(logits):
+            dt = _DT[logits.dtype]
+            wsb = lib.mp_beam_select_workspace_bytes(batch, beams, vocab, count, dt)
+            ws = torch.empty((wsb,), dtype=torch.uint8, device=logits.device)
+            _lib.check(lib.mp_beam_select(
+                logits.data_ptr(), stride, batch, beams, vocab, dt, scores.data_ptr(), _ptr(ended), pad, count, best.data_ptr(),
+                parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), wsb, _stream()), "mp_beam_select")
+    return best, parents, tokens
+
+
+@beam_select.register_fake
+def _(logits, scores, count, ended=None, pad=0):
+    shape = (scores.shape[0], count)
+    return (scores.new_empty(shape), logits.new_empty(shape, dtype=torch.int64), logits.new_empty(shape, dtype=torch.int64))
+
+
 @_op("sample_tokens", "mindpipe_amd_serve")
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
                   top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
@@ -1339,17 +1605,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[t
     what is kept exceeds ``u`` times the whole, and its logprob the logarithm of its share (0 with ``temperature <= 0``).
     Weights are summed in units of 2^-44 of the largest: a token of less than half of that is never taken, nor are NaN and
     ``-inf``; a row of nothing else gives -1 and ``-inf``.  The same inputs give the same tokens."""
-    if not isinstance(logits, torch.Tensor):
-        raise TypeError("logits must be a tensor")
-    if not logits.is_cuda:
-        raise RuntimeError("logits must be on the GPU (mindpipe_amd has no CPU path)")
-    if logits.dtype not in _DT or logits.dim() != 2:
-        raise RuntimeError(f"logits must be fp16, bf16 or fp32 [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
+    stride = _need_logits(logits)
     rows, vocab = logits.shape
-    stride = logits.stride(0) if rows > 1 else vocab
-    if vocab < 1 or vocab > 1 << 19 or (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
-        raise RuntimeError(f"logits must be rows of 1 to 2^19 contiguous values, got {tuple(logits.shape)} with strides "
-                           f"{logits.stride()}")
     for name, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
                         ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
         if t is not None or name == "u":
