@@ -73,7 +73,7 @@ def _stale(src: Path) -> bool:
     obj = BUILD_DIR / (src.stem + ".o")
     if not obj.exists():
         return True
-    deps = [src, *CSRC.glob("*.h"), PKG.parent / "include" / "mindpipe_amd.h", Path(__file__)]
+    deps = [src, *CSRC.glob("*.h"), *CSRC.glob("*.inc"), PKG.parent / "include" / "mindpipe_amd.h", Path(__file__)]
     return any(d.stat().st_mtime > obj.stat().st_mtime for d in deps if d.exists())
 
 

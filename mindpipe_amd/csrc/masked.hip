@@ -4,13 +4,17 @@
 //     mask names (a node's ancestors and itself);
 //   * windows: a row sees the last `window` positions up to its own, and the first `sinks`.
 //
-// The products are those of prompt.hip (prompt_tile.h): rows are tokens times the heads that share a key-value head, 32 to a
-// wave and kRows to a workgroup, over tiles of 64 positions in LDS.  What a row sees of a tile is a word of 64 bits.
+// The queries of the heads that share a key-value head are rows of one problem: row = token * group + head.  Two forms:
 //
-// Work is cut into equal runs.  An item is up to kRows rows of a sequence and key-value head; its tiles, those that hold
-// nothing seen left out, follow each other, and so do the items.  The workgroups of a head take equal runs of that row of tiles,
-// however ragged the sequences are.  An item that lies in several runs is joined from its parts: a workgroup leaves at most
-// two, that of the item its run begins inside of (slot 2 w) and that of the item its run ends inside of (slot 2 w + 1).
+//   * wide: the products of prompt.hip (prompt_tile.h), 128 rows to a workgroup, 32 to a wave, over tiles of 64 positions in LDS;
+//   * narrow: those of the decode kernel (attn_common.h), 16 rows to a workgroup, whose four waves take 32 positions each of a
+//     tile of 128, from memory to registers.
+//
+// An item is up to 128 (16) rows of a sequence and key-value head.  It walks over the tiles that hold what its rows see, those that
+// hold nothing seen left out.  Items that are much longer than an equal share of all tiles are cut into parts, which leave their
+// outputs, unnormalised, maxima and sums in the workspace, and a second launch joins them, always in the same order.  A
+// workgroup takes a part, and the longest come first, so that the short ones fill what the long ones leave.
+#include <algorithm>
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -70,16 +74,35 @@ struct MaskedSeq {
       gap_from = min((min(rule.sinks, to) + 63) & ~63, gap_to);
     }
   }
-  // All of tile t (64 positions) is seen by tokens a .. b.
-  __device__ __forceinline__ bool whole(int a, int b, int t) const {
-    if (t + 64 > end()) return false;
-    if constexpr (MODE == kTree) return t + 64 <= context();
+  // All of positions t .. upto - 1 are seen by tokens a .. b.
+  __device__ __forceinline__ bool whole(int a, int b, int t, int upto) const {
+    if (upto > end()) return false;
+    if constexpr (MODE == kTree) return upto <= context();
     const int64_t pos = context();
-    return t + 64 <= pos + a + 1 && (t + 64 <= rule.sinks || t >= pos + b - rule.window + 1);
+    return upto <= pos + a + 1 && (upto <= rule.sinks || t >= pos + b - rule.window + 1);
   }
 };
 
+// The form of a kernel: rows of an item, positions of a tile, and by how many tiles an item may pass an equal share and stay whole
+// (half a share at most): joining costs what so many tiles do.
+struct Wide {
+  static constexpr int kItem = kRows, kStep = kTile, kSlack = 8;
+};
+struct Narrow {
+  static constexpr int kItem = 16, kStep = 128, kSlack = 2;
+};
+
+// What a workgroup takes: tiles of an item.
 template <int MODE>
+struct MaskedPart {
+  MaskedSeq<MODE> seq;
+  int b, item, part, parts;
+  int slot;               // of the part, if there are others
+  int to, gap_from, gap;  // positions looked at lie below `to`; virtual positions from gap_from on lie `gap` further
+  int from, end;          // virtual positions of the part
+};
+
+template <int MODE, class FORM>
 struct MaskedPlan {
   PackedPlan rows;
   const int32_t *lens;
@@ -96,37 +119,79 @@ struct MaskedPlan {
     return s;
   }
   __device__ __forceinline__ int items(const MaskedSeq<MODE> &s) const {
-    return static_cast<int>((static_cast<int64_t>(s.n) * rows.grp + kRows - 1) / kRows);
+    return static_cast<int>((static_cast<int64_t>(s.n) * rows.grp + FORM::kItem - 1) / FORM::kItem);
   }
-  // Tiles of an item (one at least, which writes its zeros), with the gap among them.
-  __device__ __forceinline__ int tiles(const MaskedSeq<MODE> &s, int item, int &to, int &gap_from, int &gap_to) const {
-    const int a = item * kRows / rows.grp, b = min((item * kRows + kRows - 1) / rows.grp, s.n - 1);
+  // The tokens of an item, and where it looks.
+  __device__ __forceinline__ void span(const MaskedSeq<MODE> &s, int item, int &to, int &gap_from, int &gap) const {
+    const int a = item * FORM::kItem / rows.grp, b = min((item * FORM::kItem + FORM::kItem - 1) / rows.grp, s.n - 1);
+    int gap_to;
     s.span(a, b, to, gap_from, gap_to);
-    return max((to - (gap_to - gap_from) + kTile - 1) / kTile, 1);
+    gap = gap_to - gap_from;
   }
-  __device__ __forceinline__ int tiles(const MaskedSeq<MODE> &s, int item) const {
-    int to, from, upto;
-    return tiles(s, item, to, from, upto);
+  // Tiles of a sequence's longest item: its last one's, one more at most where windows begin inside of a tile.  One at least.
+  __device__ __forceinline__ int tiles(const MaskedSeq<MODE> &s, int items) const {
+    int to, from, gap;
+    span(s, items - 1, to, from, gap);
+    return max((to - gap + FORM::kStep - 1) / FORM::kStep, 1);
   }
-  // Tiles of a sequence.  Its items are at most (rows grp) / kRows + 1, the launch holds their tiles below 2^31.
-  __device__ __forceinline__ int operator()(int b, int) const {
-    const MaskedSeq<MODE> s = seq(b);
-    const int n = items(s);
-    if (n == 0) return 0;
-    if constexpr (MODE == kTree) return n * tiles(s, 0);
-    int sum = 0;
-    for (int i = 0; i < n; ++i) sum += tiles(s, i);
-    return sum;
-  }
-  // Tiles of all; 0 where the offsets do not ascend (then the sequences' rows add up to more than there are).
-  __device__ __forceinline__ uint32_t all() const {
-    uint32_t n = 0;
-    uint64_t held = 0;
-    for (int b = threadIdx.x & 63; b < rows.batch + 2; b += 64) {
-      n += (*this)(b, 0);
-      held += rows.end(b) - rows.first(b);
+  // The part that this workgroup, number `at` of its head's, takes.  `share`: workgroups of a head that the card holds at once.
+  // Uniform; every wave looks at all sequences, one a lane.
+  __device__ __forceinline__ bool find(int at, int share, MaskedPart<MODE> &p) const {
+    const int lane = threadIdx.x & 63, n = rows.batch + 2;
+    struct Row {
+      int items, tiles;
+    };
+    const auto row = [&](int b) {
+      Row r{0, 1};
+      if (b < n) {
+        const MaskedSeq<MODE> s = seq(b);
+        r.items = items(s);
+        if (r.items) r.tiles = tiles(s, r.items);
+      }
+      return r;
+    };
+    const Row near = row(lane);
+    uint64_t all = 0, held = 0;
+    for (int b0 = 0; b0 < n; b0 += 64) {
+      const Row r = b0 ? row(b0 + lane) : near;
+      all += static_cast<uint64_t>(r.items) * r.tiles;
+      held += b0 + lane < n ? rows.end(b0 + lane) - rows.first(b0 + lane) : 0;
     }
-    return wave_sum(held) == static_cast<uint64_t>(rows.rows) ? wave_sum(n) : 0;
+    all = wave_sum(all);
+    // offsets that do not ascend: the sequences' rows add up to more than there are
+    if (wave_sum(held) != static_cast<uint64_t>(rows.rows)) return false;
+    const int equal = static_cast<int>(all / share), limit = equal + min(equal / 2, FORM::kSlack) + 1;
+    const auto parts = [&](const Row &r) { return r.tiles > limit ? (r.tiles + limit - 1) / limit : 1; };
+    const int index = at;
+    for (int order = 0; order < 4; ++order) {  // those in parts, then the whole ones, by halves
+      for (int b0 = 0; b0 < n; b0 += 64) {
+        const Row r = b0 ? row(b0 + lane) : near;
+        const int mine = r.tiles > limit ? 0 : 2 * r.tiles > limit ? 1 : 4 * r.tiles > limit ? 2 : 3;
+        const int count = mine == order ? r.items * parts(r) : 0;
+        const int upto = static_cast<int>(wave_scan(static_cast<uint32_t>(count)));
+        const uint64_t past = __ballot(upto > at);
+        if (past) {
+          const int l = __builtin_ctzll(past);
+          p.b = b0 + l;
+          p.parts = __builtin_amdgcn_readlane(parts(r), l);
+          at -= __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l);
+          p.item = at / p.parts;
+          p.part = at - p.item * p.parts;
+          p.slot = index;  // those in parts come first: below 2 share, for each has more than half of `limit` tiles
+          p.seq = seq(p.b);
+          p.seq.first = __builtin_amdgcn_readfirstlane(p.seq.first);
+          p.seq.n = __builtin_amdgcn_readfirstlane(p.seq.n);
+          p.seq.len = __builtin_amdgcn_readfirstlane(p.seq.len);
+          span(p.seq, p.item, p.to, p.gap_from, p.gap);
+          const int64_t tiles = (p.to - p.gap + FORM::kStep - 1) / FORM::kStep;
+          p.from = static_cast<int>(p.part * tiles / p.parts) * FORM::kStep;
+          p.end = min(static_cast<int>((p.part + 1) * tiles / p.parts) * FORM::kStep, p.to - p.gap);
+          return true;
+        }
+        at -= __builtin_amdgcn_readlane(upto, 63);
+      }
+    }
+    return false;
   }
 };
 
@@ -142,13 +207,13 @@ struct MaskedOut {
 template <int MODE>
 struct MaskedSeen {
   MaskedSeq<MODE> s;
-  int token, gap_from, gap;  // the gap in virtual positions
-  uint32_t mine, wave;
+  int token, a, b, gap_from, gap;  // this lane's token, and the wave's
+  uint32_t mine;
   bool every;
   __device__ __forceinline__ int place(int v) const { return v < gap_from ? v : v + gap; }
   __device__ __forceinline__ void look(int tile) {
-    mine = static_cast<uint32_t>(s.bits(token, tile));
-    every = __all(mine == ~0u);
+    every = s.whole(a, b, tile, tile + 32);
+    if (!every) mine = static_cast<uint32_t>(s.bits(token, tile));
   }
   __device__ __forceinline__ bool sees(int p) const { return (mine >> (p & 31)) & 1; }
   __device__ __forceinline__ bool any(int) const { return true; }
@@ -202,194 +267,265 @@ __device__ __attribute__((noinline)) void masked_rows16(const MaskedRows<MODE> &
 }
 
 // Number of an item among all of a head, of rows that begin at packed row `first` of sequence b: no two are alike.
+template <class FORM>
 __device__ __forceinline__ int64_t masked_item(int first, int grp, int b, int item) {
-  return static_cast<int64_t>(first) * grp / kRows + b + item;
+  return static_cast<int64_t>(first) * grp / FORM::kItem + b + item;
 }
 // Sequences in the order of their rows: what lies before the first (batch + 1), the sequences, what lies behind the last (batch).
 __device__ __forceinline__ int masked_order(int b, int batch) { return b == batch + 1 ? 0 : b + 1; }
 
-// A run has kLeast tiles at least.
-constexpr int kLeast = 4;
+// Where an item's parts are: the first slot, how many.
+template <class FORM, int MODE>
+__device__ __forceinline__ void masked_tell(const MaskedPart<MODE> &p, int2 *joins, int grp, int batch, int kvh, int kh) {
+  if (p.part == 0 && threadIdx.x == 0)
+    joins[masked_item<FORM>(p.seq.first, grp, masked_order(p.b, batch), p.item) * kvh + kh] = make_int2(p.slot, p.parts);
+}
 
 template <int D, int DT, int MODE>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void masked_attention_kernel(
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void masked_wide_kernel(
     const uint16_t *__restrict__ q, int64_t q_row, int64_t q_head, const uint16_t *__restrict__ k, int64_t kpage,
     int64_t khead, int64_t krow, const uint16_t *__restrict__ v, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
     int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
     const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, MaskedRule rule, int share, int slot_rows,
-    float scale2, uint32_t flip, float *__restrict__ parts, int4 *__restrict__ joins, uint16_t *__restrict__ out) {
+    float scale2, uint32_t flip, float *__restrict__ parts, int2 *__restrict__ joins, uint16_t *__restrict__ out) {
   using T = PromptTile<D>;
   constexpr int kStage = T::kStage, kS = kTile / 32;
   extern __shared__ __attribute__((aligned(1024))) int8_t masked_smem[];  // two stages of K and V
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i32 = lane & 31, h = lane >> 5;
-  const int kh = blockIdx.x % kvh, run = blockIdx.x / kvh;
-  const MaskedPlan<MODE> plan{{starts, batch, rows, grp}, lens, width << shift, rule};
-  const uint64_t all = plan.all();
-  share = static_cast<int>(max(min(static_cast<uint64_t>(share), all / kLeast), uint64_t(1)));
-  if (run >= share || all == 0) return;  // uniform over the workgroup
-  const int begin = static_cast<int>(run * all / share), stop = static_cast<int>((run + 1) * all / share);
+  const int kh = blockIdx.x % kvh;
+  const MaskedPlan<MODE, Wide> plan{{starts, batch, rows, grp}, lens, width << shift, rule};
+  MaskedPart<MODE> p;
+  if (!plan.find(blockIdx.x / kvh, share, p)) return;
+  const MaskedSeq<MODE> &seq = p.seq;
+  masked_tell<Wide>(p, joins, grp, batch, kvh, kh);
+  const int from = __builtin_amdgcn_readfirstlane(p.from), end = __builtin_amdgcn_readfirstlane(p.end);
   const int mask = (1 << shift) - 1;
+  // Of this lane's 16 bytes of a load: their chunk in LDS, and their bytes behind the load's first row.  The chunks of a wave's
+  // loads differ by constants, for a wave's rows are 16.
+  constexpr int kOf = 64 / T::kChunks;  // rows of a load
+  static_assert(T::kLoads * kOf == 16, "a wave loads 16 rows");
+  const uint32_t kx = T::k_chunk(lane / T::kChunks, lane % T::kChunks), kl = 2 * (lane / T::kChunks) * static_cast<uint32_t>(krow);
+  const uint32_t vx = T::v_chunk(lane / T::kChunks, lane % T::kChunks), vl = 2 * (lane / T::kChunks) * static_cast<uint32_t>(vrow);
 
-  for (int at = begin; at < stop;) {
-    // the item that this part of the run lies in, and which of its tiles
-    int b, part, unused;
-    if (!attn_find_part(plan, batch + 2, 0, at, b, part, unused)) return;
-    MaskedSeq<MODE> seq = plan.seq(b);
-    seq.first = __builtin_amdgcn_readfirstlane(seq.first);  // uniform: in scalar registers
-    seq.n = __builtin_amdgcn_readfirstlane(seq.n);
-    seq.len = __builtin_amdgcn_readfirstlane(seq.len);
-    int item, tile0, tiles;
-    if constexpr (MODE == kTree) {
-      tiles = plan.tiles(seq, 0);
-      item = part / tiles;
-      tile0 = part - item * tiles;
-    } else {
-      attn_find_part([&](int i, int) { return plan.tiles(seq, i); }, plan.items(seq), 0, part, item, tile0, tiles);
-    }
-    int to, gap_from, gap_to;
-    plan.tiles(seq, item, to, gap_from, gap_to);
-    const int tile1 = min(tiles, tile0 + stop - at), gap = gap_to - gap_from;
-    const bool entire = tile0 == 0 && tile1 == tiles;
-    // virtual positions of this part, and its last real one
-    const int from = tile0 * kTile, end = min(tile1 * kTile, to - gap), last = end > 0 ? (end <= gap_from ? end : end + gap) - 1 : 0;
-    const auto place = [&](int vp) { return vp < gap_from ? vp : vp + gap; };
+  const auto place = [&](int vp) { return vp < p.gap_from ? vp : vp + p.gap; };
+  const int last = end > 0 ? (end <= p.gap_from ? end : end + p.gap) - 1 : 0;  // the part's last position
 
-    const int n_rows = seq.n * grp, r0 = item * kRows + wave * 32, row_at = r0 + i32;
-    const bool row = row_at < n_rows;
-    const int token = row ? row_at / grp : 0, head = kh * grp + (row ? row_at - token * grp : 0);
-    const int wave_a = r0 / grp, wave_b = min((r0 + 31) / grp, seq.n - 1);
-    uint4 qf[D / 16];
-    const uint16_t *qp = q + (seq.first + token) * q_row + head * q_head + 8 * h;
+  const int n_rows = seq.n * grp, r0 = p.item * kRows + wave * 32, row_at = r0 + i32;
+  const bool row = row_at < n_rows;
+  const int token = row ? row_at / grp : 0, head = kh * grp + (row ? row_at - token * grp : 0);
+  const int wave_a = r0 / grp, wave_b = min((r0 + 31) / grp, seq.n - 1);
+  uint4 qf[D / 16];
+  const uint16_t *qp = q + (seq.first + token) * q_row + head * q_head + 8 * h;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      const uint4 x = *reinterpret_cast<const uint4 *>(qp + 16 * c);
-      qf[c] = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
-    }
+  for (int c = 0; c < D / 16; ++c) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(qp + 16 * c);
+    qf[c] = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+  }
 
-    const uint16_t *kb = k + kh * khead, *vb = v + kh * vhead;
-    const int32_t *pg = table + static_cast<int64_t>(min(b, batch - 1)) * width;
-    const auto entry = [&](int vp) { return pg[min(place(vp) + lane, last) >> shift]; };
-    const auto load = [&](int vp, int id, int8_t *stage) {
-      const int tile = min(place(vp), last);  // past the last tile: rows that nothing reads
+  const uint16_t *kb = k + kh * khead, *vb = v + kh * vhead;
+  const int32_t *pg = table + static_cast<int64_t>(min(p.b, batch - 1)) * width;
+  const auto entry = [&](int vp) { return pg[min(place(vp) + lane, last) >> shift]; };
+  const auto load = [&](int vp, int id, int8_t *stage) {
+    const int tile = min(place(vp), last);  // past the last tile: rows that nothing reads
+    if (tile + kTile <= last + 1) {
 #pragma unroll
       for (int i = 0; i < T::kLoads; ++i) {
         const int slot = (wave * T::kLoads + i) * 64;
         const int64_t pid = __builtin_amdgcn_readlane(id, slot / T::kChunks);  // the rows of one load lie in one page
-        const int r = slot / T::kChunks + lane / T::kChunks, c = lane % T::kChunks, p = min(tile + r, last) & mask;
-        prompt_lds_load16(kb + pid * kpage, 2 * (p * static_cast<uint32_t>(krow) + 8 * T::k_chunk(r, c)), stage + slot * 16);
-        prompt_lds_load16(vb + pid * vpage, 2 * (p * static_cast<uint32_t>(vrow) + 8 * T::v_chunk(r, c)), stage + T::kBytes + slot * 16);
+        const int64_t in = (tile + slot / T::kChunks) & mask;
+        prompt_lds_load16(kb + pid * kpage + in * krow, ((kx ^ T::k_chunk(i * kOf, 0)) << 4) + kl, stage + slot * 16);
+        prompt_lds_load16(vb + pid * vpage + in * vrow, ((vx ^ T::v_chunk(i * kOf, 0)) << 4) + vl, stage + T::kBytes + slot * 16);
       }
-    };
-    const auto fix = [&](int id, uint64_t &there) {  // page numbers outside the pool: page 0, unseen
-      const bool ok = id >= 0 && id < pages;
-      there = __ballot(ok);
-      return ok ? id : 0;
-    };
+      return;
+    }
+    // the last tile, with rows past the end in place of which it takes the last one.  (The lane is new to the compiler, which
+    // would work these offsets out ahead of the loop and keep them.)
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) {
+      const int slot = (wave * T::kLoads + i) * 64;
+      const int64_t pid = __builtin_amdgcn_readlane(id, slot / T::kChunks);
+      const int r = slot / T::kChunks + ln / T::kChunks, c = ln % T::kChunks, pos = min(tile + r, last) & mask;
+      prompt_lds_load16(kb + pid * kpage, 2 * (pos * static_cast<uint32_t>(krow) + 8 * T::k_chunk(r, c)), stage + slot * 16);
+      prompt_lds_load16(vb + pid * vpage, 2 * (pos * static_cast<uint32_t>(vrow) + 8 * T::v_chunk(r, c)), stage + T::kBytes + slot * 16);
+    }
+  };
+  const auto fix = [&](int id, uint64_t &there) {  // page numbers outside the pool: page 0, unseen
+    const bool ok = id >= 0 && id < pages;
+    there = __ballot(ok);
+    return ok ? id : 0;
+  };
 
-    f16_t o[D / 32];
+  f16_t o[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  uint64_t there = 0;  // which positions of the tile that is on its way exist
+  int next_entry = 0, stage = 0;
+  if (end > from) {
+    load(from, fix(entry(from), there), masked_smem);
+    next_entry = entry(from + kTile);
+  }
+  uint32_t odd = 0;  // an infinity or NaN in V where only some of the wave's rows see it
+  for (int vp = from; vp < end; vp += kTile) {
+    // this tile's loads have landed, every wave's, and the stage of the last tile has been read
+    prompt_wait();
+    const uint64_t ok = there;
+    load(vp + kTile, fix(next_entry, there), masked_smem + (kStage - stage));
+    next_entry = entry(vp + 2 * kTile);
+    const int8_t *ks = masked_smem + stage, *vs = ks + T::kBytes;
+    stage = kStage - stage;
+    if (r0 >= n_rows) continue;  // no rows: it loads for the others
+    const int tile = place(vp);
+    uint64_t vis = ~uint64_t(0);
+    const bool some = !seq.whole(wave_a, wave_b, tile, tile + kTile) || ok != ~uint64_t(0);
+    if (some) {
+      vis = row ? seq.bits(token, tile) & ok : 0;
+      if (!__any(vis != 0)) continue;
+    }
+    f16_t s[kS];
+    prompt_scores<D, DT>(ks, qf, s, i32, h);
+    if (some) {
+      vis >>= 4 * h;
+#pragma unroll
+      for (int t = 0; t < kS; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = (vis >> (32 * t + 8 * (r >> 2) + (r & 3))) & 1 ? s[t][r] : -INFINITY;
+      prompt_odd_values<D, DT>(odd, vs, lane);
+    }
+#include "prompt_weigh.inc"
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing on its way to LDS when the workgroup ends
+  if (r0 >= n_rows) return;
+  const MaskedOut dst{out + (static_cast<int64_t>(seq.first) * kvh * grp + kh * grp) * D, static_cast<int64_t>(kvh) * grp * D,
+                      p.parts > 1 ? parts + (static_cast<int64_t>(p.slot) * kvh + kh) * slot_rows * (D + 2) : nullptr};
+  if (__any(odd)) {
+    // 0 times an infinity is no zero: these rows once more, with what they do not see left out one position at a time
+    MaskedRows<MODE> w;
+    w.src = {kb, vb, kpage, krow, vpage, vrow, pg, shift, mask, pages, last >> shift};
+    w.seen = {seq, 0, wave_a, wave_b, p.gap_from, p.gap, 0, false};
+    w.q = q + seq.first * q_row + kh * grp * q_head;
+    w.q_row = q_row;
+    w.q_head = q_head;
+    w.to = dst;
+    w.all = n_rows;
+    w.grp = grp;
+    w.r0 = p.item * kRows;
+    w.from = from;
+    w.end = end;
+    w.scale2 = flip ? -scale2 : scale2;
+    for (int half = 0; half < 2; ++half)
+      if (r0 + 16 * half < n_rows) masked_rows16<D, DT, MODE>(w, 32 * wave + 16 * half);
+    return;
+  }
+  if (!row) return;
+  l += __shfl_xor(l, 32, 64);
+  if (p.parts > 1) {
+    float *z = dst.part + (wave * 32 + i32) * (D + 2);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-    float m = -INFINITY, l = 0.f;
-    uint64_t there = 0;  // which positions of the tile that is on its way exist
-    int next_entry = 0, stage = 0;
-    __syncthreads();  // the last item's tiles have been read
-    if (end > from) {
-      load(from, fix(entry(from), there), masked_smem);
-      next_entry = entry(from + kTile);
+      for (int r = 0; r < 16; r += 2)
+        *reinterpret_cast<float2 *>(z + 32 * d + 8 * (r >> 2) + 4 * h + (r & 3)) = make_float2(o[d][r], o[d][r + 1]);
+    if (h == 0) *reinterpret_cast<float2 *>(z + D) = make_float2(m, l);
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  uint16_t *y = dst.out + token * dst.row + (head - kh * grp) * D + 4 * h;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = l == 0.f ? 0.f : o[d][r + i] * inv;
+      *reinterpret_cast<uint2 *>(y + 32 * d + 2 * r) = make_uint2(attn_pack2<DT>(x[0], x[1]), attn_pack2<DT>(x[2], x[3]));
     }
-    uint32_t odd = 0;  // an infinity or NaN in V where only some of the wave's rows see it
-    for (int vp = from; vp < end; vp += kTile) {
-      // this tile's loads have landed, every wave's, and the stage of the last tile has been read
-      prompt_wait();
-      const uint64_t ok = there;
-      load(vp + kTile, fix(next_entry, there), masked_smem + (kStage - stage));
-      next_entry = entry(vp + 2 * kTile);
-      const int8_t *ks = masked_smem + stage, *vs = ks + T::kBytes;
-      stage = kStage - stage;
-      if (r0 >= n_rows) continue;  // no rows: it loads for the others
-      const int tile = place(vp);
-      uint64_t vis = ~uint64_t(0);
-      const bool some = !seq.whole(wave_a, wave_b, tile) || ok != ~uint64_t(0);
-      if (some) {
-        vis = row ? seq.bits(token, tile) & ok : 0;
-        if (!__any(vis != 0)) continue;
+}
+
+// Workgroups of a CU whose registers hold two tiles each.
+constexpr int masked_round(int dim) { return dim == 64 ? 4 : dim == 128 ? 2 : 1; }
+
+template <int D, int DT, int MODE>
+__global__ __launch_bounds__(64 * kWaves, masked_round(D)) void masked_narrow_kernel(
+    const uint16_t *__restrict__ q, int64_t q_row, int64_t q_head, const uint16_t *__restrict__ k, int64_t kpage,
+    int64_t khead, int64_t krow, const uint16_t *__restrict__ v, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
+    int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
+    const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, MaskedRule rule, int share, int slot_rows,
+    float scale2, uint32_t flip, float *__restrict__ parts, int2 *__restrict__ joins, uint16_t *__restrict__ out) {
+  extern __shared__ float narrow_smem[];  // [kWaves][16][D] outputs, then [kWaves][16][2] maxima and sums
+  float *sm = narrow_smem, *ml = sm + kWaves * 16 * D;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, j = lane >> 4;
+  const int kh = blockIdx.x % kvh;
+  const MaskedPlan<MODE, Narrow> plan{{starts, batch, rows, grp}, lens, width << shift, rule};
+  MaskedPart<MODE> p;
+  if (!plan.find(blockIdx.x / kvh, share, p)) return;
+  const MaskedSeq<MODE> &seq = p.seq;
+  masked_tell<Narrow>(p, joins, grp, batch, kvh, kh);
+  const int n_rows = seq.n * grp, r0 = p.item * 16, held = min(n_rows - r0, 16), row_at = r0 + min(i16, held - 1);
+  const int token = row_at / grp, head = kh * grp + row_at - token * grp;
+  uint4 qf[D / 32];
+  const uint16_t *qp = q + (seq.first + token) * q_row + head * q_head + 8 * j;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) qf[c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
+  const KvSource<true> src{k + kh * khead, v + kh * vhead, kpage, krow, vpage, vrow,
+                           table + static_cast<int64_t>(min(p.b, batch - 1)) * width, shift, (1 << shift) - 1, pages,
+                           p.to > 0 ? (p.to - 1) >> shift : 0};
+  const MaskedSeen<MODE> seen{seq, token, r0 / grp, min((r0 + 15) / grp, seq.n - 1), p.gap_from, p.gap, 0, false};
+  AttnRows<D> a;
+  attn_clear(a);
+  attn_walk<D, DT, true>(a, src, qf, p.from + 32 * wave, p.end, Narrow::kStep, seen, flip ? -scale2 : scale2, lane);
+  a.l = attn_row_sum(a.l);
+
+  // the four waves' states meet
+  if (i16 < held) {
+    float *o = sm + (wave * 16 + i16) * D + (D / 16) * 4 * j;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) o[(D / 16) * r + c] = a.o[c][r];
+    if (j == 0) {
+      ml[(wave * 16 + i16) * 2] = a.m;
+      ml[(wave * 16 + i16) * 2 + 1] = a.l;
+    }
+  }
+  __syncthreads();
+  float *part = parts + (static_cast<int64_t>(p.slot) * kvh + kh) * slot_rows * (D + 2);
+  for (int e = threadIdx.x; e < held * D; e += 64 * kWaves) {
+    const int row = e / D, d = e % D;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[(w * 16 + row) * 2]);
+    float o = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float mw = ml[(w * 16 + row) * 2];
+      const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+      o += f * sm[(w * 16 + row) * D + d];
+      l += f * ml[(w * 16 + row) * 2 + 1];
+    }
+    if (p.parts == 1) {
+      const float x = l == 0.f ? 0.f : o / l;
+      const int t = (r0 + row) / grp;
+      out[((seq.first + static_cast<int64_t>(t)) * kvh * grp + kh * grp + r0 + row - t * grp) * D + d] = DT == MP_F16 ? mp_f2h(x) : mp_f2bf(x);
+    } else {
+      part[row * (D + 2) + d] = o;
+      if (d == 0) {
+        part[row * (D + 2) + D] = m;
+        part[row * (D + 2) + D + 1] = l;
       }
-      f16_t s[kS];
-      prompt_scores<D, DT>(ks, qf, s, i32, h);
-      if (some) {
-        vis >>= 4 * h;
-#pragma unroll
-        for (int t = 0; t < kS; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[t][r] = (vis >> (32 * t + 8 * (r >> 2) + (r & 3))) & 1 ? s[t][r] : -INFINITY;
-        odd |= prompt_odd_values<D, DT>(vs, lane);
-      }
-      prompt_weigh<D, DT>(s, vs, o, m, l, scale2, lane);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing on its way to LDS when the item ends
-    const int64_t slot = (static_cast<int64_t>(2 * run + (at > begin ? 1 : 0)) * kvh + kh) * slot_rows;
-    MaskedOut dst{out + (static_cast<int64_t>(seq.first) * kvh * grp + kh * grp) * D, static_cast<int64_t>(kvh) * grp * D,
-                  entire ? nullptr : parts + slot * (D + 2)};
-    if (tile0 == 0 && threadIdx.x == 0) {
-      const int last_run = static_cast<int>(((at + tiles) * static_cast<uint64_t>(share) - 1) / all);  // run of its last tile
-      joins[masked_item(seq.first, grp, masked_order(b, batch), item) * kvh + kh] = make_int4(run, last_run - run + 1, at > begin ? 1 : 0, 0);
-    }
-    at += tile1 - tile0;
-    if (r0 >= n_rows) continue;
-    if (__any(odd)) {
-      // 0 times an infinity is no zero: these rows once more, with what they do not see left out one position at a time
-      MaskedRows<MODE> p;
-      p.src = {kb, vb, kpage, krow, vpage, vrow, pg, shift, mask, pages, last >> shift};
-      p.seen.s = seq;
-      p.seen.gap_from = gap_from;
-      p.seen.gap = gap;
-      p.q = q + seq.first * q_row + kh * grp * q_head;
-      p.q_row = q_row;
-      p.q_head = q_head;
-      p.to = dst;
-      p.all = n_rows;
-      p.grp = grp;
-      p.r0 = item * kRows;
-      p.from = from;
-      p.end = end;
-      p.scale2 = flip ? -scale2 : scale2;
-      for (int half = 0; half < 2; ++half)
-        if (r0 + 16 * half < n_rows) masked_rows16<D, DT, MODE>(p, 32 * wave + 16 * half);
-      continue;
-    }
-    if (!row) continue;
-    l += __shfl_xor(l, 32, 64);
-    if (!entire) {
-      float *z = dst.part + (wave * 32 + i32) * (D + 2);
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2)
-          *reinterpret_cast<float2 *>(z + 32 * d + 8 * (r >> 2) + 4 * h + (r & 3)) = make_float2(o[d][r], o[d][r + 1]);
-      if (h == 0) *reinterpret_cast<float2 *>(z + D) = make_float2(m, l);
-      continue;
-    }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    uint16_t *y = dst.out + token * dst.row + (head - kh * grp) * D + 4 * h;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = l == 0.f ? 0.f : o[d][r + i] * inv;
-        *reinterpret_cast<uint2 *>(y + 32 * d + 2 * r) = make_uint2(attn_pack2<DT>(x[0], x[1]), attn_pack2<DT>(x[2], x[3]));
-      }
   }
 }
 
 // The parts of a row meet, one wave each.
-template <int D, int DT>
+template <int D, int DT, class FORM>
 __global__ __launch_bounds__(256) void masked_join_kernel(const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp,
-                                                          int slot_rows, int share, const float *__restrict__ parts,
-                                                          const int4 *__restrict__ joins, uint16_t *__restrict__ out) {
+                                                          int slot_rows, int slots, const float *__restrict__ parts,
+                                                          const int2 *__restrict__ joins, uint16_t *__restrict__ out) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int nh = kvh * grp, lane = threadIdx.x & 63;
   if (at >= static_cast<int64_t>(rows) * nh) return;
@@ -399,13 +535,15 @@ __global__ __launch_bounds__(256) void masked_join_kernel(const int32_t *__restr
   int b = 0;
   for (int b0 = 0; b0 <= batch; b0 += 64) b += __popcll(__ballot(b0 + lane <= batch && starts[min(b0 + lane, batch)] <= t));
   b = b == 0 ? batch + 1 : b - 1;
-  const int first = plan.first(b), r = (t - first) * grp + qh - kh * grp, item = r / kRows;
+  const int first = plan.first(b), r = (t - first) * grp + qh - kh * grp, item = r / FORM::kItem;
   if (t < first || t >= plan.end(b)) return;  // offsets that do not ascend: nothing was left
-  const int4 of = joins[masked_item(first, grp, masked_order(b, batch), item) * kvh + kh];
-  if (of.y == 1) return;  // written already
-  if (of.x < 0 || of.y < 1 || of.x >= share || of.y > share - of.x) return;
+  const int2 of = joins[masked_item<FORM>(first, grp, masked_order(b, batch), item) * kvh + kh];
+  // written already; the rest: offsets that do not ascend, nothing was left
+  if (of.y < 2 || of.x < 0 || of.x >= slots) return;
+  const int64_t from_slot = of.x;
+  if (of.y > slots - from_slot) return;
   const auto at_part = [&](int p) {
-    return parts + ((static_cast<int64_t>(2 * (of.x + p) + (p == 0 ? of.z & 1 : 0)) * kvh + kh) * slot_rows + r % kRows) * (D + 2);
+    return parts + (((from_slot + p) * kvh + kh) * slot_rows + r % FORM::kItem) * (D + 2);
   };
   float m = -INFINITY;
   for (int p = lane; p < of.y; p += 64) m = fmaxf(m, at_part(p)[D]);
@@ -429,13 +567,23 @@ __global__ __launch_bounds__(256) void masked_join_kernel(const int32_t *__restr
   }
 }
 
-// Workgroups of a head: as many as fit the card at once (two a CU; one of heads of 256).
-inline int masked_share(int64_t kvh, int dim) {
-  const int64_t n = static_cast<int64_t>(dim == 256 ? 1 : 2) * mp_cu_count() / kvh;
-  return static_cast<int>(n > 1 ? n : 1);
+// Workgroups of a head: as many as fit the card at once.
+template <class FORM>
+int64_t masked_share(int64_t kvh, int dim) {
+  const int64_t round = FORM::kItem == kRows ? (dim == 256 ? 1 : 2) : masked_round(dim);
+  const int64_t n = round * mp_cu_count() / kvh;
+  return n > 1 ? n : 1;
 }
-inline int64_t masked_slot_rows(int64_t rows, int64_t grp) { return rows * grp < kRows ? rows * grp : kRows; }
-inline int64_t masked_items(int64_t rows, int64_t grp, int64_t batch) { return rows * grp / kRows + batch + 4; }
+template <class FORM>
+int64_t masked_slot_rows(int64_t rows, int64_t grp) {
+  return rows * grp < FORM::kItem ? rows * grp : FORM::kItem;
+}
+template <class FORM>
+int64_t masked_items(int64_t rows, int64_t grp, int64_t batch) {
+  return rows * grp / FORM::kItem + batch + 4;
+}
+// Few rows of a sequence and key-value head, on the average, are narrow.
+inline bool masked_narrow(int64_t rows, int64_t grp, int64_t batch) { return rows * grp <= 32 * batch; }
 
 struct MaskedCall {
   const void *q;
@@ -453,40 +601,62 @@ struct MaskedCall {
   hipStream_t stream;
 };
 
+template <class FORM>
 size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim, int64_t batch) {
   const int64_t grp = nh / kvh;
-  return static_cast<size_t>(masked_items(rows, grp, batch) * kvh) * sizeof(int4) +
-         static_cast<size_t>(2 * masked_share(kvh, dim) * kvh * masked_slot_rows(rows, grp)) * (dim + 2) * sizeof(float);
+  return static_cast<size_t>(masked_items<FORM>(rows, grp, batch) * kvh) * sizeof(int2) +
+         static_cast<size_t>(2 * masked_share<FORM>(kvh, dim) * kvh * masked_slot_rows<FORM>(rows, grp)) * (dim + 2) * sizeof(float);
+}
+size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim, int64_t batch) {
+  return masked_narrow(rows, nh / kvh, batch) ? masked_workspace<Narrow>(rows, nh, kvh, dim, batch)
+                                              : masked_workspace<Wide>(rows, nh, kvh, dim, batch);
 }
 
-template <int D, int DT, int MODE>
+// Whether an item can be cut: no share has less than a tile, and what passes a share by one at most stays whole.
+template <class FORM>
+bool masked_splits(const MaskedCall &c, int mode) {
+  const int64_t grp = c.nh / c.kvh, span = mp_cdiv(FORM::kItem, grp) + 1;  // positions that an item's tokens spread over
+  int64_t reach = c.cache->width * c.cache->page_size;
+  if (mode == kWindow) reach = std::min(reach, static_cast<int64_t>(c.rule.window) + c.rule.sinks + span + 2 * 64);
+  return mp_cdiv(reach, FORM::kStep) > 1;
+}
+
+template <int D, int DT, int MODE, class FORM>
 int masked_start(const MaskedCall &c, int shift) {
-  const int grp = c.nh / c.kvh, share = masked_share(c.kvh, D), slot_rows = static_cast<int>(masked_slot_rows(c.rows, grp));
-  int4 *joins = static_cast<int4 *>(c.workspace);
-  float *parts = reinterpret_cast<float *>(joins + masked_items(c.rows, grp, c.batch) * c.kvh);
+  constexpr bool kIsWide = FORM::kItem == kRows;
+  const int grp = c.nh / c.kvh, share = static_cast<int>(masked_share<FORM>(c.kvh, D));
+  const int slot_rows = static_cast<int>(masked_slot_rows<FORM>(c.rows, grp));
+  int2 *joins = static_cast<int2 *>(c.workspace);
+  float *parts = reinterpret_cast<float *>(joins + masked_items<FORM>(c.rows, grp, c.batch) * c.kvh);
   // the sign of the scale goes to the queries, so that the largest product gives the largest score; a scale of 0 becomes the
   // smallest normal number, which leaves every finite score 0 and a masked one -inf
   const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
   const float scale2 = fmaxf(fabsf(c.scale) * kLog2e, FLT_MIN);
-  constexpr int kLds = 2 * PromptTile<D>::kStage;
-  if (kLds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(masked_attention_kernel<D, DT, MODE>),
-                                              hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
+  constexpr int kLds = kIsWide ? 2 * PromptTile<D>::kStage : kWaves * 16 * (D + 2) * static_cast<int>(sizeof(float));
+  constexpr auto kKernel = kIsWide ? &masked_wide_kernel<D, DT, MODE> : &masked_narrow_kernel<D, DT, MODE>;
+  if (kLds > 64 * 1024 &&
+      hipFuncSetAttribute(reinterpret_cast<const void *>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
     return MP_ERR_HIP;
   const mp_pages &p = *c.cache;
-  hipLaunchKernelGGL((masked_attention_kernel<D, DT, MODE>), dim3(static_cast<unsigned>(share) * c.kvh), dim3(64 * kWaves), kLds,
-                     c.stream, static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(p.k), p.k_page,
+  hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>((masked_items<FORM>(c.rows, grp, c.batch) + share) * c.kvh)), dim3(64 * kWaves), kLds, c.stream,
+                     static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(p.k), p.k_page,
                      p.k_head, p.k_row, static_cast<const uint16_t *>(p.v), p.v_page, p.v_head, p.v_row, static_cast<int>(p.pages),
                      shift, p.table, static_cast<int>(p.width), c.lens, c.starts, static_cast<int>(c.batch),
                      static_cast<int>(c.rows), c.kvh, grp, c.rule, share, slot_rows, scale2, flip, parts, joins,
                      static_cast<uint16_t *>(c.out));
   MP_CHECK_LAUNCH();
-  if (share > 1) {
-    hipLaunchKernelGGL((masked_join_kernel<D, DT>), dim3(static_cast<unsigned>(mp_cdiv(c.rows * c.nh, 4))), dim3(256), 0, c.stream,
-                       c.starts, static_cast<int>(c.batch), static_cast<int>(c.rows), c.kvh, grp, slot_rows, share, parts, joins,
-                       static_cast<uint16_t *>(c.out));
+  if (masked_splits<FORM>(c, MODE)) {
+    hipLaunchKernelGGL((masked_join_kernel<D, DT, FORM>), dim3(static_cast<unsigned>(mp_cdiv(c.rows * c.nh, 4))), dim3(256), 0,
+                       c.stream, c.starts, static_cast<int>(c.batch), static_cast<int>(c.rows), c.kvh, grp, slot_rows, 2 * share, parts,
+                       joins, static_cast<uint16_t *>(c.out));
     MP_CHECK_LAUNCH();
   }
   return MP_OK;
+}
+template <int D, int DT, int MODE>
+int masked_start(const MaskedCall &c, int shift) {
+  return masked_narrow(c.rows, c.nh / c.kvh, c.batch) ? masked_start<D, DT, MODE, Narrow>(c, shift)
+                                                      : masked_start<D, DT, MODE, Wide>(c, shift);
 }
 
 template <int MODE>
@@ -512,7 +682,7 @@ int masked_launch(const MaskedCall &c) {
   const int64_t grp = c.nh / c.kvh, reach = (int64_t(1) << 30) - 256, span = int64_t(1) << shift;
   if (p.k_row > reach / span || p.v_row > reach / span) return MP_ERR_SHAPE;
   if (c.rows * c.nh > INT32_MAX - kRows) return MP_ERR_SHAPE;
-  if (masked_items(c.rows, grp, c.batch) * mp_cdiv(p.width << shift, kTile) > INT32_MAX) return MP_ERR_SHAPE;
+  if (masked_items<Narrow>(c.rows, grp, c.batch) * mp_cdiv(p.width << shift, kTile) > INT32_MAX) return MP_ERR_SHAPE;
   if (c.rows == 0) return MP_OK;
   if (mp_cu_count() <= 0) return MP_ERR_HIP;
   if (c.workspace_bytes < masked_workspace(c.rows, c.nh, c.kvh, c.head_dim, c.batch)) return MP_ERR_WORKSPACE;

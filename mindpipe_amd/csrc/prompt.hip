@@ -207,9 +207,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_attentio
           const int p = 32 * t + 8 * (r >> 2) + (r & 3);
           s[t][r] = tile + p + 4 * h < sees && ((vis >> p) & 1) ? s[t][r] : -INFINITY;
         }
-      odd |= prompt_odd_values<D, DT>(vs, lane);
+      prompt_odd_values<D, DT>(odd, vs, lane);
     }
-    prompt_weigh<D, DT>(s, vs, o, m, l, scale2, lane);
+#include "prompt_weigh.inc"
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing on its way to LDS when the workgroup ends
   if (__any(odd)) {

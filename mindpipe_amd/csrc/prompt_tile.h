@@ -89,86 +89,14 @@ __device__ __forceinline__ void prompt_scores(const int8_t *ks, const uint4 (&qf
   }
 }
 
-// 16 bytes of the values' tile hold an infinity or NaN.
+// odd: whether the values' tile holds an infinity or NaN.
 template <int D, int DT>
-__device__ __forceinline__ uint32_t prompt_odd_values(const int8_t *vs, int lane) {
-  uint32_t odd = 0;
+__device__ __forceinline__ void prompt_odd_values(uint32_t &odd, const int8_t *vs, int lane) {
   for (int e = lane; e < PromptTile<D>::kBytes / 16; e += 64) {
     const i4_t x = *reinterpret_cast<const i4_t *>(vs + 16 * e);
 #pragma unroll
     for (int i = 0; i < 4; ++i) odd |= attn_odd16<DT>(x[i]) || attn_odd16<DT>(static_cast<uint32_t>(x[i]) >> 16);
   }
-  return odd;
-}
-
-// The tile's scores (-inf where masked) into the row's maximum m, sum l and outputs o.
-template <int D, int DT>
-__device__ __forceinline__ void prompt_weigh(const f16_t (&s)[kTile / 32], const int8_t *vs, f16_t (&o)[D / 32], float &m, float &l,
-                                             float scale2, int lane) {
-  using T = PromptTile<D>;
-  constexpr int kS = kTile / 32;
-  const int h = lane >> 5;
-  float top = s[0][0];
-#pragma unroll
-  for (int t = 0; t < kS; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
-  top *= scale2;
-  if (__any(top > m + kMaxLag)) {
-    const float new_m = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
-    const float f = m == new_m ? 1.0f : __builtin_amdgcn_exp2f(m - new_m);
-    l *= f;
-    m = new_m;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][r] *= f;
-  }
-  const float base = m == -INFINITY ? 0.f : m - kRaise<DT>;
-  // O^T: step c of 16 positions, whose weights are those of positions 16 c + 4 h + {0..3, 8..11}: s[c / 2][8 (c & 1) ..].  The
-  // next step's weights are made between the matrix instructions of this one.
-  constexpr int kSteps = kTile / 16, kD = D / 32;
-  const int trow = 4 * h + ((lane & 15) >> 2), tcol = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-  uint32_t w[2][4];
-  constexpr int kAheadV = 2;  // operands of V that are read before they are used (1: 461 -> 470 us, 4: 463, heads of 256 92 -> 101 and 94)
-  uint4 vf[kAheadV + 1];
-  // Weights are rounded to the values' type, off by up to 2^-11 (fp16) or 2^-8 (bf16) of themselves each, and their sum takes
-  // them as rounded: errors (rms) are 1.2 (fp16) to 1.3 times (bf16; heads of 256 1.4) those of 32-bit weights, 2.1e-3 for
-  // 1.6e-3 of the packed prompts' outputs.  A second product with what the rounding leaves would take that away for 471 -> 611 us
-  // there, 153 -> 209 for chunks of 32 heads and 91 -> 107 for heads of 256.
-  const auto weight = [&](int c, int i) {
-    const int r = 8 * (c & 1) + 2 * i;
-    w[c & 1][i] = attn_pack2<DT>(__builtin_amdgcn_exp2f(fmaf(s[c / 2][r], scale2, -base)),
-                                 __builtin_amdgcn_exp2f(fmaf(s[c / 2][r + 1], scale2, -base)));
-    l = attn_add2<DT>(w[c & 1][i], l);
-  };
-  const auto values = [&](int j) {
-    const int c = j / kD, d = j % kD;
-    const int ra = 16 * c + trow, rb = ra + 8;
-    const uint2 lo = prompt_read_tr(vs + ra * (D * 2) + 16 * T::v_chunk(ra, 4 * d + tcol) + 8 * (lane & 1));
-    const uint2 hi = prompt_read_tr(vs + rb * (D * 2) + 16 * T::v_chunk(rb, 4 * d + tcol) + 8 * (lane & 1));
-    vf[j % (kAheadV + 1)] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-  };
-#pragma unroll
-  for (int j = 0; j < kAheadV; ++j) values(j);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) weight(0, i);
-#pragma unroll
-  for (int c = 0; c < kSteps; ++c) {
-    const uint4 wf = make_uint4(w[c & 1][0], w[c & 1][1], w[c & 1][2], w[c & 1][3]);
-#pragma unroll
-    for (int d = 0; d < kD; ++d) {
-      __builtin_amdgcn_sched_barrier(0);
-      const int j = c * kD + d;
-      o[d] = prompt_mfma<DT>(vf[j % (kAheadV + 1)], wf, o[d]);
-      if (j + kAheadV < kSteps * kD) values(j + kAheadV);
-      if (c + 1 < kSteps) {
-#pragma unroll
-        for (int i = 4 * d / kD; i < 4 * (d + 1) / kD; ++i) weight(c + 1, i);
-      }
-    }
-  }
-  __builtin_amdgcn_sched_barrier(0);
 }
 
 }  // namespace
