@@ -343,6 +343,56 @@ __device__ __forceinline__ float attn_row_sum(float l) {
   return l + __shfl_xor(l, 32, 64);
 }
 
+// The states of W waves' rows (up to `rows` of 16 each, every wave the same) meet in LDS: f(row, d, o, m, l) gets values d .. d + 3
+// of a row, unnormalised, its maximum and its sum.  Rows of LDS are four values apart, so that 16 rows do not meet in a bank.
+template <int D>
+constexpr int kMeetRow = D + 4;
+inline int attn_meet_bytes(int dim, int waves, int rows) { return waves * rows * (dim + 6) * static_cast<int>(sizeof(float)); }
+template <int D, int W, class F>
+__device__ __forceinline__ void attn_meet(const AttnRows<D> &a, float *sm, int rows, int lane, int wave, F f) {
+  const int i16 = lane & 15, j = lane >> 4;
+  float *ml = sm + W * rows * kMeetRow<D>;  // maxima and sums
+  if (i16 < rows) {
+    float *o = sm + (wave * rows + i16) * kMeetRow<D> + (D / 16) * 4 * j;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < D / 16; c += 4)
+        *reinterpret_cast<float4 *>(o + (D / 16) * r + c) = make_float4(a.o[c][r], a.o[c + 1][r], a.o[c + 2][r], a.o[c + 3][r]);
+    if (j == 0) *reinterpret_cast<float2 *>(ml + (wave * rows + i16) * 2) = make_float2(a.m, a.l);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < rows * (D / 4); e += 64 * W) {
+    const int row = e / (D / 4), d = e % (D / 4) * 4;
+    float2 of[W];
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      of[w] = *reinterpret_cast<const float2 *>(ml + (w * rows + row) * 2);
+      m = fmaxf(m, of[w].x);
+    }
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float x = of[w].x == m ? 1.0f : __builtin_amdgcn_exp2f(of[w].x - m);
+      const float4 v = *reinterpret_cast<const float4 *>(sm + (w * rows + row) * kMeetRow<D> + d);
+      o.x += x * v.x;
+      o.y += x * v.y;
+      o.z += x * v.z;
+      o.w += x * v.w;
+      l += x * of[w].y;
+    }
+    f(row, d, o, m, l);
+  }
+}
+// A row's values, normalised, in their type.
+template <int DT>
+__device__ __forceinline__ uint2 attn_outputs(float4 o, float l) {
+  const bool none = l == 0.f;
+  return make_uint2(attn_pack2<DT>(none ? 0.f : o.x / l, none ? 0.f : o.y / l), attn_pack2<DT>(none ? 0.f : o.z / l, none ? 0.f : o.w / l));
+}
+
 // ---- packed sequences
 // Of the sequences' counts n(b), b < batch, in parts of `per`: which sequence the part `at` belongs to and which of its parts
 // it is.  Called by whole waves with uniform arguments, each lane looks at one sequence.

@@ -28,11 +28,29 @@ enum { kTree = 0, kWindow = 1 };
 // The lowest n bits.
 __device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1; }
 
+// Division of numbers below 2^31 by a number that the host knows: (x m) >> shift with m = ceil(2^shift / d), shift = 31 + ceil(log2
+// d): the quotient is too large by less than x / 2^shift < 1 / d, which no floor notices.  A launch of few tiles is bound by the
+// instructions on its way to them.
+struct MaskedDivisor {
+  uint32_t m;
+  int shift;
+  __device__ __forceinline__ int operator()(int x) const {
+    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * m >> shift);
+  }
+};
+inline MaskedDivisor masked_divisor(int d) {
+  int l = 0;
+  while (1 << l < d) ++l;
+  const int shift = 31 + l;
+  return {static_cast<uint32_t>(((uint64_t(1) << shift) + d - 1) / d), shift};
+}
+
 // What the rows see: plain arguments of a launch.
 struct MaskedRule {
   const int64_t *masks;  // kTree: [rows, words]
   int words;
   int window, sinks;     // kWindow
+  MaskedDivisor group;   // rows / group: tokens
 };
 
 // A sequence's rows and what they see, by the launch's rule.
@@ -119,73 +137,99 @@ struct MaskedPlan {
     return s;
   }
   __device__ __forceinline__ int items(const MaskedSeq<MODE> &s) const {
-    return static_cast<int>((static_cast<int64_t>(s.n) * rows.grp + FORM::kItem - 1) / FORM::kItem);
+    return (s.n * rows.grp + FORM::kItem - 1) / FORM::kItem;  // rows of all are below 2^31 - kItem
   }
-  // The tokens of an item, and where it looks.
+  // Where an item looks.
   __device__ __forceinline__ void span(const MaskedSeq<MODE> &s, int item, int &to, int &gap_from, int &gap) const {
-    const int a = item * FORM::kItem / rows.grp, b = min((item * FORM::kItem + FORM::kItem - 1) / rows.grp, s.n - 1);
+    int a = 0, b = 0;
+    if constexpr (MODE == kWindow) {
+      a = rule.group(item * FORM::kItem);
+      b = min(rule.group(item * FORM::kItem + FORM::kItem - 1), s.n - 1);
+    }
     int gap_to;
     s.span(a, b, to, gap_from, gap_to);
     gap = gap_to - gap_from;
   }
-  // Tiles of a sequence's longest item: its last one's, one more at most where windows begin inside of a tile.  One at least.
-  __device__ __forceinline__ int tiles(const MaskedSeq<MODE> &s, int items) const {
-    int to, from, gap;
-    span(s, items - 1, to, from, gap);
-    return max((to - gap + FORM::kStep - 1) / FORM::kStep, 1);
+  static __device__ __forceinline__ int tiles(int to, int gap) { return (to - gap + FORM::kStep - 1) / FORM::kStep; }
+  // Items of a sequence, and the tiles of its last one (one at least), which is the longest but for a tile where windows begin
+  // inside of one.
+  struct Row {
+    int items, tiles;
+  };
+  __device__ __forceinline__ Row row(int b, uint64_t &held) const {
+    Row r{0, 1};
+    if (b < rows.batch + 2) {
+      const MaskedSeq<MODE> s = seq(b);
+      held += s.n;
+      r.items = items(s);
+      int to, from, gap;
+      span(s, max(r.items - 1, 0), to, from, gap);
+      r.tiles = max(tiles(to, gap), 1);
+    }
+    return r;
   }
-  // The part that this workgroup, number `at` of its head's, takes.  `share`: workgroups of a head that the card holds at once.
-  // Uniform; every wave looks at all sequences, one a lane.
-  __device__ __forceinline__ bool find(int at, int share, MaskedPart<MODE> &p) const {
+  // The part that this workgroup, number `at` of its head's, takes.  `share`: workgroups of a head that the card holds at once;
+  // cut: how many of the parts have others.  Uniform; every wave looks at all sequences, one a lane.
+  __device__ __forceinline__ bool find(int at, int share, MaskedPart<MODE> &p, uint32_t &cut) const {
     const int lane = threadIdx.x & 63, n = rows.batch + 2;
-    struct Row {
-      int items, tiles;
-    };
-    const auto row = [&](int b) {
-      Row r{0, 1};
-      if (b < n) {
-        const MaskedSeq<MODE> s = seq(b);
-        r.items = items(s);
-        if (r.items) r.tiles = tiles(s, r.items);
-      }
-      return r;
-    };
-    const Row near = row(lane);
-    uint64_t all = 0, held = 0;
-    for (int b0 = 0; b0 < n; b0 += 64) {
-      const Row r = b0 ? row(b0 + lane) : near;
-      all += static_cast<uint64_t>(r.items) * r.tiles;
-      held += b0 + lane < n ? rows.end(b0 + lane) - rows.first(b0 + lane) : 0;
+    uint64_t held = 0, unused = 0;
+    const Row near = row(lane, held);
+    uint32_t all = near.items * near.tiles;
+    for (int b = lane + 64; b - lane < n; b += 64) {
+      const Row r = row(b, held);
+      all += r.items * r.tiles;
     }
     all = wave_sum(all);
+    cut = 0;
     // offsets that do not ascend: the sequences' rows add up to more than there are
     if (wave_sum(held) != static_cast<uint64_t>(rows.rows)) return false;
-    const int equal = static_cast<int>(all / share), limit = equal + min(equal / 2, FORM::kSlack) + 1;
-    const auto parts = [&](const Row &r) { return r.tiles > limit ? (r.tiles + limit - 1) / limit : 1; };
-    const int index = at;
+    const int equal = static_cast<int>(all / static_cast<uint32_t>(share)), limit = equal + min(equal / 2, FORM::kSlack) + 1;
+    const auto parts = [&](const Row &r) { return r.tiles > limit ? static_cast<int>(static_cast<uint32_t>(r.tiles + limit - 1) / static_cast<uint32_t>(limit)) : 1; };
+    const int near_parts = parts(near), index = at;
+    if (at == 0) {
+      uint32_t c = near_parts > 1 ? near.items * near_parts : 0;
+      for (int b = lane + 64; b - lane < n; b += 64) {
+        const Row r = row(b, unused);
+        c += r.tiles > limit ? r.items * parts(r) : 0;
+      }
+      cut = wave_sum(c);
+    }
     for (int order = 0; order < 4; ++order) {  // those in parts, then the whole ones, by halves
       for (int b0 = 0; b0 < n; b0 += 64) {
-        const Row r = b0 ? row(b0 + lane) : near;
+        Row r = near;
+        int in = near_parts;
+        if (b0) {
+          r = row(b0 + lane, unused);
+          in = parts(r);
+        }
         const int mine = r.tiles > limit ? 0 : 2 * r.tiles > limit ? 1 : 4 * r.tiles > limit ? 2 : 3;
-        const int count = mine == order ? r.items * parts(r) : 0;
+        const int count = mine == order ? r.items * in : 0;
         const int upto = static_cast<int>(wave_scan(static_cast<uint32_t>(count)));
         const uint64_t past = __ballot(upto > at);
         if (past) {
           const int l = __builtin_ctzll(past);
           p.b = b0 + l;
-          p.parts = __builtin_amdgcn_readlane(parts(r), l);
-          at -= __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l);
-          p.item = at / p.parts;
-          p.part = at - p.item * p.parts;
+          p.parts = __builtin_amdgcn_readlane(in, l);
+          p.item = at - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l));
+          p.part = 0;
           p.slot = index;  // those in parts come first: below 2 share, for each has more than half of `limit` tiles
           p.seq = seq(p.b);
           p.seq.first = __builtin_amdgcn_readfirstlane(p.seq.first);
           p.seq.n = __builtin_amdgcn_readfirstlane(p.seq.n);
           p.seq.len = __builtin_amdgcn_readfirstlane(p.seq.len);
+          if (p.parts > 1) {
+            at = p.item;
+            p.item = at / p.parts;
+            p.part = at - p.item * p.parts;
+          }
           span(p.seq, p.item, p.to, p.gap_from, p.gap);
-          const int64_t tiles = (p.to - p.gap + FORM::kStep - 1) / FORM::kStep;
-          p.from = static_cast<int>(p.part * tiles / p.parts) * FORM::kStep;
-          p.end = min(static_cast<int>((p.part + 1) * tiles / p.parts) * FORM::kStep, p.to - p.gap);
+          p.from = 0;
+          p.end = p.to - p.gap;
+          if (p.parts > 1) {  // the first ones take a tile more where they do not come out even
+            const int t = tiles(p.to, p.gap), each = t / p.parts, more = t - each * p.parts;
+            p.from = (p.part * each + min(p.part, more)) * FORM::kStep;
+            p.end = min(((p.part + 1) * each + min(p.part + 1, more)) * FORM::kStep, p.end);
+          }
           return true;
         }
         at -= __builtin_amdgcn_readlane(upto, 63);
@@ -266,19 +310,20 @@ __device__ __attribute__((noinline)) void masked_rows16(const MaskedRows<MODE> &
     }
 }
 
-// Number of an item among all of a head, of rows that begin at packed row `first` of sequence b: no two are alike.
-template <class FORM>
-__device__ __forceinline__ int64_t masked_item(int first, int grp, int b, int item) {
-  return static_cast<int64_t>(first) * grp / FORM::kItem + b + item;
-}
-// Sequences in the order of their rows: what lies before the first (batch + 1), the sequences, what lies behind the last (batch).
-__device__ __forceinline__ int masked_order(int b, int batch) { return b == batch + 1 ? 0 : b + 1; }
-
-// Where an item's parts are: the first slot, how many.
-template <class FORM, int MODE>
-__device__ __forceinline__ void masked_tell(const MaskedPart<MODE> &p, int2 *joins, int grp, int batch, int kvh, int kh) {
-  if (p.part == 0 && threadIdx.x == 0)
-    joins[masked_item<FORM>(p.seq.first, grp, masked_order(p.b, batch), p.item) * kvh + kh] = make_int2(p.slot, p.parts);
+// Of an item's first part: its slot, how many there are, the item's first row counted from the sequence's, and the packed row that
+// the sequence begins at.  Of the others: no parts.  And how many slots there are, from the first workgroup.
+template <int MODE, class FORM>
+__device__ __forceinline__ bool masked_find(const MaskedPlan<MODE, FORM> &plan, int kvh, int kh, int share, int4 *joins, MaskedPart<MODE> &p) {
+  uint32_t cut;
+  const int at = blockIdx.x / kvh;
+  const bool found = plan.find(at, share, p, cut);
+  if (threadIdx.x == 0) {
+    if (blockIdx.x == 0) joins->x = cut;
+    if (found && p.parts > 1)
+      joins[1 + p.slot * kvh + kh] = make_int4(p.part == 0 ? p.parts : 0, min(p.seq.n * plan.rows.grp - p.item * FORM::kItem, FORM::kItem),
+                                               p.item * FORM::kItem, p.seq.first);
+  }
+  return found;
 }
 
 template <int D, int DT, int MODE>
@@ -287,7 +332,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void masked_wide_ker
     int64_t khead, int64_t krow, const uint16_t *__restrict__ v, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
     int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
     const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, MaskedRule rule, int share, int slot_rows,
-    float scale2, uint32_t flip, float *__restrict__ parts, int2 *__restrict__ joins, uint16_t *__restrict__ out) {
+    float scale2, uint32_t flip, float *__restrict__ parts, int4 *__restrict__ joins, uint16_t *__restrict__ out) {
   using T = PromptTile<D>;
   constexpr int kStage = T::kStage, kS = kTile / 32;
   extern __shared__ __attribute__((aligned(1024))) int8_t masked_smem[];  // two stages of K and V
@@ -295,9 +340,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void masked_wide_ker
   const int kh = blockIdx.x % kvh;
   const MaskedPlan<MODE, Wide> plan{{starts, batch, rows, grp}, lens, width << shift, rule};
   MaskedPart<MODE> p;
-  if (!plan.find(blockIdx.x / kvh, share, p)) return;
+  if (!masked_find(plan, kvh, kh, share, joins, p)) return;
   const MaskedSeq<MODE> &seq = p.seq;
-  masked_tell<Wide>(p, joins, grp, batch, kvh, kh);
   const int from = __builtin_amdgcn_readfirstlane(p.from), end = __builtin_amdgcn_readfirstlane(p.end);
   const int mask = (1 << shift) - 1;
   // Of this lane's 16 bytes of a load: their chunk in LDS, and their bytes behind the load's first row.  The chunks of a wave's
@@ -312,8 +356,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void masked_wide_ker
 
   const int n_rows = seq.n * grp, r0 = p.item * kRows + wave * 32, row_at = r0 + i32;
   const bool row = row_at < n_rows;
-  const int token = row ? row_at / grp : 0, head = kh * grp + (row ? row_at - token * grp : 0);
-  const int wave_a = r0 / grp, wave_b = min((r0 + 31) / grp, seq.n - 1);
+  const int token = row ? rule.group(row_at) : 0, head = kh * grp + (row ? row_at - token * grp : 0);
+  const int wave_a = rule.group(r0), wave_b = min(rule.group(r0 + 31), seq.n - 1);
   uint4 qf[D / 16];
   const uint16_t *qp = q + (seq.first + token) * q_row + head * q_head + 8 * h;
 #pragma unroll
@@ -455,18 +499,16 @@ __global__ __launch_bounds__(64 * kWaves, masked_round(D)) void masked_narrow_ke
     int64_t khead, int64_t krow, const uint16_t *__restrict__ v, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
     int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
     const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, MaskedRule rule, int share, int slot_rows,
-    float scale2, uint32_t flip, float *__restrict__ parts, int2 *__restrict__ joins, uint16_t *__restrict__ out) {
-  extern __shared__ float narrow_smem[];  // [kWaves][16][D] outputs, then [kWaves][16][2] maxima and sums
-  float *sm = narrow_smem, *ml = sm + kWaves * 16 * D;
+    float scale2, uint32_t flip, float *__restrict__ parts, int4 *__restrict__ joins, uint16_t *__restrict__ out) {
+  extern __shared__ __attribute__((aligned(16))) float narrow_smem[];  // the four waves' states (attn_meet)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, j = lane >> 4;
   const int kh = blockIdx.x % kvh;
   const MaskedPlan<MODE, Narrow> plan{{starts, batch, rows, grp}, lens, width << shift, rule};
   MaskedPart<MODE> p;
-  if (!plan.find(blockIdx.x / kvh, share, p)) return;
+  if (!masked_find(plan, kvh, kh, share, joins, p)) return;
   const MaskedSeq<MODE> &seq = p.seq;
-  masked_tell<Narrow>(p, joins, grp, batch, kvh, kh);
   const int n_rows = seq.n * grp, r0 = p.item * 16, held = min(n_rows - r0, 16), row_at = r0 + min(i16, held - 1);
-  const int token = row_at / grp, head = kh * grp + row_at - token * grp;
+  const int token = rule.group(row_at), head = kh * grp + row_at - token * grp;
   uint4 qf[D / 32];
   const uint16_t *qp = q + (seq.first + token) * q_row + head * q_head + 8 * j;
 #pragma unroll
@@ -474,96 +516,74 @@ __global__ __launch_bounds__(64 * kWaves, masked_round(D)) void masked_narrow_ke
   const KvSource<true> src{k + kh * khead, v + kh * vhead, kpage, krow, vpage, vrow,
                            table + static_cast<int64_t>(min(p.b, batch - 1)) * width, shift, (1 << shift) - 1, pages,
                            p.to > 0 ? (p.to - 1) >> shift : 0};
-  const MaskedSeen<MODE> seen{seq, token, r0 / grp, min((r0 + 15) / grp, seq.n - 1), p.gap_from, p.gap, 0, false};
+  const MaskedSeen<MODE> seen{seq, token, rule.group(r0), min(rule.group(r0 + 15), seq.n - 1), p.gap_from, p.gap, 0, false};
   AttnRows<D> a;
   attn_clear(a);
   attn_walk<D, DT, true>(a, src, qf, p.from + 32 * wave, p.end, Narrow::kStep, seen, flip ? -scale2 : scale2, lane);
   a.l = attn_row_sum(a.l);
 
-  // the four waves' states meet
-  if (i16 < held) {
-    float *o = sm + (wave * 16 + i16) * D + (D / 16) * 4 * j;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) o[(D / 16) * r + c] = a.o[c][r];
-    if (j == 0) {
-      ml[(wave * 16 + i16) * 2] = a.m;
-      ml[(wave * 16 + i16) * 2 + 1] = a.l;
-    }
-  }
-  __syncthreads();
   float *part = parts + (static_cast<int64_t>(p.slot) * kvh + kh) * slot_rows * (D + 2);
-  for (int e = threadIdx.x; e < held * D; e += 64 * kWaves) {
-    const int row = e / D, d = e % D;
-    float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[(w * 16 + row) * 2]);
-    float o = 0.f, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float mw = ml[(w * 16 + row) * 2];
-      const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-      o += f * sm[(w * 16 + row) * D + d];
-      l += f * ml[(w * 16 + row) * 2 + 1];
-    }
+  attn_meet<D, kWaves>(a, narrow_smem, held, lane, wave, [&](int row, int d, float4 o, float m, float l) {
     if (p.parts == 1) {
-      const float x = l == 0.f ? 0.f : o / l;
-      const int t = (r0 + row) / grp;
-      out[((seq.first + static_cast<int64_t>(t)) * kvh * grp + kh * grp + r0 + row - t * grp) * D + d] = DT == MP_F16 ? mp_f2h(x) : mp_f2bf(x);
+      const int t = rule.group(r0 + row);
+      *reinterpret_cast<uint2 *>(out + ((seq.first + static_cast<int64_t>(t)) * kvh * grp + kh * grp + r0 + row - t * grp) * D + d) =
+          attn_outputs<DT>(o, l);
     } else {
-      part[row * (D + 2) + d] = o;
-      if (d == 0) {
-        part[row * (D + 2) + D] = m;
-        part[row * (D + 2) + D + 1] = l;
-      }
+      float2 *z = reinterpret_cast<float2 *>(part + row * (D + 2));  // rows are 8 bytes apart
+      z[d / 2] = make_float2(o.x, o.y);
+      z[d / 2 + 1] = make_float2(o.z, o.w);
+      if (d == 0) z[D / 2] = make_float2(m, l);
     }
-  }
+  });
 }
 
-// The parts of a row meet, one wave each.
+// The parts of an item meet: 16 of its rows in a workgroup, four in a wave, whose loads are under way together.
 template <int D, int DT, class FORM>
-__global__ __launch_bounds__(256) void masked_join_kernel(const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp,
-                                                          int slot_rows, int slots, const float *__restrict__ parts,
-                                                          const int2 *__restrict__ joins, uint16_t *__restrict__ out) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int nh = kvh * grp, lane = threadIdx.x & 63;
-  if (at >= static_cast<int64_t>(rows) * nh) return;
-  const int t = static_cast<int>(at / nh), qh = static_cast<int>(at - static_cast<int64_t>(t) * nh), kh = qh / grp;
-  // the sequence of packed row t: how many of them begin at or before it
-  const PackedPlan plan{starts, batch, rows, grp};
-  int b = 0;
-  for (int b0 = 0; b0 <= batch; b0 += 64) b += __popcll(__ballot(b0 + lane <= batch && starts[min(b0 + lane, batch)] <= t));
-  b = b == 0 ? batch + 1 : b - 1;
-  const int first = plan.first(b), r = (t - first) * grp + qh - kh * grp, item = r / FORM::kItem;
-  if (t < first || t >= plan.end(b)) return;  // offsets that do not ascend: nothing was left
-  const int2 of = joins[masked_item<FORM>(first, grp, masked_order(b, batch), item) * kvh + kh];
-  // written already; the rest: offsets that do not ascend, nothing was left
-  if (of.y < 2 || of.x < 0 || of.x >= slots) return;
-  const int64_t from_slot = of.x;
-  if (of.y > slots - from_slot) return;
-  const auto at_part = [&](int p) {
-    return parts + (((from_slot + p) * kvh + kh) * slot_rows + r % FORM::kItem) * (D + 2);
-  };
+__global__ __launch_bounds__(256) void masked_join_kernel(int kvh, int grp, int slot_rows, MaskedDivisor group,
+                                                          const float *__restrict__ parts, const int4 *__restrict__ joins,
+                                                          uint16_t *__restrict__ out) {
+  const int slot = blockIdx.x / kvh, kh = blockIdx.x - slot * kvh, lane = threadIdx.x & 63;
+  const int4 of = joins[1 + blockIdx.x];  // open past the last slot
+  const int r0 = blockIdx.y * 16 + 4 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (slot >= joins->x || of.x < 2 || r0 >= of.y) return;
+  const int64_t step = static_cast<int64_t>(kvh) * slot_rows * (D + 2);  // from part to part
+  const float *item = parts + static_cast<int64_t>(blockIdx.x) * slot_rows * (D + 2);
+  const auto row = [&](int k) { return item + min(r0 + k, of.y - 1) * (D + 2); };
+  // maxima: 16 lanes to a row
   float m = -INFINITY;
-  for (int p = lane; p < of.y; p += 64) m = fmaxf(m, at_part(p)[D]);
-  m = mp_wave_max(m);
-  float o[D / 64], l = 0.f;
+  for (int p = lane & 15; p < of.x; p += 16) m = fmaxf(m, row(lane >> 4)[p * step + D]);
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
-#pragma unroll 4
-  for (int p = 0; p < of.y; ++p) {
-    const float *z = at_part(p);
-    const float f = z[D] == m ? 1.0f : __builtin_amdgcn_exp2f(z[D] - m);
-    l += f * z[D + 1];
+  for (int i = 8; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+  float o[4][D / 64], l[4], top[4];
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] += f * z[64 * i + lane];
+  for (int k = 0; k < 4; ++k) {
+    top[k] = __shfl(m, 16 * k, 64);
+    l[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) o[k][i] = 0.f;
   }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll 2
+  for (int p = 0; p < of.x; ++p) {
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const float x = l == 0.f ? 0.f : o[i] * inv;
-    out[at * D + 64 * i + lane] = DT == MP_F16 ? mp_f2h(x) : mp_f2bf(x);
+    for (int k = 0; k < 4; ++k) {
+      const float *z = row(k) + p * step;
+      const float f = z[D] == top[k] ? 1.0f : __builtin_amdgcn_exp2f(z[D] - top[k]);
+      l[k] += f * z[D + 1];
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) o[k][i] += f * z[64 * i + lane];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (r0 + k >= of.y) return;
+    const float inv = l[k] == 0.f ? 0.f : 1.0f / l[k];
+    const int token = group(of.z + r0 + k), head = kh * grp + of.z + r0 + k - token * grp;
+    uint16_t *y = out + ((static_cast<int64_t>(of.w) + token) * kvh * grp + head) * D + lane;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const float x = l[k] == 0.f ? 0.f : o[k][i] * inv;
+      y[64 * i] = DT == MP_F16 ? mp_f2h(x) : mp_f2bf(x);
+    }
   }
 }
 
@@ -602,14 +622,15 @@ struct MaskedCall {
 };
 
 template <class FORM>
-size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim, int64_t batch) {
+size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim) {
   const int64_t grp = nh / kvh;
-  return static_cast<size_t>(masked_items<FORM>(rows, grp, batch) * kvh) * sizeof(int2) +
-         static_cast<size_t>(2 * masked_share<FORM>(kvh, dim) * kvh * masked_slot_rows<FORM>(rows, grp)) * (dim + 2) * sizeof(float);
+  const int64_t slots = 2 * masked_share<FORM>(kvh, dim) * kvh;
+  return static_cast<size_t>(1 + slots) * sizeof(int4) +
+         static_cast<size_t>(slots * masked_slot_rows<FORM>(rows, grp)) * (dim + 2) * sizeof(float);
 }
 size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim, int64_t batch) {
-  return masked_narrow(rows, nh / kvh, batch) ? masked_workspace<Narrow>(rows, nh, kvh, dim, batch)
-                                              : masked_workspace<Wide>(rows, nh, kvh, dim, batch);
+  return masked_narrow(rows, nh / kvh, batch) ? masked_workspace<Narrow>(rows, nh, kvh, dim)
+                                              : masked_workspace<Wide>(rows, nh, kvh, dim);
 }
 
 // Whether an item can be cut: no share has less than a tile, and what passes a share by one at most stays whole.
@@ -626,13 +647,13 @@ int masked_start(const MaskedCall &c, int shift) {
   constexpr bool kIsWide = FORM::kItem == kRows;
   const int grp = c.nh / c.kvh, share = static_cast<int>(masked_share<FORM>(c.kvh, D));
   const int slot_rows = static_cast<int>(masked_slot_rows<FORM>(c.rows, grp));
-  int2 *joins = static_cast<int2 *>(c.workspace);
-  float *parts = reinterpret_cast<float *>(joins + masked_items<FORM>(c.rows, grp, c.batch) * c.kvh);
+  int4 *joins = static_cast<int4 *>(c.workspace);
+  float *parts = reinterpret_cast<float *>(joins + 1 + 2 * static_cast<int64_t>(share) * c.kvh);
   // the sign of the scale goes to the queries, so that the largest product gives the largest score; a scale of 0 becomes the
   // smallest normal number, which leaves every finite score 0 and a masked one -inf
   const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
   const float scale2 = fmaxf(fabsf(c.scale) * kLog2e, FLT_MIN);
-  constexpr int kLds = kIsWide ? 2 * PromptTile<D>::kStage : kWaves * 16 * (D + 2) * static_cast<int>(sizeof(float));
+  constexpr int kLds = kIsWide ? 2 * PromptTile<D>::kStage : kWaves * 16 * (D + 6) * static_cast<int>(sizeof(float));
   constexpr auto kKernel = kIsWide ? &masked_wide_kernel<D, DT, MODE> : &masked_narrow_kernel<D, DT, MODE>;
   if (kLds > 64 * 1024 &&
       hipFuncSetAttribute(reinterpret_cast<const void *>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
@@ -646,9 +667,8 @@ int masked_start(const MaskedCall &c, int shift) {
                      static_cast<uint16_t *>(c.out));
   MP_CHECK_LAUNCH();
   if (masked_splits<FORM>(c, MODE)) {
-    hipLaunchKernelGGL((masked_join_kernel<D, DT, FORM>), dim3(static_cast<unsigned>(mp_cdiv(c.rows * c.nh, 4))), dim3(256), 0,
-                       c.stream, c.starts, static_cast<int>(c.batch), static_cast<int>(c.rows), c.kvh, grp, slot_rows, 2 * share, parts,
-                       joins, static_cast<uint16_t *>(c.out));
+    hipLaunchKernelGGL((masked_join_kernel<D, DT, FORM>), dim3(static_cast<unsigned>(2 * share * c.kvh), FORM::kItem / 16), dim3(256), 0,
+                       c.stream, c.kvh, grp, slot_rows, c.rule.group, parts, joins, static_cast<uint16_t *>(c.out));
     MP_CHECK_LAUNCH();
   }
   return MP_OK;
@@ -660,7 +680,7 @@ int masked_start(const MaskedCall &c, int shift) {
 }
 
 template <int MODE>
-int masked_launch(const MaskedCall &c) {
+int masked_launch(MaskedCall c) {
   if (!c.q || !c.cache || !c.cache->k || !c.cache->v || !c.cache->table || !c.lens || !c.starts || !c.out || !c.workspace)
     return MP_ERR_ARG;
   if (c.dtype != MP_F16 && c.dtype != MP_BF16) return MP_ERR_DTYPE;
@@ -686,6 +706,7 @@ int masked_launch(const MaskedCall &c) {
   if (c.rows == 0) return MP_OK;
   if (mp_cu_count() <= 0) return MP_ERR_HIP;
   if (c.workspace_bytes < masked_workspace(c.rows, c.nh, c.kvh, c.head_dim, c.batch)) return MP_ERR_WORKSPACE;
+  c.rule.group = masked_divisor(static_cast<int>(grp));
 #define MP_MASKED(DT)                                                        \
   return c.head_dim == 64 ? masked_start<64, DT, MODE>(c, shift)             \
                           : c.head_dim == 128 ? masked_start<128, DT, MODE>(c, shift) : masked_start<256, DT, MODE>(c, shift)
@@ -710,7 +731,7 @@ extern "C" int mp_paged_tree_attention(const void *q, int64_t q_row, int64_t q_h
   if (!masks) return MP_ERR_ARG;
   if (words < 1 || words > 1024) return MP_ERR_SHAPE;
   return masked_launch<kTree>({q, q_row, q_head, rows, nh, kvh, head_dim, cache, lens, starts, batch,
-                               {masks, static_cast<int>(words), 0, 0}, scale, out, dtype, workspace, workspace_bytes,
+                               {masks, static_cast<int>(words), 0, 0, {}}, scale, out, dtype, workspace, workspace_bytes,
                                reinterpret_cast<hipStream_t>(stream)});
 }
 
@@ -720,6 +741,6 @@ extern "C" int mp_paged_prompt_window_attention(const void *q, int64_t q_row, in
                                                 void *workspace, size_t workspace_bytes, mp_stream_t stream) {
   if (window < 1 || window > 1 << 30 || sinks < 0 || sinks > 1 << 30) return MP_ERR_SHAPE;
   return masked_launch<kWindow>({q, q_row, q_head, rows, nh, kvh, head_dim, cache, lens, starts, batch,
-                                 {nullptr, 0, static_cast<int>(window), static_cast<int>(sinks)}, scale, out, dtype, workspace,
+                                 {nullptr, 0, static_cast<int>(window), static_cast<int>(sinks), {}}, scale, out, dtype, workspace,
                                  workspace_bytes, reinterpret_cast<hipStream_t>(stream)});
 }

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(64 * kWaves, decode_round(D)) void paged_decode_ker
     int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens, int batch, int kvh, int grp,
     int tiles, int share, int window, int sinks, float scale2, float *__restrict__ part_o, float *__restrict__ part_ml, int4 *__restrict__ joins,
     uint16_t *__restrict__ out) {
-  extern __shared__ float sm[];  // [kWaves][rows][D] outputs, then [kWaves][rows][2] maxima and sums
+  extern __shared__ __attribute__((aligned(16))) float sm[];  // the four waves' states (attn_meet)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, j = lane >> 4;
   const int heads = kvh * tiles, h = blockIdx.x % heads, kh = h / tiles, run = blockIdx.x / heads;
   const DecodePlan<WIN> plan{lens, batch, width << shift, window, sinks};
@@ -183,7 +183,6 @@ __global__ __launch_bounds__(64 * kWaves, decode_round(D)) void paged_decode_ker
   if (run >= share || !attn_find_part(plan, batch, 0, from, b, at, blocks)) return;  // uniform over the workgroup
   const int g0 = h % tiles * 16, rows = min(16, grp - g0);  // query heads of this workgroup
   const int nh = kvh * grp;
-  float *ml = sm + kWaves * rows * D;
   KvSource<true> src{k_pages + kh * khead, v_pages + kh * vhead, kpage, krow, vpage, vrow, nullptr, shift, (1 << shift) - 1, pages, 0};
 
   for (int left = to - from; left > 0; ++b, at = 0) {
@@ -203,48 +202,19 @@ __global__ __launch_bounds__(64 * kWaves, decode_round(D)) void paged_decode_ker
     else attn_walk<D, DT, false>(a, src, qf, at * kBlock + 32 * wave, t1, kBlock, SeenUpTo{t1, t1, t1}, scale2, lane);
     a.l = attn_row_sum(a.l);
 
-    // the four waves' states meet
-    if (i16 < rows) {
-      float *o = sm + (wave * rows + i16) * D + (D / 16) * 4 * j;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) o[(D / 16) * r + c] = a.o[c][r];
-      if (j == 0) {
-        ml[(wave * rows + i16) * 2] = a.m;
-        ml[(wave * rows + i16) * 2 + 1] = a.l;
-      }
-    }
-    __syncthreads();
     const int64_t slot = (static_cast<int64_t>(2 * run + (left < to - from ? 1 : 0)) * heads + h) * min(grp, 16);
     if (at == 0 && threadIdx.x == 0) {
       const int last = static_cast<int>(((to - left + blocks) * static_cast<uint64_t>(share) - 1) / all);  // run of its last block
       joins[b * heads + h] = make_int4(run, last - run + 1, left < to - from ? 1 : 0, 0);
     }
-    for (int e = threadIdx.x; e < rows * D; e += 64 * kWaves) {
-      const int row = e / D, d = e % D;
-      float m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[(w * rows + row) * 2]);
-      float o = 0.f, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float mw = ml[(w * rows + row) * 2];
-        const float f = mw == m ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-        o += f * sm[(w * rows + row) * D + d];
-        l += f * ml[(w * rows + row) * 2 + 1];
-      }
+    attn_meet<D, kWaves>(a, sm, rows, lane, wave, [&](int row, int d, float4 o, float m, float l) {
       if (whole) {
-        const float v = l == 0.f ? 0.f : o / l;
-        out[(static_cast<int64_t>(b) * nh + kh * grp + g0 + row) * D + d] = DT == MP_F16 ? mp_f2h(v) : mp_f2bf(v);
+        *reinterpret_cast<uint2 *>(out + (static_cast<int64_t>(b) * nh + kh * grp + g0 + row) * D + d) = attn_outputs<DT>(o, l);
       } else {
-        part_o[(slot + row) * D + d] = o;
-        if (d == 0) {
-          part_ml[(slot + row) * 2] = m;
-          part_ml[(slot + row) * 2 + 1] = l;
-        }
+        *reinterpret_cast<float4 *>(part_o + (slot + row) * D + d) = o;
+        if (d == 0) *reinterpret_cast<float2 *>(part_ml + (slot + row) * 2) = make_float2(m, l);
       }
-    }
+    });
     left -= end - at;
     if (left > 0) __syncthreads();  // the next sequence's states go to the same place
   }
@@ -403,7 +373,7 @@ int decode_launch(const void *q, int64_t q_row, int64_t q_head, int64_t batch, i
   const int64_t capacity = cache->width << shift;
   if (blocks > INT32_MAX || batch * nh > INT32_MAX || batch * mp_cdiv(capacity, kBlock) > INT32_MAX) return MP_ERR_SHAPE;
   const float scale2 = scale * kLog2e;
-  const int lds = kWaves * per * (head_dim + 2) * static_cast<int>(sizeof(float));
+  const int lds = attn_meet_bytes(head_dim, kWaves, per);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define MP_DECODE(D, DT)                                                                                                  \
   do {                                                                                                                    \
