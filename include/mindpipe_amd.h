@@ -495,10 +495,11 @@ int mp_paged_prompt_attention(const void *q, int64_t q_row, int64_t q_head, int6
  * tree: the positions before the sequence's new tokens, and of those the ones whose bits are set: bit i of word w of masks
  *   int64 [rows, words] (1 to 1024 words) is new token 64 w + i of the row's sequence;
  * window: of the positions up to its own the last `window` (1 to 2^30) and the first `sinks` of the sequence (0 to 2^30).
- * Otherwise as mp_paged_prompt_attention.  Rows that see nothing are zeros.  The tiles of all rows are split into equal runs and
- * joined in a fixed order.  workspace: mp_masked_workspace_bytes of the current device, 16-byte aligned, not shared by calls that
- * may run at once.  Offsets that do not ascend leave the outputs open. */
-size_t mp_masked_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch);
+ * Otherwise as mp_paged_prompt_attention.  Rows that see nothing are zeros.  Rows with much more to see than others are split and
+ * joined in a fixed order.  workspace: mp_masked_workspace_bytes of the current device (capacity: width * page_size; window and sinks
+ * 0 for a tree), 16-byte aligned, not shared by calls that may run at once.  Offsets that do not ascend leave the outputs open. */
+size_t mp_masked_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch, int64_t capacity, int64_t window,
+                                 int64_t sinks);
 int mp_paged_tree_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh, int head_dim,
                             const mp_pages *cache, const int32_t *lens, const int32_t *starts, int64_t batch,
                             const int64_t *masks, int64_t words, float scale, void *out, int dtype, void *workspace,

@@ -101,14 +101,15 @@ struct MaskedSeq {
   }
 };
 
-// The form of a kernel: rows of an item, positions of a tile, and by how many tiles an item may pass an equal share and stay whole
-// (half a share at most): joining costs what so many tiles do.
+// The form of a kernel: rows of an item, positions of a tile, by how many tiles an item may pass an equal share and stay whole (half
+// a share at most: joining costs what so many tiles do), and the share from which on items are cut finer, once one has to be.
 struct Wide {
-  static constexpr int kItem = kRows, kStep = kTile, kSlack = 8;
+  static constexpr int kItem = kRows, kStep = kTile, kSlack = 8, kFiner = 12;
 };
 struct Narrow {
-  static constexpr int kItem = 16, kStep = 128, kSlack = 2;
+  static constexpr int kItem = 16, kStep = 128, kSlack = 2, kFiner = INT_MAX;
 };
+constexpr int kSlots = 3;  // parts that have others, in shares: each has more than half of two thirds of a share
 
 // What a workgroup takes: tiles of an item.
 template <int MODE>
@@ -183,8 +184,31 @@ struct MaskedPlan {
     cut = 0;
     // offsets that do not ascend: the sequences' rows add up to more than there are
     if (wave_sum(held) != static_cast<uint64_t>(rows.rows)) return false;
-    const int equal = static_cast<int>(all / static_cast<uint32_t>(share)), limit = equal + min(equal / 2, FORM::kSlack) + 1;
+    // Items stay whole where none is much longer than an equal share.  Otherwise parts are as long as such an item, or two thirds of
+    // a share, as the longest part and the number of rounds have it (24 sequences of up to 8192 positions with trees of up to 64
+    // nodes, 58 items of 1 to 129 tiles for 64 workgroups: 186 us, 152 with the finer ones).
+    const int equal = static_cast<int>(all / static_cast<uint32_t>(share));
+    int limit = equal + min(equal / 2, FORM::kSlack) + 1;
     const auto parts = [&](const Row &r) { return r.tiles > limit ? static_cast<int>(static_cast<uint32_t>(r.tiles + limit - 1) / static_cast<uint32_t>(limit)) : 1; };
+    if (equal >= FORM::kFiner) {
+      const int keep = limit;
+      int took[2] = {0, 0};
+      for (int i = 0; i < 2; ++i) {
+        limit = i ? equal * 2 / 3 + 1 : keep;
+        uint32_t count = near.items * parts(near);
+        int longest = near.items ? (near.tiles + parts(near) - 1) / parts(near) : 0;
+        for (int b = lane + 64; b - lane < n; b += 64) {
+          const Row r = row(b, unused);
+          count += r.items * parts(r);
+          longest = max(longest, r.items ? (r.tiles + parts(r) - 1) / parts(r) : 0);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
+        const int rounds = static_cast<int>((wave_sum(count) + share - 1) / static_cast<uint32_t>(share));
+        took[i] = min(rounds * longest, equal + longest) + 2 * rounds;  // two tiles to start a part
+      }
+      limit = took[1] && took[1] < took[0] ? limit : keep;
+    }
     const int near_parts = parts(near), index = at;
     if (at == 0) {
       uint32_t c = near_parts > 1 ? near.items * near_parts : 0;
@@ -212,7 +236,7 @@ struct MaskedPlan {
           p.parts = __builtin_amdgcn_readlane(in, l);
           p.item = at - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l));
           p.part = 0;
-          p.slot = index;  // those in parts come first: below 2 share, for each has more than half of `limit` tiles
+          p.slot = index;  // those in parts come first, below kSlots share: each has more than half of `limit` tiles
           p.seq = seq(p.b);
           p.seq.first = __builtin_amdgcn_readfirstlane(p.seq.first);
           p.seq.n = __builtin_amdgcn_readfirstlane(p.seq.n);
@@ -257,6 +281,7 @@ struct MaskedSeen {
   __device__ __forceinline__ int place(int v) const { return v < gap_from ? v : v + gap; }
   __device__ __forceinline__ void look(int tile) {
     every = s.whole(a, b, tile, tile + 32);
+    mine = ~0u;
     if (!every) mine = static_cast<uint32_t>(s.bits(token, tile));
   }
   __device__ __forceinline__ bool sees(int p) const { return (mine >> (p & 31)) & 1; }
@@ -537,54 +562,40 @@ __global__ __launch_bounds__(64 * kWaves, masked_round(D)) void masked_narrow_ke
   });
 }
 
-// The parts of an item meet: 16 of its rows in a workgroup, four in a wave, whose loads are under way together.
+// The parts of an item meet: 16 of its rows in a workgroup, four in a wave, 16 lanes to each.
 template <int D, int DT, class FORM>
 __global__ __launch_bounds__(256) void masked_join_kernel(int kvh, int grp, int slot_rows, MaskedDivisor group,
                                                           const float *__restrict__ parts, const int4 *__restrict__ joins,
                                                           uint16_t *__restrict__ out) {
-  const int slot = blockIdx.x / kvh, kh = blockIdx.x - slot * kvh, lane = threadIdx.x & 63;
+  const int slot = blockIdx.x / kvh, kh = blockIdx.x - slot * kvh, i16 = threadIdx.x & 15;
   const int4 of = joins[1 + blockIdx.x];  // open past the last slot
-  const int r0 = blockIdx.y * 16 + 4 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (slot >= joins->x || of.x < 2 || r0 >= of.y) return;
-  const int64_t step = static_cast<int64_t>(kvh) * slot_rows * (D + 2);  // from part to part
-  const float *item = parts + static_cast<int64_t>(blockIdx.x) * slot_rows * (D + 2);
-  const auto row = [&](int k) { return item + min(r0 + k, of.y - 1) * (D + 2); };
-  // maxima: 16 lanes to a row
-  float m = -INFINITY;
-  for (int p = lane & 15; p < of.x; p += 16) m = fmaxf(m, row(lane >> 4)[p * step + D]);
+  const int r = blockIdx.y * 16 + (threadIdx.x >> 4);
+  if (slot >= joins->x || of.x < 2 || r >= of.y) return;
+  const int64_t step = static_cast<int64_t>(kvh) * slot_rows * (D + 2) / 2;  // from part to part
+  const float2 *z = reinterpret_cast<const float2 *>(parts + (static_cast<int64_t>(blockIdx.x) * slot_rows + r) * (D + 2));
+  float m = -INFINITY, l = 0.f;
+  float2 o[D / 32];
 #pragma unroll
-  for (int i = 8; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
-  float o[4][D / 64], l[4], top[4];
+  for (int c = 0; c < D / 32; ++c) o[c] = make_float2(0.f, 0.f);
+#pragma unroll 8
+  for (int p = 0; p < of.x; ++p, z += step) {
+    const float2 ml = z[D / 2];
+    float2 x[D / 32];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    top[k] = __shfl(m, 16 * k, 64);
-    l[k] = 0.f;
+    for (int c = 0; c < D / 32; ++c) x[c] = z[16 * c + i16];
+    const float top = fmaxf(m, ml.x), f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+    const float g = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
+    m = top;
+    l = l * f + ml.y * g;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[k][i] = 0.f;
+    for (int c = 0; c < D / 32; ++c) o[c] = make_float2(o[c].x * f + x[c].x * g, o[c].y * f + x[c].y * g);
   }
-#pragma unroll 2
-  for (int p = 0; p < of.x; ++p) {
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const bool none = l == 0.f;
+  const int token = group(of.z + r), head = kh * grp + of.z + r - token * grp;
+  uint32_t *y = reinterpret_cast<uint32_t *>(out + ((static_cast<int64_t>(of.w) + token) * kvh * grp + head) * D);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float *z = row(k) + p * step;
-      const float f = z[D] == top[k] ? 1.0f : __builtin_amdgcn_exp2f(z[D] - top[k]);
-      l[k] += f * z[D + 1];
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) o[k][i] += f * z[64 * i + lane];
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (r0 + k >= of.y) return;
-    const float inv = l[k] == 0.f ? 0.f : 1.0f / l[k];
-    const int token = group(of.z + r0 + k), head = kh * grp + of.z + r0 + k - token * grp;
-    uint16_t *y = out + ((static_cast<int64_t>(of.w) + token) * kvh * grp + head) * D + lane;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      const float x = l[k] == 0.f ? 0.f : o[k][i] * inv;
-      y[64 * i] = DT == MP_F16 ? mp_f2h(x) : mp_f2bf(x);
-    }
-  }
+  for (int c = 0; c < D / 32; ++c) y[16 * c + i16] = attn_pack2<DT>(none ? 0.f : o[c].x * inv, none ? 0.f : o[c].y * inv);
 }
 
 // Workgroups of a head: as many as fit the card at once.
@@ -602,8 +613,25 @@ template <class FORM>
 int64_t masked_items(int64_t rows, int64_t grp, int64_t batch) {
   return rows * grp / FORM::kItem + batch + 4;
 }
-// Few rows of a sequence and key-value head, on the average, are narrow.
-inline bool masked_narrow(int64_t rows, int64_t grp, int64_t batch) { return rows * grp <= 32 * batch; }
+// The most positions that a row's tile looks at.
+int64_t masked_reach(int64_t capacity, int64_t window, int64_t sinks) {
+  return window ? std::min(capacity, window + sinks + 3 * 64) : capacity;
+}
+// Narrow: few rows of a sequence and key-value head, on the average, for the positions of an item are read once and again by
+// every 16 rows; or little work in all, counted in rounds of narrow tiles, which start sooner.  Trees of bf16, us in the narrow and
+// the wide form, by rows of a sequence and head:
+//   one sequence of 1500, 32 / 8 heads of 128      64: 15, 22   256: 22, 35 (6 rounds)
+//   one of 16000, 64 / 8                           64: 37, 44 (18)  128: 54, 56 (27)  192: 69, 47
+//   16 of 3000, 64 / 8                             16: 39, 40   32: 41, 42         64: 66, 45 (39)
+//   64 of 2000, 64 / 8                              8: 103, 108  32: 129, 113      64: 191, 117
+//   4 of 2000, 16 / 4 heads of 256                128: 39, 45 (14)                192: 68, 42 (19)
+//   32 of 3000, 8 / 8 heads of 256                 16: 153, 191  24: 191, 193      48: 258, 199
+//   16 of 2000, 28 / 4 heads of 64                 28: 15, 18                     56: 22, 20 (7)
+bool masked_narrow(int64_t rows, int64_t grp, int64_t kvh, int dim, int64_t batch, int64_t reach) {
+  const int64_t slots = masked_round(dim) * mp_cu_count(), rounds = dim == 64 ? 4 : dim == 128 ? 18 : 12;
+  const int64_t tiles = mp_cdiv(reach, Narrow::kStep) + 6;  // an item starts and ends in the time of six
+  return rows * grp <= 32 * batch || masked_items<Narrow>(rows, grp, batch) * tiles * kvh <= rounds * slots;
+}
 
 struct MaskedCall {
   const void *q;
@@ -619,27 +647,19 @@ struct MaskedCall {
   void *workspace;
   size_t workspace_bytes;
   hipStream_t stream;
+  int64_t reach;
 };
 
 template <class FORM>
 size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim) {
   const int64_t grp = nh / kvh;
-  const int64_t slots = 2 * masked_share<FORM>(kvh, dim) * kvh;
+  const int64_t slots = kSlots * masked_share<FORM>(kvh, dim) * kvh;
   return static_cast<size_t>(1 + slots) * sizeof(int4) +
          static_cast<size_t>(slots * masked_slot_rows<FORM>(rows, grp)) * (dim + 2) * sizeof(float);
 }
-size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim, int64_t batch) {
-  return masked_narrow(rows, nh / kvh, batch) ? masked_workspace<Narrow>(rows, nh, kvh, dim)
+size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim, int64_t batch, int64_t reach) {
+  return masked_narrow(rows, nh / kvh, kvh, dim, batch, reach) ? masked_workspace<Narrow>(rows, nh, kvh, dim)
                                               : masked_workspace<Wide>(rows, nh, kvh, dim);
-}
-
-// Whether an item can be cut: no share has less than a tile, and what passes a share by one at most stays whole.
-template <class FORM>
-bool masked_splits(const MaskedCall &c, int mode) {
-  const int64_t grp = c.nh / c.kvh, span = mp_cdiv(FORM::kItem, grp) + 1;  // positions that an item's tokens spread over
-  int64_t reach = c.cache->width * c.cache->page_size;
-  if (mode == kWindow) reach = std::min(reach, static_cast<int64_t>(c.rule.window) + c.rule.sinks + span + 2 * 64);
-  return mp_cdiv(reach, FORM::kStep) > 1;
 }
 
 template <int D, int DT, int MODE, class FORM>
@@ -648,7 +668,7 @@ int masked_start(const MaskedCall &c, int shift) {
   const int grp = c.nh / c.kvh, share = static_cast<int>(masked_share<FORM>(c.kvh, D));
   const int slot_rows = static_cast<int>(masked_slot_rows<FORM>(c.rows, grp));
   int4 *joins = static_cast<int4 *>(c.workspace);
-  float *parts = reinterpret_cast<float *>(joins + 1 + 2 * static_cast<int64_t>(share) * c.kvh);
+  float *parts = reinterpret_cast<float *>(joins + 1 + kSlots * static_cast<int64_t>(share) * c.kvh);
   // the sign of the scale goes to the queries, so that the largest product gives the largest score; a scale of 0 becomes the
   // smallest normal number, which leaves every finite score 0 and a masked one -inf
   const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
@@ -659,15 +679,15 @@ int masked_start(const MaskedCall &c, int shift) {
       hipFuncSetAttribute(reinterpret_cast<const void *>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
     return MP_ERR_HIP;
   const mp_pages &p = *c.cache;
-  hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>((masked_items<FORM>(c.rows, grp, c.batch) + share) * c.kvh)), dim3(64 * kWaves), kLds, c.stream,
+  hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>((masked_items<FORM>(c.rows, grp, c.batch) + kSlots * share / 2 + 1) * c.kvh)), dim3(64 * kWaves), kLds, c.stream,
                      static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(p.k), p.k_page,
                      p.k_head, p.k_row, static_cast<const uint16_t *>(p.v), p.v_page, p.v_head, p.v_row, static_cast<int>(p.pages),
                      shift, p.table, static_cast<int>(p.width), c.lens, c.starts, static_cast<int>(c.batch),
                      static_cast<int>(c.rows), c.kvh, grp, c.rule, share, slot_rows, scale2, flip, parts, joins,
                      static_cast<uint16_t *>(c.out));
   MP_CHECK_LAUNCH();
-  if (masked_splits<FORM>(c, MODE)) {
-    hipLaunchKernelGGL((masked_join_kernel<D, DT, FORM>), dim3(static_cast<unsigned>(2 * share * c.kvh), FORM::kItem / 16), dim3(256), 0,
+  if (c.reach > FORM::kStep) {  // else items of one tile, which are never cut
+    hipLaunchKernelGGL((masked_join_kernel<D, DT, FORM>), dim3(static_cast<unsigned>(kSlots * share * c.kvh), FORM::kItem / 16), dim3(256), 0,
                        c.stream, c.kvh, grp, slot_rows, c.rule.group, parts, joins, static_cast<uint16_t *>(c.out));
     MP_CHECK_LAUNCH();
   }
@@ -675,8 +695,8 @@ int masked_start(const MaskedCall &c, int shift) {
 }
 template <int D, int DT, int MODE>
 int masked_start(const MaskedCall &c, int shift) {
-  return masked_narrow(c.rows, c.nh / c.kvh, c.batch) ? masked_start<D, DT, MODE, Narrow>(c, shift)
-                                                      : masked_start<D, DT, MODE, Wide>(c, shift);
+  return masked_narrow(c.rows, c.nh / c.kvh, c.kvh, D, c.batch, c.reach) ? masked_start<D, DT, MODE, Narrow>(c, shift)
+                                                                         : masked_start<D, DT, MODE, Wide>(c, shift);
 }
 
 template <int MODE>
@@ -705,7 +725,8 @@ int masked_launch(MaskedCall c) {
   if (masked_items<Narrow>(c.rows, grp, c.batch) * mp_cdiv(p.width << shift, kTile) > INT32_MAX) return MP_ERR_SHAPE;
   if (c.rows == 0) return MP_OK;
   if (mp_cu_count() <= 0) return MP_ERR_HIP;
-  if (c.workspace_bytes < masked_workspace(c.rows, c.nh, c.kvh, c.head_dim, c.batch)) return MP_ERR_WORKSPACE;
+  c.reach = masked_reach(p.width << shift, c.rule.window, c.rule.sinks);
+  if (c.workspace_bytes < masked_workspace(c.rows, c.nh, c.kvh, c.head_dim, c.batch, c.reach)) return MP_ERR_WORKSPACE;
   c.rule.group = masked_divisor(static_cast<int>(grp));
 #define MP_MASKED(DT)                                                        \
   return c.head_dim == 64 ? masked_start<64, DT, MODE>(c, shift)             \
@@ -717,11 +738,12 @@ int masked_launch(MaskedCall c) {
 
 }  // namespace
 
-extern "C" size_t mp_masked_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch) {
+extern "C" size_t mp_masked_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch, int64_t capacity,
+                                            int64_t window, int64_t sinks) {
   if (rows <= 0 || rows > INT32_MAX || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || batch <= 0 || batch > INT32_MAX ||
-      mp_cu_count() <= 0)
+      capacity <= 0 || window < 0 || sinks < 0 || mp_cu_count() <= 0)
     return 0;
-  return masked_workspace(rows, nh, kvh, head_dim, batch);
+  return masked_workspace(rows, nh, kvh, head_dim, batch, masked_reach(capacity, window, sinks));
 }
 
 extern "C" int mp_paged_tree_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh, int head_dim,
@@ -732,7 +754,7 @@ extern "C" int mp_paged_tree_attention(const void *q, int64_t q_row, int64_t q_h
   if (words < 1 || words > 1024) return MP_ERR_SHAPE;
   return masked_launch<kTree>({q, q_row, q_head, rows, nh, kvh, head_dim, cache, lens, starts, batch,
                                {masks, static_cast<int>(words), 0, 0, {}}, scale, out, dtype, workspace, workspace_bytes,
-                               reinterpret_cast<hipStream_t>(stream)});
+                               reinterpret_cast<hipStream_t>(stream), 0});
 }
 
 extern "C" int mp_paged_prompt_window_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh,
@@ -742,5 +764,5 @@ extern "C" int mp_paged_prompt_window_attention(const void *q, int64_t q_row, in
   if (window < 1 || window > 1 << 30 || sinks < 0 || sinks > 1 << 30) return MP_ERR_SHAPE;
   return masked_launch<kWindow>({q, q_row, q_head, rows, nh, kvh, head_dim, cache, lens, starts, batch,
                                  {nullptr, 0, static_cast<int>(window), static_cast<int>(sinks), {}}, scale, out, dtype, workspace,
-                                 workspace_bytes, reinterpret_cast<hipStream_t>(stream)});
+                                 workspace_bytes, reinterpret_cast<hipStream_t>(stream), 0});
 }

@@ -1387,7 +1387,7 @@ def paged_prompt_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_page
         return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
     out, qs, lib = q.new_empty((rows, nh, dim)), _steps(q), _lib.load()
     with _dev(q):
-        wsb = lib.mp_masked_workspace_bytes(rows, nh, kvh, dim, batch)
+        wsb = lib.mp_masked_workspace_bytes(rows, nh, kvh, dim, batch, table.shape[1] * k_pages.shape[2], window, sinks)
         ws = torch.empty((wsb,), dtype=torch.uint8, device=q.device)
         _lib.check(lib.mp_paged_prompt_window_attention(
             q.data_ptr(), qs[0], qs[1], rows, nh, kvh, dim, cache, lens.data_ptr(), starts.data_ptr(), batch, window, sinks, scale,
@@ -1423,7 +1423,7 @@ def paged_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.
         return torch.zeros((rows, nh, dim), dtype=q.dtype, device=q.device)
     out, qs, lib = q.new_empty((rows, nh, dim)), _steps(q), _lib.load()
     with _dev(q):
-        wsb = lib.mp_masked_workspace_bytes(rows, nh, kvh, dim, batch)
+        wsb = lib.mp_masked_workspace_bytes(rows, nh, kvh, dim, batch, table.shape[1] * k_pages.shape[2], 0, 0)
         ws = torch.empty((wsb,), dtype=torch.uint8, device=q.device)
         _lib.check(lib.mp_paged_tree_attention(
             q.data_ptr(), qs[0], qs[1], rows, nh, kvh, dim, cache, lens.data_ptr(), starts.data_ptr(), batch, masks.data_ptr(),

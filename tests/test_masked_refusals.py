@@ -146,7 +146,8 @@ def test_c_entry_points_refuse():
         for bad in (dict(window=0), dict(window=1 << 31), dict(sinks=-1), dict(sinks=1 << 31)):
             assert call(cache(), **bad) == SHAPE
     assert chunk(cache(), starts=None) == ARG and chunk(cache(), b=0) == SHAPE and chunk(cache(), row=252) == SHAPE
-    assert lib.mp_masked_workspace_bytes(0, 4, 2, 64, 3) == 0 and lib.mp_masked_workspace_bytes(9, 5, 2, 64, 3) == 0
+    assert lib.mp_masked_workspace_bytes(0, 4, 2, 64, 3, 64, 0, 0) == 0
+    assert lib.mp_masked_workspace_bytes(9, 5, 2, 64, 3, 64, 0, 0) == 0 and lib.mp_masked_workspace_bytes(9, 4, 2, 64, 3, 0, 0, 0) == 0
 
     def copy(c, layers=2, kvh=2, d=64, src=p, n=3):
         return lib.mp_paged_copy_pages(c, layers, 12288, 12288, kvh, d, src, p, None, n, None)
