@@ -28,29 +28,12 @@ enum { kTree = 0, kWindow = 1 };
 // The lowest n bits.
 __device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1; }
 
-// Division of numbers below 2^31 by a number that the host knows: (x m) >> shift with m = ceil(2^shift / d), shift = 31 + ceil(log2
-// d): the quotient is too large by less than x / 2^shift < 1 / d, which no floor notices.  A launch of few tiles is bound by the
-// instructions on its way to them.
-struct MaskedDivisor {
-  uint32_t m;
-  int shift;
-  __device__ __forceinline__ int operator()(int x) const {
-    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * m >> shift);
-  }
-};
-inline MaskedDivisor masked_divisor(int d) {
-  int l = 0;
-  while (1 << l < d) ++l;
-  const int shift = 31 + l;
-  return {static_cast<uint32_t>(((uint64_t(1) << shift) + d - 1) / d), shift};
-}
-
 // What the rows see: plain arguments of a launch.
 struct MaskedRule {
   const int64_t *masks;  // kTree: [rows, words]
   int words;
   int window, sinks;     // kWindow
-  MaskedDivisor group;   // rows / group: tokens
+  MpDivisor group;   // rows / group: tokens
 };
 
 // A sequence's rows and what they see, by the launch's rule.
@@ -564,7 +547,7 @@ __global__ __launch_bounds__(64 * kWaves, masked_round(D)) void masked_narrow_ke
 
 // The parts of an item meet: 16 of its rows in a workgroup, four in a wave, 16 lanes to each.
 template <int D, int DT, class FORM>
-__global__ __launch_bounds__(256) void masked_join_kernel(int kvh, int grp, int slot_rows, MaskedDivisor group,
+__global__ __launch_bounds__(256) void masked_join_kernel(int kvh, int grp, int slot_rows, MpDivisor group,
                                                           const float *__restrict__ parts, const int4 *__restrict__ joins,
                                                           uint16_t *__restrict__ out) {
   const int slot = blockIdx.x / kvh, kh = blockIdx.x - slot * kvh, i16 = threadIdx.x & 15;
@@ -727,7 +710,7 @@ int masked_launch(MaskedCall c) {
   if (mp_cu_count() <= 0) return MP_ERR_HIP;
   c.reach = masked_reach(p.width << shift, c.rule.window, c.rule.sinks);
   if (c.workspace_bytes < masked_workspace(c.rows, c.nh, c.kvh, c.head_dim, c.batch, c.reach)) return MP_ERR_WORKSPACE;
-  c.rule.group = masked_divisor(static_cast<int>(grp));
+  c.rule.group = mp_divisor(static_cast<int>(grp));
 #define MP_MASKED(DT)                                                        \
   return c.head_dim == 64 ? masked_start<64, DT, MODE>(c, shift)             \
                           : c.head_dim == 128 ? masked_start<128, DT, MODE>(c, shift) : masked_start<256, DT, MODE>(c, shift)

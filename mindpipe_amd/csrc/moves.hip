@@ -10,6 +10,7 @@ struct MovePools {
   const uint16_t *k, *v;  // written as well
   int64_t k_layer, k_page, k_head, k_row, v_layer, v_page, v_head, v_row;
   int layers, pages, kvh, shift, chunks;  // chunks: of 16 bytes in a position of a head
+  MpDivisor by_chunks, by_heads;
 };
 
 __device__ __forceinline__ uint16_t *move_at(const MovePools &p, bool values, int layer, int64_t page, int head, int64_t row) {
@@ -23,27 +24,28 @@ constexpr int kPieces = 4;  // 16-byte pieces of a thread
 // A workgroup copies 256 x kPieces pieces of one page, layer and pool.
 __global__ __launch_bounds__(256) void paged_copy_kernel(MovePools p, const int32_t *__restrict__ src, const int32_t *__restrict__ dst,
                                                          const int32_t *__restrict__ filled, int per) {
-  const int part = blockIdx.x % per, pair = blockIdx.x / per, layer = blockIdx.y >> 1;
+  const int pair = blockIdx.x / per, part = blockIdx.x - pair * per, layer = blockIdx.y >> 1;
   const bool values = blockIdx.y & 1;
   const int from = src[pair], to = dst[pair], size = 1 << p.shift;
   if (from < 0 || from >= p.pages || to < 0 || to >= p.pages || from == to) return;
-  const int rows = filled ? min(max(filled[pair], 0), size) : size;
-  const uint32_t per_head = static_cast<uint32_t>(rows) * p.chunks, all = per_head * p.kvh;
+  const int rows = filled ? min(max(filled[pair], 0), size) : size, all = (p.kvh * p.chunks) << p.shift;
+  const uint16_t *x0 = move_at(p, values, layer, from, 0, 0);
+  uint16_t *y0 = move_at(p, values, layer, to, 0, 0);
+  const int64_t to_head = values ? p.v_head : p.k_head, to_row = values ? p.v_row : p.k_row;
   uint4 x[kPieces];
-  uint16_t *y[kPieces];
+  int64_t at[kPieces];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    const uint32_t at = (part * kPieces + i) * 256 + threadIdx.x;
-    y[i] = nullptr;
-    if (at < all) {
-      const uint32_t head = at / per_head, in = at - head * per_head, row = in / p.chunks, c = in - row * p.chunks;
-      x[i] = *reinterpret_cast<const uint4 *>(move_at(p, values, layer, from, head, row) + 8 * c);
-      y[i] = move_at(p, values, layer, to, head, row) + 8 * c;
+    const int piece = (part * kPieces + i) * 256 + threadIdx.x, position = p.by_chunks(piece), row = position & (size - 1);
+    at[i] = -1;
+    if (piece < all && row < rows) {
+      at[i] = (position >> p.shift) * to_head + row * to_row + 8 * (piece - position * p.chunks);
+      x[i] = *reinterpret_cast<const uint4 *>(x0 + at[i]);
     }
   }
 #pragma unroll
   for (int i = 0; i < kPieces; ++i)
-    if (y[i]) *reinterpret_cast<uint4 *>(y[i]) = x[i];
+    if (at[i] >= 0) *reinterpret_cast<uint4 *>(y0 + at[i]) = x[i];
 }
 
 constexpr int kAhead = 8;  // positions that are read before the first of them is written
@@ -53,9 +55,8 @@ constexpr int kAhead = 8;  // positions that are read before the first of them i
 __global__ __launch_bounds__(256) void paged_keep_kernel(MovePools p, const int32_t *__restrict__ table, int width,
                                                          const int32_t *__restrict__ first, const int32_t *__restrict__ keep,
                                                          const int32_t *__restrict__ starts, int total, int per) {
-  const int b = blockIdx.x / per;
-  const int column = (blockIdx.x % per) * 256 + threadIdx.x;
-  const int c = column % p.chunks, of = column / p.chunks, head = of % p.kvh, pool = of / p.kvh;
+  const int b = blockIdx.x / per, column = (blockIdx.x - b * per) * 256 + threadIdx.x;
+  const int of = p.by_chunks(column), c = column - of * p.chunks, pool = p.by_heads(of), head = of - pool * p.kvh;
   if (pool >= 2 * p.layers) return;
   const int begin = min(max(starts[b], 0), total), end = min(max(starts[b + 1], begin), total);
   const int64_t base = first[b], room = static_cast<int64_t>(width) << p.shift;
@@ -100,7 +101,8 @@ int move_pools(const mp_pages *c, int64_t layers, int64_t k_layer, int64_t v_lay
     if (s < 0 || s % 8) return MP_ERR_SHAPE;
   if (!mp_aligned(c->k, 16) || !mp_aligned(c->v, 16)) return MP_ERR_ALIGN;
   p = {static_cast<const uint16_t *>(c->k), static_cast<const uint16_t *>(c->v), k_layer, c->k_page, c->k_head, c->k_row, v_layer,
-       c->v_page, c->v_head, c->v_row, static_cast<int>(layers), static_cast<int>(c->pages), kvh, shift, head_dim / 8};
+       c->v_page, c->v_head, c->v_row, static_cast<int>(layers), static_cast<int>(c->pages), kvh, shift, head_dim / 8,
+       mp_divisor(head_dim / 8), mp_divisor(kvh)};
   return MP_OK;
 }
 

@@ -27,6 +27,23 @@ static inline bool mp_aligned(const void *p, size_t a) {
 
 static inline int64_t mp_cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Division of numbers below 2^31 by a number that the host knows: (x m) >> shift with m = ceil(2^shift / d), shift = 31 + ceil(log2
+// d): the quotient is too large by less than x / 2^shift < 1 / d, which no floor notices.  A launch of few tiles is bound by the
+// instructions on its way to them.
+struct MpDivisor {
+  uint32_t m;
+  int shift;
+  __device__ __forceinline__ int operator()(int x) const {
+    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * m >> shift);
+  }
+};
+static inline MpDivisor mp_divisor(int d) {
+  int l = 0;
+  while (1 << l < d) ++l;
+  const int shift = 31 + l;
+  return {static_cast<uint32_t>(((uint64_t(1) << shift) + d - 1) / d), shift};
+}
+
 // Compute units of the current device (cached per device id).
 static inline int mp_cu_count() {
   static int cache[64] = {0};
