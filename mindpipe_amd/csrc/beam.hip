@@ -4,11 +4,11 @@
 //   the `count` largest totals of a request, from the largest down; of equal ones those of the lowest beam, then token
 //
 // Which of two totals is larger decides a whole number, so they are made in 64 bits: the order inside of a row is that of its
-// logits, and between rows the sums of exponentials decide, each off by less than 2^-36 of itself.
+// logits, and between rows the sums of exponentials decide, each off by less than 2^-34 of itself.
 //
 // Two launches.  Of each row, workgroups take a part of the vocabulary each (a row is read once and stays in registers): they leave
 // the part's maximum, its sum of exponentials and its `count` largest values in order.  No value can be among a request's best
-// that is not among those.  Then one wave a request merges the parts' lists, taking the best of their heads each time.
+// that is not among those.  Then a workgroup a request puts the best of its lists in order.
 #include "logits.h"
 
 namespace {
@@ -19,25 +19,22 @@ constexpr int kBeamListed = 512;               // candidates of a part that LDS 
 constexpr int kQuads = kBeamThreads / 4;       // a lane of a wave to each
 constexpr double kLog2eD = 1.4426950408889634;
 
-// exp(d) for d <= 0, in 64 bits: 2^n from the whole part of d log2 e and 2^r, r in [-1/2, 1/2], by the series of exp(r ln 2) up to
-// its ninth power, which leaves less than 2^-37.  Below e^-800: 0.
+// exp(d) for d from -690 to 0, in 64 bits (below -kBeamLost, 2^-865, no part of a sum): 2^n from the whole part of d log2 e and 2^r, r in [-1/2, 1/2], by the polynomial of
+// degree seven that is off by the least share there, 2^-34.5.
+constexpr float kBeamLost = 600.f;
 __device__ __forceinline__ double beam_exp(double d) {
   const double magic = 1.5 * 0x1p52;  // a sum with it is whole
-  d = fmax(d, -800.0);
   const double t = fma(d, kLog2eD, magic), r = fma(d, kLog2eD, magic - t);
-  double p = 1.017808600923970e-7;                         // (ln 2)^9 / 9!
-  p = fma(p, r, 1.321548679014431e-6);
-  p = fma(p, r, 1.525273380405984e-5);
-  p = fma(p, r, 1.540353039338161e-4);
-  p = fma(p, r, 1.333355814642844e-3);
-  p = fma(p, r, 9.618129107628477e-3);
-  p = fma(p, r, 5.550410866482158e-2);
-  p = fma(p, r, 2.402265069591007e-1);
-  p = fma(p, r, 6.931471805599453e-1);
-  p = fma(p, r, 1.0);
-  return ldexp(p, __double2loint(t));
+  double p = 1.5201921594169677e-05;
+  p = fma(p, r, 0.00015469291141683767);
+  p = fma(p, r, 0.001333392256354045);
+  p = fma(p, r, 0.00961802725366847);
+  p = fma(p, r, 0.05550410353447978);
+  p = fma(p, r, 0.24022651198157585);
+  p = fma(p, r, 0.693147180728447);
+  p = fma(p, r, 0.9999999999616819);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));  // no underflow: n is above -1000
 }
-
 struct BeamPart {  // of a part of a row: its largest value and sum_v exp(x_v - top); top +inf: how many such values
   double sum;
   float top;
@@ -83,7 +80,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(const uint8_t *
   for (int g = 0; g < H; ++g) held[g].load(at, first + 8 * kBeamThreads * g, vocab, vec);
   if (tid == 0) listed = 0;
 
-  const auto each = [&](auto f) {  // f(index, its eight values), NaN as -inf
+  const auto each = [&](auto f, float least = -INFINITY) {  // f(index, its eight values), NaN and lower ones as `least`
 #pragma unroll
     for (int g = 0; g < H; ++g) {
 #pragma unroll
@@ -91,7 +88,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(const uint8_t *
       float v[8];
       held[g].get(v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = fmaxf(v[e], -INFINITY);
+      for (int e = 0; e < 8; ++e) v[e] = fmaxf(v[e], least);
       f(first + 8 * kBeamThreads * g, v);
     }
   };
@@ -118,10 +115,16 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(const uint8_t *
     });
   } else if (most > -INFINITY) {
     const double base = most;
-    each([&](int, const float (&v)[8]) {
+    if (fabsf(most) < 0x1p29f) {  // fp32's steps are below 64: raised to `most` - kBeamLost, values count for nothing
+      each([&](int, const float (&v)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += beam_exp(static_cast<double>(v[e]) - base);
-    });
+        for (int e = 0; e < 8; ++e) sum += beam_exp(static_cast<double>(v[e]) - base);
+      }, most - kBeamLost);
+    } else {
+      each([&](int, const float (&v)[8]) {
+        for (int e = 0; e < 8; ++e) sum += beam_exp(fmax(static_cast<double>(v[e]) - base, -kBeamLost));
+      });
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -210,105 +213,131 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(const uint8_t *
 
 struct BeamBest {
   double total;
-  int beam, token;
-  __device__ __forceinline__ bool before(const BeamBest &o) const {
-    return total > o.total || (total == o.total && (beam < o.beam || (beam == o.beam && token < o.token)));
-  }
+  int at;  // beam * vocab + token
+  __device__ __forceinline__ bool before(double t, int i) const { return total > t || (total == t && at < i); }
 };
 
-constexpr int kBeamLists = 8192;  // values of the lists that LDS has room for
+constexpr int kBeamNear = 2048;  // continuations that LDS has room for
 
+// One workgroup a request.  The best of the lists' heads, one a lane, that `count` of them reach is reached by `count`
+// continuations; the few that reach it are put in order by counting, for each, those before it.
 __global__ __launch_bounds__(256) void beam_merge_kernel(const BeamPart *__restrict__ parts, const BeamValue *__restrict__ lists,
                                                          const float *__restrict__ scores, const uint8_t *__restrict__ ended,
-                                                         int beams, int splits, int count, int pad, float *__restrict__ out_scores,
+                                                         int beams, int splits, int count, int vocab, int pad, MpDivisor by_count,
+                                                         MpDivisor by_splits, float *__restrict__ out_scores,
                                                          int64_t *__restrict__ out_beams, int64_t *__restrict__ out_tokens) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t beam_smem[];
-  __shared__ double base[kMaxBeams];  // log sum exp
-  __shared__ bool infinite[kMaxBeams];
+  __shared__ double base[kMaxBeams], score[kMaxBeams], near_total[kBeamNear];  // base: log sum exp
+  __shared__ int near_at[kBeamNear], listed;
+  __shared__ uint8_t state[kMaxBeams];
+  enum { kPlain, kInfinite, kEnded };
   const int64_t b = blockIdx.x;
-  const int n_lists = beams * splits, values = n_lists * count;
+  const int n_lists = beams * splits, values = n_lists * count, tid = threadIdx.x;
   const BeamValue *from = lists + b * values;
-  if (values <= kBeamLists) {
-    BeamValue *near = reinterpret_cast<BeamValue *>(beam_smem);
-    for (int i = threadIdx.x; i < values; i += 256) near[i] = from[i];
-    from = near;
-  }
-  if (threadIdx.x < beams) {
-    const BeamPart *p = parts + (b * beams + threadIdx.x) * splits;
+  if (tid < beams) {
+    const BeamPart *p = parts + (b * beams + tid) * splits;
+    score[tid] = scores[b * beams + tid];
+    const bool done = ended && ended[b * beams + tid];
     float top = -INFINITY;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, p[s].top);
     double sum = 0.0;
-    if (top == INFINITY) {
-      for (int s = 0; s < splits; ++s) sum += p[s].top == INFINITY ? p[s].sum : 0.0;
-    } else if (top > -INFINITY) {
-      for (int s = 0; s < splits; ++s)
-        if (p[s].top > -INFINITY) sum += p[s].sum * beam_exp(static_cast<double>(p[s].top) - static_cast<double>(top));
+    if (!done) {
+      for (int s = 0; s < splits; ++s) {
+        const BeamPart q = p[s];
+        if (q.top > top) {
+          sum = top > -INFINITY && q.top < INFINITY ? sum * beam_exp(fmax(static_cast<double>(top) - q.top, -kBeamLost)) : 0.0;
+          top = q.top;
+          sum += q.sum;
+        } else if (q.top > -INFINITY) {
+          sum += q.top == top ? q.sum : top < INFINITY ? q.sum * beam_exp(fmax(static_cast<double>(q.top) - top, -kBeamLost)) : 0.0;
+        }
+      }
     }
     // with infinite logits those alone count, as if they were 0, and all others are -inf
-    infinite[threadIdx.x] = top == INFINITY;
-    base[threadIdx.x] = (top == INFINITY ? 0.0 : static_cast<double>(top)) + log(sum);
+    state[tid] = done ? kEnded : top == INFINITY ? kInfinite : kPlain;
+    base[tid] = (top == INFINITY ? 0.0 : static_cast<double>(top)) + log(sum);
   }
+  if (tid == 0) listed = 0;
   __syncthreads();
-  if (threadIdx.x >= 64) return;
-  const int lane = threadIdx.x;
   const double none = -INFINITY;
-
-  // entry `at` of a list as a candidate; nothing there: -inf
+  // Entry `at` of a list; nothing there, or a total of -inf or NaN: -inf.
   const auto candidate = [&](int list, int at) {
-    BeamBest c{none, INT32_MAX, INT32_MAX};
-    const int k = list / splits;
-    const double score = scores[b * beams + k];
-    if (ended && ended[b * beams + k]) {  // the row's first list has its one continuation
-      if (list % splits == 0 && at == 0) c = BeamBest{score, k, pad};
-    } else if (at < count) {
+    const int k = by_splits(list);
+    BeamBest c{none, 0};
+    if (state[k] == kEnded) {  // the row's first list has its one continuation
+      if (list == k * splits && at == 0) c = BeamBest{score[k], k * vocab + pad};
+    } else {
       const BeamValue v = from[list * count + at];
       if (v.token >= 0) {
-        const double x = infinite[k] ? (v.value == INFINITY ? 0.0 : none) : static_cast<double>(v.value);
-        c = BeamBest{score + (x - base[k]), k, v.token};
+        const double x = state[k] == kInfinite ? (v.value == INFINITY ? 0.0 : none) : static_cast<double>(v.value);
+        c = BeamBest{score[k] + (x - base[k]), k * vocab + v.token};
       }
     }
-    if (!(c.total > none)) c = BeamBest{none, INT32_MAX, INT32_MAX};  // -inf and NaN
+    if (!(c.total > none)) c.total = none;
     return c;
   };
-  // a lane's lists are lane, lane + 64, ..; taken[i] of each are gone, the best of their heads is `mine`
-  uint8_t *taken = beam_smem + (values <= kBeamLists ? values * sizeof(BeamValue) : 0);
-  for (int i = lane; i < n_lists; i += 64) taken[i] = 0;
-  int of = 0;
-  const auto best_own = [&]() {
-    BeamBest m{none, INT32_MAX, INT32_MAX};
-    for (int i = lane; i < n_lists; i += 64) {
-      const BeamBest c = candidate(i, taken[i]);
-      if (c.before(m)) {
-        m = c;
-        of = i;
+  // in 32 bits, rounded down, so that whatever reaches a head reaches it here
+  const auto order = [&](double total) { return total > none ? beam_order(__double2float_rd(total)) : 0u; };
+  uint32_t head = 0;
+  for (int i = tid & 63; i < n_lists; i += 64) head = max(head, order(candidate(i, 0).total));
+  uint32_t least = 0;
+#pragma unroll 1
+  for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+    if (__popcll(__ballot(head >= (least | bit))) >= count) least |= bit;
+  least = max(least, 1u);
+  for (int i = tid; i < values; i += 256) {
+    const int list = by_count(i);
+    const BeamBest c = candidate(list, i - list * count);
+    if (order(c.total) >= least) {
+      const int n = atomicAdd(&listed, 1);
+      if (n < kBeamNear) {
+        near_total[n] = c.total;
+        near_at[n] = c.at;
       }
     }
-    return m;
+  }
+  __syncthreads();
+  const int n = listed;
+  const auto put = [&](int i, BeamBest c) {
+    const bool found = c.total > none;
+    const int k = found ? c.at / vocab : -1;
+    out_scores[b * count + i] = static_cast<float>(c.total);
+    out_beams[b * count + i] = k;
+    out_tokens[b * count + i] = found ? c.at - k * vocab : -1;
   };
-  BeamBest mine = best_own();
+  if (n <= kBeamNear) {
+    for (int e = tid; e < n; e += 256) {
+      const BeamBest me{near_total[e], near_at[e]};
+      int rank = 0;
+      for (int i = 0; i < n; ++i) rank += BeamBest{near_total[i], near_at[i]}.before(me.total, me.at) ? 1 : 0;
+      if (rank < count) put(rank, me);
+    }
+    for (int e = n + tid; e < count; e += 256) put(e, BeamBest{none, 0});
+    return;
+  }
+  // More are equal than LDS has room for: one after the other, each the best of those behind the last.
+  BeamBest last{INFINITY, -1};
   for (int i = 0; i < count; ++i) {
-    BeamBest best = mine;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const BeamBest other{__shfl_xor(best.total, o, 64), __shfl_xor(best.beam, o, 64), __shfl_xor(best.token, o, 64)};
-      if (other.before(best)) best = other;
+    BeamBest best{none, INT32_MAX};
+    for (int e = tid; e < values; e += 256) {
+      const int list = by_count(e);
+      const BeamBest c = candidate(list, e - list * count);
+      if (last.before(c.total, c.at) && c.before(best.total, best.at)) best = c;
     }
-    if (lane == 0) {
-      const bool found = best.total > none;
-      out_scores[b * count + i] = static_cast<float>(best.total);
-      out_beams[b * count + i] = found ? best.beam : -1;
-      out_tokens[b * count + i] = found ? best.token : -1;
+    __syncthreads();  // the last round's have been read
+    near_total[tid] = best.total;
+    near_at[tid] = best.at;
+    __syncthreads();
+    for (int e = 0; e < 256; ++e) {
+      const BeamBest c{near_total[e], near_at[e]};
+      if (c.before(best.total, best.at)) best = c;
     }
-    if (best.total > none && mine.beam == best.beam && mine.token == best.token) {
-      ++taken[of];
-      mine = best_own();
-    }
+    if (tid == 0) put(i, best);
+    last = best;
   }
 }
 
 // Eights of a thread: as many as hold a row in few parts, but as few as keep 512 workgroups or more in the launch.
 inline int beam_eights(int64_t rows, int64_t vocab, int dtype) {
-  int h = dtype == MP_F32 ? 8 : 16;
+  int h = 8;
   while (h > 2 && rows * mp_cdiv(vocab, 8 * h * kBeamThreads) < 512) h /= 2;
   return h;
 }
@@ -351,8 +380,7 @@ extern "C" int mp_beam_select(const void *logits, int64_t stride, int64_t batch,
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define MP_BEAM(DT)                                                                                                        \
   do {                                                                                                                     \
-    if (h == 16) beam_rows_launch<DT, DT == MP_F32 ? 8 : 16>(logits, stride, rows, n, ended, splits, k, parts, lists, s);  \
-    else if (h == 8) beam_rows_launch<DT, 8>(logits, stride, rows, n, ended, splits, k, parts, lists, s);                  \
+    if (h == 8) beam_rows_launch<DT, 8>(logits, stride, rows, n, ended, splits, k, parts, lists, s);                  \
     else if (h == 4) beam_rows_launch<DT, 4>(logits, stride, rows, n, ended, splits, k, parts, lists, s);                  \
     else beam_rows_launch<DT, 2>(logits, stride, rows, n, ended, splits, k, parts, lists, s);                              \
   } while (0)
@@ -361,13 +389,9 @@ extern "C" int mp_beam_select(const void *logits, int64_t stride, int64_t batch,
   else MP_BEAM(MP_F32);
 #undef MP_BEAM
   MP_CHECK_LAUNCH();
-  const int64_t values = beams * splits * count;
-  const size_t lds = (values <= kBeamLists ? values * sizeof(BeamValue) : 0) + beams * splits;
-  if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(beam_merge_kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)) != hipSuccess)
-    return MP_ERR_HIP;
-  hipLaunchKernelGGL(beam_merge_kernel, dim3(static_cast<unsigned>(batch)), dim3(256), lds, s, parts, lists, scores, ended,
-                     static_cast<int>(beams), splits, k, static_cast<int>(pad), out_scores, out_beams, out_tokens);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3(static_cast<unsigned>(batch)), dim3(256), 0, s, parts, lists, scores, ended,
+                     static_cast<int>(beams), splits, k, n, static_cast<int>(pad), mp_divisor(k), mp_divisor(splits), out_scores,
+                     out_beams, out_tokens);
   MP_CHECK_LAUNCH();
   return MP_OK;
 }

@@ -19,33 +19,20 @@ __device__ __forceinline__ uint16_t *move_at(const MovePools &p, bool values, in
                 : base + layer * p.k_layer + page * p.k_page + head * p.k_head + row * p.k_row;
 }
 
-constexpr int kPieces = 4;  // 16-byte pieces of a thread
-
-// A workgroup copies 256 x kPieces pieces of one page, layer and pool.
+// A workgroup copies 256 16-byte pieces of one page, layer and pool, a piece a thread.  Bound by the memory: 40 whole pages of 131 KB
+// in 32 layers, 671 MB read and written, 101 us, 6.6 TB/s, where a copy of as much in one piece takes 134; three partial pages of 16
+// positions of 32 heads (22 MB) 7 us.  Two, four and eight pieces a thread: 118, 125 and 197 us, and 19, 19 and 10.
 __global__ __launch_bounds__(256) void paged_copy_kernel(MovePools p, const int32_t *__restrict__ src, const int32_t *__restrict__ dst,
                                                          const int32_t *__restrict__ filled, int per) {
-  const int pair = blockIdx.x / per, part = blockIdx.x - pair * per, layer = blockIdx.y >> 1;
+  const int pair = blockIdx.x / per, piece = (blockIdx.x - pair * per) * 256 + threadIdx.x, layer = blockIdx.y >> 1;
   const bool values = blockIdx.y & 1;
   const int from = src[pair], to = dst[pair], size = 1 << p.shift;
   if (from < 0 || from >= p.pages || to < 0 || to >= p.pages || from == to) return;
-  const int rows = filled ? min(max(filled[pair], 0), size) : size, all = (p.kvh * p.chunks) << p.shift;
-  const uint16_t *x0 = move_at(p, values, layer, from, 0, 0);
-  uint16_t *y0 = move_at(p, values, layer, to, 0, 0);
-  const int64_t to_head = values ? p.v_head : p.k_head, to_row = values ? p.v_row : p.k_row;
-  uint4 x[kPieces];
-  int64_t at[kPieces];
-#pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int piece = (part * kPieces + i) * 256 + threadIdx.x, position = p.by_chunks(piece), row = position & (size - 1);
-    at[i] = -1;
-    if (piece < all && row < rows) {
-      at[i] = (position >> p.shift) * to_head + row * to_row + 8 * (piece - position * p.chunks);
-      x[i] = *reinterpret_cast<const uint4 *>(x0 + at[i]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kPieces; ++i)
-    if (at[i] >= 0) *reinterpret_cast<uint4 *>(y0 + at[i]) = x[i];
+  const int rows = filled ? min(max(filled[pair], 0), size) : size;
+  const int position = p.by_chunks(piece), row = position & (size - 1), head = position >> p.shift, c = piece - position * p.chunks;
+  if (head >= p.kvh || row >= rows) return;
+  *reinterpret_cast<uint4 *>(move_at(p, values, layer, to, head, row) + 8 * c) =
+      *reinterpret_cast<const uint4 *>(move_at(p, values, layer, from, head, row) + 8 * c);
 }
 
 constexpr int kAhead = 8;  // positions that are read before the first of them is written
@@ -114,7 +101,7 @@ extern "C" int mp_paged_copy_pages(const mp_pages *cache, int64_t layers, int64_
   MovePools p;
   const int rc = move_pools(cache, layers, k_layer, v_layer, kvh, head_dim, false, p);
   if (rc != MP_OK) return rc;
-  const int64_t per = mp_cdiv(static_cast<int64_t>(kvh) * p.chunks << p.shift, 256 * kPieces);
+  const int64_t per = mp_cdiv(static_cast<int64_t>(kvh) * p.chunks << p.shift, 256);
   if (count < 0 || count > INT32_MAX / per) return MP_ERR_SHAPE;
   if (count == 0) return MP_OK;
   hipLaunchKernelGGL(paged_copy_kernel, dim3(static_cast<unsigned>(count * per), static_cast<unsigned>(2 * layers)), dim3(256), 0,
