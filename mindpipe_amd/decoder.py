@@ -21,13 +21,15 @@ uses PyTorch attention (SDPA) around the same W4A16 linears and fused norm / SiL
 ``PagedKVCache`` holds sequences of different lengths in pages instead.  ``forward_paged`` runs packed
 new tokens of any of them (whole prompts, chunks of prompts, one token each) on the paged operators:
 append with rotation, decode or prompt attention.  ``generate_paged`` serves prompts with it, the
-tokens drawn by ``ops.sample_tokens``.
+tokens drawn by ``ops.sample_tokens``.  ``generate_drafted`` has drafted tokens verified, a tree of them per sequence and pass
+(``forward_tree``), ``beam_search_paged`` searches with beams that share their pages, and a model whose configuration has a
+window keeps only the pages that its tokens still see.
 """
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import List, Optional, Sequence
+from typing import Callable, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -45,6 +47,8 @@ class DecoderConfig:
     group: int = 128
     rope_theta: float = 10000.0
     eps: float = 1e-5
+    window: int = 0  # positions that a token sees, its own among them (0: all), on a paged cache
+    sinks: int = 0   # first positions that stay visible with a window
 
     @staticmethod
     def llama2_7b():
@@ -109,7 +113,8 @@ class PagedKVCache:
 
     ``k`` / ``v [layers, pages, kv_heads, page, head_dim]`` are the pools; ``table`` (int32, a row of pages for each
     sequence) and ``lens`` (int32) are what the paged operators read, in device memory and updated in place, so a
-    captured step goes on working while the sequences grow.  Which pages are free is kept on the host."""
+    captured step goes on working while the sequences grow.  Which pages are free is kept on the host.  Sequences that were
+    forked share their pages; one that goes on has a shared page that it would write to copied first (``extend``)."""
 
     def __init__(self, cfg: DecoderConfig, sequences: int, positions: int, page: int = 64, max_len: Optional[int] = None,
                  device="cuda", dtype=torch.float16):
@@ -123,11 +128,32 @@ class PagedKVCache:
         self.table = torch.zeros(sequences, -(-self.max_len // page), device=device, dtype=torch.int32)
         self.lens = torch.zeros(sequences, device=device, dtype=torch.int32)
         self.length = [0] * sequences                      # of lens, on the host
-        self._held: List[List[int]] = [[] for _ in range(sequences)]
+        self._held: List[List[int]] = [[] for _ in range(sequences)]  # -1: a page that was trimmed
+        self._uses = [0] * pages                           # sequences that hold a page
         self._free = list(range(pages - 1, -1, -1))
 
     def free_positions(self) -> int:
         return len(self._free) * self.page
+
+    def _take(self) -> int:
+        page = self._free.pop()
+        self._uses[page] = 1
+        return page
+
+    def _drop(self, pages: Sequence[int]) -> None:
+        for page in pages:
+            if page >= 0:
+                self._uses[page] -= 1
+                if not self._uses[page]:
+                    self._free.append(page)
+
+    def _set_table(self, rows: List[int], cols: List[int], pages: List[int]) -> None:
+        if rows:
+            at = torch.tensor([rows, cols], device=self.table.device)
+            self.table[at[0], at[1]] = torch.tensor(pages, device=self.table.device, dtype=torch.int32)
+
+    def _set_lens(self) -> None:
+        self.lens.copy_(torch.tensor(self.length, dtype=torch.int32))
 
     @torch.no_grad()
     def extend(self, news: Sequence[int]) -> Optional[torch.Tensor]:
@@ -140,21 +166,38 @@ class PagedKVCache:
         want = [-(-(l + n) // self.page) - len(h) for l, n, h in zip(self.length, news, self._held)]
         if any(l + n > self.max_len for l, n in zip(self.length, news)):
             raise RuntimeError(f"a sequence would pass {self.max_len} positions")
-        if sum(want) > len(self._free):
-            raise RuntimeError(f"{sum(want)} pages are wanted and {len(self._free)} are free")
+        # begun pages that others hold as well: all but the last of their holders that go on have them copied
+        uses, copies = {}, []
+        for b, (l, n, held) in enumerate(zip(self.length, news, self._held)):
+            if n and l % self.page:
+                page = held[l // self.page]
+                uses[page] = uses.get(page, self._uses[page])
+                if uses[page] > 1:
+                    uses[page] -= 1
+                    copies.append((b, page))
+        if sum(want) + len(copies) > len(self._free):
+            raise RuntimeError(f"{sum(want) + len(copies)} pages are wanted and {len(self._free)} are free")
         device = self.table.device
         rows, cols, pages = [], [], []
+        for b, page in copies:
+            rows.append(b)
+            cols.append(self.length[b] // self.page)
+            pages.append(self._take())
+            self._held[b][cols[-1]] = pages[-1]
+            self._uses[page] -= 1
+        if copies:
+            move = torch.tensor([[page for _, page in copies], pages, [self.length[b] % self.page for b, _ in copies]],
+                                device=device, dtype=torch.int32)
+            ops.paged_copy_pages(self.k, self.v, move[0], move[1], move[2])
         for b, n in enumerate(want):
             for _ in range(n):
                 rows.append(b)
                 cols.append(len(self._held[b]))
-                pages.append(self._free.pop())
+                pages.append(self._take())
                 self._held[b].append(pages[-1])
-        if pages:
-            self.table[torch.tensor(rows, device=device), torch.tensor(cols, device=device)] = \
-                torch.tensor(pages, device=device, dtype=torch.int32)
+        self._set_table(rows, cols, pages)
         self.length = [l + n for l, n in zip(self.length, news)]
-        self.lens.copy_(torch.tensor(self.length, dtype=torch.int32))
+        self._set_lens()
         if all(n == 1 for n in news):
             return None
         starts = torch.zeros(len(news) + 1, dtype=torch.int32)
@@ -163,11 +206,104 @@ class PagedKVCache:
 
     @torch.no_grad()
     def release(self, sequence: int) -> None:
-        """Ends a sequence: its pages are free again."""
-        self._free += reversed(self._held[sequence])
+        """Ends a sequence: the pages that it alone held are free again."""
+        self._drop(reversed(self._held[sequence]))
         self._held[sequence] = []
         self.length[sequence] = 0
         self.lens[sequence] = 0
+
+    @torch.no_grad()
+    def reorder(self, order: Sequence[int]) -> None:
+        """Sequence b goes on as what sequence ``order[b]`` was: tables and lengths change, pages are shared and nothing is
+        copied before ``extend`` writes.  What no sequence goes on as is released."""
+        if len(order) != len(self.length) or not all(0 <= o < len(order) for o in order):
+            raise ValueError(f"one of the {len(self.length)} sequences for each of them, got {list(order)}")
+        if all(o == b for b, o in enumerate(order)):
+            return
+        held = [list(self._held[o]) for o in order]
+        for pages in held:
+            for page in pages:
+                if page >= 0:
+                    self._uses[page] += 1
+        for pages in self._held:
+            self._drop(reversed(pages))
+        self._held = held
+        self.length = [self.length[o] for o in order]
+        self.table.copy_(self.table[torch.tensor(list(order), device=self.table.device)])
+        self._set_lens()
+
+    @torch.no_grad()
+    def fork(self, source: int, target: int) -> None:
+        """The empty sequence ``target`` begins as what ``source`` is."""
+        if self.length[target] or source == target:
+            raise ValueError(f"sequence {target} must be empty and another than {source}")
+        order = list(range(len(self.length)))
+        order[target] = source
+        self.reorder(order)
+
+    @torch.no_grad()
+    def keep(self, drafted: Sequence[int], kept: Sequence[Sequence[int]]) -> None:
+        """Of the last ``drafted[b]`` positions of each sequence b those that ``kept[b]`` names stay, ascending from 0, one behind
+        the other; pages behind them are free again."""
+        if len(drafted) != len(self.length) or len(kept) != len(self.length):
+            raise ValueError(f"a count and a list for each of the {len(self.length)} sequences")
+        for l, n, at in zip(self.length, drafted, kept):
+            if not 0 <= n <= l or any(not 0 <= i < n for i in at) or any(i >= j for i, j in zip(at, at[1:])):
+                raise ValueError(f"{list(at)} must ascend below the {n} drafted positions of {l}")
+        for l, n, held in zip(self.length, drafted, self._held):
+            if n and any(page < 0 or self._uses[page] > 1 for page in held[(l - n) // self.page:]):
+                raise RuntimeError("a sequence that was forked or trimmed since its draft keeps it as it is")
+        if any(i != j for at in kept for j, i in enumerate(at)):
+            device, first = self.table.device, [l - n for l, n in zip(self.length, drafted)]
+            starts = [0]
+            for at in kept:
+                starts.append(starts[-1] + len(at))
+            ints = torch.tensor([*first, *starts, *(i for at in kept for i in at)], dtype=torch.int32).to(device)
+            n = len(first)
+            # views of one transfer
+            ops.paged_keep_positions(self.k, self.v, self.table, ints[:n], ints[2 * n + 1:], ints[n:2 * n + 1])
+        for b, (n, at) in enumerate(zip(drafted, kept)):
+            self.length[b] += len(at) - n
+            stay = -(-self.length[b] // self.page)
+            self._drop(reversed(self._held[b][stay:]))
+            del self._held[b][stay:]
+        self._set_lens()
+
+    @torch.no_grad()
+    def trim(self, window: int, sinks: int = 0) -> int:
+        """Frees the pages that no later token sees with a window of ``window`` positions and ``sinks`` first ones; how many."""
+        if window < 1 or sinks < 0:
+            raise ValueError(f"a window has a position at least, and sinks are not negative: {window}, {sinks}")
+        rows, cols = [], []
+        for b, held in enumerate(self._held):
+            for i in range(-(-sinks // self.page), max(0, self.length[b] - window + 1) // self.page):
+                if held[i] >= 0:
+                    rows.append(b)
+                    cols.append(i)
+        for b, i in zip(rows, cols):
+            self._drop([self._held[b][i]])
+            self._held[b][i] = -1
+        self._set_table(rows, cols, [-1] * len(rows))
+        return len(rows)
+
+
+def lookup_draft(match: int = 2, nodes: int = 8, branches: int = 2) -> Callable[[List[int]], Tuple[List[int], List[int]]]:
+    """Drafts from the sequence itself for ``W4Decoder.generate_drafted``: what followed the last ``match`` tokens where they
+    stood before, the latest places first, up to ``branches`` of them and ``nodes`` tokens in all."""
+    def draft(tokens: List[int]) -> Tuple[List[int], List[int]]:
+        found: List[int] = []
+        parents: List[int] = []
+        places = [i for i in range(len(tokens) - match - 1, -1, -1) if tokens[i:i + match] == tokens[-match:]] if match < len(tokens) else []
+        for i in places[:branches]:
+            node = -1
+            for t in tokens[i + match:i + match + max(1, nodes // branches)]:
+                same = [j for j, p in enumerate(parents) if p == node and found[j] == t]
+                if not same:
+                    found.append(t)
+                    parents.append(node)
+                node = same[0] if same else len(found) - 1
+        return found[:nodes], parents[:nodes]
+    return draft
 
 
 class W4Decoder:
@@ -199,6 +335,10 @@ class W4Decoder:
         self.cos = freqs.cos().half()
         self.sin = freqs.sin().half()
 
+    def _contiguous(self):
+        if self.cfg.window:
+            raise RuntimeError("a model with a window runs on a paged cache")
+
     def weight_bytes(self):
         return sum(l[n].nbytes() for l in self.layers for n in ("qkv", "o", "gate_up", "down")) + self.lm_head.nbytes()
 
@@ -218,6 +358,7 @@ class W4Decoder:
         (or the last position's logits).  The residual adds and RMSNorms run on the fused
         kernels (one launch each), the SiLU-mul in the gate/up GEMM's epilogue, RoPE and the
         cache writes in one launch; attention is PyTorch SDPA."""
+        self._contiguous()
         cfg = self.cfg
         b, t = tokens.shape
         hd, nh, kvh = cfg.head_dim, cfg.heads, cfg.kv_heads
@@ -249,6 +390,7 @@ class W4Decoder:
     def prefill_torch(self, tokens, return_logits=False):
         """The prefill in PyTorch ops (reference path): every linear is F.linear on the
         pseudo-quantized fp16 weight (fp32 accumulation), attention in fp32."""
+        self._contiguous()
         cfg = self.cfg
         b, t = tokens.shape
         hd, nh, kvh = cfg.head_dim, cfg.heads, cfg.kv_heads
@@ -301,6 +443,7 @@ class W4Decoder:
         """One greedy step for a batch on the fused kernels.  tokens [B] int64 (the last
         token), cur_len [1] int64 device tensor = position of that token; writes its K/V
         and returns the next ids (or the logits)."""
+        self._contiguous()
         cfg = self.cfg
         b = tokens.shape[0]
         hd, nh, kvh = cfg.head_dim, cfg.heads, cfg.kv_heads
@@ -339,6 +482,7 @@ class W4Decoder:
         """The decode step in PyTorch ops (reference path): RMSNorm on the rounded residual, every
         linear F.linear on the pseudo-quantized fp16 weight (fp32 accumulation), fp32 attention over the
         whole cache masked by the current length."""
+        self._contiguous()
         cfg = self.cfg
         b = tokens.shape[0]
         hd, nh, kvh = cfg.head_dim, cfg.heads, cfg.kv_heads
@@ -390,27 +534,21 @@ class W4Decoder:
         ``starts`` each sequence has one.  A sequence without new tokens gets -inf everywhere, from which
         ``ops.sample_tokens`` takes no token (-1).  Reads lengths and pages from device memory: a step without ``starts`` can be
         captured and replayed after each ``extend``."""
-        cfg = self.cfg
-        if tokens.dim() != 1 or not tokens.numel():
-            raise ValueError(f"tokens must be packed in one dimension and hold one at least, got {tuple(tokens.shape)}")
-        if max(cache.length) > self.max_len:
-            raise RuntimeError(f"a sequence of {max(cache.length)} positions, the model has {self.max_len}")
-        hd, nh, kvh = cfg.head_dim, cfg.heads, cfg.kv_heads
-        scale, (cos, sin) = 1.0 / math.sqrt(hd), self._angles()
-        x, delta = self.embed[tokens], None
-        for li, l in enumerate(self.layers):
-            if delta is None:
-                hn = ops.add_rms_norm_quant(x, None, l["ln1"], cfg.eps, quant=False)[0]
-            else:
-                hn, _, _, x = ops.add_rms_norm_quant(delta, x, l["ln1"], cfg.eps, quant=False)
+        cfg, scale = self.cfg, 1.0 / math.sqrt(self.cfg.head_dim)
+        cos, sin = self._paged_checks(tokens, cache)
+
+        def attend(li, qkv):
             k, v = cache.k[li], cache.v[li]
-            q = ops.paged_rope_append(l["qkv"](hn), cos, sin, k, v, cache.table, cache.lens, starts)
+            q = ops.paged_rope_append(qkv, cos, sin, k, v, cache.table, cache.lens, starts)
+            if starts is None and cfg.window:
+                return ops.paged_decode_window_attention(q, k, v, cache.table, cache.lens, scale, cfg.window, cfg.sinks)
             if starts is None:
-                att = ops.paged_decode_attention(q, k, v, cache.table, cache.lens, scale)
-            else:
-                att = ops.paged_prompt_attention(q, k, v, cache.table, cache.lens, starts, scale)
-            hn, _, _, x = ops.add_rms_norm_quant(l["o"](att.view(-1, nh * hd)), x, l["ln2"], cfg.eps, quant=False)
-            delta = l["down"](l["gate_up"].swiglu(hn))
+                return ops.paged_decode_attention(q, k, v, cache.table, cache.lens, scale)
+            if cfg.window:
+                return ops.paged_prompt_window_attention(q, k, v, cache.table, cache.lens, starts, scale, cfg.window, cfg.sinks)
+            return ops.paged_prompt_attention(q, k, v, cache.table, cache.lens, starts, scale)
+
+        x, delta = self._paged_layers(tokens, attend)
         if starts is not None:  # the last row of each sequence
             last = (starts[1:].long() - 1).clamp(0, len(tokens) - 1)
             delta, x = delta[last], x[last]
@@ -418,6 +556,66 @@ class W4Decoder:
         if starts is not None:
             logits.masked_fill_((starts[1:] <= starts[:-1]).unsqueeze(1), -math.inf)
         return logits
+
+    def _paged_checks(self, tokens, cache: PagedKVCache):
+        if tokens.dim() != 1 or not tokens.numel():
+            raise ValueError(f"tokens must be packed in one dimension and hold one at least, got {tuple(tokens.shape)}")
+        if max(cache.length) > self.max_len:
+            raise RuntimeError(f"a sequence of {max(cache.length)} positions, the model has {self.max_len}")
+        return self._angles()
+
+    def _paged_layers(self, tokens, attend):
+        """The layers over packed new tokens, ``attend(layer, qkv)`` their attention: (residual, its last addend)."""
+        cfg = self.cfg
+        x, delta = self.embed[tokens], None
+        for li, l in enumerate(self.layers):
+            if delta is None:
+                hn = ops.add_rms_norm_quant(x, None, l["ln1"], cfg.eps, quant=False)[0]
+            else:
+                hn, _, _, x = ops.add_rms_norm_quant(delta, x, l["ln1"], cfg.eps, quant=False)
+            att = attend(li, l["qkv"](hn))
+            hn, _, _, x = ops.add_rms_norm_quant(l["o"](att.view(-1, cfg.heads * cfg.head_dim)), x, l["ln2"], cfg.eps, quant=False)
+            delta = l["down"](l["gate_up"].swiglu(hn))
+        return x, delta
+
+    @torch.no_grad()
+    def forward_tree(self, tokens, cache: PagedKVCache, parents: Sequence[Sequence[int]]):
+        """Logits ``[tokens, vocab]`` after each of the sequences' drafted tokens, packed in ``tokens`` (int64), for the positions that
+        ``cache.extend`` has just made room for.  ``parents[b]`` says of each node of sequence b which earlier node it follows,
+        or -1 for what the cache held before; a node sees that, its ancestors and itself, and turns by its depth.
+        ``cache.keep`` takes up the accepted ones."""
+        cfg, scale = self.cfg, 1.0 / math.sqrt(self.cfg.head_dim)
+        if cfg.window:
+            raise RuntimeError("trees are verified without a window")
+        cos, sin = self._paged_checks(tokens, cache)
+        if len(parents) != len(cache.length) or sum(map(len, parents)) != tokens.numel():
+            raise ValueError(f"a list of parents for each of the {len(cache.length)} sequences, a parent for each of the "
+                             f"{tokens.numel()} tokens")
+        words = max(1, -(-max(map(len, parents)) // 64))
+        starts, turns, masks = [0], [], []
+        for length, nodes in zip(cache.length, parents):
+            if len(nodes) > length or any(not -1 <= p < i for i, p in enumerate(nodes)):
+                raise ValueError(f"a node follows an earlier one or -1, {list(nodes)} of {length} positions")
+            depth, seen = [], []
+            for i, p in enumerate(nodes):
+                depth.append(depth[p] + 1 if p >= 0 else 0)
+                seen.append((seen[p] if p >= 0 else 0) | 1 << i)
+            starts.append(starts[-1] + len(nodes))
+            turns += [length - len(nodes) + d for d in depth]
+            for s in seen:
+                row = [s >> 64 * w & (1 << 64) - 1 for w in range(words)]
+                masks.append([w - (1 << 64) if w >> 63 else w for w in row])
+        device = tokens.device
+        masks = torch.tensor(masks, dtype=torch.int64).to(device)
+        starts, turns = (torch.tensor(t, dtype=torch.int32).to(device) for t in (starts, turns))
+
+        def attend(li, qkv):
+            k, v = cache.k[li], cache.v[li]
+            q = ops.paged_rope_append(qkv, cos, sin, k, v, cache.table, cache.lens, starts, turns=turns)
+            return ops.paged_tree_attention(q, k, v, cache.table, cache.lens, starts, masks, scale)
+
+        x, delta = self._paged_layers(tokens, attend)
+        return self.lm_head(ops.add_rms_norm_quant(delta, x, self.norm, cfg.eps, quant=False)[0])
 
     @torch.no_grad()
     def generate_paged(self, prompts: Sequence[torch.Tensor], new_tokens: int, cache: Optional[PagedKVCache] = None,
@@ -444,8 +642,117 @@ class W4Decoder:
         tokens = sample(self.forward_paged(torch.cat([p.reshape(-1) for p in prompts]).to(device), cache, starts))
         out = [tokens]
         for _ in range(new_tokens - 1):
+            if self.cfg.window:
+                cache.trim(self.cfg.window, self.cfg.sinks)
             cache.extend([1] * len(prompts))
             # a sequence that has ended goes on with the vocabulary's first token, and stays ended
             tokens = sample(self.forward_paged(out[-1].clamp(min=0), cache))
             out.append(torch.where(out[-1] < 0, -1, tokens))
         return torch.stack(out, 1)
+
+    @torch.no_grad()
+    def generate_drafted(self, prompts: Sequence[torch.Tensor], new_tokens: int,
+                         draft: Optional[Callable[[List[int]], Tuple[List[int], List[int]]]] = None,
+                         cache: Optional[PagedKVCache] = None):
+        """``generate_paged`` that takes the largest logit, with several tokens a pass where drafts come true: ``draft`` gets a
+        sequence's tokens and returns ``(tokens, parents)`` of a tree of tokens that may follow (a parent: an earlier one
+        of them, or -1), ``lookup_draft()`` if ``None``.  A pass verifies every sequence's tree, takes the path along which each
+        token is the one that the model takes, and a token more.  Returns ``[prompts, new_tokens]``, -1 from where a sequence has
+        nothing to take."""
+        device, draft = self.embed.device, draft or lookup_draft()
+        history = [p.reshape(-1).tolist() for p in prompts]
+        lengths = [len(h) for h in history]
+        if not lengths or min(lengths) < 1 or new_tokens < 1:
+            raise ValueError("prompts must hold a token at least, and new_tokens must be positive")
+        if cache is None:
+            page, spare = 64, 64
+            cache = self.paged_cache(len(prompts), sum(-(-(n + new_tokens + spare) // page) * page for n in lengths), page)
+
+        def best(logits):
+            zero = torch.zeros(len(logits), device=device)
+            return ops.sample_tokens(logits, zero, zero)[0].tolist()
+
+        starts = cache.extend(lengths)
+        packed = torch.cat([p.reshape(-1) for p in prompts]).to(device)
+        for h, t in zip(history, best(self.forward_paged(packed, cache, starts))):
+            h.append(t)
+        while True:
+            tokens, parents = [], []
+            room = cache.free_positions() // cache.page // len(history) * cache.page  # of a sequence's pages still to be taken
+            for h, n, length in zip(history, lengths, cache.length):
+                left = n + new_tokens - len(h)  # to be generated yet
+                if left < 1 or h[-1] < 0:
+                    tokens.append([])
+                    parents.append([])
+                    continue
+                more, follow = draft(list(h)) if left > 1 else ([], [])
+                if len(more) != len(follow) or any(not -1 <= p < i for i, p in enumerate(follow)) or \
+                        any(not 0 <= t < self.cfg.vocab for t in more):
+                    raise ValueError("a draft has a token of the vocabulary and an earlier parent or -1 for each node")
+                most = max(0, min(cache.max_len, self.max_len, -(-length // cache.page) * cache.page + room) - length - 1)
+                tokens.append([h[-1], *more[:most]])
+                parents.append([-1, *(p + 1 for p in follow[:most])])
+            news = [len(t) for t in tokens]
+            if not any(news):
+                break
+            cache.extend(news)
+            took = best(self.forward_tree(torch.tensor([t for of in tokens for t in of], device=device), cache, parents))
+            kept, first = [], 0
+            for h, of, follow in zip(history, tokens, parents):
+                path, node = [], 0 if of else -1
+                while node >= 0:
+                    path.append(node)
+                    t = took[first + node]
+                    h.append(t)
+                    node = next((i for i, p in enumerate(follow) if p == node and of[i] == t and i > node), -1)
+                kept.append(path)
+                first += len(of)
+            cache.keep(news, kept)
+        out = torch.full((len(history), new_tokens), -1, dtype=torch.int64)
+        for row, h, n in zip(out, history, lengths):
+            new = h[n:n + new_tokens]
+            row[:len(new)] = torch.tensor(new)
+        return out.to(device)
+
+    @torch.no_grad()
+    def beam_search_paged(self, prompts: Sequence[torch.Tensor], new_tokens: int, beams: int, end: Optional[int] = None,
+                          cache: Optional[PagedKVCache] = None):
+        """The ``beams`` best continuations of each prompt by ``new_tokens`` tokens that a search with as many beams finds, from the
+        best down: ``(tokens [prompts, beams, new_tokens], scores fp32 [prompts, beams])``, a score being the sum of the tokens' log
+        probabilities.  A beam that takes the token ``end`` is over: ``end`` fills the rest and its score stays.  A request's
+        beams share the pages of what they have in common.  ``cache``, if given, has ``beams`` sequences for each prompt.
+        Where fewer continuations are left, scores are -inf and tokens -1."""
+        device, n = self.embed.device, len(prompts)
+        lengths = [int(p.numel()) for p in prompts]
+        if not lengths or min(lengths) < 1 or new_tokens < 1 or not 1 <= beams <= 64:
+            raise ValueError("prompts must hold a token at least, new_tokens be positive, and beams 1 to 64")
+        if end is not None and not 0 <= end < self.cfg.vocab:
+            raise ValueError(f"end must be a token of the {self.cfg.vocab}, got {end}")
+        if cache is None:
+            page = 64
+            cache = self.paged_cache(n * beams, sum(-(-l // page) + beams * (-(-new_tokens // page) + 1) for l in lengths) * page, page)
+        elif len(cache.length) != n * beams:
+            raise ValueError(f"the cache must have {n * beams} sequences, {beams} for each prompt, got {len(cache.length)}")
+        base = torch.arange(0, n * beams, beams, device=device).unsqueeze(1)
+        scores = torch.full((n, beams), -math.inf, device=device)
+        scores[:, 0] = 0
+        starts = cache.extend([l if b == 0 else 0 for l in lengths for b in range(beams)])
+        logits = self.forward_paged(torch.cat([p.reshape(-1) for p in prompts]).to(device), cache, starts)
+        ended = None if end is None else torch.zeros(n, beams, dtype=torch.bool, device=device)
+        history = torch.zeros(n, beams, 0, dtype=torch.int64, device=device)
+        for step in range(new_tokens):
+            if step:
+                if self.cfg.window:
+                    cache.trim(self.cfg.window, self.cfg.sinks)
+                cache.extend([1] * (n * beams))
+                # a beam that has ended, or never was, goes on with any token and stays as it is
+                logits = self.forward_paged(history[:, :, -1].reshape(-1).clamp(min=0), cache)
+            scores, parents, tokens = ops.beam_select(logits, scores, beams, ended, end or 0)
+            alive = parents.clamp(min=0)
+            history = torch.cat((history.gather(1, alive.unsqueeze(2).expand(-1, -1, step)), tokens.unsqueeze(2)), 2)
+            history = torch.where((parents < 0).unsqueeze(2), -1, history)
+            if step + 1 < new_tokens:
+                cache.reorder((base + alive).reshape(-1).tolist())
+            if end is not None:
+                ended = ended.gather(1, alive) | (tokens == end)
+        return history, scores

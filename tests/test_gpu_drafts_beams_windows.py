@@ -1,0 +1,239 @@
+"""Drafts, beams and windows on the decoder stack, the operators together as a server runs them, against the same stack in PyTorch ops."""
+import sys
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+VOCAB = 512
+
+
+def _say(*a):
+    print(*a, flush=True)
+    sys.stdout.flush()
+
+
+def _rel(a, b):
+    return ((a - b).norm() / b.norm()).item()
+
+
+def _model(heads, kv_heads, max_len=200, seed=5, **cfg):
+    from mindpipe_amd.decoder import DecoderConfig, W4Decoder
+    cfg = DecoderConfig(layers=2, hidden=heads * 128, heads=heads, kv_heads=kv_heads, ffn=512, vocab=VOCAB, **cfg)
+    return W4Decoder(cfg, max_batch=1, max_len=max_len, device=DEV, seed=seed)
+
+
+def _tokens(*lengths, seed=6):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return [torch.randint(0, VOCAB, (n,), device=DEV, generator=g) for n in lengths]
+
+
+def _reference(model, tokens):
+    """Logits after every token of one sequence, with the configuration's window, in PyTorch ops (fp32 attention)."""
+    from mindpipe_amd.decoder import _rms
+    cfg, n = model.cfg, tokens.numel()
+    hd, nh, kvh = cfg.head_dim, cfg.heads, cfg.kv_heads
+    pos = torch.arange(n, device=DEV)
+    seen = pos <= pos[:, None]
+    if cfg.window:
+        seen &= (pos < cfg.sinks) | (pos > pos[:, None] - cfg.window)
+    x = model.embed[tokens][None]
+    for l in model.layers:
+        hn = _rms(x, l["ln1"], cfg.eps)
+        qkv = l["qkv"].reference(hn[0]).view(1, n, nh + 2 * kvh, hd).transpose(1, 2)
+        q, k, v = qkv[:, :nh], qkv[:, nh:nh + kvh], qkv[:, nh + kvh:]
+        q, k = model._rope(q, pos), model._rope(k, pos)
+        k, v = (t.repeat_interleave(nh // kvh, 1).float().contiguous() for t in (k, v))
+        s = (q.float() @ k.transpose(-1, -2).contiguous()) * hd ** -0.5
+        att = (torch.softmax(s.masked_fill(~seen, float("-inf")), -1) @ v).half()
+        x = x + l["o"].reference(att.transpose(1, 2).reshape(n, nh * hd))[None]
+        hn = _rms(x, l["ln2"], cfg.eps)
+        gu = l["gate_up"].reference(hn[0])
+        act = torch.nn.functional.silu(gu[:, :cfg.ffn]) * gu[:, cfg.ffn:]
+        x = x + l["down"].reference(act.contiguous())[None]
+    return model.lm_head.reference(_rms(x[0], model.norm, cfg.eps).contiguous()).float()
+
+
+# Bounds as for the stack's other paths: fp16 hidden states through two layers, fused kernels on one side and PyTorch ops
+# with other roundings on the other, 2e-2 of the norm of a row of logits.
+def _near_best(logits, token):
+    """The token is the largest of the reference's logits, or as near to it as 2e-2 of the row's norm (both sides' errors)."""
+    return bool(logits[token] >= logits.max() - 2e-2 * logits.norm())
+
+
+@pytest.mark.parametrize("heads,kv_heads,page", [(2, 2, 8), (4, 1, 64), (8, 2, 16)])
+def test_trees_match_their_paths(heads, kv_heads, page):
+    """Every node's logits are those of its path alone; what is taken up of it is what the next tokens see."""
+    _say("tree decoder", heads, kv_heads, page)
+    model = _model(heads, kv_heads)
+    prompts = _tokens(40, 3, 17)
+    cache = model.paged_cache(3, 3 * 200, page)
+    model.forward_paged(torch.cat(prompts), cache, cache.extend([40, 3, 17]))
+    parents = [[-1, 0, 0, 1, 2, 2, 4, -1], [], [-1]]
+    nodes = _tokens(8, 0, 1, seed=8)
+    cache.extend([8, 0, 1])
+    logits = model.forward_tree(torch.cat(nodes), cache, parents).float()
+    for b, first in ((0, 0), (2, 8)):
+        for i, p in enumerate(parents[b]):
+            path, j = [], i
+            while j >= 0:
+                path.insert(0, j)
+                j = parents[b][j]
+            want = _reference(model, torch.cat((prompts[b], nodes[b][path])))[-1]
+            assert _rel(logits[first + i], want) <= 2e-2, (b, i)
+    cache.keep([8, 0, 1], [[0, 2, 4, 6], [], []])
+    assert cache.length == [44, 3, 17]
+    steps = _tokens(3, seed=9)[0]
+    cache.extend([1, 1, 1])
+    after = model.forward_paged(steps, cache).float()
+    for b, have in enumerate((torch.cat((prompts[0], nodes[0][[0, 2, 4, 6]])), prompts[1], prompts[2])):
+        assert _rel(after[b], _reference(model, torch.cat((have, steps[b:b + 1])))[-1]) <= 2e-2
+
+
+def test_drafted_tokens_are_the_models_own():
+    """Whatever is drafted, the tokens are those that the model takes; drafts that come true save passes."""
+    model = _model(4, 2)
+    prompts, new = _tokens(20, 33, 6), 12
+    plain = model.generate_paged(prompts, new)
+    runs, forward = [], model.forward_tree
+    model.forward_tree = lambda *a: (runs.append(1), forward(*a))[1]
+    def knows(tokens):  # the true next tokens, beside others
+        for p, t in zip(prompts, plain.tolist()):
+            n = p.numel()
+            if tokens[:n] == p.tolist() and len(tokens) > n:
+                at = len(tokens) - n
+                true = t[at:at + 4]
+                wrong = [(x + 1) % VOCAB for x in true]
+                return wrong + true, [-1] * min(1, len(true)) + list(range(len(true) - 1)) + [-1] * min(1, len(true)) + \
+                    [len(true) + i for i in range(len(true) - 1)]
+        return [], []
+
+    for draft in (None, knows, lambda t: ([], []), lambda t: ([7] * 70, [-1] * 70)):
+        runs.clear()
+        got = model.generate_drafted(prompts, new, draft)
+        assert got.shape == (3, new) and int(got.min()) >= 0
+        for p, row in zip(prompts, got):
+            logits = _reference(model, torch.cat((p, row)))
+            for i in range(new):
+                assert _near_best(logits[p.numel() - 1 + i], row[i])
+        if draft is knows and torch.equal(got, plain):
+            assert len(runs) <= 4  # one, four and a token more at a time: 1 + 5 + 5 + 1
+    with pytest.raises(ValueError, match="draft"):
+        model.generate_drafted(prompts, 4, lambda t: ([1, 2], [-1, 1]))
+    with pytest.raises(ValueError, match="draft"):
+        model.generate_drafted(prompts, 4, lambda t: ([VOCAB], [-1]))
+    with pytest.raises(ValueError):
+        model.generate_drafted([], 4)
+
+
+def test_drafts_fit_the_cache_and_the_model():
+    model = _model(2, 2, max_len=40)
+    prompts = _tokens(30, 20)
+    got = model.generate_drafted(prompts, 10, lambda t: (list(range(50)), list(range(-1, 49))), model.paged_cache(2, 96, 16))
+    assert got.shape == (2, 10) and int(got.min()) >= 0
+
+
+def test_beams():
+    """Scores are the log probabilities of their tokens, from the best down, no two beams alike; one beam is the greedy run."""
+    model = _model(4, 2)
+    prompts, new, beams = _tokens(20, 65, 1), 6, 4
+    tokens, scores = model.beam_search_paged(prompts, new, beams)
+    assert tokens.shape == (3, beams, new) and scores.shape == (3, beams)
+    assert (scores[:, :-1] >= scores[:, 1:]).all()
+    for p, of, have in zip(prompts, tokens, scores):
+        assert len({tuple(t) for t in of.tolist()}) == beams
+        for t, score in zip(of, have):
+            logits = _reference(model, torch.cat((p, t)))
+            logp = torch.log_softmax(logits, -1)[p.numel() - 1:-1].gather(1, t[:, None]).sum()
+            # a log probability is off by no more than twice its row's largest error, 2e-2 of the norm of logits spread over 512
+            assert abs(float(score - logp)) <= new * 2 * 2e-2 * float(logits.norm(dim=1).max())
+    one, score = model.beam_search_paged(prompts, new, 1)
+    for p, row in zip(prompts, one[:, 0]):
+        logits = _reference(model, torch.cat((p, row)))
+        assert all(_near_best(logits[p.numel() - 1 + i], row[i]) for i in range(new))
+    assert (scores[:, 0] >= score[:, 0] - 1e-2).all()
+
+
+def test_beams_find_the_best_pair():
+    """The best of 64 beams is the best pair of tokens that the same stack finds from each of the likeliest first ones."""
+    model = _model(2, 2)
+    prompt = _tokens(9)[0]
+    tokens, scores = model.beam_search_paged([prompt], 2, 64)
+    logits = _reference(model, prompt)[-1]
+    first, best, norm = torch.log_softmax(logits, -1), -1e9, 0.0
+    for t in first.topk(64).indices:
+        after = _reference(model, torch.cat((prompt, t[None])))[-1]
+        best = max(best, float(first[t] + torch.log_softmax(after, -1).max()))
+        norm = max(norm, float(after.norm()))
+    # both log probabilities off by no more than twice their row's largest error
+    assert abs(float(scores[0, 0]) - best) <= 2 * 2e-2 * (float(logits.norm()) + norm)
+
+
+def test_beams_that_end_keep_their_scores():
+    model = _model(2, 2)
+    prompts = _tokens(12, 30)
+    plain, _ = model.beam_search_paged(prompts, 8, 3)
+    end = int(plain[0, 0, 2])  # what the best beam takes third
+    tokens, scores = model.beam_search_paged(prompts, 8, 3, end)
+    for p, of, have in zip(prompts, tokens, scores):
+        for t, score in zip(of.tolist(), have):
+            if end in t:
+                at = t.index(end)
+                assert all(x == end for x in t[at:])
+                t = t[:at + 1]
+            logits = _reference(model, torch.cat((p, torch.tensor(t, device=DEV))))
+            logp = torch.log_softmax(logits, -1)[p.numel() - 1:-1].gather(1, torch.tensor(t, device=DEV)[:, None]).sum()
+            assert abs(float(score - logp)) <= len(t) * 2 * 2e-2 * float(logits.norm(dim=1).max())
+    cache = model.paged_cache(6, 6 * 64, 8)
+    model.beam_search_paged(prompts, 8, 3, end, cache)
+    for b in range(6):
+        cache.release(b)
+    assert cache.free_positions() == 6 * 64
+    for bad in (dict(beams=0), dict(beams=65), dict(end=VOCAB), dict(cache=model.paged_cache(5, 500))):
+        with pytest.raises(ValueError):
+            model.beam_search_paged(prompts, 8, **{"beams": 3, **bad})
+
+
+@pytest.mark.parametrize("heads,kv_heads,page,window,sinks", [(2, 2, 8, 20, 3), (4, 1, 16, 1, 0), (8, 2, 8, 33, 8), (4, 2, 8, 1000, 4)])
+def test_windows_match_torch(heads, kv_heads, page, window, sinks):
+    """Prompts, chunks and single tokens of a model with a window, its pages trimmed between them."""
+    _say("window decoder", heads, kv_heads, page, window, sinks)
+    model = _model(heads, kv_heads, window=window, sinks=sinks)
+    prompts = _tokens(90, 5, 64)
+    cache = model.paged_cache(3, 3 * 200, page)
+    model.forward_paged(torch.cat((prompts[0][:50], prompts[2])), cache, cache.extend([50, 0, 64]))
+    freed = cache.trim(window, sinks)
+    assert (freed > 0) == (window < 60)
+    logits = model.forward_paged(torch.cat((prompts[0][50:], prompts[1])), cache, cache.extend([40, 5, 0])).float()
+    cache.trim(window, sinks)
+    steps = _tokens(3, seed=7)[0]
+    cache.extend([1, 1, 1])
+    after = model.forward_paged(steps, cache).float()
+    for b in range(3):
+        want = _reference(model, torch.cat((prompts[b], steps[b:b + 1])))
+        if b < 2:
+            assert _rel(logits[b], want[-2]) <= 2e-2
+        assert _rel(after[b], want[-1]) <= 2e-2
+    got = model.generate_paged(prompts, 5)
+    for p, row in zip(prompts, got):
+        logits = _reference(model, torch.cat((p, row)))
+        assert all(_near_best(logits[p.numel() - 1 + i], row[i]) for i in range(5))
+    found, _ = model.beam_search_paged(prompts, 4, 2)
+    assert found.shape == (3, 2, 4) and int(found.min()) >= 0
+    for call in (lambda: model.prefill(prompts[0][None]), lambda: model.decode_step(steps[:1], torch.tensor([3], device=DEV)),
+                 lambda: model.forward_tree(steps[:1], cache, [[-1], [], []])):
+        with pytest.raises(RuntimeError, match="window"):
+            call()
+
+
+def test_tree_refusals():
+    model = _model(2, 2)
+    cache = model.paged_cache(2, 200, 8)
+    cache.extend([3, 2])
+    t = _tokens(5)[0]
+    for parents in ([[-1, 0, 1]], [[-1, 0], [-1, 0]], [[-1, 1, 0], [-1, 0]], [[-2, 0, 0], [-1, 0]], [[-1, 0, 0, 0], [-1]]):
+        with pytest.raises(ValueError):
+            model.forward_tree(t, cache, parents)
+    with pytest.raises(ValueError, match="tokens"):
+        model.forward_tree(t.view(1, 5), cache, [[-1, 0, 0], [-1, 0]])
