@@ -92,11 +92,14 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(const uint8_t *
       f(first + 8 * kBeamThreads * g, v);
     }
   };
-  float top = -INFINITY;
-  each([&](int, const float (&v)[8]) {
+  float top = -INFINITY, eight[H];  // the largest of each eight: only those that have a candidate are looked at again
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = fmaxf(top, v[e]);
-  });
+  for (int g = 0; g < H; ++g) {
+    float v[8];
+    held[g].get(v);
+    eight[g] = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+    top = fmaxf(top, eight[g]);  // eight NaN are no part of it
+  }
   const float four = fmaxf(fmaxf(top, __shfl_xor(top, 1, 64)), fmaxf(__shfl_xor(top, 2, 64), __shfl_xor(top, 3, 64)));
   if ((tid & 3) == 0) quad[tid >> 2] = beam_order(four);
   const float wtop = mp_wave_max(top);
@@ -142,15 +145,18 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(const uint8_t *
     if (n < kBeamListed) list[n] = static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~i);
   };
   const float limit = sample_value<MP_F32>(least);
-  each([&](int i, const float (&v)[8]) {
-    float eight = v[0];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) eight = fmaxf(eight, v[e]);
-    if (eight < limit) return;
+  for (int g = 0; g < H; ++g) {
+    if (!__any(eight[g] >= limit)) continue;
+    float v[8];
+    held[g].get(v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (v[e] >= limit) want(beam_order(v[e]), i + e);
-  });
+    for (int e = 0; e < 8; ++e) {  // (a branch for the wave: the lanes' own cost more than all the rest of the pass)
+      if (__any(v[e] >= limit)) {
+        if (v[e] >= limit) want(beam_order(v[e]), first + 8 * kBeamThreads * g + e);
+      }
+    }
+  }
   __syncthreads();
   int n = static_cast<int>(listed);
   if (tid == 0) {
