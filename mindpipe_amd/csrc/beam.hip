@@ -9,6 +9,9 @@
 // Two launches.  Of each row, workgroups take a part of the vocabulary each (a row is read once and stays in registers): they leave
 // the part's maximum, its sum of exponentials and its `count` largest values in order.  No value can be among a request's best
 // that is not among those.  Then a workgroup a request puts the best of its lists in order.
+//
+// Bound by vector instructions, 26 for a value, of which the exponential in 64 bits (as fast as 32 bits here) is 17: 48 requests of 8
+// beams over 128256 bf16, 98 MB, 45 us, and the merge 10, where the reads alone would take 15.  One request of 4 over 32000: 6.4 and 7.2.
 #include "logits.h"
 
 namespace {
@@ -341,7 +344,9 @@ __global__ __launch_bounds__(256) void beam_merge_kernel(const BeamPart *__restr
   }
 }
 
-// Eights of a thread: as many as hold a row in few parts, but as few as keep 512 workgroups or more in the launch.
+// Eights of a thread: eight, of which 116 registers leave four workgroups to a CU, but as few as keep 512 workgroups or more in the
+// launch.  48 requests as above: sixteen 57 us, eight 50, four 50 with a merge of 14 in place of 10 us (before the looks for candidates
+// were cut down to 45).
 inline int beam_eights(int64_t rows, int64_t vocab, int dtype) {
   int h = 8;
   while (h > 2 && rows * mp_cdiv(vocab, 8 * h * kBeamThreads) < 512) h /= 2;

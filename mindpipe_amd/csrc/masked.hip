@@ -14,6 +14,13 @@
 // hold nothing seen left out.  Items that are much longer than an equal share of all tiles are cut into parts, which leave their
 // outputs, unnormalised, maxima and sums in the workspace, and a second launch joins them, always in the same order.  A
 // workgroup takes a part, and the longest come first, so that the short ones fill what the long ones leave.
+//
+// The wide form is bound as the prompts' attention is, by matrix and vector instructions in turn: 2.2 us for a tile of a workgroup, two to
+// a CU.  2048 tokens behind 8192 positions with a window of 4096, 64 / 8 heads of 128 in bf16, 309 us, 0.9 PFLOP/s of what is seen; 24
+// sequences of up to 8192 positions with trees of up to 64 nodes 149 us, 53 tiles an equal share and about 66 the longest path.  (Equal
+// runs of tiles over all items, with a loop over items in the kernel, took 171 us there for as many tiles a share: the loop's state took the
+// registers that hold the loads' offsets.)  The narrow form is bound by the chain from the lengths to a page and by the reads: 26 nodes
+// behind 1531 positions, 32 / 32 heads, 13.6 us and a join of 4.
 #include <algorithm>
 #include <cfloat>
 #include <climits>

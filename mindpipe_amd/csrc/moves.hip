@@ -38,7 +38,8 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(MovePools p, const int3
 constexpr int kAhead = 8;  // positions that are read before the first of them is written
 
 // A thread takes one 16-byte column (layer, pool, head, piece) of a sequence and moves its entries in their order.  They ascend
-// and none lies before its new place, so what is read later has not been written.
+// and none lies before its new place, so what is read later has not been written.  Bound by its chain of loads, offsets, entries,
+// pages and values: 40 sequences, up to seven of 64 positions, 8 heads of 128 in 32 layers (18 MB) 11 us, one sequence of 32 heads 3.8.
 __global__ __launch_bounds__(256) void paged_keep_kernel(MovePools p, const int32_t *__restrict__ table, int width,
                                                          const int32_t *__restrict__ first, const int32_t *__restrict__ keep,
                                                          const int32_t *__restrict__ starts, int total, int per) {

@@ -38,7 +38,7 @@ def _logits(rows, vocab, dtype, seed, spread=1.7):
 
 def _select(logits, scores, count, ended=None, pad=0):
     """The kernel's answer, checked.  Beams and tokens are those of the totals in 64 bits; a score is a total rounded to fp32 once,
-    half a step of it, and the total's own error (2^-36 of the sum of exponentials) is far below that."""
+    half a step of it, and the total's own error (2^-34 of the sum of exponentials) is far below that."""
     got = _ops().beam_select(logits, scores, count, ended, pad)
     best, parent, token = mref.beams(logits, scores.cpu(), count, None if ended is None else ended.cpu(), pad)
     assert torch.equal(got[1].cpu(), parent) and torch.equal(got[2].cpu(), token)
