@@ -530,7 +530,7 @@ int mp_paged_keep_positions(const mp_pages *cache, int64_t layers, int64_t k_lay
  * and -inf totals are never taken; missing ones are score -inf, beam and token -1.  With infinite logits in a row those share its
  * weight.  logits [batch * beams, vocab] (row stride `stride`; fp16, bf16 or fp32), scores fp32 [batch, beams], outputs [batch,
  * count].  workspace: mp_beam_select_workspace_bytes, 16-byte aligned, not shared by calls that may run at once. */
-size_t mp_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t count, int dtype);
+size_t mp_beam_select_workspace_bytes(int64_t batch, int64_t beams, int64_t vocab, int64_t count);
 int mp_beam_select(const void *logits, int64_t stride, int64_t batch, int64_t beams, int64_t vocab, int dtype, const float *scores,
                    const uint8_t *ended, int64_t pad, int64_t count, float *out_scores, int64_t *out_beams, int64_t *out_tokens,
                    void *workspace, size_t workspace_bytes, mp_stream_t stream);

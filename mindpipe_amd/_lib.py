@@ -102,7 +102,7 @@ SIGNATURES = {
                                                 C.c_float, _vp, _i32, _vp, _sz, _vp]),
     "mp_paged_copy_pages": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _vp]),
     "mp_paged_keep_positions": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i64, _vp, _vp, _i64, _vp, _vp]),
-    "mp_beam_select_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32]),
+    "mp_beam_select_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "mp_beam_select": (_i32, [_vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "mp_sample_tokens": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mp_moe_unpermute_combine": (_i32, [_vp, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _i32, _vp]),

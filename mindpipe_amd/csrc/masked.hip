@@ -15,12 +15,12 @@
 // outputs, unnormalised, maxima and sums in the workspace, and a second launch joins them, always in the same order.  A
 // workgroup takes a part, and the longest come first, so that the short ones fill what the long ones leave.
 //
-// The wide form is bound as the prompts' attention is, by matrix and vector instructions in turn: 2.2 us for a tile of a workgroup, two to
-// a CU.  2048 tokens behind 8192 positions with a window of 4096, 64 / 8 heads of 128 in bf16, 309 us, 0.9 PFLOP/s of what is seen; 24
-// sequences of up to 8192 positions with trees of up to 64 nodes 149 us, 53 tiles an equal share and about 66 the longest path.  (Equal
-// runs of tiles over all items, with a loop over items in the kernel, took 171 us there for as many tiles a share: the loop's state took the
-// registers that hold the loads' offsets.)  The narrow form is bound by the chain from the lengths to a page and by the reads: 26 nodes
-// behind 1531 positions, 32 / 32 heads, 13.6 us and a join of 4.
+// The wide form is bound as the prompts' attention is, by matrix and vector instructions in turn: 2.2 us for a tile of a
+// workgroup, two to a CU.  2048 tokens behind 8192 positions with a window of 4096, 64 / 8 heads of 128 in bf16, 309 us, 0.9
+// PFLOP/s of what is seen; 24 sequences of up to 8192 positions with trees of up to 64 nodes 149 us, 53 tiles an equal share and
+// about 66 the longest path.  (Equal runs of tiles over all items, with a loop over items in the kernel, took 171 us there: the
+// loop's state took the registers that hold the loads' offsets.)  The narrow form is bound by the chain from the lengths to a
+// page and by the reads: 26 nodes behind 1531 positions, 32 / 32 heads, 13.6 us and a join of 4.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -40,19 +40,21 @@ struct MaskedRule {
   const int64_t *masks;  // kTree: [rows, words]
   int words;
   int window, sinks;     // kWindow
-  MpDivisor group;   // rows / group: tokens
+  MpDivisor group;       // rows / group: tokens
 };
 
 // A sequence's rows and what they see, by the launch's rule.
 template <int MODE>
 struct MaskedSeq {
   int first, n;          // its packed rows
-  int len, room;         // its positions, the new tokens' included, and those that the table has room for; none outside of the sequences
+  int len, room;         // its positions, the new tokens' included, and those that there is room for; none outside of the sequences
   MaskedRule rule;
 
   __device__ __forceinline__ int context() const { return len - n; }  // position of its first row (negative: rows without a place)
   __device__ __forceinline__ int end() const { return min(len, room); }
-  __device__ __forceinline__ int clamped(int64_t p) const { return static_cast<int>(max(min(p, static_cast<int64_t>(end())), int64_t(0))); }
+  __device__ __forceinline__ int clamped(int64_t p) const {
+    return static_cast<int>(max(min(p, static_cast<int64_t>(end())), int64_t(0)));
+  }
   // Positions t .. t + 63 that token `token` of the sequence sees, as bits.  t is a multiple of 32.
   __device__ __forceinline__ uint64_t bits(int token, int t) const {
     if constexpr (MODE == kTree) {
@@ -99,7 +101,9 @@ struct Wide {
 struct Narrow {
   static constexpr int kItem = 16, kStep = 128, kSlack = 2, kFiner = INT_MAX;
 };
-constexpr int kSlots = 3;  // parts that have others, in shares: each has more than half of two thirds of a share
+// Parts that have others, in shares at most: an item of T > limit tiles has up to 2 T / (limit + 1), and with limit from two thirds of
+// a share e on, 2 (e + 1) / (2 e / 3 + 2) is below 3.  They are half as many more than the items that they replace.
+constexpr int kSlots = 3;
 
 // What a workgroup takes: tiles of an item.
 template <int MODE>
@@ -179,7 +183,9 @@ struct MaskedPlan {
     // nodes, 58 items of 1 to 129 tiles for 64 workgroups: 186 us, 152 with the finer ones).
     const int equal = static_cast<int>(all / static_cast<uint32_t>(share));
     int limit = equal + min(equal / 2, FORM::kSlack) + 1;
-    const auto parts = [&](const Row &r) { return r.tiles > limit ? static_cast<int>(static_cast<uint32_t>(r.tiles + limit - 1) / static_cast<uint32_t>(limit)) : 1; };
+    const auto parts = [&](const Row &r) {
+      return r.tiles > limit ? static_cast<int>(static_cast<uint32_t>(r.tiles + limit - 1) / static_cast<uint32_t>(limit)) : 1;
+    };
     if (equal >= FORM::kFiner) {
       const int keep = limit;
       int took[2] = {0, 0};
@@ -226,7 +232,7 @@ struct MaskedPlan {
           p.parts = __builtin_amdgcn_readlane(in, l);
           p.item = at - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l));
           p.part = 0;
-          p.slot = index;  // those in parts come first, below kSlots share: each has more than half of `limit` tiles
+          p.slot = index;  // those in parts come first, below kSlots share
           p.seq = seq(p.b);
           p.seq.first = __builtin_amdgcn_readfirstlane(p.seq.first);
           p.seq.n = __builtin_amdgcn_readfirstlane(p.seq.n);
@@ -328,7 +334,8 @@ __device__ __attribute__((noinline)) void masked_rows16(const MaskedRows<MODE> &
 // Of an item's first part: its slot, how many there are, the item's first row counted from the sequence's, and the packed row that
 // the sequence begins at.  Of the others: no parts.  And how many slots there are, from the first workgroup.
 template <int MODE, class FORM>
-__device__ __forceinline__ bool masked_find(const MaskedPlan<MODE, FORM> &plan, int kvh, int kh, int share, int4 *joins, MaskedPart<MODE> &p) {
+__device__ __forceinline__ bool masked_find(const MaskedPlan<MODE, FORM> &plan, int kvh, int kh, int share, int4 *joins,
+                                            MaskedPart<MODE> &p) {
   uint32_t cut;
   const int at = blockIdx.x / kvh;
   const bool found = plan.find(at, share, p, cut);
@@ -669,7 +676,8 @@ int masked_start(const MaskedCall &c, int shift) {
       hipFuncSetAttribute(reinterpret_cast<const void *>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
     return MP_ERR_HIP;
   const mp_pages &p = *c.cache;
-  hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>((masked_items<FORM>(c.rows, grp, c.batch) + kSlots * share / 2 + 1) * c.kvh)), dim3(64 * kWaves), kLds, c.stream,
+  const int64_t blocks = (masked_items<FORM>(c.rows, grp, c.batch) + kSlots * share / 2 + 1) * c.kvh;
+  hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), kLds, c.stream,
                      static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(p.k), p.k_page,
                      p.k_head, p.k_row, static_cast<const uint16_t *>(p.v), p.v_page, p.v_head, p.v_row, static_cast<int>(p.pages),
                      shift, p.table, static_cast<int>(p.width), c.lens, c.starts, static_cast<int>(c.batch),
@@ -677,8 +685,8 @@ int masked_start(const MaskedCall &c, int shift) {
                      static_cast<uint16_t *>(c.out));
   MP_CHECK_LAUNCH();
   if (c.reach > FORM::kStep) {  // else items of one tile, which are never cut
-    hipLaunchKernelGGL((masked_join_kernel<D, DT, FORM>), dim3(static_cast<unsigned>(kSlots * share * c.kvh), FORM::kItem / 16), dim3(256), 0,
-                       c.stream, c.kvh, grp, slot_rows, c.rule.group, parts, joins, static_cast<uint16_t *>(c.out));
+    hipLaunchKernelGGL((masked_join_kernel<D, DT, FORM>), dim3(static_cast<unsigned>(kSlots * share * c.kvh), FORM::kItem / 16),
+                       dim3(256), 0, c.stream, c.kvh, grp, slot_rows, c.rule.group, parts, joins, static_cast<uint16_t *>(c.out));
     MP_CHECK_LAUNCH();
   }
   return MP_OK;

@@ -1577,7 +1577,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int, ended: O
         lib = _lib.load()
         with _dev(logits):
             dt = _DT[logits.dtype]
-            wsb = lib.mp_beam_select_workspace_bytes(batch, beams, vocab, count, dt)
+            wsb = lib.mp_beam_select_workspace_bytes(batch, beams, vocab, count)
             ws = torch.empty((wsb,), dtype=torch.uint8, device=logits.device)
             _lib.check(lib.mp_beam_select(
                 logits.data_ptr(), stride, batch, beams, vocab, dt, scores.data_ptr(), _ptr(ended), pad, count, best.data_ptr(),

@@ -90,6 +90,19 @@ def test_select_equal_and_ordered_values(dtype):
     _select(rows[[0, 0, 5, 5]], torch.zeros(2, 2, device=DEV), 40)  # equal beams: the lowest first
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("beams,count", [(5, 60), (40, 64), (64, 2)])
+def test_select_equal_beams(dtype, beams, count):
+    """Equal totals in many lists, from a few hundred of them to more than LDS holds: those of the lowest beams, then tokens."""
+    x = torch.zeros(beams, 9000, dtype=dtype, device=DEV)
+    x[:, 17:8999:2] = -1.0
+    got = _select(x, torch.zeros(1, beams, device=DEV), count)
+    assert (got[1] == 0).all() and got[2][0].tolist() == [*range(17), *range(18, 9000, 2)][:count]
+    _select(x, -0.5 * (torch.arange(beams, device=DEV) % 2)[None].float(), count)
+    ended = torch.arange(beams, device=DEV)[None] < beams - 1
+    _select(x, torch.zeros(1, beams, device=DEV), count, ended, 5)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 def test_select_what_is_masked(dtype):
     """-inf, NaN and infinities among the logits and scores, rows of nothing else, fewer candidates than are asked for."""

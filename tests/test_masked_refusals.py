@@ -172,7 +172,7 @@ def test_c_entry_points_refuse():
     for bad in (dict(stride=49), dict(batch=-1), dict(beams=0), dict(beams=65), dict(vocab=0), dict(vocab=(1 << 19) + 1, stride=1 << 20),
                 dict(pad=50), dict(pad=-1), dict(count=0), dict(count=65), dict(batch=1 << 40)):
         assert beam(**bad) == SHAPE
-    assert beam(wsb=0) == WORKSPACE and beam(batch=0) == 0 and lib.mp_beam_select_workspace_bytes(1, 65, 50, 6, 0) == 0
+    assert beam(wsb=0) == WORKSPACE and beam(batch=0) == 0 and lib.mp_beam_select_workspace_bytes(1, 65, 50, 6) == 0
 
 
 def test_the_reference_forms():
