@@ -102,8 +102,12 @@ struct Narrow {
   static constexpr int kItem = 16, kStep = 128, kSlack = 2, kFiner = INT_MAX;
 };
 // Parts that have others, in shares at most: an item of T > limit tiles has up to 2 T / (limit + 1), and with limit from two thirds of
-// a share e on, 2 (e + 1) / (2 e / 3 + 2) is below 3.  They are half as many more than the items that they replace.
+// a share e on, 2 (e + 1) / (2 e / 3 + 2) is below 3.
 constexpr int kSlots = 3;
+// How many more parts than items there are, at most: T / limit for an item that is cut, together (e + 1) / limit of a share, which is
+// below 1 with a limit above e and at most 14 / 9 (e = 13, limit 9) with the finer one, for which e >= kFiner.
+constexpr int64_t masked_more(int64_t share) { return share * 14 / 9 + 1; }
+static_assert(Wide::kFiner >= 12 && Narrow::kFiner >= 12, "(e + 1) / (2 e / 3 + 1) is more for e of 7 and 10");
 
 // What a workgroup takes: tiles of an item.
 template <int MODE>
@@ -676,7 +680,7 @@ int masked_start(const MaskedCall &c, int shift) {
       hipFuncSetAttribute(reinterpret_cast<const void *>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
     return MP_ERR_HIP;
   const mp_pages &p = *c.cache;
-  const int64_t blocks = (masked_items<FORM>(c.rows, grp, c.batch) + kSlots * share / 2 + 1) * c.kvh;
+  const int64_t blocks = (masked_items<FORM>(c.rows, grp, c.batch) + masked_more(share)) * c.kvh;
   hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), kLds, c.stream,
                      static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(p.k), p.k_page,
                      p.k_head, p.k_row, static_cast<const uint16_t *>(p.v), p.v_page, p.v_head, p.v_row, static_cast<int>(p.pages),

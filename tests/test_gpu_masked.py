@@ -178,6 +178,16 @@ def test_tree_runs_that_cut_items():
     _tree(k, v, table, ln, news, 8, BF16, _trees(news, 8), 1)
 
 
+def test_tree_long_and_alone():
+    """One sequence whose tiles make many more parts than there are items: one less than 17 equal shares of them, with the one that
+    the rows behind it have."""
+    shares = torch.cuda.get_device_properties(0).multi_processor_count  # two workgroups to a CU, two key-value heads
+    n = 64 * (17 * shares - 2)
+    k, v, table, ln = _cache([n], 2, 64, 64, BF16, 12)
+    v[table[0, -100:].long()] += 40  # of a part that is not there much is missing
+    _tree(k, v, table, ln, [3], 16, BF16, _trees([3], 6), 1)
+
+
 def test_far_pages_and_strided_queries():
     """Pools of more than 2^31 values: offsets pass 32 bits.  Only the pages used are written."""
     pages = (1 << 31) // (8 * 128 * 128) + 40
