@@ -109,6 +109,9 @@ constexpr int kSlots = 3;
 constexpr int64_t masked_more(int64_t share) { return share * 14 / 9 + 1; }
 static_assert(Wide::kFiner >= 12 && Narrow::kFiner >= 12, "(e + 1) / (2 e / 3 + 1) is more for e of 7 and 10");
 
+constexpr int64_t kMaxBatch = 1 << 28;
+constexpr int kPlanNear = 64;  // sequences, with the two that hold the other rows, which a wave sees at once
+
 // What a workgroup takes: tiles of an item.
 template <int MODE>
 struct MaskedPart {
@@ -125,6 +128,7 @@ struct MaskedPlan {
   const int32_t *lens;
   int capacity;  // positions that the table has room for
   MaskedRule rule;
+  const int32_t *plan;  // of masked_plan_kernel
 
   __device__ __forceinline__ MaskedSeq<MODE> seq(int b) const {
     MaskedSeq<MODE> s;
@@ -167,101 +171,183 @@ struct MaskedPlan {
     }
     return r;
   }
+  // How long parts may be, from all items' tiles.  each(f): f of every row; sum and most: over those who call it.  Items stay whole
+  // where none is much longer than an equal share.  Otherwise parts are as long as such an item, or two thirds of a share, as the
+  // longest part and the number of rounds have it (24 sequences of up to 8192 positions with trees of up to 64 nodes, 58 items of 1 to
+  // 129 tiles for 64 workgroups: 186 us, 152 with the finer ones).
+  template <class EACH, class SUM, class MOST>
+  static __device__ __forceinline__ int limit_of(uint32_t all, int share, EACH each, SUM sum, MOST most) {
+    const int equal = static_cast<int>(all / static_cast<uint32_t>(share)), keep = equal + min(equal / 2, FORM::kSlack) + 1;
+    if (equal < FORM::kFiner) return keep;
+    const int finer = equal * 2 / 3 + 1;
+    int took[2] = {0, 0};
+    for (int i = 0; i < 2; ++i) {
+      uint32_t count = 0;
+      int longest = 0;
+      each([&](const Row &r) {
+        const int in = parts(r, i ? finer : keep);
+        count += r.items * in;
+        longest = max(longest, r.items ? (r.tiles + in - 1) / in : 0);
+      });
+      longest = most(longest);
+      const int rounds = static_cast<int>((sum(count) + share - 1) / static_cast<uint32_t>(share));
+      took[i] = min(rounds * longest, equal + longest) + 2 * rounds;  // two tiles to start a part
+    }
+    return took[1] && took[1] < took[0] ? finer : keep;
+  }
+  static __device__ __forceinline__ int parts(const Row &r, int limit) {
+    return r.tiles > limit ? static_cast<int>(static_cast<uint32_t>(r.tiles + limit - 1) / static_cast<uint32_t>(limit)) : 1;
+  }
+  // Items in parts come first, then the whole ones, by halves.
+  static __device__ __forceinline__ int order(const Row &r, int limit) {
+    return r.tiles > limit ? 0 : 2 * r.tiles > limit ? 1 : 4 * r.tiles > limit ? 2 : 3;
+  }
+  // Part `at` of sequence b's items, whose number in all is `index`.  Uniform.
+  __device__ __forceinline__ void take(MaskedPart<MODE> &p, int b, int in, int at, int index) const {
+    p.b = b;
+    p.parts = in;
+    p.item = at;
+    p.part = 0;
+    p.slot = index;  // those in parts come first, below kSlots share
+    p.seq = seq(b);
+    p.seq.first = __builtin_amdgcn_readfirstlane(p.seq.first);
+    p.seq.n = __builtin_amdgcn_readfirstlane(p.seq.n);
+    p.seq.len = __builtin_amdgcn_readfirstlane(p.seq.len);
+    if (in > 1) {
+      p.item = at / in;
+      p.part = at - p.item * in;
+    }
+    span(p.seq, p.item, p.to, p.gap_from, p.gap);
+    p.from = 0;
+    p.end = p.to - p.gap;
+    if (in > 1) {  // the first ones take a tile more where they do not come out even
+      const int t = tiles(p.to, p.gap), each = t / in, more = t - each * in;
+      p.from = (p.part * each + min(p.part, more)) * FORM::kStep;
+      p.end = min(((p.part + 1) * each + min(p.part + 1, more)) * FORM::kStep, p.end);
+    }
+  }
   // The part that this workgroup, number `at` of its head's, takes.  `share`: workgroups of a head that the card holds at once;
-  // cut: how many of the parts have others.  Uniform; every wave looks at all sequences, one a lane.
+  // cut: how many of the parts have others.  Uniform; every wave looks at all sequences, one a lane, or where they are more at
+  // what masked_plan_kernel left.
   __device__ __forceinline__ bool find(int at, int share, MaskedPart<MODE> &p, uint32_t &cut) const {
     const int lane = threadIdx.x & 63, n = rows.batch + 2;
-    uint64_t held = 0, unused = 0;
-    const Row near = row(lane, held);
-    uint32_t all = near.items * near.tiles;
-    for (int b = lane + 64; b - lane < n; b += 64) {
-      const Row r = row(b, held);
-      all += r.items * r.tiles;
-    }
-    all = wave_sum(all);
     cut = 0;
+    if (n > kPlanNear) {
+      const int limit = plan[0];
+      cut = plan[1];
+      const int32_t *upto = plan + 2;  // running counts of parts, [order, sequence]
+      int lo = 0, size = 4 * n;
+      if (!limit || at >= upto[size - 1]) return false;
+      while (size > 1) {  // the first above `at`
+        const int step = (size + 63) / 64, i = min((lane + 1) * step, size) - 1;
+        const int l = __builtin_ctzll(__ballot(upto[lo + i] > at));
+        lo += l * step;
+        size = min(step, size - l * step);
+      }
+      uint64_t unused = 0;
+      const int b = lo % n, before = lo ? __builtin_amdgcn_readfirstlane(upto[lo - 1]) : 0;
+      take(p, b, __builtin_amdgcn_readfirstlane(parts(row(b, unused), limit)), at - before, at);
+      return true;
+    }
+    uint64_t held = 0;
+    const Row near = row(lane, held);
+    const uint32_t all = wave_sum(static_cast<uint32_t>(near.items * near.tiles));
     // offsets that do not ascend: the sequences' rows add up to more than there are
     if (wave_sum(held) != static_cast<uint64_t>(rows.rows)) return false;
-    // Items stay whole where none is much longer than an equal share.  Otherwise parts are as long as such an item, or two thirds of
-    // a share, as the longest part and the number of rounds have it (24 sequences of up to 8192 positions with trees of up to 64
-    // nodes, 58 items of 1 to 129 tiles for 64 workgroups: 186 us, 152 with the finer ones).
-    const int equal = static_cast<int>(all / static_cast<uint32_t>(share));
-    int limit = equal + min(equal / 2, FORM::kSlack) + 1;
-    const auto parts = [&](const Row &r) {
-      return r.tiles > limit ? static_cast<int>(static_cast<uint32_t>(r.tiles + limit - 1) / static_cast<uint32_t>(limit)) : 1;
-    };
-    if (equal >= FORM::kFiner) {
-      const int keep = limit;
-      int took[2] = {0, 0};
-      for (int i = 0; i < 2; ++i) {
-        limit = i ? equal * 2 / 3 + 1 : keep;
-        uint32_t count = near.items * parts(near);
-        int longest = near.items ? (near.tiles + parts(near) - 1) / parts(near) : 0;
-        for (int b = lane + 64; b - lane < n; b += 64) {
-          const Row r = row(b, unused);
-          count += r.items * parts(r);
-          longest = max(longest, r.items ? (r.tiles + parts(r) - 1) / parts(r) : 0);
-        }
+    const auto most = [](int x) {
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
-        const int rounds = static_cast<int>((wave_sum(count) + share - 1) / static_cast<uint32_t>(share));
-        took[i] = min(rounds * longest, equal + longest) + 2 * rounds;  // two tiles to start a part
+      for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
+      return x;
+    };
+    const int limit = limit_of(all, share, [&](auto f) { f(near); }, [](uint32_t x) { return wave_sum(x); }, most);
+    const int near_parts = parts(near, limit), mine = order(near, limit), index = at;
+    if (at == 0) cut = wave_sum(static_cast<uint32_t>(near_parts > 1 ? near.items * near_parts : 0));
+    for (int o = 0; o < 4; ++o) {
+      const int count = mine == o ? near.items * near_parts : 0;
+      const int upto = static_cast<int>(wave_scan(static_cast<uint32_t>(count)));
+      const uint64_t past = __ballot(upto > at);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        take(p, l, __builtin_amdgcn_readlane(near_parts, l),
+             at - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l)), index);
+        return true;
       }
-      limit = took[1] && took[1] < took[0] ? limit : keep;
-    }
-    const int near_parts = parts(near), index = at;
-    if (at == 0) {
-      uint32_t c = near_parts > 1 ? near.items * near_parts : 0;
-      for (int b = lane + 64; b - lane < n; b += 64) {
-        const Row r = row(b, unused);
-        c += r.tiles > limit ? r.items * parts(r) : 0;
-      }
-      cut = wave_sum(c);
-    }
-    for (int order = 0; order < 4; ++order) {  // those in parts, then the whole ones, by halves
-      for (int b0 = 0; b0 < n; b0 += 64) {
-        Row r = near;
-        int in = near_parts;
-        if (b0) {
-          r = row(b0 + lane, unused);
-          in = parts(r);
-        }
-        const int mine = r.tiles > limit ? 0 : 2 * r.tiles > limit ? 1 : 4 * r.tiles > limit ? 2 : 3;
-        const int count = mine == order ? r.items * in : 0;
-        const int upto = static_cast<int>(wave_scan(static_cast<uint32_t>(count)));
-        const uint64_t past = __ballot(upto > at);
-        if (past) {
-          const int l = __builtin_ctzll(past);
-          p.b = b0 + l;
-          p.parts = __builtin_amdgcn_readlane(in, l);
-          p.item = at - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l));
-          p.part = 0;
-          p.slot = index;  // those in parts come first, below kSlots share
-          p.seq = seq(p.b);
-          p.seq.first = __builtin_amdgcn_readfirstlane(p.seq.first);
-          p.seq.n = __builtin_amdgcn_readfirstlane(p.seq.n);
-          p.seq.len = __builtin_amdgcn_readfirstlane(p.seq.len);
-          if (p.parts > 1) {
-            at = p.item;
-            p.item = at / p.parts;
-            p.part = at - p.item * p.parts;
-          }
-          span(p.seq, p.item, p.to, p.gap_from, p.gap);
-          p.from = 0;
-          p.end = p.to - p.gap;
-          if (p.parts > 1) {  // the first ones take a tile more where they do not come out even
-            const int t = tiles(p.to, p.gap), each = t / p.parts, more = t - each * p.parts;
-            p.from = (p.part * each + min(p.part, more)) * FORM::kStep;
-            p.end = min(((p.part + 1) * each + min(p.part + 1, more)) * FORM::kStep, p.end);
-          }
-          return true;
-        }
-        at -= __builtin_amdgcn_readlane(upto, 63);
-      }
+      at -= __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
   }
 };
+
+// Of more sequences than a wave has lanes: the limit of parts (0: offsets that do not ascend), how many parts have others, and the
+// running counts of parts over orders and sequences.  One workgroup, before the others.  (Where each of them walked over all sequences
+// itself, trees of 4 nodes behind 496 positions, 32 / 8 heads, took 1599 us for 1024 sequences, and 409 with this; 194 and 113 for 256.)
+constexpr int kPlanThreads = 1024;
+template <int MODE, class FORM>
+__global__ __launch_bounds__(kPlanThreads) void masked_plan_kernel(const int32_t *__restrict__ starts, const int32_t *__restrict__ lens,
+                                                                   int batch, int rows, int grp, int capacity, MaskedRule rule,
+                                                                   int share, int32_t *__restrict__ out) {
+  using Plan = MaskedPlan<MODE, FORM>;
+  constexpr int kPlanWaves = kPlanThreads / 64;
+  __shared__ uint64_t of_wave[kPlanWaves];
+  const Plan plan{{starts, batch, rows, grp}, lens, capacity, rule, nullptr};
+  const int n = batch + 2, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const auto gather = [&](uint64_t x, auto join) {  // of_wave[w] for every wave
+    __syncthreads();  // what was there has been read
+    if (lane == 0) of_wave[wave] = x;
+    __syncthreads();
+    uint64_t y = of_wave[0];
+    for (int w = 1; w < kPlanWaves; ++w) y = join(y, of_wave[w]);
+    return y;
+  };
+  const auto sum = [&](uint64_t x) { return gather(wave_sum(x), [](uint64_t p, uint64_t q) { return p + q; }); };
+  const auto most = [&](int x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
+    return static_cast<int>(gather(static_cast<uint64_t>(x), [](uint64_t p, uint64_t q) { return max(p, q); }));
+  };
+  uint64_t held = 0, unused = 0;
+  const typename Plan::Row near = plan.row(threadIdx.x, held);
+  uint32_t own = near.items * near.tiles;
+  for (int b = threadIdx.x + kPlanThreads; b < n; b += kPlanThreads) {
+    const typename Plan::Row r = plan.row(b, held);
+    own += r.items * r.tiles;
+  }
+  const uint32_t all = static_cast<uint32_t>(sum(own));
+  if (sum(held) != static_cast<uint64_t>(rows)) {
+    if (threadIdx.x == 0) out[0] = out[1] = 0;
+    return;
+  }
+  const auto each = [&](auto f) {
+    f(near);
+    for (int b = threadIdx.x + kPlanThreads; b < n; b += kPlanThreads) f(plan.row(b, unused));
+  };
+  const int limit = Plan::limit_of(all, share, each, [&](uint32_t x) { return static_cast<uint32_t>(sum(x)); }, most);
+  uint32_t before = 0, cut = 0;
+  for (int o = 0; o < 4; ++o) {
+    for (int b0 = 0; b0 < n; b0 += kPlanThreads) {
+      const int b = b0 + threadIdx.x;
+      const typename Plan::Row r = b0 ? plan.row(b, unused) : near;
+      const uint32_t upto = wave_scan(static_cast<uint32_t>(Plan::order(r, limit) == o ? r.items * Plan::parts(r, limit) : 0));
+      __syncthreads();  // what was there has been read
+      if (lane == 63) of_wave[wave] = upto;
+      __syncthreads();
+      uint32_t ahead = 0, total = 0;
+      for (int w = 0; w < kPlanWaves; ++w) {
+        ahead += w < wave ? static_cast<uint32_t>(of_wave[w]) : 0;
+        total += static_cast<uint32_t>(of_wave[w]);
+      }
+      if (b < n) out[2 + o * n + b] = static_cast<int32_t>(before + ahead + upto);
+      before += total;
+    }
+    if (o == 0) cut = before;
+  }
+  if (threadIdx.x == 0) {
+    out[0] = limit;
+    out[1] = static_cast<int32_t>(cut);
+  }
+}
+// Its words, if it runs.
+constexpr int64_t masked_plan_words(int64_t batch) { return batch + 2 > kPlanNear ? 2 + 4 * (batch + 2) : 0; }
 
 // Where an item's parts and its outputs go.
 struct MaskedOut {
@@ -358,13 +444,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void masked_wide_ker
     int64_t khead, int64_t krow, const uint16_t *__restrict__ v, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
     int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
     const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, MaskedRule rule, int share, int slot_rows,
-    float scale2, uint32_t flip, float *__restrict__ parts, int4 *__restrict__ joins, uint16_t *__restrict__ out) {
+    float scale2, uint32_t flip, const int32_t *__restrict__ planned, float *__restrict__ parts, int4 *__restrict__ joins,
+    uint16_t *__restrict__ out) {
   using T = PromptTile<D>;
   constexpr int kStage = T::kStage, kS = kTile / 32;
   extern __shared__ __attribute__((aligned(1024))) int8_t masked_smem[];  // two stages of K and V
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i32 = lane & 31, h = lane >> 5;
   const int kh = blockIdx.x % kvh;
-  const MaskedPlan<MODE, Wide> plan{{starts, batch, rows, grp}, lens, width << shift, rule};
+  const MaskedPlan<MODE, Wide> plan{{starts, batch, rows, grp}, lens, width << shift, rule, planned};
   MaskedPart<MODE> p;
   if (!masked_find(plan, kvh, kh, share, joins, p)) return;
   const MaskedSeq<MODE> &seq = p.seq;
@@ -525,11 +612,12 @@ __global__ __launch_bounds__(64 * kWaves, masked_round(D)) void masked_narrow_ke
     int64_t khead, int64_t krow, const uint16_t *__restrict__ v, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
     int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens,
     const int32_t *__restrict__ starts, int batch, int rows, int kvh, int grp, MaskedRule rule, int share, int slot_rows,
-    float scale2, uint32_t flip, float *__restrict__ parts, int4 *__restrict__ joins, uint16_t *__restrict__ out) {
+    float scale2, uint32_t flip, const int32_t *__restrict__ planned, float *__restrict__ parts, int4 *__restrict__ joins,
+    uint16_t *__restrict__ out) {
   extern __shared__ __attribute__((aligned(16))) float narrow_smem[];  // the four waves' states (attn_meet)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, j = lane >> 4;
   const int kh = blockIdx.x % kvh;
-  const MaskedPlan<MODE, Narrow> plan{{starts, batch, rows, grp}, lens, width << shift, rule};
+  const MaskedPlan<MODE, Narrow> plan{{starts, batch, rows, grp}, lens, width << shift, rule, planned};
   MaskedPart<MODE> p;
   if (!masked_find(plan, kvh, kh, share, joins, p)) return;
   const MaskedSeq<MODE> &seq = p.seq;
@@ -652,15 +740,16 @@ struct MaskedCall {
 };
 
 template <class FORM>
-size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim) {
+size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim, int64_t batch) {
   const int64_t grp = nh / kvh;
   const int64_t slots = kSlots * masked_share<FORM>(kvh, dim) * kvh;
   return static_cast<size_t>(1 + slots) * sizeof(int4) +
-         static_cast<size_t>(slots * masked_slot_rows<FORM>(rows, grp)) * (dim + 2) * sizeof(float);
+         static_cast<size_t>(slots * masked_slot_rows<FORM>(rows, grp)) * (dim + 2) * sizeof(float) +
+         static_cast<size_t>(masked_plan_words(batch)) * sizeof(int32_t);
 }
 size_t masked_workspace(int64_t rows, int64_t nh, int64_t kvh, int dim, int64_t batch, int64_t reach) {
-  return masked_narrow(rows, nh / kvh, kvh, dim, batch, reach) ? masked_workspace<Narrow>(rows, nh, kvh, dim)
-                                              : masked_workspace<Wide>(rows, nh, kvh, dim);
+  return masked_narrow(rows, nh / kvh, kvh, dim, batch, reach) ? masked_workspace<Narrow>(rows, nh, kvh, dim, batch)
+                                                               : masked_workspace<Wide>(rows, nh, kvh, dim, batch);
 }
 
 template <int D, int DT, int MODE, class FORM>
@@ -670,6 +759,7 @@ int masked_start(const MaskedCall &c, int shift) {
   const int slot_rows = static_cast<int>(masked_slot_rows<FORM>(c.rows, grp));
   int4 *joins = static_cast<int4 *>(c.workspace);
   float *parts = reinterpret_cast<float *>(joins + 1 + kSlots * static_cast<int64_t>(share) * c.kvh);
+  int32_t *planned = reinterpret_cast<int32_t *>(parts + kSlots * static_cast<int64_t>(share) * c.kvh * slot_rows * (D + 2));
   // the sign of the scale goes to the queries, so that the largest product gives the largest score; a scale of 0 becomes the
   // smallest normal number, which leaves every finite score 0 and a masked one -inf
   const uint32_t flip = c.scale < 0.f ? 0x80008000u : 0u;
@@ -680,12 +770,17 @@ int masked_start(const MaskedCall &c, int shift) {
       hipFuncSetAttribute(reinterpret_cast<const void *>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
     return MP_ERR_HIP;
   const mp_pages &p = *c.cache;
+  if (masked_plan_words(c.batch)) {
+    hipLaunchKernelGGL((masked_plan_kernel<MODE, FORM>), dim3(1), dim3(kPlanThreads), 0, c.stream, c.starts, c.lens,
+                       static_cast<int>(c.batch), static_cast<int>(c.rows), grp, static_cast<int>(p.width << shift), c.rule, share, planned);
+    MP_CHECK_LAUNCH();
+  }
   const int64_t blocks = (masked_items<FORM>(c.rows, grp, c.batch) + masked_more(share)) * c.kvh;
   hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), kLds, c.stream,
                      static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(p.k), p.k_page,
                      p.k_head, p.k_row, static_cast<const uint16_t *>(p.v), p.v_page, p.v_head, p.v_row, static_cast<int>(p.pages),
                      shift, p.table, static_cast<int>(p.width), c.lens, c.starts, static_cast<int>(c.batch),
-                     static_cast<int>(c.rows), c.kvh, grp, c.rule, share, slot_rows, scale2, flip, parts, joins,
+                     static_cast<int>(c.rows), c.kvh, grp, c.rule, share, slot_rows, scale2, flip, planned, parts, joins,
                      static_cast<uint16_t *>(c.out));
   MP_CHECK_LAUNCH();
   if (c.reach > FORM::kStep) {  // else items of one tile, which are never cut
@@ -712,7 +807,7 @@ int masked_launch(MaskedCall c) {
   for (int s = 3; s < 16; ++s)
     if (p.page_size == 1 << s) shift = s;
   if (shift < 0 || p.pages < 1 || p.pages > INT32_MAX || p.width < 1 || p.width > (1 << 30) >> shift) return MP_ERR_SHAPE;
-  if (c.rows < 0 || c.rows > INT32_MAX || c.batch < 1 || c.batch > INT32_MAX - 64) return MP_ERR_SHAPE;
+  if (c.rows < 0 || c.rows > INT32_MAX || c.batch < 1 || c.batch > kMaxBatch) return MP_ERR_SHAPE;
   if (c.nh < 1 || c.kvh < 1 || c.nh > 65536 || c.nh % c.kvh) return MP_ERR_SHAPE;
   if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return MP_ERR_SHAPE;
   for (int64_t s : {c.q_row, c.q_head, p.k_page, p.k_head, p.k_row, p.v_page, p.v_head, p.v_row})
@@ -742,8 +837,8 @@ int masked_launch(MaskedCall c) {
 
 extern "C" size_t mp_masked_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch, int64_t capacity,
                                             int64_t window, int64_t sinks) {
-  if (rows <= 0 || rows > INT32_MAX || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || batch <= 0 || batch > INT32_MAX ||
-      capacity <= 0 || window < 0 || sinks < 0 || mp_cu_count() <= 0)
+  if (rows <= 0 || rows > INT32_MAX || nh <= 0 || kvh <= 0 || nh % kvh || head_dim <= 0 || batch <= 0 || batch > kMaxBatch ||
+      capacity <= 0 || window < 0 || window > 1 << 30 || sinks < 0 || sinks > 1 << 30 || mp_cu_count() <= 0)
     return 0;
   return masked_workspace(rows, nh, kvh, head_dim, batch, masked_reach(capacity, window, sinks));
 }

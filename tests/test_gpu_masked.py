@@ -171,6 +171,25 @@ def test_tree_many_sequences():
     _tree(k, v, table, ln, news, 2, BF16, _trees(news, 6), 1)
 
 
+@pytest.mark.parametrize("count", [61, 62, 63, 64, 130, 1021, 1022, 1023, 2100])
+def test_any_number_of_sequences(count):
+    """Sequences of many lengths, one of them so long that it is cut, in trees of few rows and of many, and with windows."""
+    g = random.Random(count)
+    news = [g.choice((0, 0, 1, 2)) for _ in range(count)]
+    ctxs = [g.randrange(0, 20) for _ in news]
+    at = (count - 1, count // 2, 0)
+    for b, n, c in zip(at, (40, 3, 0), (5000, 0, 900)):
+        news[b], ctxs[b] = n, c
+    k, v, table, ln = _cache([a + b for a, b in zip(news, ctxs)], 1, 64, 16, F16, 7)
+    _tree(k, v, table, ln, news, 2, F16, _trees(news, 8), 1)
+    _tree(k, v, table, ln, news, 70, F16, _trees(news, 8), 1)  # more rows to a sequence
+    q = _queries(sum(news) + 1, 2, 64, F16)
+    starts = _ints(_starts(news))
+    got = _ops().paged_prompt_window_attention(q, k, v, table, ln, starts, 0.125, 30, 4)
+    want, tol = mref.masked_attention(q, k, v, table, ln, starts, mref.in_window(30, 4), 0.125)
+    ref.check(got, want, tol)
+
+
 def test_tree_runs_that_cut_items():
     """Long and short sequences with several row tiles each: runs begin and end inside of items."""
     news, ctxs = [40, 64, 2, 33], [4000, 100, 1500, 0]
