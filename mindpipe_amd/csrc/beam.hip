@@ -467,7 +467,7 @@ extern "C" int mp_beam_select(const void *logits, int64_t stride, int64_t batch,
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define MP_BEAM(DT)                                                                                                        \
   do {                                                                                                                     \
-    if (h == 8) beam_rows_launch<DT, 8>(logits, stride, rows, n, ended, splits, k, parts, lists, s);                  \
+    if (h == 8) beam_rows_launch<DT, 8>(logits, stride, rows, n, ended, splits, k, parts, lists, s);                       \
     else if (h == 4) beam_rows_launch<DT, 4>(logits, stride, rows, n, ended, splits, k, parts, lists, s);                  \
     else beam_rows_launch<DT, 2>(logits, stride, rows, n, ended, splits, k, parts, lists, s);                              \
   } while (0)

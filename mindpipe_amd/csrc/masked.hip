@@ -772,7 +772,8 @@ int masked_start(const MaskedCall &c, int shift) {
   const mp_pages &p = *c.cache;
   if (masked_plan_words(c.batch)) {
     hipLaunchKernelGGL((masked_plan_kernel<MODE, FORM>), dim3(1), dim3(kPlanThreads), 0, c.stream, c.starts, c.lens,
-                       static_cast<int>(c.batch), static_cast<int>(c.rows), grp, static_cast<int>(p.width << shift), c.rule, share, planned);
+                       static_cast<int>(c.batch), static_cast<int>(c.rows), grp, static_cast<int>(p.width << shift), c.rule, share,
+                       planned);
     MP_CHECK_LAUNCH();
   }
   const int64_t blocks = (masked_items<FORM>(c.rows, grp, c.batch) + masked_more(share)) * c.kvh;

@@ -137,7 +137,8 @@ struct DecodePlan {
     DecodeSeen s;
     s.len = len(b);
     s.sinks = sinks;
-    s.low = min(max(lens[b], 0) - min(window, max(lens[b], 0)), capacity);  // the window ends at the sequence's end, whatever the table holds
+    // the window ends at the sequence's end, whatever the table holds
+    s.low = min(max(lens[b], 0) - min(window, max(lens[b], 0)), capacity);
     const int low = min(s.low, s.len) & ~31;
     s.gap_from = min((min(sinks, s.len) + 31) & ~31, low);
     s.gap = low - s.gap_from;
@@ -170,8 +171,8 @@ __global__ __launch_bounds__(64 * kWaves, decode_round(D)) void paged_decode_ker
     const uint16_t *__restrict__ q, int64_t q_row, int64_t q_head, const uint16_t *__restrict__ k_pages, int64_t kpage,
     int64_t khead, int64_t krow, const uint16_t *__restrict__ v_pages, int64_t vpage, int64_t vhead, int64_t vrow, int pages,
     int shift, const int32_t *__restrict__ table, int width, const int32_t *__restrict__ lens, int batch, int kvh, int grp,
-    int tiles, int share, int window, int sinks, float scale2, float *__restrict__ part_o, float *__restrict__ part_ml, int4 *__restrict__ joins,
-    uint16_t *__restrict__ out) {
+    int tiles, int share, int window, int sinks, float scale2, float *__restrict__ part_o, float *__restrict__ part_ml,
+    int4 *__restrict__ joins, uint16_t *__restrict__ out) {
   extern __shared__ __attribute__((aligned(16))) float sm[];  // the four waves' states (attn_meet)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, j = lane >> 4;
   const int heads = kvh * tiles, h = blockIdx.x % heads, kh = h / tiles, run = blockIdx.x / heads;
@@ -375,24 +376,25 @@ int decode_launch(const void *q, int64_t q_row, int64_t q_head, int64_t batch, i
   const float scale2 = scale * kLog2e;
   const int lds = attn_meet_bytes(head_dim, kWaves, per);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define MP_DECODE(D, DT)                                                                                                  \
-  do {                                                                                                                    \
-    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(paged_decode_kernel<D, DT, WIN>),               \
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)            \
-      return MP_ERR_HIP;                                                                                                  \
-    hipLaunchKernelGGL((paged_decode_kernel<D, DT, WIN>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),              \
-                       lds, s, static_cast<const uint16_t *>(q), q_row, q_head,        \
-                       static_cast<const uint16_t *>(cache->k), cache->k_page, cache->k_head, cache->k_row,               \
-                       static_cast<const uint16_t *>(cache->v), cache->v_page, cache->v_head, cache->v_row,               \
-                       static_cast<int>(cache->pages), shift, cache->table, static_cast<int>(cache->width), lens,         \
-                       static_cast<int>(batch), kvh, grp, tiles, static_cast<int>(share), window, sinks, scale2, part_o, part_ml, joins,                    \
-                       static_cast<uint16_t *>(out));                                                                     \
-    MP_CHECK_LAUNCH();                                                                                                    \
-    if (capacity > kBlock) { /* else every sequence is one block */                                                       \
-      hipLaunchKernelGGL((paged_decode_join_kernel<D, DT>), dim3(static_cast<unsigned>(batch * nh)), dim3(256), 0, s,     \
-                         static_cast<int>(heads), kvh, grp, part_o, part_ml, joins, static_cast<uint16_t *>(out));        \
-      MP_CHECK_LAUNCH();                                                                                                  \
-    }                                                                                                                     \
+#define MP_DECODE(D, DT)                                                                                                \
+  do {                                                                                                                  \
+    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(paged_decode_kernel<D, DT, WIN>),         \
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)          \
+      return MP_ERR_HIP;                                                                                                \
+    hipLaunchKernelGGL((paged_decode_kernel<D, DT, WIN>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),       \
+                       lds, s, static_cast<const uint16_t *>(q), q_row, q_head,                                         \
+                       static_cast<const uint16_t *>(cache->k), cache->k_page, cache->k_head, cache->k_row,             \
+                       static_cast<const uint16_t *>(cache->v), cache->v_page, cache->v_head, cache->v_row,             \
+                       static_cast<int>(cache->pages), shift, cache->table, static_cast<int>(cache->width), lens,       \
+                       static_cast<int>(batch), kvh, grp, tiles, static_cast<int>(share), window, sinks, scale2, part_o,\
+                       part_ml, joins,                                                                                  \
+                       static_cast<uint16_t *>(out));                                                                   \
+    MP_CHECK_LAUNCH();                                                                                                  \
+    if (capacity > kBlock) { /* else every sequence is one block */                                                     \
+      hipLaunchKernelGGL((paged_decode_join_kernel<D, DT>), dim3(static_cast<unsigned>(batch * nh)), dim3(256), 0, s,   \
+                         static_cast<int>(heads), kvh, grp, part_o, part_ml, joins, static_cast<uint16_t *>(out));      \
+      MP_CHECK_LAUNCH();                                                                                                \
+    }                                                                                                                   \
   } while (0)
   if (dtype == MP_F16) {
     if (head_dim == 64) MP_DECODE(64, MP_F16);

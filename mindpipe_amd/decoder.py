@@ -293,7 +293,7 @@ def lookup_draft(match: int = 2, nodes: int = 8, branches: int = 2) -> Callable[
     def draft(tokens: List[int]) -> Tuple[List[int], List[int]]:
         found: List[int] = []
         parents: List[int] = []
-        places = [i for i in range(len(tokens) - match - 1, -1, -1) if tokens[i:i + match] == tokens[-match:]] if match < len(tokens) else []
+        places = [i for i in range(len(tokens) - match - 1, -1, -1) if tokens[i:i + match] == tokens[-match:]]
         for i in places[:branches]:
             node = -1
             for t in tokens[i + match:i + match + max(1, nodes // branches)]:
