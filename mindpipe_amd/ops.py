@@ -1444,12 +1444,12 @@ def _move_pools(k_pages: torch.Tensor, v_pages: torch.Tensor, table: Optional[to
         ndim = 4
     _need_strided(k_pages, "k_pages", _HALF, ndim)
     _need_strided(v_pages, "v_pages", k_pages.dtype, ndim)
-    if v_pages.shape != k_pages.shape:
-        raise RuntimeError(f"v_pages {tuple(v_pages.shape)} must have the shape of k_pages {tuple(k_pages.shape)}")
+    shape = k_pages.shape
+    if v_pages.shape != shape:
+        raise RuntimeError(f"v_pages {tuple(v_pages.shape)} must have the shape of k_pages {tuple(shape)}")
     if v_pages.device != k_pages.device:
         _same_device(k_pages, v_pages=v_pages)
-    pages, kvh, size, dim = k_pages.shape[-4:]
-    layers = k_pages.shape[0] if ndim == 5 else 1
+    layers, pages, kvh, size, dim = shape if ndim == 5 else (1, *shape)
     if size < 8 or size > 32768 or size & (size - 1):
         raise RuntimeError(f"a page holds a power of two of positions from 8 to 32768, got {size}")
     if dim % 8 or not 8 <= dim <= 1024:
@@ -1457,7 +1457,7 @@ def _move_pools(k_pages: torch.Tensor, v_pages: torch.Tensor, table: Optional[to
     if not pages or not kvh or not layers:
         raise RuntimeError("k_pages and v_pages must hold at least one layer, page and head")
     ks, vs = _steps(k_pages), _steps(v_pages)
-    if any(n > 1 and not s for t, steps in ((k_pages, ks), (v_pages, vs)) for n, s in zip(t.shape, steps)):
+    if (0 in ks or 0 in vs) and any(n > 1 and not s for steps in (ks, vs) for n, s in zip(shape, steps)):
         raise RuntimeError("k_pages and v_pages are written to: no two of their values may lie in one place")
     address, width = (0, 0) if table is None else (table.data_ptr(), table.shape[1])
     cache = _lib.PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), *ks[-4:-1], *vs[-4:-1], pages, size, address, width)
@@ -1571,8 +1571,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int, ended: O
         if ended.shape != scores.shape:
             raise RuntimeError(f"ended {tuple(ended.shape)} must have the shape of scores {tuple(scores.shape)}")
     best = scores.new_empty((batch, count))
-    parents = torch.empty((batch, count), dtype=torch.int64, device=logits.device)
-    tokens = torch.empty((batch, count), dtype=torch.int64, device=logits.device)
+    parents = scores.new_empty((batch, count), dtype=torch.int64)
+    tokens = scores.new_empty((batch, count), dtype=torch.int64)
     if batch:
         lib = _lib.load()
         with _dev(logits):
