@@ -664,6 +664,8 @@ class W4Decoder:
         lengths = [len(h) for h in history]
         if not lengths or min(lengths) < 1 or new_tokens < 1:
             raise ValueError("prompts must hold a token at least, and new_tokens must be positive")
+        if self.cfg.window:
+            raise RuntimeError("trees are verified without a window")
         if cache is None:
             page, spare = 64, 64
             cache = self.paged_cache(len(prompts), sum(-(-(n + new_tokens + spare) // page) * page for n in lengths), page)

@@ -237,3 +237,11 @@ def test_tree_refusals():
             model.forward_tree(t, cache, parents)
     with pytest.raises(ValueError, match="tokens"):
         model.forward_tree(t.view(1, 5), cache, [[-1, 0, 0], [-1, 0]])
+
+
+def test_drafts_with_a_window_are_refused_before_they_begin():
+    model = _model(4, 4, window=16)
+    cache = model.paged_cache(1, 64, 64)
+    with pytest.raises(RuntimeError, match="window"):
+        model.generate_drafted(_tokens(5), 3, cache=cache)
+    assert cache.length == [0]
