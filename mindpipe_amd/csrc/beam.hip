@@ -4,14 +4,15 @@
 //   the `count` largest totals of a request, from the largest down; of equal ones those of the lowest beam, then token
 //
 // Which of two totals is larger decides a whole number, so they are made in 64 bits: the order inside of a row is that of its
-// logits, and between rows the sums of exponentials decide, each off by less than 2^-34 of itself.
+// logits, and between rows the sums of exponentials decide, each off by less than 2^-39 of what its other values add to the largest
+// one's 1, and by the roundings of some hundred additions, 2^-45.
 //
 // Two launches.  Of each row, workgroups take a part of the vocabulary each (a row is read once and stays in registers): they leave
 // the part's maximum, its sum of exponentials and its `count` largest values in order.  No value can be among a request's best
 // that is not among those.  Then a workgroup a request puts the best of its lists in order.
 //
-// Bound by vector instructions, 26 for a value, of which the exponential in 64 bits (as fast as 32 bits here) is 17: 48 requests of 8
-// beams over 128256 bf16, 98 MB, 46 us, and the merge 11, where the reads alone would take 15.  One request of 4 over 32000: 6.2 and 8.4.
+// Bound by vector instructions, 27 for a value, of which the exponential in 64 bits (as fast as 32 bits here) is 18: 48 requests of 8
+// beams over 128256 bf16, 98 MB, 47 us, and the merge 10, where the reads alone would take 15.  One request of 4 over 32000: 6.2 and 8.4.
 #include "logits.h"
 
 namespace {
@@ -22,19 +23,22 @@ constexpr int kBeamListed = 512;               // candidates of a part that LDS 
 constexpr double kLog2eD = 1.4426950408889634;
 
 // exp(d) for d from -690 to 0, in 64 bits (below -kBeamLost, 2^-865, no part of a sum): 2^n from the whole part of d log2 e and 2^r,
-// r in [-1/2, 1/2], by the polynomial of degree seven that is off by the least share there, 2^-34.5.
+// r in [-1/2, 1/2], by the polynomial of degree eight that is 1 at 0 and otherwise off by the least share there, 2^-39.7.  A row's
+// largest value so counts as 1: where nothing else has weight the logarithm of the sum is 0, and a certain token's total is its
+// beam's score.  (Degree seven is off by 2^-34.5 where its constant term is free, and makes that token likelier than 1.)
 constexpr float kBeamLost = 600.f;
 __device__ __forceinline__ double beam_exp(double d) {
   const double magic = 1.5 * 0x1p52;  // a sum with it is whole
   const double t = fma(d, kLog2eD, magic), r = fma(d, kLog2eD, magic - t);
-  double p = 1.5201921594169677e-05;
-  p = fma(p, r, 0.00015469291141683767);
-  p = fma(p, r, 0.001333392256354045);
-  p = fma(p, r, 0.00961802725366847);
-  p = fma(p, r, 0.05550410353447978);
-  p = fma(p, r, 0.24022651198157585);
-  p = fma(p, r, 0.693147180728447);
-  p = fma(p, r, 0.9999999999616819);
+  double p = 1.3344183484134179e-06;
+  p = fma(p, r, 1.5314209223349525e-05);
+  p = fma(p, r, 0.0001540309828656179);
+  p = fma(p, r, 0.0013333434157560176);
+  p = fma(p, r, 0.009618129558838935);
+  p = fma(p, r, 0.05550410959228811);
+  p = fma(p, r, 0.2402265069474259);
+  p = fma(p, r, 0.6931471805412327);
+  p = fma(p, r, 1.0);
   return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));  // no underflow: n is above -1000
 }
 struct BeamPart {  // of a part of a row: its largest value and sum_v exp(x_v - top); top +inf: how many such values
