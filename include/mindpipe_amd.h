@@ -500,6 +500,9 @@ int mp_paged_prompt_attention(const void *q, int64_t q_row, int64_t q_head, int6
  * 0 for a tree), 16-byte aligned, not shared by calls that may run at once.  Offsets that do not ascend leave the outputs open. */
 size_t mp_masked_workspace_bytes(int64_t rows, int nh, int kvh, int head_dim, int64_t batch, int64_t capacity, int64_t window,
                                  int64_t sinks);
+/* How many rows (tokens times heads that share a key-value head) a workgroup of such a call takes at a time, 16 or 128, which the same
+ * numbers decide; 0 where there is no such call. */
+int mp_masked_item_rows(int64_t rows, int nh, int kvh, int head_dim, int64_t batch, int64_t capacity, int64_t window, int64_t sinks);
 int mp_paged_tree_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh, int head_dim,
                             const mp_pages *cache, const int32_t *lens, const int32_t *starts, int64_t batch,
                             const int64_t *masks, int64_t words, float scale, void *out, int dtype, void *workspace,

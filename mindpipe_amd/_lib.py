@@ -96,6 +96,7 @@ SIGNATURES = {
     "mp_paged_decode_window_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i64, _i64, C.c_float, _vp,
                                                 _i32, _vp, _sz, _vp]),
     "mp_masked_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64]),
+    "mp_masked_item_rows": (_i32, [_i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64]),
     "mp_paged_tree_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp, _i64, C.c_float, _vp,
                                        _i32, _vp, _sz, _vp]),
     "mp_paged_prompt_window_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i64,

@@ -706,20 +706,25 @@ int64_t masked_items(int64_t rows, int64_t grp, int64_t batch) {
 int64_t masked_reach(int64_t capacity, int64_t window, int64_t sinks) {
   return window ? std::min(capacity, window + sinks + 3 * 64) : capacity;
 }
-// Narrow: few rows of a sequence and key-value head, on the average, for the positions of an item are read once and again by
-// every 16 rows; or little work in all, counted in rounds of narrow tiles, which start sooner.  Trees of bf16, us in the narrow and
-// the wide form, by rows of a sequence and head:
+// Narrow: little work in all, counted in rounds of narrow tiles, which start sooner, though every 16 rows read an item's positions
+// again; or few rows of a sequence and key-value head on the average, if it were little work with all rows in one of them, for the
+// host does not know which sequences have new tokens.  Trees of bf16, us in the narrow and the wide form, by rows of a sequence and
+// head:
 //   one sequence of 1500, 32 / 8 heads of 128      64: 15, 22   256: 22, 35 (6 rounds)
 //   one of 16000, 64 / 8                           64: 37, 44 (18)  128: 54, 56 (27)  192: 69, 47
 //   16 of 3000, 64 / 8                             16: 39, 40   32: 41, 42         64: 66, 45 (39)
-//   64 of 2000, 64 / 8                              8: 103, 108  32: 129, 113      64: 191, 117
+//   64 of 2000, 64 / 8                              8: 102, 113  16: 104, 113   32: 123, 114   64: 189, 119
 //   4 of 2000, 16 / 4 heads of 256                128: 39, 45 (14)                192: 68, 42 (19)
-//   32 of 3000, 8 / 8 heads of 256                 16: 153, 191  24: 191, 193      48: 258, 199
+//   32 of 3000, 8 / 8 heads of 256                 4: 147, 157  16: 150, 157   24: 191, 193      48: 258, 199
+//   64 of 1000, 32 / 8 heads of 64                  4: 33, 41   16: 34, 41     32: 40, 41
 //   16 of 2000, 28 / 4 heads of 64                 28: 15, 18                     56: 22, 20 (7)
+// New tokens of one sequence among 64 that the call names, behind 8000 positions, 32 / 8 heads of 128:
+//                                                128: 42, 65  256: 59, 48   512: 94, 54   2048: 317, 105
 bool masked_narrow(int64_t rows, int64_t grp, int64_t kvh, int dim, int64_t batch, int64_t reach) {
   const int64_t slots = masked_round(dim) * mp_cu_count(), rounds = dim == 64 ? 4 : dim == 128 ? 18 : 12;
   const int64_t tiles = mp_cdiv(reach, Narrow::kStep) + 6;  // an item starts and ends in the time of six
-  return rows * grp <= 32 * batch || masked_items<Narrow>(rows, grp, batch) * tiles * kvh <= rounds * slots;
+  const int64_t items = rows * grp <= 32 * batch ? mp_cdiv(rows * grp, Narrow::kItem) : masked_items<Narrow>(rows, grp, batch);
+  return items * tiles * kvh <= rounds * slots;
 }
 
 struct MaskedCall {
@@ -842,6 +847,12 @@ extern "C" size_t mp_masked_workspace_bytes(int64_t rows, int nh, int kvh, int h
       capacity <= 0 || window < 0 || window > 1 << 30 || sinks < 0 || sinks > 1 << 30 || mp_cu_count() <= 0)
     return 0;
   return masked_workspace(rows, nh, kvh, head_dim, batch, masked_reach(capacity, window, sinks));
+}
+
+extern "C" int mp_masked_item_rows(int64_t rows, int nh, int kvh, int head_dim, int64_t batch, int64_t capacity, int64_t window,
+                                   int64_t sinks) {
+  if (!mp_masked_workspace_bytes(rows, nh, kvh, head_dim, batch, capacity, window, sinks)) return 0;
+  return masked_narrow(rows, nh / kvh, kvh, head_dim, batch, masked_reach(capacity, window, sinks)) ? Narrow::kItem : Wide::kItem;
 }
 
 extern "C" int mp_paged_tree_attention(const void *q, int64_t q_row, int64_t q_head, int64_t rows, int nh, int kvh, int head_dim,
