@@ -203,9 +203,10 @@ struct SeenUpTo {
 // One tile into the rows' state.  Rows that see nothing of the tile are left as they are, whatever its masked places hold: masked scores
 // become -inf, V rows that no row sees are cleared, and a tile whose V has an infinity or NaN where only some rows see it
 // is added position by position, to those rows alone (0 times an infinity is no zero).  APART: rows see different positions.
-// Otherwise the second product takes the weights and then what their rounding leaves, so that they count with 16 (bf16) or 22
-// bits.  That rest may be 0 or negative, which beside an infinity gives NaN: a tile whose V has one takes halves of the weights.
-template <int D, int DT, bool APART, class Seen>
+// REST: the second product takes the weights and then what their rounding leaves, so that they count with 16 (bf16) or 22
+// bits.  That rest may be 0 or negative, which beside an infinity gives NaN: a tile whose V has one takes halves of the weights
+// twice, and one that is added position by position takes them once, as they are rounded.
+template <int D, int DT, bool APART, bool REST, class Seen>
 __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const uint4 (&q)[D / 32], int tile, const Seen &seen,
                                           float scale2, int lane) {
   const int j = lane >> 4, p0 = tile + 8 * j;
@@ -247,14 +248,14 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
     for (int c = 0; c < D / 16; ++c) a.o[c] *= f;
   }
   bool odd = false;  // an infinity or NaN in V
-  if constexpr (!APART) {
+  if constexpr (REST) {
     au2_t most = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int c = 0; c < D / 32; ++c)
         most = __builtin_elementwise_max(most, __builtin_bit_cast(au2_t, t.v[i][c] & 0x7FFF7FFFu));
-    odd = __any(max(most.x, most.y) >= (DT == MP_F16 ? 0x7C00 : 0x7F80));
+    odd = !apart && __any(max(most.x, most.y) >= (DT == MP_F16 ? 0x7C00 : 0x7F80));
   }
   const float base = (a.m == -INFINITY ? 0.f : a.m - kRaise<DT>) + (odd ? 1.f : 0.f);
   float p[8];
@@ -271,7 +272,7 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
                       __builtin_amdgcn_perm(t.v[5][c / 2], t.v[4][c / 2], sel),
                       __builtin_amdgcn_perm(t.v[7][c / 2], t.v[6][c / 2], sel));
   };
-  if constexpr (!APART) {
+  if (REST && !apart) {
     uint4 rest = make_uint4(attn_rest2<DT>(w.x, p[0], p[1]), attn_rest2<DT>(w.y, p[2], p[3]), attn_rest2<DT>(w.z, p[4], p[5]),
                             attn_rest2<DT>(w.w, p[6], p[7]));
     if (odd) rest = w;
@@ -316,7 +317,7 @@ __device__ __forceinline__ void attn_tile(AttnRows<D> &a, KvTile<D> &t, const ui
 
 // Tiles first, first + step, ... below `to`, virtual positions, into the rows' state.  The next tile's rows and the table
 // entries of the one after it are asked for before a tile is computed.
-template <int D, int DT, bool APART, bool PAGED, class Seen>
+template <int D, int DT, bool APART, bool REST, bool PAGED, class Seen>
 __device__ __forceinline__ void attn_walk(AttnRows<D> &a, const KvSource<PAGED> &src, const uint4 (&q)[D / 32], int first,
                                           int to, int step, Seen seen, float scale2, int lane) {
   if (first >= to) return;
@@ -332,7 +333,7 @@ __device__ __forceinline__ void attn_walk(AttnRows<D> &a, const KvSource<PAGED> 
       next = after;
     }
     seen.look(seen.place(tile));
-    attn_tile<D, DT, APART>(a, cur, q, seen.place(tile), seen, scale2, lane);
+    attn_tile<D, DT, APART, REST>(a, cur, q, seen.place(tile), seen, scale2, lane);
     cur = ahead;
   }
 }

@@ -10,6 +10,11 @@
 //   * narrow: those of the decode kernel (attn_common.h), 16 rows to a workgroup, whose four waves take 32 positions each of a
 //     tile of 128, from memory to registers.
 //
+// The narrow form takes its weights and then what their rounding to 16 bits leaves, as decode does, whose tokens a draft's stand in
+// for: the matrix cores idle there (26 nodes behind 1531 positions 17.9 -> 18.3 us, errors 2.6e-4 -> 2.1e-4).  The wide form takes
+// them as rounded, like the prompts: with the rest 157 -> 204, 71 -> 86 and 305 -> 412 us for the batch of trees, short windows and the
+// long chunk, errors (rms) 1.77e-3 -> 1.64e-3, 2.6e-4 -> 2.0e-4 and 2.3e-3 -> 1.7e-3.
+//
 // An item is up to 128 (16) rows of a sequence and key-value head.  It walks over the tiles that hold what its rows see, those that
 // hold nothing seen left out.  Items that are much longer than an equal share of all tiles are cut into parts, which leave their
 // outputs, unnormalised, maxima and sums in the workspace, and a second launch joins them, always in the same order.  A
@@ -396,7 +401,7 @@ __device__ __attribute__((noinline)) void masked_rows16(const MaskedRows<MODE> &
   seen.token = token;
   AttnRows<D> a;
   attn_clear(a);
-  attn_walk<D, DT, true>(a, p.src, qf, p.from, p.end, 32, seen, p.scale2, lane);
+  attn_walk<D, DT, true, true>(a, p.src, qf, p.from, p.end, 32, seen, p.scale2, lane);
   const float l = attn_row_sum(a.l);
   if (p.r0 + at0 + i16 >= p.all) return;
   if (p.to.part) {
@@ -633,7 +638,7 @@ __global__ __launch_bounds__(64 * kWaves, masked_round(D)) void masked_narrow_ke
   const MaskedSeen<MODE> seen{seq, token, rule.group(r0), min(rule.group(r0 + 15), seq.n - 1), p.gap_from, p.gap, 0, false};
   AttnRows<D> a;
   attn_clear(a);
-  attn_walk<D, DT, true>(a, src, qf, p.from + 32 * wave, p.end, Narrow::kStep, seen, flip ? -scale2 : scale2, lane);
+  attn_walk<D, DT, true, true>(a, src, qf, p.from + 32 * wave, p.end, Narrow::kStep, seen, flip ? -scale2 : scale2, lane);
   a.l = attn_row_sum(a.l);
 
   float *part = parts + (static_cast<int64_t>(p.slot) * kvh + kh) * slot_rows * (D + 2);

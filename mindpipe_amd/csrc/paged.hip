@@ -199,8 +199,8 @@ __global__ __launch_bounds__(64 * kWaves, decode_round(D)) void paged_decode_ker
     src.last = len > 0 ? (len - 1) >> shift : 0;
     AttnRows<D> a;
     attn_clear(a);
-    if constexpr (WIN) attn_walk<D, DT, false>(a, src, qf, at * kBlock + 32 * wave, t1, kBlock, plan.seen(b), scale2, lane);
-    else attn_walk<D, DT, false>(a, src, qf, at * kBlock + 32 * wave, t1, kBlock, SeenUpTo{t1, t1, t1}, scale2, lane);
+    if constexpr (WIN) attn_walk<D, DT, false, true>(a, src, qf, at * kBlock + 32 * wave, t1, kBlock, plan.seen(b), scale2, lane);
+    else attn_walk<D, DT, false, true>(a, src, qf, at * kBlock + 32 * wave, t1, kBlock, SeenUpTo{t1, t1, t1}, scale2, lane);
     a.l = attn_row_sum(a.l);
 
     const int64_t slot = (static_cast<int64_t>(2 * run + (left < to - from ? 1 : 0)) * heads + h) * min(grp, 16);

@@ -54,7 +54,7 @@ __device__ __attribute__((noinline)) void prompt_rows16(const PromptRows<PAGED> 
   for (int c = 0; c < D / 32; ++c) qf[c] = *reinterpret_cast<const uint4 *>(qp + 32 * c);
   AttnRows<D> a;
   attn_clear(a);
-  attn_walk<D, DT, true>(a, p.src, qf, p.from, min(end, p.to), 32, SeenUpTo{seen(at), end, full}, p.scale2, lane);
+  attn_walk<D, DT, true, false>(a, p.src, qf, p.from, min(end, p.to), 32, SeenUpTo{seen(at), end, full}, p.scale2, lane);
   const float l = attn_row_sum(a.l);
   if (r0 + i16 >= p.all) return;
   if (p.part) {
