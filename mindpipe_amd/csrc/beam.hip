@@ -466,6 +466,7 @@ extern "C" int mp_beam_select(const void *logits, int64_t stride, int64_t batch,
   const int64_t rows = batch * beams;
   const int h = beam_eights(rows, vocab), n = static_cast<int>(vocab), k = static_cast<int>(count);
   const int splits = static_cast<int>(beam_splits(rows, vocab));
+  if (rows * splits > kMpMaxGroups) return MP_ERR_SHAPE;
   BeamPart *parts = static_cast<BeamPart *>(workspace);
   BeamValue *lists = reinterpret_cast<BeamValue *>(parts + rows * splits);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);

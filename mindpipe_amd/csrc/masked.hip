@@ -780,13 +780,14 @@ int masked_start(const MaskedCall &c, int shift) {
       hipFuncSetAttribute(reinterpret_cast<const void *>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)
     return MP_ERR_HIP;
   const mp_pages &p = *c.cache;
+  const int64_t blocks = (masked_items<FORM>(c.rows, grp, c.batch) + masked_more(share)) * c.kvh;
+  if (blocks > kMpMaxGroups) return MP_ERR_SHAPE;
   if (masked_plan_words(c.batch)) {
     hipLaunchKernelGGL((masked_plan_kernel<MODE, FORM>), dim3(1), dim3(kPlanThreads), 0, c.stream, c.starts, c.lens,
                        static_cast<int>(c.batch), static_cast<int>(c.rows), grp, static_cast<int>(p.width << shift), c.rule, share,
                        planned);
     MP_CHECK_LAUNCH();
   }
-  const int64_t blocks = (masked_items<FORM>(c.rows, grp, c.batch) + masked_more(share)) * c.kvh;
   hipLaunchKernelGGL(kKernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), kLds, c.stream,
                      static_cast<const uint16_t *>(c.q), c.q_row, c.q_head, static_cast<const uint16_t *>(p.k), p.k_page,
                      p.k_head, p.k_row, static_cast<const uint16_t *>(p.v), p.v_page, p.v_head, p.v_row, static_cast<int>(p.pages),

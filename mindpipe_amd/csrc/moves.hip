@@ -103,7 +103,7 @@ extern "C" int mp_paged_copy_pages(const mp_pages *cache, int64_t layers, int64_
   const int rc = move_pools(cache, layers, k_layer, v_layer, kvh, head_dim, false, p);
   if (rc != MP_OK) return rc;
   const int64_t per = mp_cdiv(static_cast<int64_t>(kvh) * p.chunks << p.shift, 256);
-  if (count < 0 || count > INT32_MAX / per) return MP_ERR_SHAPE;
+  if (count < 0 || count > kMpMaxGroups / per) return MP_ERR_SHAPE;
   if (count == 0) return MP_OK;
   hipLaunchKernelGGL(paged_copy_kernel, dim3(static_cast<unsigned>(count * per), static_cast<unsigned>(2 * layers)), dim3(256), 0,
                      reinterpret_cast<hipStream_t>(stream), p, src, dst, filled, static_cast<int>(per));
@@ -119,7 +119,7 @@ extern "C" int mp_paged_keep_positions(const mp_pages *cache, int64_t layers, in
   const int rc = move_pools(cache, layers, k_layer, v_layer, kvh, head_dim, true, p);
   if (rc != MP_OK) return rc;
   const int64_t columns = 2 * layers * kvh * p.chunks, per = mp_cdiv(columns, 256);
-  if (columns > INT32_MAX - 256 || batch < 0 || batch > INT32_MAX / per || total < 0 || total > INT32_MAX / 2) return MP_ERR_SHAPE;
+  if (columns > INT32_MAX - 256 || batch < 0 || batch > kMpMaxGroups / per || total < 0 || total > INT32_MAX / 2) return MP_ERR_SHAPE;
   if (batch == 0 || total == 0) return MP_OK;
   hipLaunchKernelGGL(paged_keep_kernel, dim3(static_cast<unsigned>(batch * per)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
                      p, cache->table, static_cast<int>(cache->width), first, keep, starts, static_cast<int>(total), static_cast<int>(per));

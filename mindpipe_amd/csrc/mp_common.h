@@ -27,6 +27,9 @@ static inline bool mp_aligned(const void *p, size_t a) {
 
 static inline int64_t mp_cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Workgroups of 256 threads that a launch holds in a dimension: a grid has below 2^32 threads there.
+constexpr int64_t kMpMaxGroups = (int64_t(1) << 24) - 1;
+
 // Division of numbers below 2^31 by a number that the host knows: (x m) >> shift with m = ceil(2^shift / d), shift = 31 + ceil(log2
 // d): the quotient is too large by less than x / 2^shift < 1 / d, which no floor notices.  A launch of few tiles is bound by the
 // instructions on its way to them.

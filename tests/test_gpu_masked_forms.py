@@ -109,3 +109,18 @@ def test_narrow_over_infinite_values(dtype, dim, kvh, grp):
     ref.check(got, *mref.masked_attention(q, k, v, table, ln, torch.tensor(at), mref.in_tree(sets), scale))
     got = _ops().paged_prompt_window_attention(q, k, v, table, ln, _ints(at), scale, 1500, 2)
     ref.check(got, *mref.masked_attention(q, k, v, table, ln, torch.tensor(at), mref.in_window(1500, 2), scale))
+
+
+# ---------------------------------------------------------------- what a launch does not hold
+@pytest.mark.parametrize("batch,kvh", [(65536, 65536), (1 << 20, 4096), (1 << 18, 64)])
+def test_more_workgroups_than_a_launch_holds(batch, kvh):
+    """Sequences times key-value heads past what a grid has: refused, not cut to its low bits."""
+    k = torch.zeros(1, kvh, 8, 64, device=DEV, dtype=F16)
+    table, ln = torch.zeros(batch, 1, device=DEV, dtype=torch.int32), torch.ones(batch, device=DEV, dtype=torch.int32)
+    starts = torch.ones(batch + 1, device=DEV, dtype=torch.int32)
+    starts[0] = 0
+    q, m = torch.zeros(1, kvh, 64, device=DEV, dtype=F16), torch.ones(1, 1, device=DEV, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="shape"):
+        _ops().paged_tree_attention(q, k, k, table, ln, starts, m, 0.1)
+    with pytest.raises(RuntimeError, match="shape"):
+        _ops().paged_prompt_window_attention(q, k, k, table, ln, starts, 0.1, 4, 0)
