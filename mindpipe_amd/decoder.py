@@ -129,6 +129,7 @@ class PagedKVCache:
         self.lens = torch.zeros(sequences, device=device, dtype=torch.int32)
         self.length = [0] * sequences                      # of lens, on the host
         self._held: List[List[int]] = [[] for _ in range(sequences)]  # -1: a page that was trimmed
+        self._least = [0] * sequences                      # below it a next token would look at pages that were trimmed
         self._uses = [0] * pages                           # sequences that hold a page
         self._free = list(range(pages - 1, -1, -1))
 
@@ -209,7 +210,7 @@ class PagedKVCache:
         """Ends a sequence: the pages that it alone held are free again."""
         self._drop(reversed(self._held[sequence]))
         self._held[sequence] = []
-        self.length[sequence] = 0
+        self._least[sequence] = self.length[sequence] = 0
         self.lens[sequence] = 0
 
     @torch.no_grad()
@@ -228,6 +229,7 @@ class PagedKVCache:
         for pages in self._held:
             self._drop(reversed(pages))
         self._held = held
+        self._least = [self._least[o] for o in order]
         self.length = [self.length[o] for o in order]
         self.table.copy_(self.table[torch.tensor(list(order), device=self.table.device)])
         self._set_lens()
@@ -244,14 +246,15 @@ class PagedKVCache:
     @torch.no_grad()
     def keep(self, drafted: Sequence[int], kept: Sequence[Sequence[int]]) -> None:
         """Of the last ``drafted[b]`` positions of each sequence b those that ``kept[b]`` names stay, ascending from 0, one behind
-        the other; pages behind them are free again."""
+        the other; pages behind them are free again.  Raises, and changes nothing, where a sequence was forked since its draft, or
+        trimmed so far that its next token would look at a page that is gone."""
         if len(drafted) != len(self.length) or len(kept) != len(self.length):
             raise ValueError(f"a count and a list for each of the {len(self.length)} sequences")
         for l, n, at in zip(self.length, drafted, kept):
             if not 0 <= n <= l or any(not 0 <= i < n for i in at) or any(i >= j for i, j in zip(at, at[1:])):
                 raise ValueError(f"{list(at)} must ascend below the {n} drafted positions of {l}")
-        for l, n, held in zip(self.length, drafted, self._held):
-            if n and any(page < 0 or self._uses[page] > 1 for page in held[(l - n) // self.page:]):
+        for l, n, at, held, least in zip(self.length, drafted, kept, self._held, self._least):
+            if n and (l - n + len(at) < least or any(page < 0 or self._uses[page] > 1 for page in held[(l - n) // self.page:])):
                 raise RuntimeError("a sequence that was forked or trimmed since its draft keeps it as it is")
         if any(i != j for at in kept for j, i in enumerate(at)):
             device, first = self.table.device, [l - n for l, n in zip(self.length, drafted)]
@@ -283,6 +286,7 @@ class PagedKVCache:
         for b, i in zip(rows, cols):
             self._drop([self._held[b][i]])
             self._held[b][i] = -1
+            self._least[b] = max(self._least[b], (i + 1) * self.page + window - 1)
         self._set_table(rows, cols, [-1] * len(rows))
         return len(rows)
 
