@@ -124,3 +124,23 @@ def test_more_workgroups_than_a_launch_holds(batch, kvh):
         _ops().paged_tree_attention(q, k, k, table, ln, starts, m, 0.1)
     with pytest.raises(RuntimeError, match="shape"):
         _ops().paged_prompt_window_attention(q, k, k, table, ln, starts, 0.1, 4, 0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_narrow_repeats_its_bits(dtype, dim):
+    """NaN in a key, an infinity and NaN in values: the same bits again, those of the NaN included."""
+    news, lens = [5, 1, 30], [700, 90, 400]
+    g = torch.Generator().manual_seed(dim)
+    k, v, table = _pages_of(lens, 2, dim, 16, dtype, g)
+    k[int(table[0, 43]), 0, 10], v[int(table[2, 24]), 1, 3], v[int(table[0, 1]), 0, 2, 5] = float("nan"), float("nan"), float("inf")
+    at, ln = _ints(_starts(news)), _ints(lens)
+    q = torch.randn(36, 6, dim, generator=g).to(dtype).to(DEV)
+    m = mref.masks(_trees(news, 2), 1).to(DEV)
+    assert _form(36, 6, 2, dim, 3, 16 * table.shape[1]) == NARROW
+    for call in (lambda: _ops().paged_tree_attention(q, k, v, table, ln, at, m, 0.1),
+                 lambda: _ops().paged_prompt_window_attention(q, k, v, table, ln, at, 0.1, 300, 40)):
+        got = call()
+        assert got.isnan().any() and torch.isfinite(got).any()
+        for _ in range(5):
+            assert torch.equal(got.view(torch.int16), call().view(torch.int16))
