@@ -106,13 +106,28 @@ struct Wide {
 struct Narrow {
   static constexpr int kItem = 16, kStep = 128, kSlack = 2, kFiner = INT_MAX;
 };
-// Parts that have others, in shares at most: an item of T > limit tiles has up to 2 T / (limit + 1), and with limit from two thirds of
-// a share e on, 2 (e + 1) / (2 e / 3 + 2) is below 3.
+// How long a part may be, in tiles, with e tiles an equal share: as long as an item that stays whole, or finer.
+template <class FORM>
+constexpr int masked_keep(int e) { return e + (e / 2 < FORM::kSlack ? e / 2 : FORM::kSlack) + 1; }
+constexpr int masked_finer(int e) { return e * 2 / 3 + 1; }
+// Parts that have others, in shares at most: an item of T > limit tiles has up to 2 T / (limit + 1), all of them fewer than
+// 2 (e + 1) / (limit + 1) of a share.
 constexpr int kSlots = 3;
-// How many more parts than items there are, at most: T / limit for an item that is cut, together (e + 1) / limit of a share, which is
-// below 1 with a limit above e and at most 14 / 9 (e = 13, limit 9) with the finer one, for which e >= kFiner.
+// How many more parts than items there are, at most: fewer than T / limit for an item that is cut, together (e + 1) / limit of a share,
+// which is no more than 1 with a limit above e and at most 14 / 9 (e = 13, limit 9) with the finer one.
 constexpr int64_t masked_more(int64_t share) { return share * 14 / 9 + 1; }
-static_assert(Wide::kFiner >= 12 && Narrow::kFiner >= 12, "(e + 1) / (2 e / 3 + 1) is more for e of 7 and 10");
+// The grid and the workspace rest on these two: checked for every e of 16 bits, from where on the finer limit's quotients are within
+// 2e-5 of 3 / 2 and below 3.  (3 / 2 itself is too little for every e of 3 m + 1, and 14 / 9 for the 7 and 10 that are below kFiner.)
+template <class FORM>
+constexpr bool masked_bounds_hold() {
+  for (int64_t e = 0; e < 1 << 16; ++e) {
+    const int64_t keep = masked_keep<FORM>(static_cast<int>(e)), finer = e < FORM::kFiner ? keep : masked_finer(static_cast<int>(e));
+    const int64_t limit = keep < finer ? keep : finer;
+    if (2 * (e + 1) > kSlots * (limit + 1) || 9 * (e + 1) > 14 * limit) return false;
+  }
+  return true;
+}
+static_assert(masked_bounds_hold<Wide>() && masked_bounds_hold<Narrow>(), "a part without a workgroup, or without a place to join from");
 
 constexpr int64_t kMaxBatch = 1 << 28;
 constexpr int kPlanNear = 64;  // sequences, with the two that hold the other rows, which a wave sees at once
@@ -182,9 +197,9 @@ struct MaskedPlan {
   // 129 tiles for 64 workgroups: 186 us, 152 with the finer ones).
   template <class EACH, class SUM, class MOST>
   static __device__ __forceinline__ int limit_of(uint32_t all, int share, EACH each, SUM sum, MOST most) {
-    const int equal = static_cast<int>(all / static_cast<uint32_t>(share)), keep = equal + min(equal / 2, FORM::kSlack) + 1;
+    const int equal = static_cast<int>(all / static_cast<uint32_t>(share)), keep = masked_keep<FORM>(equal);
     if (equal < FORM::kFiner) return keep;
-    const int finer = equal * 2 / 3 + 1;
+    const int finer = masked_finer(equal);
     int took[2] = {0, 0};
     for (int i = 0; i < 2; ++i) {
       uint32_t count = 0;
