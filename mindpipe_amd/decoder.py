@@ -131,6 +131,7 @@ class PagedKVCache:
         self._held: List[List[int]] = [[] for _ in range(sequences)]  # -1: a page that was trimmed
         self._least = [0] * sequences                      # below it a next token would look at pages that were trimmed
         self._uses = [0] * pages                           # sequences that hold a page
+        self._shared = 0                                   # holds of pages beyond their first
         self._free = list(range(pages - 1, -1, -1))
 
     def free_positions(self) -> int:
@@ -145,7 +146,9 @@ class PagedKVCache:
         for page in pages:
             if page >= 0:
                 self._uses[page] -= 1
-                if not self._uses[page]:
+                if self._uses[page]:
+                    self._shared -= 1
+                else:
                     self._free.append(page)
 
     def _set_table(self, rows: List[int], cols: List[int], pages: List[int]) -> None:
@@ -169,7 +172,7 @@ class PagedKVCache:
             raise RuntimeError(f"a sequence would pass {self.max_len} positions")
         # begun pages that others hold as well: all but the last of their holders that go on have them copied
         uses, copies = {}, []
-        for b, (l, n, held) in enumerate(zip(self.length, news, self._held)):
+        for b, (l, n, held) in enumerate(zip(self.length, news, self._held) if self._shared else ()):
             if n and l % self.page:
                 page = held[l // self.page]
                 uses[page] = uses.get(page, self._uses[page])
@@ -185,7 +188,7 @@ class PagedKVCache:
             cols.append(self.length[b] // self.page)
             pages.append(self._take())
             self._held[b][cols[-1]] = pages[-1]
-            self._uses[page] -= 1
+            self._drop([page])
         if copies:
             move = torch.tensor([[page for _, page in copies], pages, [self.length[b] % self.page for b, _ in copies]],
                                 device=device, dtype=torch.int32)
@@ -226,6 +229,7 @@ class PagedKVCache:
             for page in pages:
                 if page >= 0:
                     self._uses[page] += 1
+                    self._shared += 1
         for pages in self._held:
             self._drop(reversed(pages))
         self._held = held
