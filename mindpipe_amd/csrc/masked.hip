@@ -22,10 +22,10 @@
 //
 // The wide form is bound as the prompts' attention is, by matrix and vector instructions in turn: 2.2 us for a tile of a
 // workgroup, two to a CU.  2048 tokens behind 8192 positions with a window of 4096, 64 / 8 heads of 128 in bf16, 309 us, 0.9
-// PFLOP/s of what is seen; 24 sequences of up to 8192 positions with trees of up to 64 nodes 149 us, 53 tiles an equal share and
+// PFLOP/s of what is seen; 24 sequences of up to 8192 positions with trees of up to 64 nodes 147 us, 53 tiles an equal share and
 // about 66 the longest path.  (Equal runs of tiles over all items, with a loop over items in the kernel, took 171 us there: the
 // loop's state took the registers that hold the loads' offsets.)  The narrow form is bound by the chain from the lengths to a
-// page and by the reads: 26 nodes behind 1531 positions, 32 / 32 heads, 13.6 us and a join of 4.
+// page and by the reads: 26 nodes behind 1531 positions, 32 / 32 heads, 13.5 us and a join of 4 to 5.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
